@@ -273,7 +273,8 @@ def _turned(x, s, inverse=False):
 
 def _codes(x):
     most = x.abs().amax(-1).clamp(min=1e-6)
-    return torch.round(x * (127.0 / most)[..., None]).clamp(-128, 127).to(torch.int8), most * (1.0 / 127.0)
+    inv = torch.full_like(most, 127.0) / most   # one division (127.0 / most is a reciprocal and a product)
+    return torch.round(x * inv[..., None]).clamp(-128, 127).to(torch.int8), most * (1.0 / 127.0)
 
 
 def _values(s):

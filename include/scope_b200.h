@@ -45,6 +45,7 @@ extern "C" {
 #define WS_DTYPE_BF16 0
 #define WS_DTYPE_F32 1
 #define WS_DTYPE_I8 2
+#define WS_DTYPE_F16 3     /* the paged entries only */
 
 /* ---- GQA output modes (what the reference wrappers return) */
 #define WS_OUT_NORM_BF16 0   /* out bf16 normalised, max/sum bf16: fused_cpu_attn on bf16 (kernel/cpu_attn.cpp:631-634) */
@@ -378,6 +379,130 @@ int ws_lse_merge(const float* o_parts, const float* lse_parts, int P, int64_t R,
 int ws_lse_merge_strided(const float* o_parts, int64_t o_part_stride, const float* lse_parts,
                          int64_t lse_part_stride, int P, int64_t R, int D, void* out, int out_dtype,
                          float* out_lse, void* stream);
+
+/* ---- Paged key-value cache
+ *
+ * A pool of pages of `page_size` tokens each; a request owns the pages its
+ * row of the page table lists, in order, so its length is bounded by the pool
+ * and not by a reserved row.  These entries have no counterpart in the
+ * reference, whose caches reserve [rows, max_seq] (system/qwenoffload.py:59-141).
+ *
+ * Keys and values of slot s = page * page_size + offset, kv head h:
+ *   k (page, offset, h, d) at k + page*k_stride_page + offset*k_stride_tok + h*k_stride_head + d   (Dk wide)
+ *   v the same with v_stride_* and Dv.
+ * dtype WS_DTYPE_BF16, WS_DTYPE_F16, or WS_DTYPE_I8 with one fp32 scale per
+ * row (value = code * scale) at k_scales + page*ks_stride_page +
+ * offset*ks_stride_tok + h*ks_stride_head, likewise v_scales.
+ * Constraints: Dk, Dv multiples of 16, at most 256; page_size >= 1; k, v
+ * 16-byte aligned with strides of whole 16 bytes.
+ */
+typedef struct ws_paged_kv {
+    void* k;
+    void* v;
+    float* k_scales;   /* WS_DTYPE_I8 only */
+    float* v_scales;
+    int64_t n_pages;
+    int64_t k_stride_page, k_stride_tok, k_stride_head;
+    int64_t v_stride_page, v_stride_tok, v_stride_head;
+    int64_t ks_stride_page, ks_stride_tok, ks_stride_head;
+    int64_t vs_stride_page, vs_stride_tok, vs_stride_head;
+    int32_t page_size, Hkv, Dk, Dv, dtype, reserved;
+} ws_paged_kv;
+
+/*
+ * One step's page tables and slot map from the requests' lengths, on the
+ * device.  Request b holds seq_lens[b] tokens in the pages page_table[b, 0 ..
+ * ceil(seq_lens[b] / page_size)) and adds new_lens[b] tokens (negative counts
+ * read as 0).  In request order each takes the pages it lacks from the ring of
+ * free pages and writes them into its table row; then token j of request b
+ * (row cu_new[b] + j of the step's packed tokens) gets
+ *   positions = seq_lens[b] + j,  slots = page * page_size + offset.
+ *   ring [3] int32: head, free count, and (output) requests refused.  Free page
+ *   i is free_pages[(head + i) % n_ring]; served requests advance the head.
+ *   A request is refused whole when its pages would pass max_pages, its tokens
+ *   would pass n_tokens, or the pages it lacks, added to those of the requests
+ *   before it that passed the first two checks, are more than are free: its
+ *   length, table row and the ring stay as they are and its tokens get slot -1,
+ *   position 0.  Rows [cu_new[B], n_tokens) get the same.
+ *   cu_new [B+1], seq_lens_out [B] and ring_out [3] are int32; seq_lens_out may
+ *   be seq_lens and ring_out may be ring.  slots int64, positions int32 [n_tokens].
+ * One launch; B <= 8192.  The workspace is the counter header only.
+ */
+int ws_paged_slots(const int32_t* seq_lens, const int32_t* new_lens, int B, int32_t* page_table, int64_t table_stride,
+                   int max_pages, const int32_t* free_pages, int n_ring, const int32_t* ring, int page_size,
+                   int64_t n_tokens, int64_t* slots, int32_t* positions, int32_t* cu_new, int32_t* seq_lens_out,
+                   int32_t* ring_out, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * Give the pages of finished requests back: for every b with done[b] != 0, in
+ * request order, the pages of row b go to the ring's end and seq_lens_out[b] is
+ * 0; the other lengths are copied.  ring_out gets head, the new free count, 0.
+ * A ring that would overflow (pages given back twice) keeps what fits and
+ * records WS_ERR_DEVICE for ws_status_take.  One launch; B <= 8192.
+ */
+int ws_paged_release(const int32_t* seq_lens, const uint8_t* done, int B, const int32_t* page_table,
+                     int64_t table_stride, int max_pages, int32_t* free_pages, int n_ring, const int32_t* ring,
+                     int page_size, int32_t* seq_lens_out, int32_t* ring_out, void* workspace, size_t workspace_bytes,
+                     void* stream);
+size_t ws_paged_slots_workspace_size(void);
+
+/*
+ * Rotary positions with up to four axes (time, height, width, ...).  Pair i of
+ * the first rope_dim dims turns by the angle of position[axis(i)]:
+ *   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin      (inverse: sin negated, also the gradient)
+ * with (cos, sin) = cos_sin[position, i], cos_sin[position, rope_dim/2 + i]
+ * (fp32 [max_pos, rope_dim]) and the pair at dims (i, rope_dim/2 + i), or
+ * (2i, 2i+1) with `adjacent`.  Each product and sum is rounded to fp32 by
+ * itself, so the result equals the formula's elementwise evaluation bit for bit.
+ *   axis(i) is two bits at axis_map[i / 16] >> (2 * (i % 16));
+ *   positions int32 (or int64 with positions_i64), axis a's at positions + a*axis_stride;
+ *   a position outside [0, max_pos) is clamped and recorded (WS_ERR_DEVICE).
+ * rope_dim: a multiple of 16, at most 256.
+ */
+typedef struct ws_rope {
+    const void* positions;
+    const float* cos_sin;
+    int64_t axis_stride;
+    int64_t max_pos;
+    int32_t positions_i64, n_axes, rope_dim, adjacent, inverse, reserved;
+    uint32_t axis_map[8];
+} ws_rope;
+
+/*
+ * Rotation of a step's queries and keys, and the scatter of its keys and
+ * values into the paged cache, in one launch.
+ *   q [N, H, Dk] -> q_out (may be q); k [N, Hkv, Dk], v [N, Hkv, Dv]: element
+ *   (t, h, d) at base + t*stride_tok + h*stride_head + d; dtype WS_DTYPE_BF16 or
+ *   WS_DTYPE_F16.  The pool holds that type, or int8 codes:
+ *   scale = max(max|x|, 1e-6) / 127, code = rne(x * 127 / max) per row (the rule
+ *   of ws_csa_kv_quantize_s8), taken from the rotated fp32 row.
+ *   slots int64 [N]: token t's keys and values go to slot slots[t]; a negative
+ *   slot drops them, one past the pool drops them and records WS_ERR_DEVICE.
+ * rope NULL: no rotation.  H = 0: no queries.  kv NULL: queries only (k, v,
+ * slots ignored; Dk is given by `D`).
+ */
+int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stride_tok, int64_t q_stride_head, int H, int D,
+                   void* q_out, int64_t qo_stride_tok, int64_t qo_stride_head, const void* k, int64_t k_stride_tok,
+                   int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head, int dtype,
+                   int64_t N, const int64_t* slots, const ws_paged_kv* kv, void* stream);
+
+/*
+ * Attention of one new token per request over the paged cache.
+ *   q [B, Hkv*G, Dk] in q_dtype (WS_DTYPE_BF16 or WS_DTYPE_F16; the pool holds
+ *   that type or int8): head (b, h) at q + b*q_stride_b + h*q_stride_h,
+ *   h = kvh * G + g, 16-byte aligned rows;
+ *   page_table int32 [B, max_pages], row b at page_table + b*table_stride;
+ *   seq_lens int32 [B]: tokens [0, seq_lens[b]) are attended (clipped to
+ *   max_pages * page_size), with window > 0 only the last `window` of them;
+ *   out [B, Hkv*G, Dv] contiguous in q_dtype, normalised; out_lse [B, Hkv*G] fp32 (NULL: none).
+ * A request without tokens gives out = 0, lse = -inf.  A page id outside the
+ * pool leaves its tokens out and records WS_ERR_DEVICE.  Nothing past a
+ * request's length is used, whatever the pages hold there.
+ */
+int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q_dtype, int B, int G,
+                    const ws_paged_kv* kv, const int32_t* page_table, int64_t table_stride, int max_pages,
+                    const int32_t* seq_lens, int window, float scale, void* out, float* out_lse, void* workspace,
+                    size_t workspace_bytes, void* stream);
+size_t ws_paged_decode_workspace_size(int B, int Hkv, int G, int Dv);
 
 #ifdef __cplusplus
 }

@@ -17,9 +17,12 @@ import os
 
 from . import cpu_attn as _cpu_attn
 from ._lib import LIB_PATH, ScopeError, lib
+from .kv_cache import PagedKVCache
 from .ops import Share, gqa_decode_shares, lse_merge
+from .paged import PagedStep, paged_decode, paged_release, paged_slots, rope, rope_append
 
 __all__ = ["build", "build_tile", "build_csa_attn", "lib", "ScopeError", "Share", "gqa_decode_shares", "lse_merge",
+           "PagedKVCache", "PagedStep", "paged_slots", "paged_release", "rope", "rope_append", "paged_decode",
            "status_take"]
 
 

@@ -8,6 +8,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -26,6 +27,7 @@ WS_ERR_DEVICE = 5
 WS_DTYPE_BF16 = 0
 WS_DTYPE_F32 = 1
 WS_DTYPE_I8 = 2
+WS_DTYPE_F16 = 3   # the paged entries only
 
 WS_OUT_NORM_BF16 = 0
 WS_OUT_UNNORM_F32 = 1
@@ -49,6 +51,12 @@ class KvShare(ctypes.Structure):
     """Mirror of `ws_kv_share` (include/scope_b200.h)."""
     _fields_ = [("k", _V), ("v", _V), ("cu_seqlens", _V), ("seqlens", _V), ("n_tok", _i64),
                 ("k_stride_t", _i64), ("k_stride_h", _i64), ("v_stride_t", _i64), ("v_stride_h", _i64)]
+
+
+# `ws_paged_kv` and `ws_rope` (include/scope_b200.h) packed in one call each: k, v, scales, pages, the twelve strides and
+# the six ints; positions, table, axis stride, max_pos, the six ints and the axis map (as 32 bytes).
+paged_kv_pack = struct.Struct("@QQQQq12q6i").pack
+rope_pack = struct.Struct("@QQqq6i32s").pack
 
 
 # exported symbol -> (restype, argtypes); the CPU tests check that every
@@ -85,6 +93,13 @@ SIGNATURES = {
     "ws_indexer_topk": (_i, [_V, _V, _i, _V, _i, _i, _i, _i64, _i, _i, _V, _V, _V, _sz, _V]),
     "ws_indexer_topk_workspace_size": (_sz, [_i, _i64]),
     "ws_kv_append": (_i, [_V, _i64, _i64, _i64, _V, _i64, _i64, _i64, _i64, _i, _i, _i64, _V]),
+    "ws_paged_slots": (_i, [_V, _V, _i, _V, _i64, _i, _V, _i, _V, _i, _i64, _V, _V, _V, _V, _V, _V, _sz, _V]),
+    "ws_paged_release": (_i, [_V, _V, _i, _V, _i64, _i, _V, _i, _V, _i, _V, _V, _V, _sz, _V]),
+    "ws_paged_slots_workspace_size": (_sz, []),
+    "ws_rope_append": (_i, [_V, _V, _i64, _i64, _i, _i, _V, _i64, _i64, _V, _i64, _i64, _V, _i64, _i64, _i, _i64, _V, _V,
+                            _V]),
+    "ws_paged_decode": (_i, [_V, _i64, _i64, _i, _i, _i, _V, _V, _i64, _i, _V, _i, _f, _V, _V, _V, _sz, _V]),
+    "ws_paged_decode_workspace_size": (_sz, [_i, _i, _i, _i]),
     "ws_peer_exchange_bytes": (_sz, [_i, _i64, _i]),
     "ws_peer_slot_offset": (_sz, [_i, _i64, _i, _i]),
     "ws_peer_buffer_create": (_i, [_sz, ctypes.POINTER(_V), _V]),

@@ -1,0 +1,296 @@
+// Page tables and slot maps of a paged key-value cache, built on the device
+// from the requests' lengths, and the return of finished requests' pages.
+//
+// With P tokens a page, request b of length L_b that adds n_b tokens lacks
+//   need_b = ceil((L_b + n_b) / P) - ceil(L_b / P)
+// pages.  The exclusive scans of n_b (where its tokens start in the packed
+// step) and of need_b (where its pages start in the ring of free pages) make
+// every token independent of every other: token t finds its request by a
+// binary search over the scan, and its page is either the request's last page
+// or a fixed place of the ring.  The token that opens a page writes the table.
+//
+// What bounds it: latency.  The reads and writes of a step are a few hundred
+// kilobytes at most.  So every CTA repeats the scan over all requests (two
+// loads a request, kept in shared memory) instead of waiting for another
+// launch, and takes kTokensPerCta tokens; a step of up to that many is one
+// CTA.  Lengths and ring may be updated in place: with one CTA after a
+// barrier, with more by the CTA that finishes last (a ticket), when no other
+// reads them any more.
+#include <cstdio>
+
+#include "common.cuh"
+#include "ws_internal.h"
+
+namespace ws {
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kTokensPerCta = 2048;
+constexpr int kMaxRequests = 8192;   // 16 bytes of shared memory each
+
+// Exclusive scan of one value per thread over the block; `carry` holds the
+// total of the earlier chunks and takes this chunk's.  All threads call it.
+struct BlockScan {
+    long long part[kThreads / 32];
+    long long total;
+};
+__device__ __forceinline__ long long block_scan(long long v, BlockScan& sh, long long& carry) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();   // the previous call's reads are done
+    if (lane == 31) sh.part[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        long long p = lane < nw ? sh.part[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, p, o);
+            if (lane >= o) p += y;
+        }
+        if (lane < nw) sh.part[lane] = p;
+        if (lane == nw - 1) sh.total = p;
+    }
+    __syncthreads();
+    const long long ex = carry + x - v + (warp ? sh.part[warp - 1] : 0);
+    carry += sh.total;
+    return ex;
+}
+
+// True in the CTA that gets here last (always, with one CTA); that CTA then
+// sees everything the others read or wrote before.  The counter returns to 0.
+__device__ __forceinline__ bool last_cta(int* counter) {
+    if (gridDim.x == 1) {
+        __syncthreads();
+        return true;
+    }
+    __shared__ int last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(counter, 1) == (int)gridDim.x - 1;
+        if (last) *counter = 0;
+        __threadfence();
+    }
+    __syncthreads();
+    return last;
+}
+
+// First b in [0, B) whose end[b] > t (ends ascend; t < end[B - 1]).
+__device__ __forceinline__ int owner_of(const int* end, int B, int t) {
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (end[mid] > t) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kThreads)
+paged_slots_kernel(const int32_t* seq_lens, const int32_t* __restrict__ new_lens, int B, int32_t* table,
+                   int64_t table_stride, int max_pages, const int32_t* __restrict__ free_pages, int n_ring,
+                   const int32_t* ring, int P, int64_t n_tokens, int64_t* __restrict__ slots,
+                   int32_t* __restrict__ positions, int32_t* __restrict__ cu_new, int32_t* seq_lens_out,
+                   int32_t* ring_out, int* counter) {
+    extern __shared__ int sm[];
+    __shared__ BlockScan sh;
+    __shared__ int n_refused;
+    int* end = sm;            // tokens of requests 0 .. b, clipped to n_tokens
+    int* len = sm + B;        // tokens before the step, or -1: refused
+    int* base = sm + 2 * B;   // first ring place (counted from the head) of b's new pages
+    int* first = sm + 3 * B;  // first token of b in the packed step
+    if (threadIdx.x == 0) n_refused = 0;
+    const int head = ring[0], n_free = min(max(ring[1], 0), n_ring);
+    long long tokens = 0, pages = 0, took = 0;
+    int refused = 0;
+    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        const long long L = b < B ? max(seq_lens[b], 0) : 0;
+        const long long n = b < B ? max(new_lens[b], 0) : 0;
+        const long long start = block_scan(n, sh, tokens);
+        const long long held = (L + P - 1) / P, want = (L + n + P - 1) / P;
+        const bool fits = want <= max_pages && start + n <= n_tokens && L + n <= INT32_MAX;
+        const long long need = fits ? want - held : 0;
+        const long long place = block_scan(need, sh, pages);
+        if (b < B) {
+            const bool served = fits && (need == 0 || place + need <= n_free);
+            end[b] = (int)min(start + n, (long long)n_tokens);
+            first[b] = (int)min(start, (long long)n_tokens);
+            len[b] = served ? (int)L : -1;
+            base[b] = (int)min(place, (long long)n_ring);
+            refused += !served;
+            if (served && need) took = max(took, place + need);
+            if (blockIdx.x == 0) {
+                if (b == 0) cu_new[0] = 0;
+                cu_new[b + 1] = (int)min(start + n, (long long)INT32_MAX);
+            }
+        }
+    }
+    if (B == 0 && blockIdx.x == 0 && threadIdx.x == 0) cu_new[0] = 0;
+    __syncthreads();
+    const int real = B > 0 ? end[B - 1] : 0;
+    const int64_t t_end = min((int64_t)(blockIdx.x + 1) * kTokensPerCta, n_tokens);
+    for (int64_t t = (int64_t)blockIdx.x * kTokensPerCta + threadIdx.x; t < t_end; t += blockDim.x) {
+        int64_t slot = -1;
+        int pos = 0;
+        if (t < real) {
+            const int b = owner_of(end, B, (int)t);
+            if (len[b] >= 0) {
+                const unsigned L = len[b];
+                const unsigned p = L + (unsigned)((int)t - first[b]), col = p / (unsigned)P, off = p - col * P;
+                const unsigned held = (L + P - 1) / (unsigned)P;
+                int32_t* row = table + (int64_t)b * table_stride;
+                int page;
+                if (col < held) {
+                    page = row[col];
+                } else {
+                    page = free_pages[(unsigned)((head + (long long)base[b] + (col - held)) % n_ring)];
+                    if (off == 0) row[col] = page;
+                }
+                pos = (int)p;
+                if (page >= 0) slot = (int64_t)page * P + off;
+            }
+        }
+        slots[t] = slot;
+        positions[t] = pos;
+    }
+    if (!last_cta(counter)) return;
+    // served requests that took pages are a prefix of those that fit, so the largest end is what was taken
+    refused = __reduce_add_sync(0xffffffffu, refused);
+    if ((threadIdx.x & 31) == 0 && refused) atomicAdd(&n_refused, refused);
+    const int taken = __reduce_max_sync(0xffffffffu, (int)took);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) reinterpret_cast<int*>(sh.part)[threadIdx.x >> 5] = taken;
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
+        const int n = max(new_lens[b], 0);
+        const int L = max(seq_lens[b], 0);
+        seq_lens_out[b] = len[b] >= 0 ? L + n : seq_lens[b];
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int all = 0;
+        for (int w = 0; w < (int)(blockDim.x >> 5); ++w) all = max(all, reinterpret_cast<int*>(sh.part)[w]);
+        ring_out[0] = (int)((head + (long long)all) % n_ring);
+        ring_out[1] = n_free - all;
+        ring_out[2] = n_refused;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads)
+paged_release_kernel(const int32_t* seq_lens, const uint8_t* __restrict__ done, int B,
+                     const int32_t* __restrict__ table, int64_t table_stride, int max_pages, int32_t* free_pages,
+                     int n_ring, const int32_t* ring, int P, int32_t* seq_lens_out, int32_t* ring_out, int* counter,
+                     int* status) {
+    extern __shared__ int sm[];
+    __shared__ BlockScan sh;
+    int* end = sm;   // pages of requests 0 .. b that go back
+    const int head = ring[0], n_free = min(max(ring[1], 0), n_ring);
+    const int room = n_ring - n_free;
+    long long pages = 0;
+    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        long long held = 0;
+        if (b < B && done[b]) held = min(((long long)max(seq_lens[b], 0) + P - 1) / P, (long long)max_pages);
+        const long long start = block_scan(held, sh, pages);
+        if (b < B) end[b] = (int)min(start + held, (long long)INT32_MAX);
+    }
+    __syncthreads();
+    const int total = (int)min(pages, (long long)room);
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
+        const int b = owner_of(end, B, i);
+        const int j = i - (b ? end[b - 1] : 0);
+        free_pages[(unsigned)((head + (long long)n_free + i) % n_ring)] = table[(int64_t)b * table_stride + j];
+    }
+    if (!last_cta(counter)) return;
+    for (int b = threadIdx.x; b < B; b += blockDim.x) seq_lens_out[b] = done[b] ? 0 : seq_lens[b];
+    if (threadIdx.x == 0) {
+        ring_out[0] = head;
+        ring_out[1] = n_free + total;
+        ring_out[2] = 0;
+        if (pages > room && status) atomicMax(status, kDevBadIndex);
+    }
+}
+
+int checked(const char* what, int B, int max_pages, int64_t table_stride, int n_ring, int page_size, void* workspace,
+            size_t workspace_bytes) {
+    char buf[160];
+    const char* why = nullptr;
+    if (B < 0 || max_pages < 1 || n_ring < 1 || page_size < 1 || (B > 1 && table_stride < max_pages))
+        why = "bad shape";
+    else if (B > kMaxRequests) why = "more than 8192 requests";
+    else if (!workspace || workspace_bytes < kCounterHeaderBytes || reinterpret_cast<uintptr_t>(workspace) % 16)
+        why = "workspace missing, unaligned or too small";
+    if (!why) return WS_OK;
+    snprintf(buf, sizeof(buf), "%s: %s", what, why);
+    return set_error(B > kMaxRequests ? WS_ERR_UNSUPPORTED : why[0] == 'w' ? WS_ERR_WORKSPACE : WS_ERR_INVALID_ARG, buf);
+}
+
+// CTAs of up to kThreads threads, as many as the requests or the CTA's tokens can use.
+int block_threads(int64_t n) { return (int)std::min<int64_t>(kThreads, std::max<int64_t>(128, (n + 31) / 32 * 32)); }
+
+int launch_status() {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace ws
+
+using namespace ws;
+
+extern "C" {
+
+size_t ws_paged_slots_workspace_size(void) { return kCounterHeaderBytes; }
+
+int ws_paged_slots(const int32_t* seq_lens, const int32_t* new_lens, int B, int32_t* page_table, int64_t table_stride,
+                   int max_pages, const int32_t* free_pages, int n_ring, const int32_t* ring, int page_size,
+                   int64_t n_tokens, int64_t* slots, int32_t* positions, int32_t* cu_new, int32_t* seq_lens_out,
+                   int32_t* ring_out, void* workspace, size_t workspace_bytes, void* stream) {
+    if (const int rc = checked("paged_slots", B, max_pages, table_stride, n_ring, page_size, workspace, workspace_bytes))
+        return rc;
+    if (n_tokens < 0 || n_tokens > INT32_MAX / 2) return set_error(WS_ERR_INVALID_ARG, "paged_slots: bad n_tokens");
+    if (!ring || !ring_out || !cu_new || !free_pages || (B > 0 && (!seq_lens || !new_lens || !page_table || !seq_lens_out)) ||
+        (n_tokens > 0 && (!slots || !positions)))
+        return set_error(WS_ERR_INVALID_ARG, "paged_slots: null pointer");
+    const size_t smem = (size_t)std::max(B, 1) * 16;
+    static thread_local int set_for = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (smem > 40 * 1024 && set_for != dev) {
+        if (cudaFuncSetAttribute(paged_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRequests * 16) !=
+            cudaSuccess)
+            return set_error(WS_ERR_CUDA, "paged_slots: shared memory");
+        set_for = dev;
+    }
+    const int64_t ctas = std::max<int64_t>(1, (n_tokens + kTokensPerCta - 1) / kTokensPerCta);
+    const int threads = block_threads(std::max<int64_t>(B, std::min<int64_t>(n_tokens, kTokensPerCta)));
+    paged_slots_kernel<<<(unsigned)ctas, threads, smem, static_cast<cudaStream_t>(stream)>>>(
+        seq_lens, new_lens, B, page_table, table_stride, max_pages, free_pages, n_ring, ring, page_size, n_tokens, slots,
+        positions, cu_new, seq_lens_out, ring_out, static_cast<int*>(workspace));
+    return launch_status();
+}
+
+int ws_paged_release(const int32_t* seq_lens, const uint8_t* done, int B, const int32_t* page_table,
+                     int64_t table_stride, int max_pages, int32_t* free_pages, int n_ring, const int32_t* ring,
+                     int page_size, int32_t* seq_lens_out, int32_t* ring_out, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+    if (const int rc = checked("paged_release", B, max_pages, table_stride, n_ring, page_size, workspace, workspace_bytes))
+        return rc;
+    if (!ring || !ring_out || !free_pages || (B > 0 && (!seq_lens || !done || !page_table || !seq_lens_out)))
+        return set_error(WS_ERR_INVALID_ARG, "paged_release: null pointer");
+    // at most n_ring pages go back, and none of more than B rows
+    const int64_t most = std::min<int64_t>(n_ring, (int64_t)B * max_pages);
+    const int threads = block_threads(std::max<int64_t>(B, most));
+    const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(device_sm_count(), most / (8 * kThreads)));
+    const size_t smem = (size_t)std::max(B, 1) * 4;   // 32 KB at most
+    paged_release_kernel<<<(unsigned)ctas, threads, smem, static_cast<cudaStream_t>(stream)>>>(
+        seq_lens, done, B, page_table, table_stride, max_pages, free_pages, n_ring, ring, page_size, seq_lens_out,
+        ring_out, static_cast<int*>(workspace), device_status_word());
+    return launch_status();
+}
+
+}  // extern "C"

@@ -1,0 +1,328 @@
+// Rotary positions with several axes, and the append of a step's keys and
+// values into a paged cache, in one pass over q, k and v.
+//
+//   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin,   (cos, sin) = cos_sin[position[axis(i)], i]
+//
+// What bounds it: memory.  Each value is read once and written once, and the
+// arithmetic is four operations a pair.  A thread owns a unit of 16 dims of a
+// head -- eight pairs, so both halves of every pair are its own: 16 bytes at
+// dim 8u and 16 at rope_dim/2 + 8u, or 32 contiguous bytes for adjacent pairs
+// and for the dims that pass unrotated -- and walks the heads of its token, so
+// the eight cosines and sines are loaded once for all of them.  The units of a
+// head are padded to a power of two and lie in one warp, which the int8 form
+// needs for the row's maximum.
+//
+// Products and sums are rounded one by one (no fused multiply-add): the result
+// is the elementwise formula's, bit for bit, so an int8 code never depends on
+// which program computed it.
+#include <cstdio>
+
+#include "common.cuh"
+#include "ws_internal.h"
+
+#include <cuda_fp16.h>
+
+namespace ws {
+namespace {
+
+constexpr int kWarps = 4;
+
+struct Heads {          // one of q, k, v: rows of (token, head)
+    const uint16_t* src;
+    int64_t src_tok, src_head;
+    uint8_t* dst;       // q: the output; k, v: the pool
+    int64_t dst_tok;    // q: per token; k, v: per slot of a page  (elements)
+    int64_t dst_head, dst_page;
+    float* scales;      // int8 pool only
+    int64_t s_page, s_tok, s_head;
+    int n, D;
+};
+
+struct RopeAppendArgs {
+    Heads h[3];
+    ws_rope rope;
+    const int64_t* slots;
+    int64_t N, n_slots;
+    int page_size, lanes;   // lanes: units of a head, padded to a power of two
+    int parts;              // warps that share a token's heads
+    int* status;
+};
+
+template <bool F16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+    if (F16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if (F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return pack_bf16(a, b);
+}
+
+// Eight 16-bit values from p; without VEC the address need not be aligned.
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const uint16_t* p) {
+    if (VEC) return *reinterpret_cast<const uint4*>(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
+    if (VEC) {
+        *reinterpret_cast<uint4*>(p) = v;
+        return;
+    }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        p[2 * i] = (uint16_t)w[i];
+        p[2 * i + 1] = (uint16_t)(w[i] >> 16);
+    }
+}
+
+// F16: fp16 inputs (else bf16); I8: the pool holds int8 codes; VEC: q, k, v and q_out are 16-byte aligned throughout.
+template <bool F16, bool I8, bool VEC>
+__global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_constant__ RopeAppendArgs a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int64_t t = item / a.parts;
+    if (t >= a.N) return;
+    const int part = (int)(item - t * a.parts);
+    const int u = lane & (a.lanes - 1), row0 = lane / a.lanes, rows = 32 / a.lanes;
+
+    // this unit's eight turns, shared by all of the token's q and k heads
+    const ws_rope& r = a.rope;
+    const bool turned = 16 * u < r.rope_dim;
+    float c[8], s[8];
+    if (turned) {
+        const int n = r.rope_dim >> 1;
+        auto position = [&](int axis) {
+            const int64_t at = axis * r.axis_stride + t;
+            int64_t p = r.positions_i64 ? static_cast<const int64_t*>(r.positions)[at]
+                                        : static_cast<const int32_t*>(r.positions)[at];
+            if ((uint64_t)p >= (uint64_t)r.max_pos) {
+                if (a.status) atomicMax(a.status, kDevBadIndex);
+                p = p < 0 ? 0 : r.max_pos - 1;
+            }
+            return p;
+        };
+        if (r.n_axes == 1) {
+            const float* row = r.cos_sin + position(0) * r.rope_dim + 8 * u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = __ldg(row + i), s[i] = __ldg(row + n + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int pair = 8 * u + i;
+                const int axis = (a.rope.axis_map[pair >> 4] >> (2 * (pair & 15))) & 3;
+                const float* row = r.cos_sin + position(axis) * r.rope_dim + pair;
+                c[i] = __ldg(row), s[i] = __ldg(row + n);
+            }
+        }
+        if (r.inverse) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = -s[i];
+        }
+    }
+    int64_t page = -1, off = 0;
+    if (a.slots) {
+        const int64_t slot = a.slots[t];
+        if (slot >= 0) {
+            if (slot < a.n_slots) {
+                page = slot / a.page_size;
+                off = slot - page * a.page_size;
+            } else if (a.status) {
+                atomicMax(a.status, kDevBadIndex);
+            }
+        }
+    }
+
+    const int total = a.h[0].n + a.h[1].n + a.h[2].n;
+    for (int base = part * rows; base < total; base += a.parts * rows) {
+        int h = base + row0, kind = 0;
+        if (h >= a.h[0].n) h -= a.h[0].n, kind = 1;
+        if (kind == 1 && h >= a.h[1].n) h -= a.h[1].n, kind = 2;
+        const Heads& x = a.h[kind];
+        const bool on = base + row0 < total && 16 * u < x.D && (kind == 0 || page >= 0);
+        const bool turn = turned && kind < 2;
+        const bool split = turn && !r.adjacent;   // the unit's two halves lie rope_dim/2 apart
+        const int d0 = split ? 8 * u : 16 * u, d1 = split ? (r.rope_dim >> 1) + 8 * u : 16 * u + 8;
+        float lo[8], hi[8];   // dims d0 .. d0+7 and d1 .. d1+7
+        if (on) {
+            const uint16_t* p = x.src + t * x.src_tok + h * x.src_head;
+            const uint4 v0 = load8<VEC>(p + d0), v1 = load8<VEC>(p + d1);
+            const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack2<F16>(w0[i]), g = unpack2<F16>(w1[i]);
+                lo[2 * i] = f.x, lo[2 * i + 1] = f.y, hi[2 * i] = g.x, hi[2 * i + 1] = g.y;
+            }
+            auto pair = [](float& x1, float& x2, float cs, float sn) {
+                const float y1 = __fsub_rn(__fmul_rn(x1, cs), __fmul_rn(x2, sn));
+                x2 = __fadd_rn(__fmul_rn(x2, cs), __fmul_rn(x1, sn));
+                x1 = y1;
+            };
+            if (split) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pair(lo[i], hi[i], c[i], s[i]);
+            } else if (turn) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    pair(lo[2 * i], lo[2 * i + 1], c[i], s[i]);
+                    pair(hi[2 * i], hi[2 * i + 1], c[4 + i], s[4 + i]);
+                }
+            }
+        }
+        if (I8) {
+            float most = 0.f;
+            if (on && kind) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+            }
+            for (int o = a.lanes >> 1; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            if (on && kind) {
+                most = fmaxf(most, 1e-6f);
+                const float inv = __fdiv_rn(127.f, most);
+                auto codes = [&](const float* f) {
+                    uint32_t w[2] = {0, 0};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int q = max(-128, min(127, __float2int_rn(__fmul_rn(f[i], inv))));
+                        w[i >> 2] |= (uint32_t)(q & 0xff) << (8 * (i & 3));
+                    }
+                    return make_uint2(w[0], w[1]);
+                };
+                uint8_t* p = x.dst + page * x.dst_page + off * x.dst_tok + h * x.dst_head;
+                *reinterpret_cast<uint2*>(p + d0) = codes(lo);
+                *reinterpret_cast<uint2*>(p + d1) = codes(hi);
+                if (u == 0) x.scales[page * x.s_page + off * x.s_tok + h * x.s_head] = __fmul_rn(most, 1.0f / 127.0f);
+            }
+            if (kind) continue;
+        }
+        if (on) {
+            uint32_t w0[4], w1[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w0[i] = pack2<F16>(lo[2 * i], lo[2 * i + 1]);
+                w1[i] = pack2<F16>(hi[2 * i], hi[2 * i + 1]);
+            }
+            const int64_t at = kind ? page * x.dst_page + off * x.dst_tok + h * x.dst_head : t * x.dst_tok + h * x.dst_head;
+            uint16_t* p = reinterpret_cast<uint16_t*>(x.dst) + at;
+            store8<VEC>(p + d0, make_uint4(w0[0], w0[1], w0[2], w0[3]));
+            store8<VEC>(p + d1, make_uint4(w1[0], w1[1], w1[2], w1[3]));
+        }
+    }
+}
+
+}  // namespace
+
+int paged_kv_check(const char* what, const ws_paged_kv* kv) {
+    char buf[200];
+    const char* why = nullptr;
+    int code = WS_ERR_INVALID_ARG;
+    const int eb = kv->dtype == WS_DTYPE_I8 ? 1 : 2;
+    const int64_t st[6] = {kv->k_stride_page, kv->k_stride_tok, kv->k_stride_head,
+                           kv->v_stride_page, kv->v_stride_tok, kv->v_stride_head};
+    if (kv->dtype != WS_DTYPE_BF16 && kv->dtype != WS_DTYPE_F16 && kv->dtype != WS_DTYPE_I8)
+        why = "the pool's dtype must be bf16, fp16 or int8";
+    else if (kv->Hkv < 1 || kv->page_size < 1 || kv->n_pages < 0 || kv->Dk < 1 || kv->Dv < 1)
+        why = "bad pool shape";
+    else if (kv->Dk % 16 || kv->Dv % 16 || kv->Dk > 256 || kv->Dv > 256)
+        why = "head dims must be multiples of 16, at most 256", code = WS_ERR_UNSUPPORTED;
+    else if (kv->n_pages > 0 && (!kv->k || !kv->v || (kv->dtype == WS_DTYPE_I8 && (!kv->k_scales || !kv->v_scales))))
+        why = "null pool pointer";
+    else if (reinterpret_cast<uintptr_t>(kv->k) % 16 || reinterpret_cast<uintptr_t>(kv->v) % 16)
+        why = "the pool must be 16-byte aligned";
+    else if (kv->n_pages > INT32_MAX)
+        why = "more than 2^31 - 1 pages", code = WS_ERR_UNSUPPORTED;
+    else
+        for (int i = 0; i < 6; ++i)
+            if (st[i] < 0 || st[i] * eb % 16) why = "pool strides must be whole 16 bytes";
+    if (!why) return WS_OK;
+    snprintf(buf, sizeof(buf), "%s: %s", what, why);
+    return set_error(code, buf);
+}
+
+}  // namespace ws
+
+using namespace ws;
+
+extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stride_tok, int64_t q_stride_head, int H,
+                              int D, void* q_out, int64_t qo_stride_tok, int64_t qo_stride_head, const void* k,
+                              int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+                              int64_t v_stride_head, int dtype, int64_t N, const int64_t* slots, const ws_paged_kv* kv,
+                              void* stream) {
+    if (N < 0 || H < 0 || (!kv && D < 1)) return set_error(WS_ERR_INVALID_ARG, "rope_append: bad shape");
+    if (dtype != WS_DTYPE_BF16 && dtype != WS_DTYPE_F16)
+        return set_error(WS_ERR_INVALID_ARG, "rope_append: q, k, v must be bf16 or fp16");
+    if (kv) {
+        if (const int rc = paged_kv_check("rope_append", kv)) return rc;
+        if (kv->dtype != WS_DTYPE_I8 && kv->dtype != dtype)
+            return set_error(WS_ERR_INVALID_ARG, "rope_append: the pool must hold the inputs' type or int8");
+        if (H > 0 && D != kv->Dk) return set_error(WS_ERR_INVALID_ARG, "rope_append: q and k differ in their head dim");
+    }
+    if (D % 16 || D > 256) return set_error(WS_ERR_UNSUPPORTED, "rope_append: head dims must be multiples of 16, at most 256");
+    if (N == 0 || (H == 0 && !kv)) return WS_OK;
+    if ((H > 0 && (!q || !q_out)) || (kv && (!k || !v || !slots)))
+        return set_error(WS_ERR_INVALID_ARG, "rope_append: null pointer");
+    if (kv && kv->n_pages == 0) return set_error(WS_ERR_INVALID_ARG, "rope_append: empty pool");
+    RopeAppendArgs a;
+    memset(&a, 0, sizeof(a));
+    int Dmax = H > 0 ? D : 16;
+    a.h[0].src = static_cast<const uint16_t*>(q);
+    a.h[0].src_tok = q_stride_tok, a.h[0].src_head = q_stride_head;
+    a.h[0].dst = static_cast<uint8_t*>(q_out);
+    a.h[0].dst_tok = qo_stride_tok, a.h[0].dst_head = qo_stride_head;
+    a.h[0].n = H, a.h[0].D = D;
+    auto aligned = [](const void* p, int64_t s0, int64_t s1) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0;
+    };
+    bool vec = H == 0 || (aligned(q, q_stride_tok, q_stride_head) && aligned(q_out, qo_stride_tok, qo_stride_head));
+    if (kv) {
+        a.h[1] = {static_cast<const uint16_t*>(k), k_stride_tok, k_stride_head, static_cast<uint8_t*>(kv->k),
+                  kv->k_stride_tok, kv->k_stride_head, kv->k_stride_page, kv->k_scales, kv->ks_stride_page,
+                  kv->ks_stride_tok, kv->ks_stride_head, kv->Hkv, kv->Dk};
+        a.h[2] = {static_cast<const uint16_t*>(v), v_stride_tok, v_stride_head, static_cast<uint8_t*>(kv->v),
+                  kv->v_stride_tok, kv->v_stride_head, kv->v_stride_page, kv->v_scales, kv->vs_stride_page,
+                  kv->vs_stride_tok, kv->vs_stride_head, kv->Hkv, kv->Dv};
+        a.slots = slots;
+        a.n_slots = kv->n_pages * kv->page_size;
+        a.page_size = kv->page_size;
+        Dmax = std::max(Dmax, std::max(kv->Dk, kv->Dv));
+        vec = vec && aligned(k, k_stride_tok, k_stride_head) && aligned(v, v_stride_tok, v_stride_head);
+    }
+    if (rope) {
+        const int Dk = kv ? kv->Dk : D;
+        if (rope->rope_dim < 16 || rope->rope_dim % 16 || rope->rope_dim > Dk)
+            return set_error(WS_ERR_INVALID_ARG, "rope_append: rope_dim must be a multiple of 16 within the head dim");
+        if (rope->n_axes < 1 || rope->n_axes > 4 || rope->max_pos < 1 || !rope->positions || !rope->cos_sin)
+            return set_error(WS_ERR_INVALID_ARG, "rope_append: bad rope");
+        for (int i = 0; i < rope->rope_dim / 2; ++i)
+            if ((int)((rope->axis_map[i >> 4] >> (2 * (i & 15))) & 3) >= rope->n_axes)
+                return set_error(WS_ERR_INVALID_ARG, "rope_append: a pair's axis has no positions");
+        a.rope = *rope;
+    }
+    a.N = N;
+    a.status = device_status_word();
+    a.lanes = 1;
+    while (a.lanes * 16 < Dmax) a.lanes *= 2;
+    // One warp walks all heads of a token when there are tokens for every SM; with fewer, its rows are shared out.
+    const int rows = 32 / a.lanes, steps = (H + (kv ? 2 * kv->Hkv : 0) + rows - 1) / rows;
+    const int64_t want = (int64_t)device_sm_count() * 32;
+    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps, (want + N - 1) / N));
+    const int64_t blocks = (N * a.parts + kWarps - 1) / kWarps;
+    if (blocks > INT32_MAX) return set_error(WS_ERR_UNSUPPORTED, "rope_append: too many tokens");
+    const bool f16 = dtype == WS_DTYPE_F16, i8 = kv && kv->dtype == WS_DTYPE_I8;
+    auto fn = f16 ? (i8 ? (vec ? rope_append_kernel<true, true, true> : rope_append_kernel<true, true, false>)
+                        : (vec ? rope_append_kernel<true, false, true> : rope_append_kernel<true, false, false>))
+                  : (i8 ? (vec ? rope_append_kernel<false, true, true> : rope_append_kernel<false, true, false>)
+                        : (vec ? rope_append_kernel<false, false, true> : rope_append_kernel<false, false, false>));
+    fn<<<(unsigned)blocks, 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
+}

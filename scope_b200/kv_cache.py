@@ -186,3 +186,82 @@ class ShardedKVCacheCompressed:
             raise RuntimeError("decode: a PartialExchange is required when world > 1")
         mla_decode(q_proj, q_pe, c, pe, scale, out_dtype=torch.float32, out=exchange.part_o, lse=exchange.part_l)
         return exchange.step(torch.bfloat16)
+
+
+class PagedKVCache:
+    """Paged GQA cache of a model's layers on one GPU: a pool of pages per layer, and one page table, length array and
+    ring of free pages that the layers share.
+
+    Where ``ShardedKVCache`` reserves max_seq tokens for every row, a request here holds only the pages its tokens
+    fill, so ``num_pages * page_size`` bounds the requests' summed length.  ``dtype`` bf16, fp16 or int8 (codes with
+    one fp32 scale per row).  Per step:
+
+        step = cache.begin_step(new_lens, n_tokens)       # pages, slots, positions; lengths advance
+        q = cache.append(li, q, k, v, step, cos_sin)      # each layer: rotate, write keys and values
+        out, lse = cache.decode(li, q_last, scale)        # each layer: one query per request
+        cache.release(done)                               # finished requests' pages go back
+
+    Nothing here waits for the device; ``free_pages()`` and ``refused()`` do.  The table, lengths and ring are updated
+    in place, so the calls can be captured in a CUDA graph.
+    """
+
+    def __init__(self, num_layers, num_pages, page_size, num_kv_heads, head_dim, max_requests, max_seq,
+                 v_head_dim=None, dtype=torch.bfloat16, device=None):
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.device, self.page_size, self.num_pages, self.max_requests = dev, page_size, num_pages, max_requests
+        vd = head_dim if v_head_dim is None else v_head_dim
+        pool = (num_pages, page_size, num_kv_heads)
+        self.k_pages = [torch.empty(*pool, head_dim, dtype=dtype, device=dev) for _ in range(num_layers)]
+        self.v_pages = [torch.empty(*pool, vd, dtype=dtype, device=dev) for _ in range(num_layers)]
+        quantised = dtype == torch.int8
+        self.k_scales = [torch.empty(pool, device=dev) if quantised else None for _ in range(num_layers)]
+        self.v_scales = [torch.empty(pool, device=dev) if quantised else None for _ in range(num_layers)]
+        self.page_table = torch.empty(max_requests, -(-max_seq // page_size), dtype=torch.int32, device=dev)
+        self.seq_lens = torch.empty(max_requests, dtype=torch.int32, device=dev)
+        self._free = torch.empty(num_pages, dtype=torch.int32, device=dev)
+        self._ring = torch.empty(3, dtype=torch.int32, device=dev)
+        self.reset()
+
+    def reset(self):
+        """Every request empty, every page free."""
+        self.page_table.fill_(-1)
+        self.seq_lens.zero_()
+        self._free.copy_(torch.arange(self.num_pages, dtype=torch.int32))
+        self._ring.copy_(torch.tensor([0, self.num_pages, 0], dtype=torch.int32))
+
+    def begin_step(self, new_lens, n_tokens):
+        """new_lens int32 [max_requests] on the device: the tokens each request adds (0: none); n_tokens: the rows of
+        the packed step.  Returns a ``paged.PagedStep``."""
+        from .paged import paged_slots
+        return paged_slots(self.seq_lens, new_lens, self.page_table, self._free, self._ring, self.page_size, n_tokens,
+                           seq_lens_out=self.seq_lens, ring_out=self._ring)
+
+    def append(self, li, q, k, v, step, cos_sin=None, positions=None, **rope):
+        """Write the step's keys and values into layer li's pool and return its rotated queries.  ``positions``
+        (default: ``step.positions``) is given for tokens with several axes; ``rope``: sections, cyclic, pairs,
+        q_out of ``paged.rope_append``."""
+        from .paged import rope_append
+        if cos_sin is not None and positions is None:
+            positions = step.positions
+        return rope_append(q, k, v, positions, cos_sin, step.slots, self.k_pages[li], self.v_pages[li],
+                           k_scales=self.k_scales[li], v_scales=self.v_scales[li], **rope)
+
+    def decode(self, li, q, scale, window=0, out=None, lse=None):
+        """q [max_requests, H, D], one query per request -> (out, lse) over the request's tokens."""
+        from .paged import paged_decode
+        return paged_decode(q, self.k_pages[li], self.v_pages[li], self.page_table, self.seq_lens, scale,
+                            window=window, k_scales=self.k_scales[li], v_scales=self.v_scales[li], out=out, lse=lse)
+
+    def release(self, done):
+        """done bool [max_requests] on the device: these requests' pages go back and their lengths become 0."""
+        from .paged import paged_release
+        paged_release(self.seq_lens, done, self.page_table, self._free, self._ring, self.page_size,
+                      seq_lens_out=self.seq_lens, ring_out=self._ring)
+
+    def free_pages(self) -> int:
+        """Pages free now (waits for the device)."""
+        return int(self._ring[1])
+
+    def refused(self) -> int:
+        """Requests the last begin_step refused (waits for the device)."""
+        return int(self._ring[2])

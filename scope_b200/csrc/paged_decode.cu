@@ -7,12 +7,10 @@
 namespace ws {
 namespace {
 
-constexpr int kMaxWarps = 8;
-
-// Heads a block: 8 (one tensor-core column tile) up to 8 query heads a kv head, 16 up to 16, and 32 beyond -- a
-// block reads its keys and values once, so fewer blocks mean fewer bytes -- but at most 16 at head dims past 128,
-// where the accumulators of 32 heads would not fit the registers.
-int tiles_of(int G, int D) { return G <= 8 ? 1 : G <= 16 || D > 128 ? 2 : 4; }
+// Heads a block: 8 (one tensor-core column tile) up to 8 query heads a kv head and at head dims past 128, else 16.  A
+// block reads its keys and values once, so fewer blocks mean fewer bytes, but more accumulators do not fit the registers.
+int tiles_of(int G, int DB) { return G <= 8 || DB > 128 ? 1 : 2; }
+int bound_of(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 }  // namespace
 }  // namespace ws
@@ -22,9 +20,10 @@ using namespace ws;
 extern "C" {
 
 size_t ws_paged_decode_workspace_size(int B, int Hkv, int G, int Dv) {
-    (void)B, (void)Hkv;
-    return kCounterHeaderBytes +
-           (size_t)device_sm_count() * (2 + kMaxWarps) * paged::piece_floats(tiles_of(G, 0), Dv) * sizeof(float);
+    (void)B, (void)Hkv, (void)G, (void)Dv;
+    // two row parts a CTA; the larger of the two forms that a key dim of up to 256 may choose
+    const size_t piece = std::max(paged::piece_floats(256, 1), paged::piece_floats(128, 2));
+    return kCounterHeaderBytes + (size_t)device_sm_count() * 2 * piece * sizeof(float);
 }
 
 int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q_dtype, int B, int G,
@@ -49,20 +48,26 @@ int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q
         return set_error(WS_ERR_WORKSPACE, "paged_decode: workspace missing, unaligned or too small");
     const bool f16 = q_dtype == WS_DTYPE_F16, i8 = kv->dtype == WS_DTYPE_I8;
     const int64_t eb = i8 ? 1 : 2;
-    const int D = std::max(kv->Dk, kv->Dv), DB = D <= 64 ? 64 : D <= 128 ? 128 : 256, NT = tiles_of(G, D);
+    const int D = std::max(kv->Dk, kv->Dv), DB = bound_of(D), NT = tiles_of(G, DB);
     paged::Args a;
     memset(&a, 0, sizeof(a));
     a.q = static_cast<const uint16_t*>(q);
     a.q_b = q_stride_b, a.q_h = q_stride_h;
     a.k = static_cast<const uint8_t*>(kv->k), a.v = static_cast<const uint8_t*>(kv->v);
-    a.kp = kv->k_stride_page * eb, a.kt = kv->k_stride_tok * eb, a.kh = kv->k_stride_head * eb;
-    a.vp = kv->v_stride_page * eb, a.vt = kv->v_stride_tok * eb, a.vh = kv->v_stride_head * eb;
+    const int64_t strides[6] = {kv->k_stride_page, kv->k_stride_tok, kv->k_stride_head,
+                                kv->v_stride_page, kv->v_stride_tok, kv->v_stride_head};
+    uint32_t* const pieces[6] = {&a.kp, &a.kt, &a.kh, &a.vp, &a.vt, &a.vh};
+    for (int i = 0; i < 6; ++i) {
+        if (strides[i] * eb / 16 > UINT32_MAX) return set_error(WS_ERR_UNSUPPORTED, "paged_decode: a pool stride of 64 GB or more");
+        *pieces[i] = (uint32_t)(strides[i] * eb / 16);
+    }
     a.ks = kv->k_scales, a.vs = kv->v_scales;
     a.ksp = kv->ks_stride_page, a.kst = kv->ks_stride_tok, a.ksh = kv->ks_stride_head;
     a.vsp = kv->vs_stride_page, a.vst = kv->vs_stride_tok, a.vsh = kv->vs_stride_head;
     a.table = page_table, a.table_stride = table_stride;
     a.seq_lens = seq_lens;
     a.cap = std::min<int64_t>((int64_t)max_pages * kv->page_size, INT32_MAX - 64);
+    a.whole = kv->page_size % paged::kTok == 0;
     a.n_pages = (int)kv->n_pages, a.page_size = kv->page_size;
     // t / page_size for t < 2^31 as a multiply and a shift: shift = ceil(log2 P), mul = floor(2^32 (2^shift - P) / P) + 1
     while ((1ull << a.div_shift) < (uint64_t)kv->page_size) ++a.div_shift;

@@ -3,22 +3,24 @@
 //   o = sum_t softmax_t(scale q.k_t) v_t,  lse = log sum_t exp(scale q.k_t),  t in [max(0, L - window), L)
 //
 // What bounds it: HBM.  Every key and value row is read once (the query heads that share it are one tensor-core
-// tile), against G multiply-adds a byte, so the whole design is about keeping enough bytes in flight on every SM
-// for any mix of lengths:
+// tile), against G multiply-adds a byte, so the design keeps enough bytes in flight on every SM for any mix of lengths,
+// at few instructions a byte:
 //
 //   * Rows (request, kv head, block of 8*NT query heads) are cut into subtiles of 16 tokens, laid end to end, and the
 //     line is split evenly over the CTAs (one a SM) and again over each CTA's warps.  Every warp runs alone over its
 //     stretch with its own ring of S stages filled by 16-byte cp.async, so no warp ever waits for another and a short
 //     row costs no barrier.  The lengths are read on the device; the host never needs them.
-//   * A subtile is one stage.  Pages need not divide it: each lane looks up one token's page (an entry fetched one
-//     subtile ahead) and the row addresses travel by shuffle.  Tokens past the length, before the window or on a page
-//     that is none are not read: their shared-memory rows are zero and their scores -inf.
+//   * A subtile is one stage.  With pages of whole subtiles it has one page, and its rows lie at one stride; else each
+//     lane looks up one token's page and the row addresses travel by shuffle.  Entries are fetched a subtile ahead.
+//     Tokens past the length, before the window or on a page that is none are not read: their shared-memory rows are
+//     zero and their scores -inf.
 //   * Rows in shared memory are an odd number of 16-byte pieces apart, so ldmatrix reads are free of bank conflicts for
 //     every head dim without a swizzle.
 //   * S^T[16 tok x 8 heads] = K . Q^T and O^T[Dv x 8] += V^T . P^T by mma.sync with the heads as the narrow dimension:
 //     at G <= 8 query heads a key there is no 128-row tile for tcgen05 to fill, and the tensor pipe is nearly idle.
-//     Running maxima and sums are fp32; P enters the second product as the sum of two 16-bit values (the rounded one
-//     and the rest), which keeps its error below the output's own rounding.
+//   * The softmax's reference moves only when a score passes it by 2^kSlack: then, and not every subtile, the lanes
+//     agree on a new maximum and the accumulators are rescaled.  Sums are fp32; P enters the second product as the sum
+//     of two 16-bit values (the rounded one and the rest), which keeps its error below the output's own rounding.
 //   * int8 rows go from shared memory to bf16 (fp16) fragments by bit operations, exactly; the row's scale multiplies
 //     the score, or the probability.
 //   * A row that ends inside one warp's stretch is written at once.  The others leave a state (o, m, l) per warp,
@@ -31,17 +33,21 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace ws {
 namespace paged {
 
-constexpr int kTok = 16;   // tokens of a subtile
+constexpr int kTok = 16;        // tokens of a subtile
+constexpr int kMinSub = 2;      // subtiles a warp takes before another CTA joins in
+constexpr float kSlack = 6.f;   // log2 of how far a probability may pass its bound before the reference moves
 
 struct Args {
     const uint16_t* q;
     int64_t q_b, q_h;                    // elements
     const uint8_t* k;
     const uint8_t* v;
-    int64_t kp, kt, kh, vp, vt, vh;      // bytes
+    uint32_t kp, kt, kh, vp, vt, vh;     // strides in 16-byte pieces
     const float* ks;
     const float* vs;
     int64_t ksp, kst, ksh, vsp, vst, vsh;
@@ -49,6 +55,7 @@ struct Args {
     int64_t table_stride;
     const int32_t* seq_lens;
     int64_t cap;                         // max_pages * page_size
+    int whole;                           // page_size is a multiple of kTok
     int n_pages, page_size;
     uint32_t div_mul, div_shift;         // t / page_size = (umulhi(t, div_mul) + t) >> div_shift
     int B, Hkv, G, hb, Dk, Dv, window;   // hb: head blocks of a kv head
@@ -56,46 +63,40 @@ struct Args {
     uint16_t* out;
     float* lse;
     int* counters;
-    float* pieces;                       // [cta][2 + warps][piece floats]
+    float* pieces;                       // [cta][2][piece floats]
     int* status;
 };
 
-// The variant for head dims up to DB, 8*NT query heads a block.
-template <bool F16, bool I8, int DB, int NT>
+// The variant for head dims up to DB, 8*NT query heads a block: as many warps, each with two stages, as shared memory and
+// the registers allow (measured at D = 128 in 16 bits, 16 ragged requests to 32768: 8 warps 160 us, 10 warps 152, 12
+// warps 157; three stages put more in flight than the memory takes, and the SMs it serves last fall behind), or more
+// stages where a stage is small.
+template <bool I8, int DB, int NT>
 struct Cfg {
-    static constexpr int kWarps = DB <= 128 ? 8 : 4;
-    static constexpr int kRow = I8 ? ((DB / 16) | 1) * 16 : DB * 2 + 16;
-    static constexpr int kStage = 2 * kTok * kRow + (I8 ? 128 : 0) + 32;
-    static constexpr int kFit = (220 << 10) / (kWarps * kStage);
-    static constexpr int kStages = kFit > 6 ? 6 : kFit;
-    static constexpr int kUnits = NT * (DB / 16);   // 16 x 8 fragments of an accumulator
-    static_assert(kStages >= 3, "ring");
+    static constexpr int kMt = DB / 16;                                   // accumulator fragments of a head tile
+    static constexpr int kWarps = DB == 256 ? (I8 ? 8 : 5) : DB == 128 ? (NT == 1 ? (I8 ? 16 : 10) : (I8 ? 12 : 8))
+                                                                       : NT == 1 ? 16 : 12;
+    static constexpr int kRow = I8 ? ((DB / 16) | 1) * 16 : DB * 2 + 16;  // bytes between rows in shared memory
+    static constexpr int kStage = 2 * kTok * kRow + (I8 ? 128 : 0) + 16;
+    static constexpr int kPiece = NT * (8 * DB + 16);                     // floats: fragments, then m and l of the heads
+    static constexpr int kUnits = NT * kMt;
+    static constexpr int kFit = ((224 << 10) / kWarps - kPiece * 4) / kStage;
+    static constexpr int kStages = kFit > 4 ? 4 : kFit;
+    static constexpr int kRing = kStages * kStage;                        // ends as the place of the last part
+    static constexpr int kWarpSmem = kRing + kPiece * 4;                  // the ring and the first part
+    static_assert(kStages >= 2 && kRing >= kPiece * 4 && kRing % 16 == 0, "ring");
 };
-__host__ __device__ inline int row_bytes(bool i8, int D) { return i8 ? ((D / 16) | 1) * 16 : D * 2 + 16; }
-// shared memory of one warp: its ring, or its last part when that is larger
-__host__ __device__ inline size_t warp_bytes(bool i8, int stages, int NT, int Dk, int Dv) {
-    const size_t ring = stages * ((size_t)kTok * (row_bytes(i8, Dk) + row_bytes(i8, Dv)) + (i8 ? 128 : 0) + 32);
-    const size_t part = ((size_t)NT * 8 * Dv + 16 * NT) * 4;
-    return ring > part ? ring : part;
-}
-// floats of one row part: the accumulator's fragments, then m and l of its 8*NT heads
-__host__ __device__ inline int piece_floats(int NT, int Dv) { return NT * 8 * Dv + 16 * NT; }
+inline int piece_floats(int DB, int NT) { return NT * (8 * DB + 16); }
 
 // What the filler of a stage leaves for its reader.
 struct __align__(16) Meta {
-    uint32_t mask;      // bit i: token i counts; bit 16: the row starts here; bit 17: the row ends here
-    int b, hr, n;       // request, kv head * hb + head block, the row's subtiles
-    long long start;    // the row's first place on the line
-    long long pad;
-};
-static_assert(sizeof(Meta) == 32, "meta");
-
-// A row part, as the CTA's last step sees it.
-struct Part {
-    long long start;   // < 0: none
-    int b, hr, n;
+    uint32_t mask;   // bit i: token i counts; bit 16: the row ends here
+    int b, row, sub; // request, row of it, place in the row
 };
 
+__device__ __forceinline__ void cp_async16_all(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
@@ -133,9 +134,10 @@ __device__ __forceinline__ float2 unpack16(uint32_t v) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
-// Bytes 0 and 2 of r, signed, as a pair of 16-bit floats (exact).  bf16: 0x4300 is 128 and holds 7 bits below it, so
-// (128 + low 7 bits) - (128 or, with the sign bit set, 256) is the value.  fp16: 0x6400 is 1024 and holds all 8 bits:
-// 1024 + (value + 128) - 1152.
+// Bytes 0 and 2 of r, signed, as a pair of 16-bit floats, exactly, times s8_unit.  With the sign bit turned the byte is
+// u = value + 128.  fp16: 0x6400 is 1024 and holds all 8 bits below it, so 1024 + u - 1152 is the value.  bf16 holds 7
+// bits below a leading one, but the pattern 0x00uu is u 2^-133 over the whole byte, where subnormal numbers run on into
+// normal ones: u 2^-133 2^120 - 2^-6 is value 2^-13.
 template <bool F16>
 __device__ __forceinline__ uint32_t s8_pair(uint32_t r) {
     uint32_t d;
@@ -143,13 +145,15 @@ __device__ __forceinline__ uint32_t s8_pair(uint32_t r) {
         const uint32_t x = (r & 0x00ff00ffu) ^ 0x64806480u;
         asm("sub.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x64806480u));
     } else {
-        const uint32_t x = (r & 0x007f007fu) | 0x43004300u, y = (r & 0x00800080u) | 0x43004300u;
-        asm("sub.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+        const uint32_t x = (r & 0x00ff00ffu) ^ 0x00800080u;
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0x7b807b80u), "r"(0xbc80bc80u));
     }
     return d;
 }
+template <bool F16>
+constexpr float s8_unit = F16 ? 1.f : 8192.f;   // the factor that s8_pair leaves out
 
-// Where request b's attended tokens lie: subtiles [first/16, first/16 + n), tokens [lo, L).
+// Where request b's attended tokens lie: subtiles from (lo & ~15), tokens [lo, L), n subtiles.
 struct Span {
     int lo, L, n;
 };
@@ -161,241 +165,243 @@ __device__ __forceinline__ Span span_of(const Args& a, int b) {
     return s;
 }
 
-// The running joint state of row parts for one lane's fragment unit (two heads, two dims each).
-struct Join {
-    float m[2], l[2], o[4];
-    __device__ __forceinline__ void reset() {
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
-        o[0] = o[1] = o[2] = o[3] = 0.f;
+// n / d, in 32 bits where that is enough.
+__device__ __forceinline__ long long quotient(long long n, long long d) {
+    if (((n | d) >> 32) == 0) return (uint32_t)n / (uint32_t)d;
+    return n / d;
+}
+// An even split of a line of N places over n CTAs: the first `more` take one place more than `each`.
+struct Split {
+    long long each, more;
+    __device__ __forceinline__ Split(long long N, int n) {
+        each = n ? quotient(N, n) : 0;
+        more = N - each * n;
     }
-    __device__ __forceinline__ void add(const float2& pm, const float2& pl, const float4& po) {
-        const float nm[2] = {pm.x, pm.y}, nl[2] = {pl.x, pl.y}, no[4] = {po.x, po.y, po.z, po.w};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float top = fmaxf(m[j], nm[j]), ref = top == -INFINITY ? 0.f : top;
-            const float x = ex2(m[j] - ref), y = ex2(nm[j] - ref);
-            l[j] = l[j] * x + nl[j] * y;
-            o[j] = o[j] * x + no[j] * y;
-            o[j + 2] = o[j + 2] * x + no[j + 2] * y;
-            m[j] = top;
-        }
+    __device__ __forceinline__ long long start(int c) const { return c * each + min((long long)c, more); }
+    __device__ __forceinline__ int owner(long long t) const {
+        const long long wide = more * (each + 1);
+        return (int)(t < wide ? quotient(t, each + 1) : more + quotient(t - wide, each));
     }
 };
-
-// Write one fragment unit of a finished row: O^T[dims x heads] of m-tile mt, heads nt*8 + 2t, +1 of the block.
-// 16-bit pools: this lane's o[0..1] are dim 16mt + g, o[2..3] dim 16mt + g + 8; int8 pools: dims 16mt + 2g and + 1.
-template <bool F16, bool I8>
-__device__ __forceinline__ void store_unit(const Args& a, int b, int hr, int heads0, int nt, int mt, const float* o,
-                                           const float* inv) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int kvh = hr / a.hb, left = a.G - heads0;
-    uint16_t* base = a.out + ((int64_t)b * a.Hkv * a.G + (int64_t)kvh * a.G + heads0) * a.Dv + 16 * mt;
-    if (I8) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int h = nt * 8 + 2 * t + j;
-            if (h < left)
-                *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 2 * g) = pack16<F16>(o[j] * inv[j], o[j + 2] * inv[j]);
-        }
-    } else {
-        // transposed: lane (g, t) gets head g, dims 2t, 2t+1 (and +8)
-        const uint32_t lo = movmatrix_t(pack16<F16>(o[0] * inv[0], o[1] * inv[1]));
-        const uint32_t hi = movmatrix_t(pack16<F16>(o[2] * inv[0], o[3] * inv[1]));
-        const int h = nt * 8 + g;
-        if (h < left) {
-            *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 2 * t) = lo;
-            *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 8 + 2 * t) = hi;
-        }
-    }
+// Adds to a counter, after everything that this CTA wrote before its last barrier and before everything it reads next.
+__device__ __forceinline__ int take_ticket(int* counter) {
+    int old;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+    return old;
 }
-// m, l of the lane's two heads -> 1/l; lanes with g == 0 write the lse when asked.
-__device__ __forceinline__ void finish(const Args& a, int b, int hr, int heads0, int nt, const float* m, const float* l,
-                                       bool write_lse, float* inv) {
+
+// Two heads' 1/l; with `write`, lanes of the first row write their lse.
+__device__ __forceinline__ void finish(const Args& a, int64_t head0, int left, int nt, const float* m, const float* l,
+                                       bool write, float* inv) {
     const int lane = threadIdx.x & 31, t = lane & 3;
-    const int kvh = hr / a.hb;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         inv[j] = l[j] > 0.f ? 1.f / l[j] : 0.f;
         const int h = nt * 8 + 2 * t + j;
-        if (write_lse && a.lse && lane < 4 && heads0 + h < a.G)
-            a.lse[(int64_t)b * a.Hkv * a.G + (int64_t)kvh * a.G + heads0 + h] =
-                l[j] > 0.f ? m[j] * kLn2 + logf(l[j]) : -INFINITY;
+        if (write && a.lse && lane < 4 && h < left) a.lse[head0 + h] = l[j] > 0.f ? m[j] * kLn2 + logf(l[j]) : -INFINITY;
     }
 }
 
 template <bool F16, bool I8, int DB, int NT>
-__global__ void __launch_bounds__(32 * Cfg<F16, I8, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
-    using C = Cfg<F16, I8, DB, NT>;
-    constexpr int kWarps = C::kWarps, S = C::kStages, kKs = DB / 16, kMt = DB / 16;
+__global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
+    using C = Cfg<I8, DB, NT>;
+    constexpr int kWarps = C::kWarps, S = C::kStages, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
     constexpr bool kPF16 = F16 && !I8;   // the type of P and V in the second product (bf16's range for scaled P)
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ long long s_scan[kWarps], s_off[kWarps];
-    __shared__ int s_b[kWarps], s_last[2];
-    __shared__ Part s_part[2 * kWarps];
+    // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
+    constexpr float kUp = kPF16 ? 8.f : 0.f;
+    extern __shared__ __align__(16) uint8_t smem[];   // [kWarps][kWarpSmem]
+    __shared__ long long s_scan[kWarps], s_off[kWarps], s_start[2 * kWarps];   // s_start < 0: no part
+    __shared__ int s_b[kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_last[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
     const int R = a.Hkv * a.hb;          // rows of a request
 
-    // ---- the line: total length, this CTA's stretch, and where each warp's begins
-    long long N;
-    const int per = (a.B + kWarps * 32 - 1) / (kWarps * 32), first_b = tid * per;
-    long long mine = 0;
-    for (int b = first_b; b < min(first_b + per, a.B); ++b) mine += span_of(a, b).n;
-    long long upto = mine;
+    // ---- the line: total length, this CTA's stretch, and where this warp's begins
+    long long N, my_off = 0;
+    int my_b = 0;
+    if (lane < 2) s_start[2 * warp + lane] = -1;
+    auto nC_of = [&](long long n) { return (int)min((long long)gridDim.x, (n + kWarps * kMinSub - 1) / (kWarps * kMinSub)); };
+    long long x0 = 0, x1 = 0;
+    auto warp_start = [&](int w) { return x0 + (uint32_t)(x1 - x0) * (uint64_t)w / kWarps; };
+    auto stretch = [&]() {
+        const Split split(N, nC_of(N));
+        if ((int)blockIdx.x < nC_of(N)) x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
+    };
+    if (a.B <= 32) {   // every warp for itself: one request a lane
+        const long long mine = lane < a.B ? (long long)span_of(a, lane).n * R : 0;
+        long long upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
-    }
-    if (lane == 31) s_scan[warp] = upto;
-    if (tid < 2 * kWarps) s_part[tid].start = -1;
-    __syncthreads();
-    long long before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_scan[w];
-        total += s_scan[w];
-    }
-    N = total * R;
-    const int nC = (int)min((long long)gridDim.x, N);
-    const bool works = (int)blockIdx.x < nC;
-    const long long x0 = works ? split_start(blockIdx.x, N, nC) : 0, x1 = works ? split_start(blockIdx.x + 1, N, nC) : 0;
-    auto warp_start = [&](int w) { return x0 + (x1 - x0) * w / kWarps; };
-    {
-        long long off = (before + upto - mine) * R;
-        for (int b = first_b; b < min(first_b + per, a.B); ++b) {
-            const long long len = (long long)span_of(a, b).n * R;
-            if (len > 0 && off < x1 && off + len > x0) {
-                for (int w = 0; w < kWarps; ++w) {
-                    const long long y = warp_start(w);
-                    if (y >= off && y < off + len) s_b[w] = b, s_off[w] = off;
-                }
-            }
-            off += len;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
         }
+        N = __shfl_sync(0xffffffffu, upto, 31);
+        stretch();
+        const long long y = warp_start(warp);
+        const uint32_t here = __ballot_sync(0xffffffffu, y >= upto - mine && y < upto);
+        my_b = here ? __ffs(here) - 1 : 0;
+        my_off = __shfl_sync(0xffffffffu, upto - mine, my_b);
+    } else {
+        const int per = (a.B + kWarps * 32 - 1) / (kWarps * 32), first_b = tid * per;
+        long long mine = 0;
+        for (int b = first_b; b < min(first_b + per, a.B); ++b) mine += span_of(a, b).n;
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane == 31) s_scan[warp] = upto;
+        __syncthreads();
+        long long before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s_scan[w];
+            total += s_scan[w];
+        }
+        N = total * R;
+        stretch();
+        long long off = (before + upto - mine) * R;
+        if (off < x1 && off + mine * R > x0) {
+            for (int b = first_b; b < min(first_b + per, a.B); ++b) {
+                const long long len = (long long)span_of(a, b).n * R;
+                if (off < x1 && off + len > x0) {
+                    for (int w = 0; w < kWarps; ++w) {
+                        const long long y = warp_start(w);
+                        if (y >= off && y < off + len) s_b[w] = b, s_off[w] = off;
+                    }
+                }
+                off += len;
+            }
+        }
+        __syncthreads();
+        my_b = s_b[warp], my_off = s_off[warp];
     }
-    __syncthreads();
     // requests without a token, dealt over the CTAs: zeros, -inf
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-        if (span_of(a, b).n) continue;
-        const int64_t row = (int64_t)b * a.Hkv * a.G;
-        for (int i = tid; i < a.Hkv * a.G * (a.Dv / 8); i += 32 * kWarps)
-            reinterpret_cast<uint4*>(a.out + row * a.Dv)[i] = make_uint4(0, 0, 0, 0);
-        for (int i = tid; a.lse && i < a.Hkv * a.G; i += 32 * kWarps) a.lse[row + i] = -INFINITY;
+    auto write_empty = [&]() {
+        for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+            if (span_of(a, b).n) continue;
+            const int64_t row = (int64_t)b * a.Hkv * a.G;
+            for (int i = tid; i < a.Hkv * a.G * (a.Dv / 8); i += 32 * kWarps)
+                reinterpret_cast<uint4*>(a.out + row * a.Dv)[i] = make_uint4(0, 0, 0, 0);
+            for (int i = tid; a.lse && i < a.Hkv * a.G; i += 32 * kWarps) a.lse[row + i] = -INFINITY;
+        }
+    };
+    if (x0 == x1) {
+        write_empty();
+        return;
     }
-    if (!works) return;
 
     // ---- this warp's stretch
     const long long w0 = warp_start(warp);
     const int count = (int)(warp_start(warp + 1) - w0);
-    const int krow = row_bytes(I8, a.Dk), vrow = row_bytes(I8, a.Dv);
-    const uint32_t stage_sz = kTok * (krow + vrow) + (I8 ? 128 : 0) + 32;
-    const size_t warp_sz = warp_bytes(I8, S, NT, a.Dk, a.Dv);
-    uint8_t* const ring = smem + warp * warp_sz;
+    uint8_t* const ring = smem + warp * C::kWarpSmem;
     const uint32_t ring_u = smem_u32(ring);
-    const uint32_t v_at = kTok * krow, s_at = v_at + kTok * vrow, m_at = s_at + (I8 ? 128 : 0);
-    const int pf = piece_floats(NT, a.Dv);
-    float* const cta_pieces = a.pieces + (int64_t)blockIdx.x * (2 + kWarps) * pf;
+    // a stage: key rows, value rows, int8 scales (16 of keys, 16 of values), meta
+    constexpr int kRow = C::kRow, kV = kTok * kRow, kS = 2 * kV, kM = kS + (I8 ? 128 : 0);
+    float* const cta_pieces = a.pieces + (int64_t)blockIdx.x * 2 * kPiece;
 
-    // filler state: the row being filled and the next subtile's page entry
-    int fb = 0, fhr = 0, fsub = 0;
-    long long fstart = 0;
+    // filler: the row being filled, and the next subtile's page entry (of this lane's token where pages are not whole
+    // subtiles)
     Span fs = {0, 0, 0};
-    int f_entry = 0, f_off = 0;   // this lane's token: page entry and place in the page
-    bool f_ok = false;
-    int left = count;
-    const int tok = lane & 15;
-
-    auto look_up = [&]() {   // the page of this lane's token of subtile fsub
-        const uint32_t t = (uint32_t)(fs.lo & ~(kTok - 1)) + (uint32_t)fsub * kTok + tok;
-        f_ok = (int)t >= fs.lo && (int)t < fs.L;
-        const uint32_t page = (__umulhi(t, a.div_mul) + t) >> a.div_shift;
-        f_off = (int)(t - page * (uint32_t)a.page_size);
-        f_entry = f_ok ? __ldg(a.table + (int64_t)fb * a.table_stride + page) : 0;
-    };
-    if (count > 0) {
-        fb = s_b[warp];
-        fs = span_of(a, fb);
-        const long long rel = w0 - s_off[warp];
-        fhr = (int)(rel / fs.n);
-        fsub = (int)(rel - (long long)fhr * fs.n);
-        fstart = w0 - fsub;
-        look_up();
-    }
-    const int l8 = lane & 7, r4 = lane >> 3;
+    int f_b = 0, f_row = 0, f_sub = 0, f_entry = -1, f_left = count;
+    uint32_t f_off = 0;
+    const int l8 = lane & 7, r4 = lane >> 3;   // copies: eight lanes a row, four rows at a time
     const int kchunks = I8 ? a.Dk >> 4 : a.Dk >> 3, vchunks = I8 ? a.Dv >> 4 : a.Dv >> 3;
-    constexpr int kCols = (I8 ? DB / 16 : DB / 8) / 8 > 0 ? (I8 ? DB / 16 : DB / 8) / 8 : 1;
+    constexpr int kCols = (I8 ? DB / 16 : DB / 8) >= 8 ? (I8 ? DB / 16 : DB / 8) / 8 : 1;
+    const uint64_t k_lane = (uint64_t)r4 * a.kt + l8, v_lane = (uint64_t)r4 * a.vt + l8;
 
+    auto look_up = [&]() {
+        uint32_t t = (uint32_t)(fs.lo & ~(kTok - 1)) + (uint32_t)f_sub * kTok;
+        if (!a.whole) t = min(max(t + (lane & 15), (uint32_t)fs.lo), (uint32_t)fs.L - 1);
+        const uint32_t page = (__umulhi(t, a.div_mul) + t) >> a.div_shift;
+        f_off = t - page * (uint32_t)a.page_size;
+        f_entry = __ldg(a.table + (int64_t)f_b * a.table_stride + page);
+    };
     auto fill = [&](int slot) {
-        if (left > 0) {
-            --left;
-            const uint32_t st = ring_u + slot * stage_sz;
-            bool ok = f_ok;
-            if (ok && (uint32_t)f_entry >= (uint32_t)a.n_pages) {
-                ok = false;
+        if (f_left > 0) {
+            const uint32_t st = ring_u + slot * C::kStage;
+            const int t0 = (fs.lo & ~(kTok - 1)) + f_sub * kTok;
+            uint32_t mask = (0xffffu >> max(t0 + kTok - fs.L, 0)) & (0xffffu << max(fs.lo - t0, 0));
+            const bool page_ok = (uint32_t)f_entry < (uint32_t)a.n_pages;
+            const uint32_t pages_ok = __ballot_sync(0xffffffffu, page_ok);
+            if (pages_ok != 0xffffffffu) {
                 if (a.status) atomicMax(a.status, kDevBadIndex);
+                mask &= a.whole ? 0u : pages_ok;
             }
-            const int kvh = fhr / a.hb;
-            const long long page = ok ? f_entry : 0, off = ok ? f_off : 0;
-            const long long ka = page * a.kp + off * a.kt + kvh * a.kh, va = page * a.vp + off * a.vt + kvh * a.vh;
-            const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+            const uint32_t page = page_ok ? f_entry : 0, kvh = a.hb == 1 ? f_row : f_row / a.hb;
+            uint64_t ka = (uint64_t)page * a.kp + (uint64_t)f_off * a.kt + (uint64_t)kvh * a.kh;
+            uint64_t va = (uint64_t)page * a.vp + (uint64_t)f_off * a.vt + (uint64_t)kvh * a.vh;
             if (I8) {
+                const int64_t off = a.whole ? f_off + (lane & 15) : f_off;
                 const float* src = lane < 16 ? a.ks + (page * a.ksp + off * a.kst + kvh * a.ksh)
                                              : a.vs + (page * a.vsp + off * a.vst + kvh * a.vsh);
-                cp_async4(st + s_at + lane * 4, src, ok);
+                cp_async4(st + kS + lane * 4, src, (mask >> (lane & 15)) & 1);
             }
             if (lane == 0) {
                 Meta m;
-                m.mask = mask | (fsub == 0 ? 1u << 16 : 0u) | (fsub == fs.n - 1 ? 1u << 17 : 0u);
-                m.b = fb, m.hr = fhr, m.n = fs.n, m.start = fstart, m.pad = 0;
-                *reinterpret_cast<Meta*>(ring + slot * stage_sz + m_at) = m;
+                m.mask = mask | (f_sub == fs.n - 1 ? 1u << 16 : 0u);
+                m.b = f_b, m.row = f_row, m.sub = f_sub;
+                *reinterpret_cast<Meta*>(ring + slot * C::kStage + kM) = m;
             }
-            // 8 lanes a row, 4 rows at a time
+            const uint32_t kd = st + r4 * kRow + l8 * 16, vd = kd + kV;
+            if (a.whole && mask == 0xffffu) {
+                const uint8_t *kp = a.k + ((ka + k_lane) << 4), *vp = a.v + ((va + v_lane) << 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 4 * i + r4;
-                const long long kr = __shfl_sync(0xffffffffu, ka, row), vr = __shfl_sync(0xffffffffu, va, row);
-                const bool on = (mask >> row) & 1;
-                const uint8_t* kp = a.k + kr + l8 * 16;
-                const uint8_t* vp = a.v + vr + l8 * 16;
-                const uint32_t kd = st + row * krow + l8 * 16, vd = st + v_at + row * vrow + l8 * 16;
+                for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int j = 0; j < kCols; ++j) {
-                    if (l8 + 8 * j < kchunks) cp_async16(kd + j * 128, kp + j * 128, on);
-                    if (l8 + 8 * j < vchunks) cp_async16(vd + j * 128, vp + j * 128, on);
+                    for (int j = 0; j < kCols; ++j) {
+                        if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * kRow + j * 128, kp + j * 128);
+                        if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * kRow + j * 128, vp + j * 128);
+                    }
+                    kp += (uint64_t)a.kt << 6, vp += (uint64_t)a.vt << 6;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 4 * i + r4;
+                    const bool on = (mask >> row) & 1;
+                    uint64_t kr = ka + (on ? row * (uint64_t)a.kt : 0), vr = va + (on ? row * (uint64_t)a.vt : 0);
+                    if (!a.whole) kr = __shfl_sync(0xffffffffu, ka, row), vr = __shfl_sync(0xffffffffu, va, row);
+                    const uint8_t *kp = a.k + ((kr + l8) << 4), *vp = a.v + ((vr + l8) << 4);
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) {
+                        if (l8 + 8 * j < kchunks) cp_async16(kd + 4 * i * kRow + j * 128, kp + j * 128, on);
+                        if (l8 + 8 * j < vchunks) cp_async16(vd + 4 * i * kRow + j * 128, vp + j * 128, on);
+                    }
                 }
             }
-            // the next subtile
-            if (++fsub == fs.n) {
-                fsub = 0;
-                fstart += fs.n;
-                if (++fhr == R && left > 0) {
-                    fhr = 0;
-                    do fs = span_of(a, ++fb);
-                    while (fs.n == 0);
+            // on to the next subtile
+            if (--f_left > 0) {
+                if (++f_sub == fs.n) {
+                    f_sub = 0;
+                    if (++f_row == R) {
+                        f_row = 0;
+                        do fs = span_of(a, ++f_b);
+                        while (fs.n == 0);
+                    }
                 }
+                look_up();
             }
-            if (left > 0) look_up();
         }
         cp_async_commit();
     };
 
-    // ---- reader state
-    float m_run[NT][2], l_run[NT][2], acc[NT][kMt][4];
-    uint32_t bq[NT][kKs][2];
-    bool began = false;
+    float m_ref[NT][2], l_run[NT][2], acc[NT][kMt][4];
+    uint32_t bq[NT][DB / 16][2];
+    bool began = false;                // the row's first subtile was this warp's
+
     const int nks = a.Dk >> 4, nmt = a.Dv >> 4;
 
-    auto load_q = [&](int b, int hr) {
-        const int kvh = hr / a.hb, h0 = (hr - kvh * a.hb) * 8 * NT;
+    auto load_q = [&](int b, int row) {
+        const int kvh = row / a.hb, h0 = (row - kvh * a.hb) * 8 * NT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int h = h0 + nt * 8 + g;
             const uint16_t* q = a.q + b * a.q_b + ((int64_t)kvh * a.G + h) * a.q_h;
 #pragma unroll
-            for (int ks = 0; ks < kKs; ++ks) {
+            for (int ks = 0; ks < DB / 16; ++ks) {
                 uint32_t x = 0, y = 0;
                 if (ks < nks && h < a.G) {
                     if (I8) {   // the order in which s8_pair gives the dims: (0, 2), (1, 3) of each four
@@ -409,103 +415,160 @@ __global__ void __launch_bounds__(32 * Cfg<F16, I8, DB, NT>::kWarps, 1) decode_k
                 }
                 bq[nt][ks][0] = x, bq[nt][ks][1] = y;
             }
-            m_run[nt][0] = m_run[nt][1] = -INFINITY;
+            m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
             l_run[nt][0] = l_run[nt][1] = 0.f;
 #pragma unroll
             for (int mt = 0; mt < kMt; ++mt) acc[nt][mt][0] = acc[nt][mt][1] = acc[nt][mt][2] = acc[nt][mt][3] = 0.f;
         }
     };
-
-    // this lane's part of the row into piece memory (shared or global)
     auto file_piece = [&](float* p) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int mt = 0; mt < kMt; ++mt)
-                if (mt < nmt)
-                    *reinterpret_cast<float4*>(p + ((nt * nmt + mt) * 32 + lane) * 4) =
-                        make_float4(acc[nt][mt][0], acc[nt][mt][1], acc[nt][mt][2], acc[nt][mt][3]);
+                *reinterpret_cast<float4*>(p + ((nt * kMt + mt) * 32 + lane) * 4) =
+                    make_float4(acc[nt][mt][0], acc[nt][mt][1], acc[nt][mt][2], acc[nt][mt][3]);
             if (lane < 4) {
-                float* ml = p + NT * 8 * a.Dv + nt * 16;
-                *reinterpret_cast<float2*>(ml + 2 * t4) = make_float2(m_run[nt][0], m_run[nt][1]);
+                float* ml = p + NT * 8 * DB + nt * 16;
+                *reinterpret_cast<float2*>(ml + 2 * t4) = make_float2(m_ref[nt][0], m_ref[nt][1]);
                 *reinterpret_cast<float2*>(ml + 8 + 2 * t4) = make_float2(l_run[nt][0], l_run[nt][1]);
             }
         }
     };
-
+    // One fragment of a finished row: O^T[16 dims x 8 heads], dims from 16mt.
+    auto store_unit = [&](int64_t head0, int left, int nt, int mt, const float* o, const float* inv) {
+        uint16_t* base = a.out + head0 * a.Dv + 16 * mt;
+        if (I8) {   // dims 2g and 2g + 1 of heads 2t, 2t + 1
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) fill(s);
-    int slot = 0;
-    for (int it = 0; it < count; ++it) {
-        cp_async_wait<S - 2>();
-        __syncwarp();
-        fill(slot == 0 ? S - 1 : slot - 1);
-        const uint32_t st = ring_u + slot * stage_sz;
-        const Meta* meta = reinterpret_cast<const Meta*>(ring + slot * stage_sz + m_at);
-        const uint32_t mask = meta->mask;
-        if (it == 0 || (mask & (1u << 16))) {
-            load_q(meta->b, meta->hr);
-            began = mask & (1u << 16);
+            for (int j = 0; j < 2; ++j) {
+                const int h = nt * 8 + 2 * t4 + j;
+                if (h < left)
+                    *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 2 * g) = pack16<F16>(o[j] * inv[j], o[j + 2] * inv[j]);
+            }
+        } else {    // dims g and g + 8; transposed, lane (g, t) gets head g, dims 2t, 2t + 1 and + 8
+            const uint32_t lo = movmatrix_t(pack16<F16>(o[0] * inv[0], o[1] * inv[1]));
+            const uint32_t hi = movmatrix_t(pack16<F16>(o[2] * inv[0], o[3] * inv[1]));
+            const int h = nt * 8 + g;
+            if (h < left) {
+                *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 2 * t4) = lo;
+                *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 8 + 2 * t4) = hi;
+            }
         }
-        // scores
-        float c[NT][4];
+    };
+
+    if (count > 0) {
+        f_b = my_b;
+        fs = span_of(a, f_b);
+        const long long rel = w0 - my_off;
+        f_row = (int)quotient(rel, fs.n);
+        f_sub = (int)(rel - (long long)f_row * fs.n);
+        look_up();
+        load_q(f_b, f_row);
+    }
+    int slot = 0;   // the stage that iteration `it` reads; the one before it is filled
+#pragma unroll 1
+    for (int it = 1 - S; it < count; ++it) {
+        if (it >= 0) {
+            cp_async_wait<S - 2>();
+            __syncwarp();
+        }
+        const int to = it < 0 ? it + S - 1 : slot == 0 ? S - 1 : slot - 1;
+        fill(to);
+        if (it < 0) {
+            if (it == 1 - S) write_empty();
+            continue;
+        }
+        const uint32_t st = ring_u + slot * C::kStage;
+        const Meta meta = *reinterpret_cast<const Meta*>(ring + slot * C::kStage + kM);
+        if (meta.sub == 0) {
+            if (it) load_q(meta.b, meta.row);
+            began = true;
+        }
+        // scores, in two chains
+        float c[NT][4], e[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
-        const uint32_t k_ld = st + (lane & 15) * krow + (lane >> 4) * 16;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[nt][i] = e[nt][i] = 0.f;
+        const uint32_t k_ld = st + (lane & 15) * kRow + (lane >> 4) * 16;
         if (I8) {
 #pragma unroll
-            for (int ks = 0; ks < kKs; ks += 2) {
-                if (ks < nks) {
-                    uint32_t r[4];
-                    ldsm_x4(k_ld + ks * 16, r[0], r[1], r[2], r[3]);
+            for (int ks = 0; ks < DB / 16; ks += 2) {
+                if (ks >= nks) break;
+                uint32_t r[4];
+                ldsm_x4(k_ld + ks * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        if (u == 0 || ks + 1 < nks) {
-                            const uint32_t a0 = s8_pair<F16>(r[2 * u]), a1 = s8_pair<F16>(r[2 * u + 1]);
-                            const uint32_t a2 = s8_pair<F16>(r[2 * u] >> 8), a3 = s8_pair<F16>(r[2 * u + 1] >> 8);
+                for (int u = 0; u < 2; ++u) {   // past an odd nks the queries are zero and what was read is finite
+                    const uint32_t a0 = s8_pair<F16>(r[2 * u]), a1 = s8_pair<F16>(r[2 * u + 1]);
+                    const uint32_t a2 = s8_pair<F16>(r[2 * u] >> 8), a3 = s8_pair<F16>(r[2 * u + 1] >> 8);
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                mma16<F16>(c[nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
-                        }
-                    }
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma16<F16>(u ? e[nt] : c[nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
                 }
             }
         } else {
 #pragma unroll
-            for (int ks = 0; ks < kKs; ++ks) {
-                if (ks < nks) {
-                    uint32_t a0, a1, a2, a3;
-                    ldsm_x4(k_ld + ks * 32, a0, a1, a2, a3);
+            for (int ks = 0; ks < DB / 16; ++ks) {
+                if (ks >= nks) break;
+                uint32_t a0, a1, a2, a3;
+                ldsm_x4(k_ld + ks * 32, a0, a1, a2, a3);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16<F16>(c[nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
+                for (int nt = 0; nt < NT; ++nt) mma16<F16>(ks & 1 ? e[nt] : c[nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
+            }
+        }
+        float f0 = a.scale_log2, f1 = f0, v0 = 1.f, v1 = 1.f;
+        if (I8) {
+            const float* sc = reinterpret_cast<const float*>(ring + slot * C::kStage + kS);
+            f0 *= sc[g] * s8_unit<F16>, f1 *= sc[g + 8] * s8_unit<F16>;
+            v0 = sc[16 + g] * s8_unit<kPF16>, v1 = sc[24 + g] * s8_unit<kPF16>;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[nt][i] = (c[nt][i] + e[nt][i]) * (i < 2 ? f0 : f1);
+        if ((meta.mask & 0xffffu) != 0xffffu) {   // tokens that do not count (their values and scales are zero)
+            const bool on0 = (meta.mask >> g) & 1, on1 = (meta.mask >> (g + 8)) & 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[nt][i] = (i < 2 ? on0 : on1) ? c[nt][i] : -INFINITY;
+        }
+        bool past = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) past |= fmaxf(c[nt][j], c[nt][j + 2]) > m_ref[nt][j] + (kUp + kSlack);
+        if (__any_sync(0xffffffffu, past)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float keep[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float top = fmaxf(c[nt][j], c[nt][j + 2]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    top = fmaxf(top - kUp, m_ref[nt][j]);
+                    keep[j] = top == -INFINITY ? 1.f : ex2(m_ref[nt][j] - top);
+                    m_ref[nt][j] = top;
+                    l_run[nt][j] *= keep[j];
+                }
+#pragma unroll
+                for (int mt = 0; mt < kMt; ++mt) {
+                    acc[nt][mt][0] *= keep[0], acc[nt][mt][1] *= keep[1];
+                    acc[nt][mt][2] *= keep[0], acc[nt][mt][3] *= keep[1];
                 }
             }
         }
-        float f0 = a.scale_log2, f1 = a.scale_log2, v0 = 1.f, v1 = 1.f;
-        if (I8) {
-            const float* sc = reinterpret_cast<const float*>(ring + slot * stage_sz + s_at);
-            f0 *= sc[g], f1 *= sc[g + 8], v0 = sc[16 + g], v1 = sc[24 + g];
-        }
-        const bool on0 = (mask >> g) & 1, on1 = (mask >> (g + 8)) & 1;
         uint32_t ph[NT][2], pl[NT][2];
-        bool moved = false;
-        float keep[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                c[nt][j] = on0 ? c[nt][j] * f0 : -INFINITY;
-                c[nt][j + 2] = on1 ? c[nt][j + 2] * f1 : -INFINITY;
-                float top = fmaxf(c[nt][j], c[nt][j + 2]);
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                const float m2 = fmaxf(m_run[nt][j], top), ref = m2 == -INFINITY ? 0.f : m2;
-                moved |= m2 > m_run[nt][j];
-                keep[nt][j] = ex2(m_run[nt][j] - ref);
-                m_run[nt][j] = m2;
+                // while every score so far is -inf the reference is too: any finite one in its place gives 0
+                const float ref = fmaxf(m_ref[nt][j], -3.0e38f);
                 const float p0 = ex2(c[nt][j] - ref), p1 = ex2(c[nt][j + 2] - ref);
-                l_run[nt][j] = l_run[nt][j] * keep[nt][j] + (p0 + p1);
+                l_run[nt][j] += p0 + p1;
                 c[nt][j] = I8 ? p0 * v0 : p0;
                 c[nt][j + 2] = I8 ? p1 * v1 : p1;
             }
@@ -515,55 +578,42 @@ __global__ void __launch_bounds__(32 * Cfg<F16, I8, DB, NT>::kWarps, 1) decode_k
             pl[nt][0] = movmatrix_t(pack16<kPF16>(c[nt][0] - e0.x, c[nt][1] - e0.y));
             pl[nt][1] = movmatrix_t(pack16<kPF16>(c[nt][2] - e1.x, c[nt][3] - e1.y));
         }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int mt = 0; mt < kMt; ++mt) {
-                    acc[nt][mt][0] *= keep[nt][0], acc[nt][mt][1] *= keep[nt][1];
-                    acc[nt][mt][2] *= keep[nt][0], acc[nt][mt][3] *= keep[nt][1];
-                }
-        }
         // values
         if (I8) {
-            const uint32_t v_ld = st + v_at + (lane & 15) * vrow + (lane >> 4) * 16;
+            const uint32_t v_ld = st + kV + (lane & 15) * kRow + (lane >> 4) * 16;
 #pragma unroll
             for (int mt = 0; mt < kMt; mt += 2) {
-                if (mt < nmt) {
-                    uint32_t r[4];
-                    ldsm_x4_t(v_ld + mt * 16, r[0], r[1], r[2], r[3]);
+                if (mt >= nmt) break;
+                uint32_t r[4];
+                ldsm_x4_t(v_ld + mt * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        if (u == 0 || mt + 1 < nmt) {
-                            const uint32_t a0 = s8_pair<kPF16>(r[2 * u]), a1 = s8_pair<kPF16>(r[2 * u] >> 8);
-                            const uint32_t a2 = s8_pair<kPF16>(r[2 * u + 1]), a3 = s8_pair<kPF16>(r[2 * u + 1] >> 8);
+                for (int u = 0; u < 2; ++u) {   // past an odd nmt: accumulators that nobody reads
+                    const uint32_t a0 = s8_pair<kPF16>(r[2 * u]), a1 = s8_pair<kPF16>(r[2 * u] >> 8);
+                    const uint32_t a2 = s8_pair<kPF16>(r[2 * u + 1]), a3 = s8_pair<kPF16>(r[2 * u + 1] >> 8);
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                                mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
-                            }
-                        }
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                        mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
                     }
                 }
             }
         } else {
-            const uint32_t v_ld = st + v_at + ((lane & 7) + ((lane >> 4) << 3)) * vrow + ((lane >> 3) & 1) * 16;
+            const uint32_t v_ld = st + kV + ((lane & 7) + ((lane >> 4) << 3)) * kRow + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int mt = 0; mt < kMt; ++mt) {
-                if (mt < nmt) {
-                    uint32_t a0, a1, a2, a3;
-                    ldsm_x4_t(v_ld + mt * 32, a0, a1, a2, a3);
+                if (mt >= nmt) break;
+                uint32_t a0, a1, a2, a3;
+                ldsm_x4_t(v_ld + mt * 32, a0, a1, a2, a3);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                        mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
-                    }
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                    mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
                 }
             }
         }
         // the row, or this warp's stretch, ends
-        const bool ends = mask & (1u << 17), last = it == count - 1;
-        if (ends || last) {
+        const bool ends = meta.mask >> 16, more = it + 1 < count;
+        if (ends || !more) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -572,26 +622,26 @@ __global__ void __launch_bounds__(32 * Cfg<F16, I8, DB, NT>::kWarps, 1) decode_k
                     l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], 8);
                     l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], 16);
                 }
-            const Meta mm = *meta;
-            const int kvh = mm.hr / a.hb, h0 = (mm.hr - kvh * a.hb) * 8 * NT;
             if (ends && began) {
+                const int kvh = meta.row / a.hb, h0 = (meta.row - kvh * a.hb) * 8 * NT, left = a.G - h0;
+                const int64_t head0 = ((int64_t)meta.b * a.Hkv + kvh) * a.G + h0;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float inv[2];
-                    finish(a, mm.b, mm.hr, h0, nt, m_run[nt], l_run[nt], true, inv);
+                    finish(a, head0, left, nt, m_ref[nt], l_run[nt], true, inv);
 #pragma unroll
                     for (int mt = 0; mt < kMt; ++mt)
-                        if (mt < nmt) store_unit<F16, I8>(a, mm.b, mm.hr, h0, nt, mt, acc[nt][mt], inv);
+                        if (mt < nmt) store_unit(head0, left, nt, mt, acc[nt][mt], inv);
                 }
             } else {
-                // the stretch's last part stays in this warp's own ring (nothing is in flight into it any more), an
-                // earlier one goes through L2
+                // the stretch's last part takes the ring's place (nothing is in flight into it any more)
+                const int part = 2 * warp + (more ? 0 : 1);
                 __syncwarp();
-                file_piece(last ? reinterpret_cast<float*>(ring) : cta_pieces + (2 + warp) * pf);
+                file_piece(reinterpret_cast<float*>(more ? ring + C::kRing : ring));
                 if (lane == 0) {
-                    Part p;
-                    p.start = mm.start, p.b = mm.b, p.hr = mm.hr, p.n = mm.n;
-                    s_part[2 * warp + (last ? 1 : 0)] = p;
+                    s_start[part] = w0 + it - meta.sub;
+                    s_row[part] = meta.b * R + meta.row;
+                    s_n[part] = span_of(a, meta.b).n;
                 }
             }
         }
@@ -599,102 +649,149 @@ __global__ void __launch_bounds__(32 * Cfg<F16, I8, DB, NT>::kWarps, 1) decode_k
     }
     __syncthreads();
 
-    // ---- join the CTA's parts row by row; a row that leaves the CTA is filed for the last of its CTAs
-    const int units = NT * nmt;
-    auto part_at = [&](int i) -> const float* {
-        return (i & 1) ? reinterpret_cast<const float*>(smem + (i >> 1) * warp_sz)
-                       : cta_pieces + (2 + (i >> 1)) * pf;
-    };
-    Part cross[2];
-    cross[0].start = cross[1].start = -1;
-    int i0 = 0;
-    while (i0 < 2 * kWarps) {
-        const Part p = s_part[i0];
-        if (p.start < 0) {
-            ++i0;
-            continue;
-        }
-        int i1 = i0 + 1;
-        while (i1 < 2 * kWarps && (s_part[i1].start < 0 || s_part[i1].start == p.start)) ++i1;
-        const bool inside = p.start >= x0 && p.start + p.n <= x1;
-        const int which = p.start >= x0 ? 1 : 0;
-        const int kvh = p.hr / a.hb, h0 = (p.hr - kvh * a.hb) * 8 * NT;
-        float* const to = cta_pieces + which * pf;
-        for (int u = warp; u < units; u += kWarps) {
-            const int nt = u / nmt, mt = u - nt * nmt;
-            Join z;
-            z.reset();
-            for (int i = i0; i < i1; ++i) {
-                if (s_part[i].start < 0) continue;
-                const float* src = part_at(i);
-                const float* ml = src + NT * 8 * a.Dv + nt * 16;
-                z.add(*reinterpret_cast<const float2*>(ml + 2 * t4), *reinterpret_cast<const float2*>(ml + 8 + 2 * t4),
-                      *reinterpret_cast<const float4*>(src + (u * 32 + lane) * 4));
-            }
-            if (inside) {
-                float inv[2];
-                finish(a, p.b, p.hr, h0, nt, z.m, z.l, mt == 0, inv);
-                store_unit<F16, I8>(a, p.b, p.hr, h0, nt, mt, z.o, inv);
-            } else {
-                *reinterpret_cast<float4*>(to + (u * 32 + lane) * 4) = make_float4(z.o[0], z.o[1], z.o[2], z.o[3]);
-                if (mt == 0 && lane < 4) {
-                    float* ml = to + NT * 8 * a.Dv + nt * 16;
-                    *reinterpret_cast<float2*>(ml + 2 * t4) = make_float2(z.m[0], z.m[1]);
-                    *reinterpret_cast<float2*>(ml + 8 + 2 * t4) = make_float2(z.l[0], z.l[1]);
+    // ---- join parts: unit (16 x 8 fragment) u of the parts at `at(0)`, `at(1)`, ..., to a piece, or (null) to the output
+    auto join = [&](auto load, auto at, int n, int u, int row, float* to) {
+        const int nt = u / kMt, mt = u - nt * kMt, ml = NT * 8 * DB + nt * 16 + 2 * t4;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < n; i += 4) {
+            float4 z[4];
+            float2 x[4], y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i + k < n) {
+                    const float* src = at(i + k);
+                    load(x[k], src + ml), load(y[k], src + ml + 8), load(z[k], src + (u * 32 + lane) * 4);
+                } else {
+                    x[k] = make_float2(-INFINITY, -INFINITY), y[k] = make_float2(0.f, 0.f), z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             }
+            const float t0 = fmaxf(fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)), m[0]);
+            const float t1 = fmaxf(fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y)), m[1]);
+            const float r0 = fmaxf(t0, -3.0e38f), r1 = fmaxf(t1, -3.0e38f), k0 = ex2(m[0] - r0), k1 = ex2(m[1] - r1);
+            l[0] *= k0, o[0] *= k0, o[2] *= k0, l[1] *= k1, o[1] *= k1, o[3] *= k1, m[0] = t0, m[1] = t1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float s0 = ex2(x[k].x - r0), s1 = ex2(x[k].y - r1);
+                l[0] += y[k].x * s0, l[1] += y[k].y * s1;
+                o[0] += z[k].x * s0, o[1] += z[k].y * s1, o[2] += z[k].z * s0, o[3] += z[k].w * s1;
+            }
         }
-        if (!inside) cross[which] = p;
-        i0 = i1;
+        if (to) {
+            *reinterpret_cast<float4*>(to + (u * 32 + lane) * 4) = make_float4(o[0], o[1], o[2], o[3]);
+            if (mt == 0 && lane < 4) {
+                *reinterpret_cast<float2*>(to + ml) = make_float2(m[0], m[1]);
+                *reinterpret_cast<float2*>(to + ml + 8) = make_float2(l[0], l[1]);
+            }
+        } else {
+            const int b = row / R, kvh = (row - b * R) / a.hb, h0 = (row - b * R - kvh * a.hb) * 8 * NT, left = a.G - h0;
+            const int64_t head0 = ((int64_t)b * a.Hkv + kvh) * a.G + h0;
+            float inv[2];
+            finish(a, head0, left, nt, m, l, mt == 0, inv);
+            if (mt < nmt) store_unit(head0, left, nt, mt, o, inv);
+        }
+    };
+    auto from_smem = [](auto& v, const float* p) { v = *reinterpret_cast<const std::remove_reference_t<decltype(v)>*>(p); };
+    auto from_l2 = [](auto& v, const float* p) { v = __ldcg(reinterpret_cast<const std::remove_reference_t<decltype(v)>*>(p)); };
+
+    // the CTA's parts, row by row; lane i looks at part i: warp i/2's first (even) or last (odd).  The units of all rows
+    // are dealt over the warps.
+    const long long my_start = lane < 2 * kWarps ? s_start[lane] : -1;
+    uint32_t todo = __ballot_sync(0xffffffffu, my_start >= 0);
+    long long cross0 = -1, cross1 = -1;   // the row that came from an earlier CTA, the one that goes on into the next
+    int row0 = 0, row1 = 0, n0 = 0, n1 = 0, turn = warp;
+#pragma unroll 1
+    while (todo) {
+        const int i = __ffs(todo) - 1;
+        const long long start = __shfl_sync(0xffffffffu, my_start, i);
+        const uint32_t parts = __ballot_sync(0xffffffffu, my_start == start);
+        const int row = s_row[i], n = s_n[i];
+        todo &= ~parts;
+        float* to = nullptr;
+        if (start < x0) cross0 = start, row0 = row, n0 = n, to = cta_pieces;
+        else if (start + n > x1) cross1 = start, row1 = row, n1 = n, to = cta_pieces + kPiece;
+#pragma unroll 1
+        for (; turn < kUnits; turn += kWarps) {
+            uint32_t next = parts;
+            auto at = [&](int) -> const float* {   // asked for in order
+                const int p = __ffs(next) - 1;
+                next &= next - 1;
+                return reinterpret_cast<const float*>(smem + (p >> 1) * C::kWarpSmem + (p & 1 ? 0 : C::kRing));
+            };
+            join(from_smem, at, __popc(parts), turn, row, to);
+        }
+        turn = (turn - kUnits) % kWarps;
     }
-    if (cross[0].start < 0 && cross[1].start < 0) return;   // the same in every thread
-    __threadfence();
+    if (cross0 < 0 && cross1 < 0) return;   // the same in every thread
+    const Split split(N, nC_of(N));
     __syncthreads();
     if (tid < 2) {
-        const Part p = tid ? cross[1] : cross[0];
+        const long long start = tid ? cross1 : cross0;
         int last = 0;
-        if (p.start >= 0) {
+        if (start >= 0) {
             // the row's first CTA keeps its counter: a CTA is the first of one crossing row at most
-            const int c0 = (int)split_owner(p.start, N, nC), c1 = (int)split_owner(p.start + p.n - 1, N, nC);
-            last = atomicAdd(a.counters + c0, 1) == c1 - c0;
+            const int c0 = split.owner(start), c1 = split.owner(start + (tid ? n1 : n0) - 1);
+            last = take_ticket(a.counters + c0) == c1 - c0;
             if (last) a.counters[c0] = 0;
         }
         s_last[tid] = last;
-        __threadfence();
     }
     __syncthreads();
+#pragma unroll 1
     for (int e = 0; e < 2; ++e) {
         if (!s_last[e]) continue;
-        const Part p = e ? cross[1] : cross[0];
-        const int c0 = (int)split_owner(p.start, N, nC), c1 = (int)split_owner(p.start + p.n - 1, N, nC);
-        const int kvh = p.hr / a.hb, h0 = (p.hr - kvh * a.hb) * 8 * NT;
-        for (int u = warp; u < units; u += kWarps) {
-            const int nt = u / nmt, mt = u - nt * nmt;
-            Join z;
-            z.reset();
-            constexpr int kDeep = 8;
-            for (int c = c0; c <= c1; c += kDeep) {
-                float2 pm[kDeep], pl[kDeep];
-                float4 po[kDeep];
+        const long long start = e ? cross1 : cross0;
+        const int row = e ? row1 : row0, c0 = split.owner(start), n = split.owner(start + (e ? n1 : n0) - 1) - c0 + 1;
+        // the first CTA filed the row as its slot 1, the others as their slot 0
+        auto at = [&](int i) -> const float* { return a.pieces + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPiece; };
+        if (n <= 8) {
+#pragma unroll 1
+            for (int u = warp; u < kUnits; u += kWarps) join(from_l2, at, n, u, row, nullptr);
+            continue;
+        }
+        // many CTAs: every warp gathers some of them, then the warps' sums are joined
+        const int from = n * warp / kWarps, to = n * (warp + 1) / kWarps;
 #pragma unroll
-                for (int i = 0; i < kDeep; ++i) {
-                    if (c + i <= c1) {
-                        // the first CTA filed the row's start as its slot 1, the others as their slot 0
-                        const float* src = a.pieces + ((int64_t)(c + i) * (2 + kWarps) + (c + i == c0 ? 1 : 0)) * pf;
-                        const float* ml = src + NT * 8 * a.Dv + nt * 16;
-                        pm[i] = __ldcg(reinterpret_cast<const float2*>(ml + 2 * t4));
-                        pl[i] = __ldcg(reinterpret_cast<const float2*>(ml + 8 + 2 * t4));
-                        po[i] = __ldcg(reinterpret_cast<const float4*>(src + (u * 32 + lane) * 4));
-                    }
+        for (int nt = 0; nt < NT; ++nt) {
+            m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
+            l_run[nt][0] = l_run[nt][1] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < kMt; ++mt) acc[nt][mt][0] = acc[nt][mt][1] = acc[nt][mt][2] = acc[nt][mt][3] = 0.f;
+        }
+#pragma unroll 1
+        for (int i = from; i < to; ++i) {
+            const float* src = at(i);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float* ml = src + NT * 8 * DB + nt * 16 + 2 * t4;
+                float2 x, y;
+                float4 z[kMt];
+                from_l2(x, ml), from_l2(y, ml + 8);
+#pragma unroll
+                for (int mt = 0; mt < kMt; ++mt) from_l2(z[mt], src + ((nt * kMt + mt) * 32 + lane) * 4);
+                const float pm[2] = {x.x, x.y}, pl[2] = {y.x, y.y};
+                float s0[2], s1[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float top = fmaxf(m_ref[nt][j], pm[j]), ref = fmaxf(top, -3.0e38f);
+                    s0[j] = ex2(m_ref[nt][j] - ref), s1[j] = ex2(pm[j] - ref);
+                    m_ref[nt][j] = top;
+                    l_run[nt][j] = l_run[nt][j] * s0[j] + pl[j] * s1[j];
                 }
 #pragma unroll
-                for (int i = 0; i < kDeep; ++i)
-                    if (c + i <= c1) z.add(pm[i], pl[i], po[i]);
+                for (int mt = 0; mt < kMt; ++mt) {
+                    acc[nt][mt][0] = acc[nt][mt][0] * s0[0] + z[mt].x * s1[0];
+                    acc[nt][mt][1] = acc[nt][mt][1] * s0[1] + z[mt].y * s1[1];
+                    acc[nt][mt][2] = acc[nt][mt][2] * s0[0] + z[mt].z * s1[0];
+                    acc[nt][mt][3] = acc[nt][mt][3] * s0[1] + z[mt].w * s1[1];
+                }
             }
-            float inv[2];
-            finish(a, p.b, p.hr, h0, nt, z.m, z.l, mt == 0, inv);
-            store_unit<F16, I8>(a, p.b, p.hr, h0, nt, mt, z.o, inv);
         }
+        __syncthreads();   // the parts in shared memory are used up
+        file_piece(reinterpret_cast<float*>(ring));
+        __syncthreads();
+        auto sums = [&](int i) -> const float* { return reinterpret_cast<const float*>(smem + i * C::kWarpSmem); };
+#pragma unroll 1
+        for (int u = warp; u < kUnits; u += kWarps) join(from_smem, sums, kWarps, u, row, nullptr);
     }
 }
 
@@ -704,33 +801,29 @@ int launch_f16(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 int launch_bf16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 int launch_f16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 
-// Launch the variant for these args (grid: one CTA a SM, capped by `ctas`).
 template <bool F16, bool I8, int DB, int NT>
 int launch(const Args& a, int ctas, cudaStream_t st) {
-    using C = Cfg<F16, I8, DB, NT>;
-    const size_t smem = C::kWarps * warp_bytes(I8, C::kStages, NT, a.Dk, a.Dv);
+    using C = Cfg<I8, DB, NT>;
+    constexpr int kSmem = C::kWarps * C::kWarpSmem;
     static thread_local int set_for = -1;
     int dev = 0;
     cudaGetDevice(&dev);
     if (set_for != dev) {
-        const size_t most = C::kWarps * warp_bytes(I8, C::kStages, NT, DB, DB);
-        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) !=
+        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
             cudaSuccess)
             return set_error(WS_ERR_CUDA, "paged_decode: shared memory");
         set_for = dev;
     }
-    decode_kernel<F16, I8, DB, NT><<<ctas, 32 * C::kWarps, smem, st>>>(a);
+    decode_kernel<F16, I8, DB, NT><<<ctas, 32 * C::kWarps, kSmem, st>>>(a);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }
 
 template <bool F16, bool I8>
 int launch_any(const Args& a, int DB, int NT, int ctas, cudaStream_t st) {
-    if (DB == 64) return NT == 1 ? launch<F16, I8, 64, 1>(a, ctas, st) : NT == 2 ? launch<F16, I8, 64, 2>(a, ctas, st)
-                                                                                 : launch<F16, I8, 64, 4>(a, ctas, st);
-    if (DB == 128) return NT == 1 ? launch<F16, I8, 128, 1>(a, ctas, st) : NT == 2 ? launch<F16, I8, 128, 2>(a, ctas, st)
-                                                                                   : launch<F16, I8, 128, 4>(a, ctas, st);
-    return NT == 1 ? launch<F16, I8, 256, 1>(a, ctas, st) : launch<F16, I8, 256, 2>(a, ctas, st);
+    if (DB == 64) return NT == 1 ? launch<F16, I8, 64, 1>(a, ctas, st) : launch<F16, I8, 64, 2>(a, ctas, st);
+    if (DB == 128) return NT == 1 ? launch<F16, I8, 128, 1>(a, ctas, st) : launch<F16, I8, 128, 2>(a, ctas, st);
+    return launch<F16, I8, 256, 1>(a, ctas, st);
 }
 
 }  // namespace paged

@@ -66,7 +66,7 @@ int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q
     a.vsp = kv->vs_stride_page, a.vst = kv->vs_stride_tok, a.vsh = kv->vs_stride_head;
     a.table = page_table, a.table_stride = table_stride;
     a.seq_lens = seq_lens;
-    a.cap = std::min<int64_t>((int64_t)max_pages * kv->page_size, INT32_MAX - 64);
+    a.cap = (int)std::min<int64_t>((int64_t)max_pages * kv->page_size, INT32_MAX - 64);
     a.whole = kv->page_size % paged::kTok == 0;
     a.n_pages = (int)kv->n_pages, a.page_size = kv->page_size;
     // t / page_size for t < 2^31 as a multiply and a shift: shift = ceil(log2 P), mul = floor(2^32 (2^shift - P) / P) + 1

@@ -33,8 +33,6 @@
 
 #include <cuda_fp16.h>
 
-#include <type_traits>
-
 namespace ws {
 namespace paged {
 
@@ -54,7 +52,7 @@ struct Args {
     const int32_t* table;
     int64_t table_stride;
     const int32_t* seq_lens;
-    int64_t cap;                         // max_pages * page_size
+    int cap;                             // max_pages * page_size, or less than 2^31
     int whole;                           // page_size is a multiple of kTok
     int n_pages, page_size;
     uint32_t div_mul, div_shift;         // t / page_size = (umulhi(t, div_mul) + t) >> div_shift
@@ -91,7 +89,7 @@ inline int piece_floats(int DB, int NT) { return NT * (8 * DB + 16); }
 // What the filler of a stage leaves for its reader.
 struct __align__(16) Meta {
     uint32_t mask;   // bit i: token i counts; bit 16: the row ends here
-    int b, row, sub; // request, row of it, place in the row
+    int b, row, sub; // request; kv head << 16 | head block; place in the row
 };
 
 __device__ __forceinline__ void cp_async16_all(uint32_t dst, const void* src) {
@@ -159,28 +157,30 @@ struct Span {
 };
 __device__ __forceinline__ Span span_of(const Args& a, int b) {
     Span s;
-    s.L = (int)min((long long)max(__ldg(a.seq_lens + b), 0), (long long)a.cap);
+    s.L = min(max(__ldg(a.seq_lens + b), 0), a.cap);
     s.lo = a.window > 0 ? max(s.L - a.window, 0) : 0;
-    s.n = s.L > 0 ? (s.L - (s.lo & ~(kTok - 1)) + kTok - 1) / kTok : 0;
+    s.n = (s.L - (s.lo & ~(kTok - 1)) + kTok - 1) / kTok;   // lo = 0 without a token
     return s;
 }
 
-// n / d, in 32 bits where that is enough.
-__device__ __forceinline__ long long quotient(long long n, long long d) {
-    if (((n | d) >> 32) == 0) return (uint32_t)n / (uint32_t)d;
-    return n / d;
-}
 // An even split of a line of N places over n CTAs: the first `more` take one place more than `each`.
 struct Split {
     long long each, more;
+    float inv;
     __device__ __forceinline__ Split(long long N, int n) {
-        each = n ? quotient(N, n) : 0;
+        // N / n in two steps of 32 bits: N < 2^48, n < 2^16
+        const uint32_t hi = (uint32_t)(N >> 16), q = hi / (uint32_t)n;
+        each = ((long long)q << 16) + (((hi - q * n) << 16) | (uint32_t)(N & 0xffff)) / (uint32_t)n;
         more = N - each * n;
+        inv = __fdividef(n, (float)N);
     }
     __device__ __forceinline__ long long start(int c) const { return c * each + min((long long)c, more); }
+    // The CTA that holds place t: a guess in fp32, which is off by one at most, and the starts beside it.
     __device__ __forceinline__ int owner(long long t) const {
-        const long long wide = more * (each + 1);
-        return (int)(t < wide ? quotient(t, each + 1) : more + quotient(t - wide, each));
+        int c = (int)((float)t * inv);
+        while (c > 0 && start(c) > t) --c;
+        while (start(c + 1) <= t) ++c;
+        return c;
     }
 };
 // Adds to a counter, after everything that this CTA wrote before its last barrier and before everything it reads next.
@@ -188,6 +188,17 @@ __device__ __forceinline__ int take_ticket(int* counter) {
     int old;
     asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
     return old;
+}
+
+// A load, from shared memory or the workspace, that sees what other SMs wrote.
+template <typename T>
+__device__ __forceinline__ T load_l2(const float* p) {
+    T v;
+    if constexpr (sizeof(T) == 16)
+        asm volatile("ld.relaxed.gpu.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    else
+        asm volatile("ld.relaxed.gpu.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+    return v;
 }
 
 // Two heads' 1/l; with `write`, lanes of the first row write their lse.
@@ -211,7 +222,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     constexpr float kUp = kPF16 ? 8.f : 0.f;
     extern __shared__ __align__(16) uint8_t smem[];   // [kWarps][kWarpSmem]
     __shared__ long long s_scan[kWarps], s_off[kWarps], s_start[2 * kWarps];   // s_start < 0: no part
-    __shared__ int s_b[kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_last[2];
+    __shared__ int s_b[kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
@@ -221,27 +232,47 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     long long N, my_off = 0;
     int my_b = 0;
     if (lane < 2) s_start[2 * warp + lane] = -1;
-    auto nC_of = [&](long long n) { return (int)min((long long)gridDim.x, (n + kWarps * kMinSub - 1) / (kWarps * kMinSub)); };
-    long long x0 = 0, x1 = 0;
-    auto warp_start = [&](int w) { return x0 + (uint32_t)(x1 - x0) * (uint64_t)w / kWarps; };
-    auto stretch = [&]() {
-        const Split split(N, nC_of(N));
-        if ((int)blockIdx.x < nC_of(N)) x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
+    // CTAs that work: all, or as many as get kMinSub subtiles a warp
+    auto nC_of = [&](long long n) {
+        return n >= (long long)gridDim.x * kWarps * kMinSub ? (int)gridDim.x
+                                                            : ((int)n + kWarps * kMinSub - 1) / (kWarps * kMinSub);
     };
-    if (a.B <= 32) {   // every warp for itself: one request a lane
-        const long long mine = lane < a.B ? (long long)span_of(a, lane).n * R : 0;
+    long long x0 = 0, x1 = 0;
+    auto warp_start = [&](int w) {
+        const uint32_t len = (uint32_t)(x1 - x0), each = len / kWarps;
+        return x0 + each * w + min((uint32_t)w, len - each * kWarps);
+    };
+    auto stretch = [&]() {
+        const int n = nC_of(N);
+        if ((int)blockIdx.x >= n) return;
+        const Split split(N, n);
+        x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
+    };
+    if (a.B <= 256) {   // every warp for itself, up to eight requests a lane
+        const int per = (a.B + 31) / 32;
+        int n[8], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n[i] = i < per && lane * per + i < a.B ? span_of(a, lane * per + i).n : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine += n[i];
         long long upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += y;
         }
-        N = __shfl_sync(0xffffffffu, upto, 31);
+        N = __shfl_sync(0xffffffffu, upto, 31) * R;
         stretch();
         const long long y = warp_start(warp);
-        const uint32_t here = __ballot_sync(0xffffffffu, y >= upto - mine && y < upto);
-        my_b = here ? __ffs(here) - 1 : 0;
-        my_off = __shfl_sync(0xffffffffu, upto - mine, my_b);
+        long long off = (upto - mine) * R;
+        const uint32_t here = __ballot_sync(0xffffffffu, y >= off && y < upto * R);
+        int b = lane * per;
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (b == lane * per + i && y >= off + (long long)n[i] * R) off += (long long)n[i] * R, ++b;
+        const int src = here ? __ffs(here) - 1 : 0;
+        my_b = __shfl_sync(0xffffffffu, b, src);
+        my_off = __shfl_sync(0xffffffffu, off, src);
     } else {
         const int per = (a.B + kWarps * 32 - 1) / (kWarps * 32), first_b = tid * per;
         long long mine = 0;
@@ -279,19 +310,15 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         my_b = s_b[warp], my_off = s_off[warp];
     }
     // requests without a token, dealt over the CTAs: zeros, -inf
-    auto write_empty = [&]() {
-        for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-            if (span_of(a, b).n) continue;
-            const int64_t row = (int64_t)b * a.Hkv * a.G;
-            for (int i = tid; i < a.Hkv * a.G * (a.Dv / 8); i += 32 * kWarps)
-                reinterpret_cast<uint4*>(a.out + row * a.Dv)[i] = make_uint4(0, 0, 0, 0);
-            for (int i = tid; a.lse && i < a.Hkv * a.G; i += 32 * kWarps) a.lse[row + i] = -INFINITY;
-        }
-    };
-    if (x0 == x1) {
-        write_empty();
-        return;
+#pragma unroll 1
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+        if (span_of(a, b).n) continue;
+        const int64_t head0 = (int64_t)b * a.Hkv * a.G;
+        for (int i = tid; i < a.Hkv * a.G * (a.Dv / 8); i += 32 * kWarps)
+            reinterpret_cast<uint4*>(a.out + head0 * a.Dv)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; a.lse && i < a.Hkv * a.G; i += 32 * kWarps) a.lse[head0 + i] = -INFINITY;
     }
+    if (x0 == x1) return;
 
     // ---- this warp's stretch
     const long long w0 = warp_start(warp);
@@ -305,7 +332,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     // filler: the row being filled, and the next subtile's page entry (of this lane's token where pages are not whole
     // subtiles)
     Span fs = {0, 0, 0};
-    int f_b = 0, f_row = 0, f_sub = 0, f_entry = -1, f_left = count;
+    int f_b = 0, f_kvh = 0, f_blk = 0, f_sub = 0, f_entry = -1, f_left = count;
     uint32_t f_off = 0;
     const int l8 = lane & 7, r4 = lane >> 3;   // copies: eight lanes a row, four rows at a time
     const int kchunks = I8 ? a.Dk >> 4 : a.Dk >> 3, vchunks = I8 ? a.Dv >> 4 : a.Dv >> 3;
@@ -330,7 +357,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 if (a.status) atomicMax(a.status, kDevBadIndex);
                 mask &= a.whole ? 0u : pages_ok;
             }
-            const uint32_t page = page_ok ? f_entry : 0, kvh = a.hb == 1 ? f_row : f_row / a.hb;
+            const uint32_t page = page_ok ? f_entry : 0, kvh = f_kvh;
             uint64_t ka = (uint64_t)page * a.kp + (uint64_t)f_off * a.kt + (uint64_t)kvh * a.kh;
             uint64_t va = (uint64_t)page * a.vp + (uint64_t)f_off * a.vt + (uint64_t)kvh * a.vh;
             if (I8) {
@@ -342,7 +369,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             if (lane == 0) {
                 Meta m;
                 m.mask = mask | (f_sub == fs.n - 1 ? 1u << 16 : 0u);
-                m.b = f_b, m.row = f_row, m.sub = f_sub;
+                m.b = f_b, m.row = f_kvh << 16 | f_blk, m.sub = f_sub;
                 *reinterpret_cast<Meta*>(ring + slot * C::kStage + kM) = m;
             }
             const uint32_t kd = st + r4 * kRow + l8 * 16, vd = kd + kV;
@@ -376,10 +403,13 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             if (--f_left > 0) {
                 if (++f_sub == fs.n) {
                     f_sub = 0;
-                    if (++f_row == R) {
-                        f_row = 0;
-                        do fs = span_of(a, ++f_b);
-                        while (fs.n == 0);
+                    if (++f_blk == a.hb) {
+                        f_blk = 0;
+                        if (++f_kvh == a.Hkv) {
+                            f_kvh = 0;
+                            do fs = span_of(a, ++f_b);
+                            while (fs.n == 0);
+                        }
                     }
                 }
                 look_up();
@@ -394,8 +424,12 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 
     const int nks = a.Dk >> 4, nmt = a.Dv >> 4;
 
+    // A row's first head of the block in the output, and how many of the kv head's heads are left from it.
+    auto head_of = [&](int b, int row) { return ((int64_t)b * a.Hkv + (row >> 16)) * a.G + (row & 0xffff) * 8 * NT; };
+    auto left_of = [&](int row) { return a.G - (row & 0xffff) * 8 * NT; };
+
     auto load_q = [&](int b, int row) {
-        const int kvh = row / a.hb, h0 = (row - kvh * a.hb) * 8 * NT;
+        const int kvh = row >> 16, h0 = (row & 0xffff) * 8 * NT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int h = h0 + nt * 8 + g;
@@ -460,11 +494,15 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         f_b = my_b;
         fs = span_of(a, f_b);
         const long long rel = w0 - my_off;
-        f_row = (int)quotient(rel, fs.n);
-        f_sub = (int)(rel - (long long)f_row * fs.n);
+        int row = (int)__fdividef((float)rel, (float)fs.n);   // off by one at most
+        if ((long long)row * fs.n > rel) --row;
+        if ((long long)(row + 1) * fs.n <= rel) ++row;
+        f_sub = (int)(rel - (long long)row * fs.n);
+        f_kvh = a.hb == 1 ? row : row / a.hb;
+        f_blk = row - f_kvh * a.hb;
         look_up();
-        load_q(f_b, f_row);
     }
+    const int first_b = f_b, first_row = f_kvh << 16 | f_blk;
     int slot = 0;   // the stage that iteration `it` reads; the one before it is filled
 #pragma unroll 1
     for (int it = 1 - S; it < count; ++it) {
@@ -474,16 +512,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         }
         const int to = it < 0 ? it + S - 1 : slot == 0 ? S - 1 : slot - 1;
         fill(to);
-        if (it < 0) {
-            if (it == 1 - S) write_empty();
-            continue;
-        }
         const uint32_t st = ring_u + slot * C::kStage;
-        const Meta meta = *reinterpret_cast<const Meta*>(ring + slot * C::kStage + kM);
-        if (meta.sub == 0) {
-            if (it) load_q(meta.b, meta.row);
-            began = true;
-        }
+        Meta meta;
+        if (it < 0) meta.b = first_b, meta.row = first_row, meta.sub = it == 1 - S ? 0 : 1;
+        else meta = *reinterpret_cast<const Meta*>(ring + slot * C::kStage + kM);
+        // a row's queries: the first row's while its first keys come
+        if (meta.sub == 0 && it != 0 && count > 0) load_q(meta.b, meta.row);
+        if (it < 0) continue;
+        began |= meta.sub == 0;
         // scores, in two chains
         float c[NT][4], e[NT][4];
 #pragma unroll
@@ -623,8 +659,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], 16);
                 }
             if (ends && began) {
-                const int kvh = meta.row / a.hb, h0 = (meta.row - kvh * a.hb) * 8 * NT, left = a.G - h0;
-                const int64_t head0 = ((int64_t)meta.b * a.Hkv + kvh) * a.G + h0;
+                const int left = left_of(meta.row);
+                const int64_t head0 = head_of(meta.b, meta.row);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float inv[2];
@@ -640,7 +676,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 file_piece(reinterpret_cast<float*>(more ? ring + C::kRing : ring));
                 if (lane == 0) {
                     s_start[part] = w0 + it - meta.sub;
-                    s_row[part] = meta.b * R + meta.row;
+                    s_req[part] = meta.b;
+                    s_row[part] = meta.row;
                     s_n[part] = span_of(a, meta.b).n;
                 }
             }
@@ -649,149 +686,146 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     }
     __syncthreads();
 
-    // ---- join parts: unit (16 x 8 fragment) u of the parts at `at(0)`, `at(1)`, ..., to a piece, or (null) to the output
-    auto join = [&](auto load, auto at, int n, int u, int row, float* to) {
-        const int nt = u / kMt, mt = u - nt * kMt, ml = NT * 8 * DB + nt * 16 + 2 * t4;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < n; i += 4) {
-            float4 z[4];
-            float2 x[4], y[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (i + k < n) {
-                    const float* src = at(i + k);
-                    load(x[k], src + ml), load(y[k], src + ml + 8), load(z[k], src + (u * 32 + lane) * 4);
-                } else {
-                    x[k] = make_float2(-INFINITY, -INFINITY), y[k] = make_float2(0.f, 0.f), z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-            }
-            const float t0 = fmaxf(fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)), m[0]);
-            const float t1 = fmaxf(fmaxf(fmaxf(x[0].y, x[1].y), fmaxf(x[2].y, x[3].y)), m[1]);
-            const float r0 = fmaxf(t0, -3.0e38f), r1 = fmaxf(t1, -3.0e38f), k0 = ex2(m[0] - r0), k1 = ex2(m[1] - r1);
-            l[0] *= k0, o[0] *= k0, o[2] *= k0, l[1] *= k1, o[1] *= k1, o[3] *= k1, m[0] = t0, m[1] = t1;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float s0 = ex2(x[k].x - r0), s1 = ex2(x[k].y - r1);
-                l[0] += y[k].x * s0, l[1] += y[k].y * s1;
-                o[0] += z[k].x * s0, o[1] += z[k].y * s1, o[2] += z[k].z * s0, o[3] += z[k].w * s1;
-            }
-        }
-        if (to) {
-            *reinterpret_cast<float4*>(to + (u * 32 + lane) * 4) = make_float4(o[0], o[1], o[2], o[3]);
-            if (mt == 0 && lane < 4) {
-                *reinterpret_cast<float2*>(to + ml) = make_float2(m[0], m[1]);
-                *reinterpret_cast<float2*>(to + ml + 8) = make_float2(l[0], l[1]);
-            }
-        } else {
-            const int b = row / R, kvh = (row - b * R) / a.hb, h0 = (row - b * R - kvh * a.hb) * 8 * NT, left = a.G - h0;
-            const int64_t head0 = ((int64_t)b * a.Hkv + kvh) * a.G + h0;
-            float inv[2];
-            finish(a, head0, left, nt, m, l, mt == 0, inv);
-            if (mt < nmt) store_unit(head0, left, nt, mt, o, inv);
-        }
-    };
-    auto from_smem = [](auto& v, const float* p) { v = *reinterpret_cast<const std::remove_reference_t<decltype(v)>*>(p); };
-    auto from_l2 = [](auto& v, const float* p) { v = __ldcg(reinterpret_cast<const std::remove_reference_t<decltype(v)>*>(p)); };
-
-    // the CTA's parts, row by row; lane i looks at part i: warp i/2's first (even) or last (odd).  The units of all rows
-    // are dealt over the warps.
+    // ---- join parts.  First the CTA's, row by row; lane i looks at part i: warp i/2's first (even) or last (odd).  Then,
+    // if this CTA is the last of a row's to file its part, the row's.  The units (16 x 8 fragments) of a row are dealt
+    // over the warps.
     const long long my_start = lane < 2 * kWarps ? s_start[lane] : -1;
     uint32_t todo = __ballot_sync(0xffffffffu, my_start >= 0);
     long long cross0 = -1, cross1 = -1;   // the row that came from an earlier CTA, the one that goes on into the next
-    int row0 = 0, row1 = 0, n0 = 0, n1 = 0, turn = warp;
+    int id0 = 0, id1 = 0, turn = warp, ended = -1;
 #pragma unroll 1
-    while (todo) {
-        const int i = __ffs(todo) - 1;
-        const long long start = __shfl_sync(0xffffffffu, my_start, i);
-        const uint32_t parts = __ballot_sync(0xffffffffu, my_start == start);
-        const int row = s_row[i], n = s_n[i];
-        todo &= ~parts;
-        float* to = nullptr;
-        if (start < x0) cross0 = start, row0 = row, n0 = n, to = cta_pieces;
-        else if (start + n > x1) cross1 = start, row1 = row, n1 = n, to = cta_pieces + kPiece;
-#pragma unroll 1
-        for (; turn < kUnits; turn += kWarps) {
-            uint32_t next = parts;
-            auto at = [&](int) -> const float* {   // asked for in order
-                const int p = __ffs(next) - 1;
-                next &= next - 1;
-                return reinterpret_cast<const float*>(smem + (p >> 1) * C::kWarpSmem + (p & 1 ? 0 : C::kRing));
-            };
-            join(from_smem, at, __popc(parts), turn, row, to);
-        }
-        turn = (turn - kUnits) % kWarps;
-    }
-    if (cross0 < 0 && cross1 < 0) return;   // the same in every thread
-    const Split split(N, nC_of(N));
-    __syncthreads();
-    if (tid < 2) {
-        const long long start = tid ? cross1 : cross0;
-        int last = 0;
-        if (start >= 0) {
-            // the row's first CTA keeps its counter: a CTA is the first of one crossing row at most
-            const int c0 = split.owner(start), c1 = split.owner(start + (tid ? n1 : n0) - 1);
-            last = take_ticket(a.counters + c0) == c1 - c0;
-            if (last) a.counters[c0] = 0;
-        }
-        s_last[tid] = last;
-    }
-    __syncthreads();
-#pragma unroll 1
-    for (int e = 0; e < 2; ++e) {
-        if (!s_last[e]) continue;
-        const long long start = e ? cross1 : cross0;
-        const int row = e ? row1 : row0, c0 = split.owner(start), n = split.owner(start + (e ? n1 : n0) - 1) - c0 + 1;
-        // the first CTA filed the row as its slot 1, the others as their slot 0
-        auto at = [&](int i) -> const float* { return a.pieces + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPiece; };
-        if (n <= 8) {
-#pragma unroll 1
-            for (int u = warp; u < kUnits; u += kWarps) join(from_l2, at, n, u, row, nullptr);
-            continue;
-        }
-        // many CTAs: every warp gathers some of them, then the warps' sums are joined
-        const int from = n * warp / kWarps, to = n * (warp + 1) / kWarps;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
-            l_run[nt][0] = l_run[nt][1] = 0.f;
-#pragma unroll
-            for (int mt = 0; mt < kMt; ++mt) acc[nt][mt][0] = acc[nt][mt][1] = acc[nt][mt][2] = acc[nt][mt][3] = 0.f;
-        }
-#pragma unroll 1
-        for (int i = from; i < to; ++i) {
-            const float* src = at(i);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float* ml = src + NT * 8 * DB + nt * 16 + 2 * t4;
-                float2 x, y;
-                float4 z[kMt];
-                from_l2(x, ml), from_l2(y, ml + 8);
-#pragma unroll
-                for (int mt = 0; mt < kMt; ++mt) from_l2(z[mt], src + ((nt * kMt + mt) * 32 + lane) * 4);
-                const float pm[2] = {x.x, x.y}, pl[2] = {y.x, y.y};
-                float s0[2], s1[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float top = fmaxf(m_ref[nt][j], pm[j]), ref = fmaxf(top, -3.0e38f);
-                    s0[j] = ex2(m_ref[nt][j] - ref), s1[j] = ex2(pm[j] - ref);
-                    m_ref[nt][j] = top;
-                    l_run[nt][j] = l_run[nt][j] * s0[j] + pl[j] * s1[j];
+    while (true) {
+        int id, n, c0 = 0;          // one of the row's parts here; how many parts, and the first CTA when they are CTAs'
+        uint32_t parts = 0;         // the parts in shared memory
+        float* to = nullptr;        // a piece in the workspace, or the output
+        if (todo) {
+            id = __ffs(todo) - 1;
+            const long long start = __shfl_sync(0xffffffffu, my_start, id);
+            parts = __ballot_sync(0xffffffffu, my_start == start);
+            todo &= ~parts;
+            n = __popc(parts);
+            if (start < x0) cross0 = start, id0 = id, to = cta_pieces;
+            else if (start + s_n[id] > x1) cross1 = start, id1 = id, to = cta_pieces + kPiece;
+        } else {
+            if (ended < 0) {
+                if (cross0 < 0 && cross1 < 0) return;   // the same in every thread
+                __syncthreads();
+                if (tid < 2) {
+                    const long long start = tid ? cross1 : cross0;
+                    int ctas = 0;
+                    if (start >= 0) {
+                        // the row's first CTA keeps its counter: a CTA is the first of one crossing row at most
+                        const Split split(N, nC_of(N));
+                        const int c = tid ? blockIdx.x : split.owner(start);
+                        ctas = split.owner(start + s_n[tid ? id1 : id0] - 1) - c + 1;
+                        if (take_ticket(a.counters + c) == ctas - 1) a.counters[c] = 0;
+                        else ctas = 0;
+                        s_first[tid] = c;
+                    }
+                    s_ctas[tid] = ctas;
                 }
+                __syncthreads();
+            }
+            if (++ended == 2) return;
+            n = s_ctas[ended], c0 = s_first[ended], id = ended ? id1 : id0;
+            if (n == 0) continue;
+            turn = warp;
+            if (n > 32) {
+                // many CTAs: every warp gathers some of them, then the warps' sums are joined
+                const int from = n * warp / kWarps, end = n * (warp + 1) / kWarps;
 #pragma unroll
-                for (int mt = 0; mt < kMt; ++mt) {
-                    acc[nt][mt][0] = acc[nt][mt][0] * s0[0] + z[mt].x * s1[0];
-                    acc[nt][mt][1] = acc[nt][mt][1] * s0[1] + z[mt].y * s1[1];
-                    acc[nt][mt][2] = acc[nt][mt][2] * s0[0] + z[mt].z * s1[0];
-                    acc[nt][mt][3] = acc[nt][mt][3] * s0[1] + z[mt].w * s1[1];
+                for (int nt = 0; nt < NT; ++nt) {
+                    m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
+                    l_run[nt][0] = l_run[nt][1] = 0.f;
+#pragma unroll
+                    for (int mt = 0; mt < kMt; ++mt) acc[nt][mt][0] = acc[nt][mt][1] = acc[nt][mt][2] = acc[nt][mt][3] = 0.f;
                 }
+#pragma unroll 1
+                for (int i = from; i < end; ++i) {
+                    const float* src = a.pieces + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPiece;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float* ml = src + NT * 8 * DB + nt * 16 + 2 * t4;
+                        const float2 x = load_l2<float2>(ml), y = load_l2<float2>(ml + 8);
+                        float4 z[kMt];
+#pragma unroll
+                        for (int mt = 0; mt < kMt; ++mt) z[mt] = load_l2<float4>(src + ((nt * kMt + mt) * 32 + lane) * 4);
+                        const float pm[2] = {x.x, x.y}, pl[2] = {y.x, y.y};
+                        float s0[2], s1[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float top = fmaxf(m_ref[nt][j], pm[j]), ref = fmaxf(top, -3.0e38f);
+                            s0[j] = ex2(m_ref[nt][j] - ref), s1[j] = ex2(pm[j] - ref);
+                            m_ref[nt][j] = top;
+                            l_run[nt][j] = l_run[nt][j] * s0[j] + pl[j] * s1[j];
+                        }
+#pragma unroll
+                        for (int mt = 0; mt < kMt; ++mt) {
+                            acc[nt][mt][0] = acc[nt][mt][0] * s0[0] + z[mt].x * s1[0];
+                            acc[nt][mt][1] = acc[nt][mt][1] * s0[1] + z[mt].y * s1[1];
+                            acc[nt][mt][2] = acc[nt][mt][2] * s0[0] + z[mt].z * s1[0];
+                            acc[nt][mt][3] = acc[nt][mt][3] * s0[1] + z[mt].w * s1[1];
+                        }
+                    }
+                }
+                __syncthreads();   // the parts in shared memory are used up
+                file_piece(reinterpret_cast<float*>(ring));
+                __syncthreads();
+                n = kWarps, parts = 0xaaaaaaaau >> (32 - 2 * kWarps);
             }
         }
-        __syncthreads();   // the parts in shared memory are used up
-        file_piece(reinterpret_cast<float*>(ring));
-        __syncthreads();
-        auto sums = [&](int i) -> const float* { return reinterpret_cast<const float*>(smem + i * C::kWarpSmem); };
+        const int req = s_req[id], row = s_row[id];
 #pragma unroll 1
-        for (int u = warp; u < kUnits; u += kWarps) join(from_smem, sums, kWarps, u, row, nullptr);
+        for (; turn < kUnits; turn += kWarps) {
+            const int u = turn, nt = u / kMt, mt = u - nt * kMt, ml = NT * 8 * DB + nt * 16 + 2 * t4;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
+            constexpr int kBatch = 8;
+            uint32_t next = parts;
+#pragma unroll 1
+            for (int i = 0; i < n; i += kBatch) {
+                float4 z[kBatch];
+                float2 x[kBatch], y[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    x[k] = make_float2(-INFINITY, -INFINITY), y[k] = make_float2(0.f, 0.f), z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (i + k < n) {
+                        const float* src;
+                        if (parts) {
+                            const int p = __ffs(next) - 1;
+                            next &= next - 1;
+                            src = reinterpret_cast<const float*>(smem + (p >> 1) * C::kWarpSmem + (p & 1 ? 0 : C::kRing));
+                        } else {   // the first CTA filed the row as its slot 1, the others as their slot 0
+                            src = a.pieces + ((int64_t)(c0 + i + k) * 2 + (i + k == 0 ? 1 : 0)) * kPiece;
+                        }
+                        x[k] = load_l2<float2>(src + ml), y[k] = load_l2<float2>(src + ml + 8);
+                        z[k] = load_l2<float4>(src + (u * 32 + lane) * 4);
+                    }
+                }
+                float t0 = m[0], t1 = m[1];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) t0 = fmaxf(t0, x[k].x), t1 = fmaxf(t1, x[k].y);
+                const float r0 = fmaxf(t0, -3.0e38f), r1 = fmaxf(t1, -3.0e38f), k0 = ex2(m[0] - r0), k1 = ex2(m[1] - r1);
+                l[0] *= k0, o[0] *= k0, o[2] *= k0, l[1] *= k1, o[1] *= k1, o[3] *= k1, m[0] = t0, m[1] = t1;
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const float s0 = ex2(x[k].x - r0), s1 = ex2(x[k].y - r1);
+                    l[0] += y[k].x * s0, l[1] += y[k].y * s1;
+                    o[0] += z[k].x * s0, o[1] += z[k].y * s1, o[2] += z[k].z * s0, o[3] += z[k].w * s1;
+                }
+            }
+            if (to) {
+                *reinterpret_cast<float4*>(to + (u * 32 + lane) * 4) = make_float4(o[0], o[1], o[2], o[3]);
+                if (mt == 0 && lane < 4) {
+                    *reinterpret_cast<float2*>(to + ml) = make_float2(m[0], m[1]);
+                    *reinterpret_cast<float2*>(to + ml + 8) = make_float2(l[0], l[1]);
+                }
+            } else {
+                float inv[2];
+                finish(a, head_of(req, row), left_of(row), nt, m, l, mt == 0, inv);
+                if (mt < nmt) store_unit(head_of(req, row), left_of(row), nt, mt, o, inv);
+            }
+        }
+        turn = (turn - kUnits) % kWarps;
     }
 }
 

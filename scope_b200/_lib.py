@@ -7,8 +7,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.util
 import os
-import struct
 import threading
 
 import torch
@@ -51,12 +51,6 @@ class KvShare(ctypes.Structure):
     """Mirror of `ws_kv_share` (include/scope_b200.h)."""
     _fields_ = [("k", _V), ("v", _V), ("cu_seqlens", _V), ("seqlens", _V), ("n_tok", _i64),
                 ("k_stride_t", _i64), ("k_stride_h", _i64), ("v_stride_t", _i64), ("v_stride_h", _i64)]
-
-
-# `ws_paged_kv` and `ws_rope` (include/scope_b200.h) packed in one call each: k, v, scales, pages, the twelve strides and
-# the six ints; positions, table, axis stride, max_pos, the six ints and the axis map (as 32 bytes).
-paged_kv_pack = struct.Struct("@QQQQq12q6i").pack
-rope_pack = struct.Struct("@QQqq6i32s").pack
 
 
 # exported symbol -> (restype, argtypes); the CPU tests check that every
@@ -143,6 +137,33 @@ def check(rc: int, what: str) -> None:
     if rc != WS_OK:
         msg = lib().ws_last_error().decode(errors="replace")
         raise ScopeError(f"{what} failed (status {rc}): {msg}")
+
+
+BINDING_PATH = os.path.join(PKG, "_binding.so")
+_binding = None
+
+
+def binding():
+    """The CPython binding of the paged cache's entries (csrc/binding.cpp), set up for the loaded library."""
+    global _binding
+    if _binding is None:
+        L = lib()
+        with _lock:
+            if _binding is None:
+                if not os.path.exists(BINDING_PATH):
+                    raise ImportError(
+                        f"{BINDING_PATH} is missing; build it with `python -m scope_b200.compile_lib` "
+                        "(there is no CPU fallback)")
+                spec = importlib.util.spec_from_file_location("scope_b200._binding", BINDING_PATH)
+                mod = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(mod)
+                from .paged import PagedStep
+                address = [ctypes.cast(getattr(L, n), _V).value for n in (
+                    "ws_last_error", "ws_paged_slots", "ws_paged_release", "ws_rope_append", "ws_paged_decode")]
+                mod.setup(*address, L.ws_paged_slots_workspace_size(), L.ws_paged_decode_workspace_size(1, 1, 1, 16),
+                          ScopeError, workspaces.get, workspaces._bufs, PagedStep)
+                _binding = mod
+    return _binding
 
 
 # The current stream's raw handle without building a Stream object (2 us per call on the host otherwise, and

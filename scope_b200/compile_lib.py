@@ -1,9 +1,12 @@
-"""Compile libscope_b200.so (the C-ABI library) in-tree with nvcc for sm_100a.
+"""Compile libscope_b200.so (the C-ABI library) in-tree with nvcc for sm_100a, and _binding.so (the CPython binding of
+the paged cache's entries) with the host compiler.
 
     python -m scope_b200.compile_lib [-v]
 
 Objects are compiled in parallel into scope_b200/_build/ and linked with the
-static CUDA runtime; the library links nothing from PyTorch.
+static CUDA runtime; the library links nothing from PyTorch.  The binding is
+compiled against PyTorch's headers and resolves its symbols from the PyTorch
+that the process has loaded.
 """
 from __future__ import annotations
 
@@ -12,11 +15,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libscope_b200.so")
+BINDING_SRC = os.path.join(CSRC, "binding.cpp")
+BINDING = os.path.join(PKG, "_binding.so")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -54,7 +60,42 @@ def _compile(src: str, verbose: bool) -> tuple[str, str]:
     return obj, out.stderr if verbose else ""
 
 
+def build_binding(verbose: bool = False, force: bool = False) -> str:
+    """Build the binding if its source is newer than it; return its path."""
+    newest = max(os.path.getmtime(BINDING_SRC), _headers_mtime())
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest:
+        return BINDING
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cxx = shutil.which("g++")
+    if cxx is None:
+        raise RuntimeError("g++ not found")
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-sign-compare",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + INCLUDE, "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(root, "include"),
+           "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(cuda, "include"), BINDING_SRC, "-o", BINDING + ".tmp",
+           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+    out = subprocess.run(cmd, capture_output=True, text=True)
+    if out.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING_SRC}:\n{out.stdout}\n{out.stderr}")
+    if verbose:
+        sys.stdout.write(out.stderr)
+    os.replace(BINDING + ".tmp", BINDING)
+    return BINDING
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
+    """Build the library and the binding where a source is newer; return the library's path."""
+    with cf.ThreadPoolExecutor(max_workers=1) as ex:
+        binding = ex.submit(build_binding, verbose, force)
+        lib = build_lib(verbose, force)
+        binding.result()
+    return lib
+
+
+def build_lib(verbose: bool = False, force: bool = False) -> str:
     """Build the library if any source is newer than it; return its path."""
     os.makedirs(BUILD, exist_ok=True)
     srcs = sources()

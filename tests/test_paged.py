@@ -1,10 +1,15 @@
 """CPU checks of the paged cache's host side: axis maps, argument checks that need no GPU."""
 import ctypes
+import struct
 
 import pytest
 import torch
 
 from scope_b200 import _lib, paged
+
+# ws_paged_kv and ws_rope (include/scope_b200.h)
+paged_kv_pack = struct.Struct("@QQQQq12q6i").pack
+rope_pack = struct.Struct("@QQqq6i32s").pack
 
 
 def axes_of(packed, n):
@@ -63,7 +68,7 @@ def test_entries_check_their_arguments_before_any_launch():
         f = dict(k=p, v=p, ks=0, vs=0, n=4, kp=2048, kt=128, kh=32, vp=2048, vt=128, vh=32, P=16, Hkv=4, Dk=32, Dv=32,
                  dt=_lib.WS_DTYPE_BF16)
         f.update(change)
-        return _lib.paged_kv_pack(f["k"], f["v"], f["ks"], f["vs"], f["n"], f["kp"], f["kt"], f["kh"], f["vp"], f["vt"],
+        return paged_kv_pack(f["k"], f["v"], f["ks"], f["vs"], f["n"], f["kp"], f["kt"], f["kh"], f["vp"], f["vt"],
                                   f["vh"], 0, 0, 0, 0, 0, 0, f["P"], f["Hkv"], f["Dk"], f["Dv"], f["dt"], 0)
 
     def decode(pool, q=p, B=2, G=2, q_dtype=_lib.WS_DTYPE_BF16, stride=128, window=0, ws=p, nbytes=1 << 30, out=p):
@@ -92,7 +97,7 @@ def test_entries_check_their_arguments_before_any_launch():
         return L.ws_rope_append(rope, p, 64, 32, H, D, p, 64, 32, k, 128, 32, p, 128, 32, dtype, 3, p, pool, None)
 
     def rope(rot=32, axes=1, top=4, positions=p, amap=b""):
-        return _lib.rope_pack(positions, p, 0, top, 0, axes, rot, 0, 0, 0, amap)
+        return rope_pack(positions, p, 0, top, 0, axes, rot, 0, 0, 0, amap)
 
     assert append(rope(rot=8)) == bad and append(rope(rot=48)) == bad and append(rope(rot=24)) == bad
     assert append(rope(axes=5)) == bad and append(rope(top=0)) == bad and append(rope(positions=0)) == bad

@@ -38,6 +38,10 @@ namespace paged {
 
 constexpr int kTok = 16;        // tokens of a subtile
 constexpr int kMinSub = 2;      // subtiles a warp takes before another CTA joins in
+// Rows up to so many subtiles are not cut by a border between two CTAs, or two warps: the border moves to the nearer end
+// of the row, which unbalances the stretches by half a row at most and saves the joining.
+constexpr int kSnapCta = 40;
+constexpr int kSnapWarp = 4;
 constexpr float kSlack = 6.f;   // log2 of how far a probability may pass its bound before the reference moves
 
 struct Args {
@@ -221,93 +225,123 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
     constexpr float kUp = kPF16 ? 8.f : 0.f;
     extern __shared__ __align__(16) uint8_t smem[];   // [kWarps][kWarpSmem]
-    __shared__ long long s_scan[kWarps], s_off[kWarps], s_start[2 * kWarps];   // s_start < 0: no part
-    __shared__ int s_b[kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
+    __shared__ long long s_scan[kWarps], s_from[32 * kWarps], s_start[2 * kWarps];   // s_start < 0: no part
+    __shared__ int s_cnt[32 * kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
     const int R = a.Hkv * a.hb;          // rows of a request
 
-    // ---- the line: total length, this CTA's stretch, and where this warp's begins
-    long long N, my_off = 0;
-    int my_b = 0;
+    // ---- the line: total length, this CTA's stretch and this warp's
     if (lane < 2) s_start[2 * warp + lane] = -1;
-    // CTAs that work: all, or as many as get kMinSub subtiles a warp
-    auto nC_of = [&](long long n) {
-        return n >= (long long)gridDim.x * kWarps * kMinSub ? (int)gridDim.x
-                                                            : ((int)n + kWarps * kMinSub - 1) / (kWarps * kMinSub);
-    };
-    long long x0 = 0, x1 = 0;
-    auto warp_start = [&](int w) {
-        const uint32_t len = (uint32_t)(x1 - x0), each = len / kWarps;
-        return x0 + each * w + min((uint32_t)w, len - each * kWarps);
-    };
-    auto stretch = [&]() {
-        const int n = nC_of(N);
-        if ((int)blockIdx.x >= n) return;
-        const Split split(N, n);
-        x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
-    };
-    if (a.B <= 256) {   // every warp for itself, up to eight requests a lane
-        const int per = (a.B + 31) / 32;
-        int n[8], mine = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) n[i] = i < per && lane * per + i < a.B ? span_of(a, lane * per + i).n : 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mine += n[i];
-        long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-        }
-        N = __shfl_sync(0xffffffffu, upto, 31) * R;
-        stretch();
-        const long long y = warp_start(warp);
-        long long off = (upto - mine) * R;
-        const uint32_t here = __ballot_sync(0xffffffffu, y >= off && y < upto * R);
-        int b = lane * per;
-#pragma unroll
-        for (int i = 0; i < 7; ++i)
-            if (b == lane * per + i && y >= off + (long long)n[i] * R) off += (long long)n[i] * R, ++b;
-        const int src = here ? __ffs(here) - 1 : 0;
-        my_b = __shfl_sync(0xffffffffu, b, src);
-        my_off = __shfl_sync(0xffffffffu, off, src);
+    long long N;
+    const int per = a.B <= 32 ? 1 : (a.B + kWarps * 32 - 1) / (kWarps * 32);   // requests a lane, or a thread, looks at
+    long long my_from = 0, my_to = 0;   // up to 32 requests: where this lane's request lies
+    int my_n = 0;                       // (with one request each) its subtiles a row
+    if (a.B <= 32) {   // every warp for itself
+        my_n = lane < a.B ? span_of(a, lane).n : 0;
+        my_to = my_n;
     } else {
-        const int per = (a.B + kWarps * 32 - 1) / (kWarps * 32), first_b = tid * per;
-        long long mine = 0;
-        for (int b = first_b; b < min(first_b + per, a.B); ++b) mine += span_of(a, b).n;
-        long long upto = mine;
+        const int first = tid * per;
+#pragma unroll 1
+        for (int b = first; b < min(first + per, a.B); ++b) my_n = span_of(a, b).n, my_to += my_n;
+    }
+    my_from = my_to;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-        }
-        if (lane == 31) s_scan[warp] = upto;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, my_to, o);
+        if (lane >= o) my_to += y;
+    }
+    my_from = (my_to - my_from) * R, my_to *= R;
+    if (a.B <= 32) {
+        N = __shfl_sync(0xffffffffu, my_to, 31);
+    } else {
+        if (lane == 31) s_scan[warp] = my_to;
         __syncthreads();
-        long long before = 0, total = 0;
+        long long before = 0;
+        N = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) before += s_scan[w];
-            total += s_scan[w];
+            if (w == warp) before = N;
+            N += s_scan[w];
         }
-        N = total * R;
-        stretch();
-        long long off = (before + upto - mine) * R;
-        if (off < x1 && off + mine * R > x0) {
-            for (int b = first_b; b < min(first_b + per, a.B); ++b) {
-                const long long len = (long long)span_of(a, b).n * R;
-                if (off < x1 && off + len > x0) {
-                    for (int w = 0; w < kWarps; ++w) {
-                        const long long y = warp_start(w);
-                        if (y >= off && y < off + len) s_b[w] = b, s_off[w] = off;
-                    }
-                }
-                off += len;
-            }
-        }
+        s_from[tid] = before + my_from;
+        s_cnt[tid] = my_n;
         __syncthreads();
-        my_b = s_b[warp], my_off = s_off[warp];
+    }
+    // The request that holds place y < N, its first place and a row's subtiles.
+    struct Place {
+        int b, n;
+        long long off;
+    };
+    auto find = [&](long long y) {
+        Place p;
+        if (a.B <= 32) {
+            const uint32_t here = __ballot_sync(0xffffffffu, y >= my_from && y < my_to);
+            p.b = here ? __ffs(here) - 1 : 0;
+            p.n = __shfl_sync(0xffffffffu, my_n, p.b);
+            p.off = __shfl_sync(0xffffffffu, my_from, p.b);
+            return p;
+        }
+        // the last thread whose requests begin at or before y: its group of kWarps threads, then itself
+        const int group = (__popc(__ballot_sync(0xffffffffu, s_from[lane * kWarps] <= y)) - 1) * kWarps;
+        const int c = group + __popc(__ballot_sync(0xffffffffu, lane < kWarps && s_from[group + lane % kWarps] <= y)) - 1;
+        p.b = c * per, p.off = s_from[c];
+        if (per == 1) {
+            p.n = s_cnt[c];
+            return p;
+        }
+        while (true) {   // and the one of them that holds it, 32 at a time
+            const int b = p.b + lane, n = b < min((c + 1) * per, a.B) ? span_of(a, b).n : 0;
+            long long to = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, to, o);
+                if (lane >= o) to += x;
+            }
+            to = p.off + to * R;
+            const uint32_t here = __ballot_sync(0xffffffffu, y < to && n > 0);
+            if (here || p.b + 32 >= (c + 1) * per) {
+                const int src = here ? __ffs(here) - 1 : 0;
+                p.b += src;
+                p.n = __shfl_sync(0xffffffffu, n, src);
+                p.off = __shfl_sync(0xffffffffu, to - (long long)n * R, src);
+                return p;
+            }
+            p.b += 32, p.off = __shfl_sync(0xffffffffu, to, 31);
+        }
+    };
+    auto row_of = [&](const Place& p, long long y) {
+        const long long rel = y - p.off;
+        int row = (int)__fdividef((float)rel, (float)p.n);   // off by one at most
+        if ((long long)row * p.n > rel) --row;
+        if ((long long)(row + 1) * p.n <= rel) ++row;
+        return row;
+    };
+    // A border at y moves to the nearer end of its row where the row is short.
+    auto snap = [&](const Place& p, long long y, int most) {
+        if (p.n > most || p.n == 0) return y;
+        const long long at = p.off + (long long)row_of(p, y) * p.n;
+        return 2 * (y - at) < p.n ? at : at + p.n;
+    };
+    // CTAs that work: all, or as many as get kMinSub subtiles a warp
+    const int nC = N >= (long long)gridDim.x * kWarps * kMinSub ? (int)gridDim.x
+                                                                 : ((int)N + kWarps * kMinSub - 1) / (kWarps * kMinSub);
+    long long x0 = 0, x1 = 0, w0 = 0, w1 = 0;
+    Place at_w0 = {0, 0, 0};
+    if ((int)blockIdx.x < nC) {
+        const Split split(N, nC);
+        x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
+        x0 = snap(find(x0), x0, kSnapCta);
+        if (x1 < N) x1 = snap(find(x1), x1, kSnapCta);
+        const uint32_t len = (uint32_t)(x1 - x0), each = len / kWarps, more = len - each * kWarps;
+        w0 = x0 + each * warp + min((uint32_t)warp, more);
+        w1 = x0 + each * (warp + 1) + min((uint32_t)warp + 1, more);
+        if (w0 < N) {
+            at_w0 = find(w0);
+            w0 = snap(at_w0, w0, kSnapWarp);
+        }
+        if (w1 < N) w1 = snap(find(w1), w1, kSnapWarp);
     }
     // requests without a token, dealt over the CTAs: zeros, -inf
 #pragma unroll 1
@@ -321,8 +355,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     if (x0 == x1) return;
 
     // ---- this warp's stretch
-    const long long w0 = warp_start(warp);
-    const int count = (int)(warp_start(warp + 1) - w0);
+    const int count = (int)(w1 - w0);
     uint8_t* const ring = smem + warp * C::kWarpSmem;
     const uint32_t ring_u = smem_u32(ring);
     // a stage: key rows, value rows, int8 scales (16 of keys, 16 of values), meta
@@ -491,13 +524,15 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     };
 
     if (count > 0) {
-        f_b = my_b;
+        f_b = at_w0.b;
         fs = span_of(a, f_b);
-        const long long rel = w0 - my_off;
-        int row = (int)__fdividef((float)rel, (float)fs.n);   // off by one at most
-        if ((long long)row * fs.n > rel) --row;
-        if ((long long)(row + 1) * fs.n <= rel) ++row;
-        f_sub = (int)(rel - (long long)row * fs.n);
+        int row = row_of(at_w0, w0);   // R when the border moved to the request's end
+        f_sub = (int)(w0 - at_w0.off - (long long)row * fs.n);
+        if (row == R) {
+            row = 0;
+            do fs = span_of(a, ++f_b);
+            while (fs.n == 0);
+        }
         f_kvh = a.hb == 1 ? row : row / a.hb;
         f_blk = row - f_kvh * a.hb;
         look_up();
@@ -715,7 +750,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     int ctas = 0;
                     if (start >= 0) {
                         // the row's first CTA keeps its counter: a CTA is the first of one crossing row at most
-                        const Split split(N, nC_of(N));
+                        const Split split(N, nC);
                         const int c = tid ? blockIdx.x : split.owner(start);
                         ctas = split.owner(start + s_n[tid ? id1 : id0] - 1) - c + 1;
                         if (take_ticket(a.counters + c) == ctas - 1) a.counters[c] = 0;

@@ -194,17 +194,6 @@ __device__ __forceinline__ int take_ticket(int* counter) {
     return old;
 }
 
-// A load, from shared memory or the workspace, that sees what other SMs wrote.
-template <typename T>
-__device__ __forceinline__ T load_l2(const float* p) {
-    T v;
-    if constexpr (sizeof(T) == 16)
-        asm volatile("ld.relaxed.gpu.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
-    else
-        asm volatile("ld.relaxed.gpu.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
-    return v;
-}
-
 // Two heads' 1/l; with `write`, lanes of the first row write their lse.
 __device__ __forceinline__ void finish(const Args& a, int64_t head0, int left, int nt, const float* m, const float* l,
                                        bool write, float* inv) {
@@ -226,11 +215,15 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     constexpr float kUp = kPF16 ? 8.f : 0.f;
     extern __shared__ __align__(16) uint8_t smem[];   // [kWarps][kWarpSmem]
     __shared__ long long s_scan[kWarps], s_from[32 * kWarps], s_start[2 * kWarps];   // s_start < 0: no part
-    __shared__ int s_cnt[32 * kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
+    __shared__ int s_list[kWarps][32], s_cnt[32 * kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
     const int R = a.Hkv * a.hb;          // rows of a request
+
+    // A programmatic dependent launch: everything before this overlaps the kernel before; its writes are seen after.
+    pdl_wait_primary();
+    pdl_launch_dependents();
 
     // ---- the line: total length, this CTA's stretch and this warp's
     if (lane < 2) s_start[2 * warp + lane] = -1;
@@ -332,16 +325,23 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     if ((int)blockIdx.x < nC) {
         const Split split(N, nC);
         x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
-        x0 = snap(find(x0), x0, kSnapCta);
-        if (x1 < N) x1 = snap(find(x1), x1, kSnapCta);
-        const uint32_t len = (uint32_t)(x1 - x0), each = len / kWarps, more = len - each * kWarps;
-        w0 = x0 + each * warp + min((uint32_t)warp, more);
-        w1 = x0 + each * (warp + 1) + min((uint32_t)warp + 1, more);
-        if (w0 < N) {
-            at_w0 = find(w0);
-            w0 = snap(at_w0, w0, kSnapWarp);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {   // x1, x0, w1, w0 (one copy of the code: most of a small call is fetching it)
+            if (i == 2) {
+                const uint32_t len = (uint32_t)(x1 - x0), each = len / kWarps, more = len - each * kWarps;
+                w0 = x0 + each * warp + min((uint32_t)warp, more);
+                w1 = x0 + each * (warp + 1) + min((uint32_t)warp + 1, more);
+            }
+            long long y = i == 0 ? x1 : i == 1 ? x0 : i == 2 ? w1 : w0;
+            if (y < N) {
+                at_w0 = find(y);
+                y = snap(at_w0, y, i < 2 ? kSnapCta : kSnapWarp);
+            }
+            if (i == 0) x1 = y;
+            else if (i == 1) x0 = y;
+            else if (i == 2) w1 = y;
+            else w0 = y;
         }
-        if (w1 < N) w1 = snap(find(w1), w1, kSnapWarp);
     }
     // requests without a token, dealt over the CTAs: zeros, -inf
 #pragma unroll 1
@@ -545,14 +545,13 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             cp_async_wait<S - 2>();
             __syncwarp();
         }
-        const int to = it < 0 ? it + S - 1 : slot == 0 ? S - 1 : slot - 1;
-        fill(to);
         const uint32_t st = ring_u + slot * C::kStage;
         Meta meta;
         if (it < 0) meta.b = first_b, meta.row = first_row, meta.sub = it == 1 - S ? 0 : 1;
         else meta = *reinterpret_cast<const Meta*>(ring + slot * C::kStage + kM);
-        // a row's queries: the first row's while its first keys come
+        // a row's queries (the first row's before anything else is asked for)
         if (meta.sub == 0 && it != 0 && count > 0) load_q(meta.b, meta.row);
+        fill(it < 0 ? it + S - 1 : slot == 0 ? S - 1 : slot - 1);
         if (it < 0) continue;
         began |= meta.sub == 0;
         // scores, in two chains
@@ -722,23 +721,26 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     __syncthreads();
 
     // ---- join parts.  First the CTA's, row by row; lane i looks at part i: warp i/2's first (even) or last (odd).  Then,
-    // if this CTA is the last of a row's to file its part, the row's.  The units (16 x 8 fragments) of a row are dealt
-    // over the warps.
+    // if this CTA is the last of a row's to file its part, the row's, copied to shared memory.  The units (16 x 8
+    // fragments) of a row are dealt over the warps.
     const long long my_start = lane < 2 * kWarps ? s_start[lane] : -1;
     uint32_t todo = __ballot_sync(0xffffffffu, my_start >= 0);
     long long cross0 = -1, cross1 = -1;   // the row that came from an earlier CTA, the one that goes on into the next
-    int id0 = 0, id1 = 0, turn = warp, ended = -1;
+    int id0 = 0, id1 = 0, turn = warp, ended = -1, done = 0;
+    constexpr int kRoom = kWarps * C::kWarpSmem / (kPiece * 4) < 32 ? kWarps * C::kWarpSmem / (kPiece * 4) : 32;
 #pragma unroll 1
     while (true) {
-        int id, n, c0 = 0;          // one of the row's parts here; how many parts, and the first CTA when they are CTAs'
-        uint32_t parts = 0;         // the parts in shared memory
-        float* to = nullptr;        // a piece in the workspace, or the output
+        int id, n;              // one of the row's parts here; how many parts to join: s_list[warp][0 .. n-1], bytes
+        float* to = nullptr;    // a piece in the workspace or in shared memory, or the output
         if (todo) {
             id = __ffs(todo) - 1;
             const long long start = __shfl_sync(0xffffffffu, my_start, id);
-            parts = __ballot_sync(0xffffffffu, my_start == start);
+            const uint32_t parts = __ballot_sync(0xffffffffu, my_start == start);
             todo &= ~parts;
             n = __popc(parts);
+            __syncwarp();
+            if ((parts >> lane) & 1)
+                s_list[warp][__popc(parts & ((1u << lane) - 1))] = (lane >> 1) * C::kWarpSmem + (lane & 1 ? 0 : C::kRing);
             if (start < x0) cross0 = start, id0 = id, to = cta_pieces;
             else if (start + s_n[id] > x1) cross1 = start, id1 = id, to = cta_pieces + kPiece;
         } else {
@@ -760,92 +762,70 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     s_ctas[tid] = ctas;
                 }
                 __syncthreads();
+                ended = 0;
             }
-            if (++ended == 2) return;
-            n = s_ctas[ended], c0 = s_first[ended], id = ended ? id1 : id0;
-            if (n == 0) continue;
-            turn = warp;
-            if (n > 32) {
-                // many CTAs: every warp gathers some of them, then the warps' sums are joined
-                const int from = n * warp / kWarps, end = n * (warp + 1) / kWarps;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
-                    l_run[nt][0] = l_run[nt][1] = 0.f;
-#pragma unroll
-                    for (int mt = 0; mt < kMt; ++mt) acc[nt][mt][0] = acc[nt][mt][1] = acc[nt][mt][2] = acc[nt][mt][3] = 0.f;
-                }
+            if (ended < 2 && done == s_ctas[ended]) {
+                ++ended, done = 0;
+                if (ended < 2 && s_ctas[ended] == 0) ++ended;
+            }
+            if (ended == 2) return;
+            const int ctas = s_ctas[ended], c0 = s_first[ended], carry = done > 0;
+            id = ended ? id1 : id0;
+            // kRoom parts at a time, with what came of the earlier ones (in place 0 or 1 by turns) as the first
+            const int take = min(ctas - done, kRoom - 2);
+            __syncthreads();
 #pragma unroll 1
-                for (int i = from; i < end; ++i) {
-                    const float* src = a.pieces + ((int64_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPiece;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const float* ml = src + NT * 8 * DB + nt * 16 + 2 * t4;
-                        const float2 x = load_l2<float2>(ml), y = load_l2<float2>(ml + 8);
-                        float4 z[kMt];
-#pragma unroll
-                        for (int mt = 0; mt < kMt; ++mt) z[mt] = load_l2<float4>(src + ((nt * kMt + mt) * 32 + lane) * 4);
-                        const float pm[2] = {x.x, x.y}, pl[2] = {y.x, y.y};
-                        float s0[2], s1[2];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const float top = fmaxf(m_ref[nt][j], pm[j]), ref = fmaxf(top, -3.0e38f);
-                            s0[j] = ex2(m_ref[nt][j] - ref), s1[j] = ex2(pm[j] - ref);
-                            m_ref[nt][j] = top;
-                            l_run[nt][j] = l_run[nt][j] * s0[j] + pl[j] * s1[j];
-                        }
-#pragma unroll
-                        for (int mt = 0; mt < kMt; ++mt) {
-                            acc[nt][mt][0] = acc[nt][mt][0] * s0[0] + z[mt].x * s1[0];
-                            acc[nt][mt][1] = acc[nt][mt][1] * s0[1] + z[mt].y * s1[1];
-                            acc[nt][mt][2] = acc[nt][mt][2] * s0[0] + z[mt].z * s1[0];
-                            acc[nt][mt][3] = acc[nt][mt][3] * s0[1] + z[mt].w * s1[1];
-                        }
-                    }
-                }
-                __syncthreads();   // the parts in shared memory are used up
-                file_piece(reinterpret_cast<float*>(ring));
-                __syncthreads();
-                n = kWarps, parts = 0xaaaaaaaau >> (32 - 2 * kWarps);
+            for (int i = tid; i < take * (kPiece / 4); i += 32 * kWarps) {
+                const int p = i / (kPiece / 4), r = i - p * (kPiece / 4), c = done + p;
+                // the first CTA filed the row as its slot 1, the others as their slot 0
+                cp_async16_all(smem_u32(smem) + ((p + 2) * (kPiece / 4) + r) * 16,
+                               a.pieces + ((int64_t)(c0 + c) * 2 + (c == 0 ? 1 : 0)) * kPiece + r * 4);
             }
+            const int round = done / (kRoom - 2);
+            done += take;
+            n = take + carry;
+            __syncwarp();
+            if (lane < n) s_list[warp][lane] = (carry && lane == 0 ? (round & 1) : lane - carry + 2) * kPiece * 4;
+            if (done < ctas) to = reinterpret_cast<float*>(smem + ((round + 1) & 1) * kPiece * 4);
+            turn = warp;
+            cp_async_commit();
+            cp_async_wait<0>();
+            __syncthreads();
         }
+        __syncwarp();
         const int req = s_req[id], row = s_row[id];
 #pragma unroll 1
         for (; turn < kUnits; turn += kWarps) {
             const int u = turn, nt = u / kMt, mt = u - nt * kMt, ml = NT * 8 * DB + nt * 16 + 2 * t4;
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
-            constexpr int kBatch = 8;
-            uint32_t next = parts;
 #pragma unroll 1
-            for (int i = 0; i < n; i += kBatch) {
-                float4 z[kBatch];
-                float2 x[kBatch], y[kBatch];
+            for (int i = 0; i < n; i += 8) {   // eight parts: lane (g, t) looks at part g's m and l of its two heads
+                const bool in = i + g < n;
+                const float* src = reinterpret_cast<const float*>(smem + s_list[warp][in ? i + g : 0]);
+                const float2 x = in ? *reinterpret_cast<const float2*>(src + ml) : make_float2(-INFINITY, -INFINITY);
+                const float2 y = in ? *reinterpret_cast<const float2*>(src + ml + 8) : make_float2(0.f, 0.f);
+                const float px[2] = {x.x, x.y}, py[2] = {y.x, y.y};
+                float w[2];
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    x[k] = make_float2(-INFINITY, -INFINITY), y[k] = make_float2(0.f, 0.f), z[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (i + k < n) {
-                        const float* src;
-                        if (parts) {
-                            const int p = __ffs(next) - 1;
-                            next &= next - 1;
-                            src = reinterpret_cast<const float*>(smem + (p >> 1) * C::kWarpSmem + (p & 1 ? 0 : C::kRing));
-                        } else {   // the first CTA filed the row as its slot 1, the others as their slot 0
-                            src = a.pieces + ((int64_t)(c0 + i + k) * 2 + (i + k == 0 ? 1 : 0)) * kPiece;
-                        }
-                        x[k] = load_l2<float2>(src + ml), y[k] = load_l2<float2>(src + ml + 8);
-                        z[k] = load_l2<float4>(src + (u * 32 + lane) * 4);
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    float top = fmaxf(px[j], __shfl_xor_sync(0xffffffffu, px[j], 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), m[j]);
+                    const float ref = fmaxf(top, -3.0e38f), keep = ex2(m[j] - ref);
+                    m[j] = top;
+                    w[j] = ex2(px[j] - ref);
+                    float sum = py[j] * w[j];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                    l[j] = l[j] * keep + sum;
+                    o[j] *= keep, o[j + 2] *= keep;
                 }
-                float t0 = m[0], t1 = m[1];
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) t0 = fmaxf(t0, x[k].x), t1 = fmaxf(t1, x[k].y);
-                const float r0 = fmaxf(t0, -3.0e38f), r1 = fmaxf(t1, -3.0e38f), k0 = ex2(m[0] - r0), k1 = ex2(m[1] - r1);
-                l[0] *= k0, o[0] *= k0, o[2] *= k0, l[1] *= k1, o[1] *= k1, o[3] *= k1, m[0] = t0, m[1] = t1;
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    const float s0 = ex2(x[k].x - r0), s1 = ex2(x[k].y - r1);
-                    l[0] += y[k].x * s0, l[1] += y[k].y * s1;
-                    o[0] += z[k].x * s0, o[1] += z[k].y * s1, o[2] += z[k].z * s0, o[3] += z[k].w * s1;
+                for (int k = 0; k < 8; ++k) {   // past the last part: the first one, with weight 0
+                    const float4 z = *reinterpret_cast<const float4*>(smem + s_list[warp][i + k < n ? i + k : 0] + (u * 32 + lane) * 16);
+                    const float w0 = __shfl_sync(0xffffffffu, w[0], 4 * k + t4), w1 = __shfl_sync(0xffffffffu, w[1], 4 * k + t4);
+                    o[0] += z.x * w0, o[1] += z.y * w1, o[2] += z.z * w0, o[3] += z.w * w1;
                 }
             }
             if (to) {
@@ -883,8 +863,7 @@ int launch(const Args& a, int ctas, cudaStream_t st) {
             return set_error(WS_ERR_CUDA, "paged_decode: shared memory");
         set_for = dev;
     }
-    decode_kernel<F16, I8, DB, NT><<<ctas, 32 * C::kWarps, kSmem, st>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_dependent(decode_kernel<F16, I8, DB, NT>, dim3(ctas), 32 * C::kWarps, kSmem, st, a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }
 

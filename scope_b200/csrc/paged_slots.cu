@@ -104,6 +104,8 @@ paged_slots_kernel(const int32_t* seq_lens, const int32_t* __restrict__ new_lens
     int* base = sm + 2 * B;   // first ring place (counted from the head) of b's new pages
     int* first = sm + 3 * B;  // first token of b in the packed step
     if (threadIdx.x == 0) n_refused = 0;
+    pdl_wait_primary();
+    pdl_launch_dependents();
     const int head = ring[0], n_free = min(max(ring[1], 0), n_ring);
     long long tokens = 0, pages = 0, took = 0;
     int refused = 0;
@@ -188,6 +190,8 @@ paged_release_kernel(const int32_t* seq_lens, const uint8_t* __restrict__ done, 
     extern __shared__ int sm[];
     __shared__ BlockScan sh;
     int* end = sm;   // pages of requests 0 .. b that go back
+    pdl_wait_primary();
+    pdl_launch_dependents();
     const int head = ring[0], n_free = min(max(ring[1], 0), n_ring);
     const int room = n_ring - n_free;
     long long pages = 0;
@@ -232,8 +236,7 @@ int checked(const char* what, int B, int max_pages, int64_t table_stride, int n_
 // CTAs of up to kThreads threads, as many as the requests or the CTA's tokens can use.
 int block_threads(int64_t n) { return (int)std::min<int64_t>(kThreads, std::max<int64_t>(128, (n + 31) / 32 * 32)); }
 
-int launch_status() {
-    const cudaError_t e = cudaGetLastError();
+int launch_status(cudaError_t e) {
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }
 
@@ -268,10 +271,10 @@ int ws_paged_slots(const int32_t* seq_lens, const int32_t* new_lens, int B, int3
     }
     const int64_t ctas = std::max<int64_t>(1, (n_tokens + kTokensPerCta - 1) / kTokensPerCta);
     const int threads = block_threads(std::max<int64_t>(B, std::min<int64_t>(n_tokens, kTokensPerCta)));
-    paged_slots_kernel<<<(unsigned)ctas, threads, smem, static_cast<cudaStream_t>(stream)>>>(
+    return launch_status(launch_dependent(
+        paged_slots_kernel, dim3((unsigned)ctas), threads, smem, static_cast<cudaStream_t>(stream),
         seq_lens, new_lens, B, page_table, table_stride, max_pages, free_pages, n_ring, ring, page_size, n_tokens, slots,
-        positions, cu_new, seq_lens_out, ring_out, static_cast<int*>(workspace));
-    return launch_status();
+        positions, cu_new, seq_lens_out, ring_out, static_cast<int*>(workspace)));
 }
 
 int ws_paged_release(const int32_t* seq_lens, const uint8_t* done, int B, const int32_t* page_table,
@@ -287,10 +290,10 @@ int ws_paged_release(const int32_t* seq_lens, const uint8_t* done, int B, const 
     const int threads = block_threads(std::max<int64_t>(B, most));
     const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(device_sm_count(), most / (8 * kThreads)));
     const size_t smem = (size_t)std::max(B, 1) * 4;   // 32 KB at most
-    paged_release_kernel<<<(unsigned)ctas, threads, smem, static_cast<cudaStream_t>(stream)>>>(
+    return launch_status(launch_dependent(
+        paged_release_kernel, dim3((unsigned)ctas), threads, smem, static_cast<cudaStream_t>(stream),
         seq_lens, done, B, page_table, table_stride, max_pages, free_pages, n_ring, ring, page_size, seq_lens_out,
-        ring_out, static_cast<int*>(workspace), device_status_word());
-    return launch_status();
+        ring_out, static_cast<int*>(workspace), device_status_word()));
 }
 
 }  // extern "C"

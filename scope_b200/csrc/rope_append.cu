@@ -88,6 +88,8 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
 // F16: fp16 inputs (else bf16); I8: the pool holds int8 codes; VEC: q, k, v and q_out are 16-byte aligned throughout.
 template <bool F16, bool I8, bool VEC>
 __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_constant__ RopeAppendArgs a) {
+    pdl_wait_primary();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int64_t t = item / a.parts;
@@ -322,7 +324,6 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
                         : (vec ? rope_append_kernel<true, false, true> : rope_append_kernel<true, false, false>))
                   : (i8 ? (vec ? rope_append_kernel<false, true, true> : rope_append_kernel<false, true, false>)
                         : (vec ? rope_append_kernel<false, false, true> : rope_append_kernel<false, false, false>));
-    fn<<<(unsigned)blocks, 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_dependent(fn, dim3((unsigned)blocks), 32 * kWarps, 0, static_cast<cudaStream_t>(stream), a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -82,8 +82,23 @@ int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q
     a.status = device_status_word();
     const int ctas = device_sm_count();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (f16) return i8 ? paged::launch_f16_i8(a, DB, NT, ctas, st) : paged::launch_f16(a, DB, NT, ctas, st);
-    return i8 ? paged::launch_bf16_i8(a, DB, NT, ctas, st) : paged::launch_bf16(a, DB, NT, ctas, st);
+    // The kernel counts subtiles in 32 bits: more requests at once than that holds, were every row of the table full,
+    // go in several launches.
+    const int64_t most = (std::min<int64_t>(a.cap, window > 0 ? (int64_t)window + paged::kTok : a.cap) / paged::kTok + 1) *
+                         kv->Hkv * a.hb;
+    if (most > INT32_MAX / 2) return set_error(WS_ERR_UNSUPPORTED, "paged_decode: too many tokens times kv heads in one request");
+    const int at_once = (int)std::min<int64_t>(B, INT32_MAX / 2 / most);
+    for (int b = 0; b < B; b += at_once) {
+        paged::Args c = a;
+        c.B = std::min(at_once, B - b);
+        c.q += b * q_stride_b, c.table += b * table_stride, c.seq_lens += b;
+        c.out += (int64_t)b * kv->Hkv * G * kv->Dv;
+        if (c.lse) c.lse += (int64_t)b * kv->Hkv * G;
+        const int rc = f16 ? (i8 ? paged::launch_f16_i8(c, DB, NT, ctas, st) : paged::launch_f16(c, DB, NT, ctas, st))
+                           : (i8 ? paged::launch_bf16_i8(c, DB, NT, ctas, st) : paged::launch_bf16(c, DB, NT, ctas, st));
+        if (rc != WS_OK) return rc;
+    }
+    return WS_OK;
 }
 
 }  // extern "C"

@@ -169,18 +169,16 @@ __device__ __forceinline__ Span span_of(const Args& a, int b) {
 
 // An even split of a line of N places over n CTAs: the first `more` take one place more than `each`.
 struct Split {
-    long long each, more;
+    int each, more;
     float inv;
-    __device__ __forceinline__ Split(long long N, int n) {
-        // N / n in two steps of 32 bits: N < 2^48, n < 2^16
-        const uint32_t hi = (uint32_t)(N >> 16), q = hi / (uint32_t)n;
-        each = ((long long)q << 16) + (((hi - q * n) << 16) | (uint32_t)(N & 0xffff)) / (uint32_t)n;
+    __device__ __forceinline__ Split(int N, int n) {
+        each = (uint32_t)N / (uint32_t)n;
         more = N - each * n;
         inv = __fdividef(n, (float)N);
     }
-    __device__ __forceinline__ long long start(int c) const { return c * each + min((long long)c, more); }
+    __device__ __forceinline__ int start(int c) const { return c * each + min(c, more); }
     // The CTA that holds place t: a guess in fp32, which is off by one at most, and the starts beside it.
-    __device__ __forceinline__ int owner(long long t) const {
+    __device__ __forceinline__ int owner(int t) const {
         int c = (int)((float)t * inv);
         while (c > 0 && start(c) > t) --c;
         while (start(c + 1) <= t) ++c;
@@ -214,7 +212,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
     constexpr float kUp = kPF16 ? 8.f : 0.f;
     extern __shared__ __align__(16) uint8_t smem[];   // [kWarps][kWarpSmem]
-    __shared__ long long s_scan[kWarps], s_from[32 * kWarps], s_start[2 * kWarps];   // s_start < 0: no part
+    __shared__ int s_scan[kWarps], s_from[32 * kWarps], s_start[2 * kWarps];   // s_start < 0: no part
     __shared__ int s_list[kWarps][32], s_cnt[32 * kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -225,13 +223,13 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     pdl_wait_primary();
     pdl_launch_dependents();
 
-    // ---- the line: total length, this CTA's stretch and this warp's
+    // ---- the line (shorter than 2^31 places): its length, this CTA's stretch and this warp's
     if (lane < 2) s_start[2 * warp + lane] = -1;
-    long long N;
+    int N;
     const int per = a.B <= 32 ? 1 : (a.B + kWarps * 32 - 1) / (kWarps * 32);   // requests a lane, or a thread, looks at
-    long long my_from = 0, my_to = 0;   // up to 32 requests: where this lane's request lies
-    int my_n = 0;                       // (with one request each) its subtiles a row
-    if (a.B <= 32) {   // every warp for itself
+    int my_from = 0, my_to = 0;   // up to 32 requests: where this lane's request lies
+    int my_n = 0;                 // (with one request each) its subtiles a row
+    if (a.B <= 32) {              // every warp for itself
         my_n = lane < a.B ? span_of(a, lane).n : 0;
         my_to = my_n;
     } else {
@@ -242,7 +240,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     my_from = my_to;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, my_to, o);
+        const int y = __shfl_up_sync(0xffffffffu, my_to, o);
         if (lane >= o) my_to += y;
     }
     my_from = (my_to - my_from) * R, my_to *= R;
@@ -251,7 +249,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     } else {
         if (lane == 31) s_scan[warp] = my_to;
         __syncthreads();
-        long long before = 0;
+        int before = 0;
         N = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
@@ -262,86 +260,72 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         s_cnt[tid] = my_n;
         __syncthreads();
     }
-    // The request that holds place y < N, its first place and a row's subtiles.
-    struct Place {
-        int b, n;
-        long long off;
+    // A border at place y: where it goes, and the row that begins or goes on there.  In a short row (of up to `most`
+    // subtiles) it moves to the row's nearer end.
+    struct Border {
+        int y, b, row, sub;   // row: R at the request's end
     };
-    auto find = [&](long long y) {
-        Place p;
+    auto border = [&](int y, int most) {
+        if (y >= N) return Border{y, 0, 0, 0};   // the line's end
+        int b = 0, from = my_from, n = my_n;
+        if (a.B <= 32) {
+            b = lane;   // the lane whose request holds y knows best
+        } else {
+            // the last thread whose requests begin at or before y: its group of kWarps threads, then itself
+            const int group = (__popc(__ballot_sync(0xffffffffu, s_from[lane * kWarps] <= y)) - 1) * kWarps;
+            const int c = group + __popc(__ballot_sync(0xffffffffu, lane < kWarps && s_from[group + lane % kWarps] <= y)) - 1;
+            b = c * per, from = s_from[c], n = s_cnt[c];
+            while (per > 1) {   // and the one of them that holds it, 32 at a time
+                const int i = b + lane, k = i < min((c + 1) * per, a.B) ? span_of(a, i).n : 0;
+                int to = k;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, to, o);
+                    if (lane >= o) to += x;
+                }
+                to = from + to * R;
+                const uint32_t here = __ballot_sync(0xffffffffu, y < to && k > 0);
+                if (here || b + 32 >= (c + 1) * per) {
+                    const int src = here ? __ffs(here) - 1 : 0;
+                    b += src;
+                    n = __shfl_sync(0xffffffffu, k, src);
+                    from = __shfl_sync(0xffffffffu, to - k * R, src);
+                    break;
+                }
+                b += 32, from = __shfl_sync(0xffffffffu, to, 31);
+            }
+        }
+        Border r = {y, b, 0, 0};
+        if (n > 0) {
+            const int rel = y - from;
+            r.row = (int)__fdividef((float)rel, (float)n);   // off by one at most
+            r.sub = rel - r.row * n;
+            if (r.sub < 0) --r.row, r.sub += n;
+            if (r.sub >= n) ++r.row, r.sub -= n;
+            if (n <= most && r.sub > 0) {
+                if (2 * r.sub < n) r.y -= r.sub;
+                else r.y += n - r.sub, ++r.row;
+                r.sub = 0;
+            }
+        }
         if (a.B <= 32) {
             const uint32_t here = __ballot_sync(0xffffffffu, y >= my_from && y < my_to);
-            p.b = here ? __ffs(here) - 1 : 0;
-            p.n = __shfl_sync(0xffffffffu, my_n, p.b);
-            p.off = __shfl_sync(0xffffffffu, my_from, p.b);
-            return p;
+            const int src = __ffs(here) - 1;
+            r.y = __shfl_sync(0xffffffffu, r.y, src), r.row = __shfl_sync(0xffffffffu, r.row, src);
+            r.sub = __shfl_sync(0xffffffffu, r.sub, src), r.b = src;
         }
-        // the last thread whose requests begin at or before y: its group of kWarps threads, then itself
-        const int group = (__popc(__ballot_sync(0xffffffffu, s_from[lane * kWarps] <= y)) - 1) * kWarps;
-        const int c = group + __popc(__ballot_sync(0xffffffffu, lane < kWarps && s_from[group + lane % kWarps] <= y)) - 1;
-        p.b = c * per, p.off = s_from[c];
-        if (per == 1) {
-            p.n = s_cnt[c];
-            return p;
-        }
-        while (true) {   // and the one of them that holds it, 32 at a time
-            const int b = p.b + lane, n = b < min((c + 1) * per, a.B) ? span_of(a, b).n : 0;
-            long long to = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, to, o);
-                if (lane >= o) to += x;
-            }
-            to = p.off + to * R;
-            const uint32_t here = __ballot_sync(0xffffffffu, y < to && n > 0);
-            if (here || p.b + 32 >= (c + 1) * per) {
-                const int src = here ? __ffs(here) - 1 : 0;
-                p.b += src;
-                p.n = __shfl_sync(0xffffffffu, n, src);
-                p.off = __shfl_sync(0xffffffffu, to - (long long)n * R, src);
-                return p;
-            }
-            p.b += 32, p.off = __shfl_sync(0xffffffffu, to, 31);
-        }
-    };
-    auto row_of = [&](const Place& p, long long y) {
-        const long long rel = y - p.off;
-        int row = (int)__fdividef((float)rel, (float)p.n);   // off by one at most
-        if ((long long)row * p.n > rel) --row;
-        if ((long long)(row + 1) * p.n <= rel) ++row;
-        return row;
-    };
-    // A border at y moves to the nearer end of its row where the row is short.
-    auto snap = [&](const Place& p, long long y, int most) {
-        if (p.n > most || p.n == 0) return y;
-        const long long at = p.off + (long long)row_of(p, y) * p.n;
-        return 2 * (y - at) < p.n ? at : at + p.n;
+        return r;
     };
     // CTAs that work: all, or as many as get kMinSub subtiles a warp
-    const int nC = N >= (long long)gridDim.x * kWarps * kMinSub ? (int)gridDim.x
-                                                                 : ((int)N + kWarps * kMinSub - 1) / (kWarps * kMinSub);
-    long long x0 = 0, x1 = 0, w0 = 0, w1 = 0;
-    Place at_w0 = {0, 0, 0};
+    const int nC = min((int)gridDim.x, (int)((uint32_t)(N + kWarps * kMinSub - 1) / (kWarps * kMinSub)));
+    int x0 = 0, x1 = 0, w0 = 0, w1 = 0;
+    Border first = {0, 0, 0, 0};
     if ((int)blockIdx.x < nC) {
         const Split split(N, nC);
-        x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {   // x1, x0, w1, w0 (one copy of the code: most of a small call is fetching it)
-            if (i == 2) {
-                const uint32_t len = (uint32_t)(x1 - x0), each = len / kWarps, more = len - each * kWarps;
-                w0 = x0 + each * warp + min((uint32_t)warp, more);
-                w1 = x0 + each * (warp + 1) + min((uint32_t)warp + 1, more);
-            }
-            long long y = i == 0 ? x1 : i == 1 ? x0 : i == 2 ? w1 : w0;
-            if (y < N) {
-                at_w0 = find(y);
-                y = snap(at_w0, y, i < 2 ? kSnapCta : kSnapWarp);
-            }
-            if (i == 0) x1 = y;
-            else if (i == 1) x0 = y;
-            else if (i == 2) w1 = y;
-            else w0 = y;
-        }
+        x0 = border(split.start(blockIdx.x), kSnapCta).y, x1 = border(split.start(blockIdx.x + 1), kSnapCta).y;
+        const int len = x1 - x0, each = (uint32_t)len / kWarps, more = len - each * kWarps;
+        first = border(x0 + each * warp + min(warp, more), kSnapWarp);
+        w0 = first.y, w1 = border(x0 + each * (warp + 1) + min(warp + 1, more), kSnapWarp).y;
     }
     // requests without a token, dealt over the CTAs: zeros, -inf
 #pragma unroll 1
@@ -355,7 +339,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     if (x0 == x1) return;
 
     // ---- this warp's stretch
-    const int count = (int)(w1 - w0);
+    const int count = w1 - w0;
     uint8_t* const ring = smem + warp * C::kWarpSmem;
     const uint32_t ring_u = smem_u32(ring);
     // a stage: key rows, value rows, int8 scales (16 of keys, 16 of values), meta
@@ -461,26 +445,57 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     auto head_of = [&](int b, int row) { return ((int64_t)b * a.Hkv + (row >> 16)) * a.G + (row & 0xffff) * 8 * NT; };
     auto left_of = [&](int row) { return a.G - (row & 0xffff) * 8 * NT; };
 
+    // A row's queries as they lie, 16 (int8 pools: 8) bytes a lane; order_q makes fragments of them once they are here.
     auto load_q = [&](int b, int row) {
         const int kvh = row >> 16, h0 = (row & 0xffff) * 8 * NT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int h = h0 + nt * 8 + g;
-            const uint16_t* q = a.q + b * a.q_b + ((int64_t)kvh * a.G + h) * a.q_h;
+            const uint16_t* q = a.q + b * a.q_b + ((int64_t)kvh * a.G + h) * a.q_h + (I8 ? 4 : 8) * t4;
+            if (I8) {
 #pragma unroll
-            for (int ks = 0; ks < DB / 16; ++ks) {
-                uint32_t x = 0, y = 0;
-                if (ks < nks && h < a.G) {
-                    if (I8) {   // the order in which s8_pair gives the dims: (0, 2), (1, 3) of each four
-                        const uint2 w = __ldg(reinterpret_cast<const uint2*>(q + 16 * ks + 4 * t4));
-                        x = __byte_perm(w.x, w.y, 0x5410);
-                        y = __byte_perm(w.x, w.y, 0x7632);
-                    } else {
-                        x = __ldg(reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * t4));
-                        y = __ldg(reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * t4 + 8));
-                    }
+                for (int ks = 0; ks < DB / 16; ++ks) {   // dims 16ks + 4t .. 4t + 3
+                    uint2 w = make_uint2(0, 0);
+                    if (ks < nks && h < a.G) w = __ldg(reinterpret_cast<const uint2*>(q + 16 * ks));
+                    bq[nt][ks][0] = w.x, bq[nt][ks][1] = w.y;
                 }
-                bq[nt][ks][0] = x, bq[nt][ks][1] = y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < DB / 32; ++i) {      // dims 32i + 8t .. 8t + 7
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (32 * i + 8 * t4 < a.Dk && h < a.G) w = __ldg(reinterpret_cast<const uint4*>(q + 32 * i));
+                    bq[nt][2 * i][0] = w.x, bq[nt][2 * i][1] = w.y, bq[nt][2 * i + 1][0] = w.z, bq[nt][2 * i + 1][1] = w.w;
+                }
+            }
+        }
+    };
+    auto order_q = [&]() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            if (I8) {   // the order in which s8_pair gives the dims: (0, 2), (1, 3) of each four
+#pragma unroll
+                for (int ks = 0; ks < DB / 16; ++ks) {
+                    const uint32_t x = bq[nt][ks][0], y = bq[nt][ks][1];
+                    bq[nt][ks][0] = __byte_perm(x, y, 0x5410), bq[nt][ks][1] = __byte_perm(x, y, 0x7632);
+                }
+            } else {    // word i of lane t to word t of lane i, within each four lanes: what ldmatrix gives of the keys
+#pragma unroll
+                for (int i = 0; i < DB / 16; i += 2) {
+                    uint32_t w[4] = {bq[nt][i][0], bq[nt][i][1], bq[nt][i + 1][0], bq[nt][i + 1][1]};
+#pragma unroll
+                    for (int o = 1; o <= 2; o <<= 1) {
+                        const bool up = t4 & o;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if (k & o) continue;
+                            const uint32_t mine = up ? w[k] : w[k + o];
+                            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, o);
+                            if (up) w[k] = other;
+                            else w[k + o] = other;
+                        }
+                    }
+                    bq[nt][i][0] = w[0], bq[nt][i][1] = w[1], bq[nt][i + 1][0] = w[2], bq[nt][i + 1][1] = w[3];
+                }
             }
             m_ref[nt][0] = m_ref[nt][1] = -INFINITY;
             l_run[nt][0] = l_run[nt][1] = 0.f;
@@ -524,10 +539,9 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     };
 
     if (count > 0) {
-        f_b = at_w0.b;
+        f_b = first.b, f_sub = first.sub;
         fs = span_of(a, f_b);
-        int row = row_of(at_w0, w0);   // R when the border moved to the request's end
-        f_sub = (int)(w0 - at_w0.off - (long long)row * fs.n);
+        int row = first.row;
         if (row == R) {
             row = 0;
             do fs = span_of(a, ++f_b);
@@ -553,7 +567,10 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         if (meta.sub == 0 && it != 0 && count > 0) load_q(meta.b, meta.row);
         fill(it < 0 ? it + S - 1 : slot == 0 ? S - 1 : slot - 1);
         if (it < 0) continue;
-        began |= meta.sub == 0;
+        if (it == 0 || meta.sub == 0) {
+            order_q();
+            began = meta.sub == 0;
+        }
         // scores, in two chains
         float c[NT][4], e[NT][4];
 #pragma unroll
@@ -723,9 +740,9 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     // ---- join parts.  First the CTA's, row by row; lane i looks at part i: warp i/2's first (even) or last (odd).  Then,
     // if this CTA is the last of a row's to file its part, the row's, copied to shared memory.  The units (16 x 8
     // fragments) of a row are dealt over the warps.
-    const long long my_start = lane < 2 * kWarps ? s_start[lane] : -1;
+    const int my_start = lane < 2 * kWarps ? s_start[lane] : -1;
     uint32_t todo = __ballot_sync(0xffffffffu, my_start >= 0);
-    long long cross0 = -1, cross1 = -1;   // the row that came from an earlier CTA, the one that goes on into the next
+    int cross0 = -1, cross1 = -1;   // the row that came from an earlier CTA, the one that goes on into the next
     int id0 = 0, id1 = 0, turn = warp, ended = -1, done = 0;
     constexpr int kRoom = kWarps * C::kWarpSmem / (kPiece * 4) < 32 ? kWarps * C::kWarpSmem / (kPiece * 4) : 32;
 #pragma unroll 1
@@ -734,7 +751,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         float* to = nullptr;    // a piece in the workspace or in shared memory, or the output
         if (todo) {
             id = __ffs(todo) - 1;
-            const long long start = __shfl_sync(0xffffffffu, my_start, id);
+            const int start = __shfl_sync(0xffffffffu, my_start, id);
             const uint32_t parts = __ballot_sync(0xffffffffu, my_start == start);
             todo &= ~parts;
             n = __popc(parts);
@@ -748,7 +765,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 if (cross0 < 0 && cross1 < 0) return;   // the same in every thread
                 __syncthreads();
                 if (tid < 2) {
-                    const long long start = tid ? cross1 : cross0;
+                    const int start = tid ? cross1 : cross0;
                     int ctas = 0;
                     if (start >= 0) {
                         // the row's first CTA keeps its counter: a CTA is the first of one crossing row at most

@@ -136,6 +136,13 @@ __device__ __forceinline__ float2 unpack16(uint32_t v) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
+// (r & m) ^ x in one instruction.
+__device__ __forceinline__ uint32_t and_xor(uint32_t r, uint32_t m, uint32_t x) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(d) : "r"(r), "r"(m), "r"(x));
+    return d;
+}
+
 // Bytes 0 and 2 of r, signed, as a pair of 16-bit floats, exactly, times s8_unit.  With the sign bit turned the byte is
 // u = value + 128.  fp16: 0x6400 is 1024 and holds all 8 bits below it, so 1024 + u - 1152 is the value.  bf16 holds 7
 // bits below a leading one, but the pattern 0x00uu is u 2^-133 over the whole byte, where subnormal numbers run on into
@@ -144,10 +151,10 @@ template <bool F16>
 __device__ __forceinline__ uint32_t s8_pair(uint32_t r) {
     uint32_t d;
     if (F16) {
-        const uint32_t x = (r & 0x00ff00ffu) ^ 0x64806480u;
+        const uint32_t x = and_xor(r, 0x00ff00ffu, 0x64806480u);
         asm("sub.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0x64806480u));
     } else {
-        const uint32_t x = (r & 0x00ff00ffu) ^ 0x00800080u;
+        const uint32_t x = and_xor(r, 0x00ff00ffu, 0x00800080u);
         asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0x7b807b80u), "r"(0xbc80bc80u));
     }
     return d;
@@ -204,7 +211,8 @@ __device__ __forceinline__ void finish(const Args& a, int64_t head0, int left, i
     }
 }
 
-template <bool F16, bool I8, int DB, int NT>
+// EXACT: Dk = Dv = DB, known when compiling: no bounds on the pieces of a row (360 instructions a subtile to 280).
+template <bool F16, bool I8, int DB, int NT, bool EXACT>
 __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
     using C = Cfg<I8, DB, NT>;
     constexpr int kWarps = C::kWarps, S = C::kStages, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
@@ -218,6 +226,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
     const int R = a.Hkv * a.hb;          // rows of a request
+    const int Dk = EXACT ? DB : a.Dk, Dv = EXACT ? DB : a.Dv;
 
     // A programmatic dependent launch: everything before this overlaps the kernel before; its writes are seen after.
     pdl_wait_primary();
@@ -332,8 +341,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
         if (span_of(a, b).n) continue;
         const int64_t head0 = (int64_t)b * a.Hkv * a.G;
-        for (int i = tid; i < a.Hkv * a.G * (a.Dv / 8); i += 32 * kWarps)
-            reinterpret_cast<uint4*>(a.out + head0 * a.Dv)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < a.Hkv * a.G * (Dv / 8); i += 32 * kWarps)
+            reinterpret_cast<uint4*>(a.out + head0 * Dv)[i] = make_uint4(0, 0, 0, 0);
         for (int i = tid; a.lse && i < a.Hkv * a.G; i += 32 * kWarps) a.lse[head0 + i] = -INFINITY;
     }
     if (x0 == x1) return;
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     int f_b = 0, f_kvh = 0, f_blk = 0, f_sub = 0, f_entry = -1, f_left = count;
     uint32_t f_off = 0;
     const int l8 = lane & 7, r4 = lane >> 3;   // copies: eight lanes a row, four rows at a time
-    const int kchunks = I8 ? a.Dk >> 4 : a.Dk >> 3, vchunks = I8 ? a.Dv >> 4 : a.Dv >> 3;
+    const int kchunks = I8 ? Dk >> 4 : Dk >> 3, vchunks = I8 ? Dv >> 4 : Dv >> 3;
     constexpr int kCols = (I8 ? DB / 16 : DB / 8) >= 8 ? (I8 ? DB / 16 : DB / 8) / 8 : 1;
     const uint64_t k_lane = (uint64_t)r4 * a.kt + l8, v_lane = (uint64_t)r4 * a.vt + l8;
 
@@ -439,7 +448,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     uint32_t bq[NT][DB / 16][2];
     bool began = false;                // the row's first subtile was this warp's
 
-    const int nks = a.Dk >> 4, nmt = a.Dv >> 4;
+    const int nks = Dk >> 4, nmt = Dv >> 4;
 
     // A row's first head of the block in the output, and how many of the kv head's heads are left from it.
     auto head_of = [&](int b, int row) { return ((int64_t)b * a.Hkv + (row >> 16)) * a.G + (row & 0xffff) * 8 * NT; };
@@ -463,7 +472,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                 for (int i = 0; i < DB / 32; ++i) {      // dims 32i + 8t .. 8t + 7
                     uint4 w = make_uint4(0, 0, 0, 0);
-                    if (32 * i + 8 * t4 < a.Dk && h < a.G) w = __ldg(reinterpret_cast<const uint4*>(q + 32 * i));
+                    if (32 * i + 8 * t4 < Dk && h < a.G) w = __ldg(reinterpret_cast<const uint4*>(q + 32 * i));
                     bq[nt][2 * i][0] = w.x, bq[nt][2 * i][1] = w.y, bq[nt][2 * i + 1][0] = w.z, bq[nt][2 * i + 1][1] = w.w;
                 }
             }
@@ -519,21 +528,21 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     };
     // One fragment of a finished row: O^T[16 dims x 8 heads], dims from 16mt.
     auto store_unit = [&](int64_t head0, int left, int nt, int mt, const float* o, const float* inv) {
-        uint16_t* base = a.out + head0 * a.Dv + 16 * mt;
+        uint16_t* base = a.out + head0 * Dv + 16 * mt;
         if (I8) {   // dims 2g and 2g + 1 of heads 2t, 2t + 1
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int h = nt * 8 + 2 * t4 + j;
                 if (h < left)
-                    *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 2 * g) = pack16<F16>(o[j] * inv[j], o[j + 2] * inv[j]);
+                    *reinterpret_cast<uint32_t*>(base + (int64_t)h * Dv + 2 * g) = pack16<F16>(o[j] * inv[j], o[j + 2] * inv[j]);
             }
         } else {    // dims g and g + 8; transposed, lane (g, t) gets head g, dims 2t, 2t + 1 and + 8
             const uint32_t lo = movmatrix_t(pack16<F16>(o[0] * inv[0], o[1] * inv[1]));
             const uint32_t hi = movmatrix_t(pack16<F16>(o[2] * inv[0], o[3] * inv[1]));
             const int h = nt * 8 + g;
             if (h < left) {
-                *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 2 * t4) = lo;
-                *reinterpret_cast<uint32_t*>(base + (int64_t)h * a.Dv + 8 + 2 * t4) = hi;
+                *reinterpret_cast<uint32_t*>(base + (int64_t)h * Dv + 2 * t4) = lo;
+                *reinterpret_cast<uint32_t*>(base + (int64_t)h * Dv + 8 + 2 * t4) = hi;
             }
         }
     };
@@ -867,7 +876,7 @@ int launch_f16(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 int launch_bf16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 int launch_f16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 
-template <bool F16, bool I8, int DB, int NT>
+template <bool F16, bool I8, int DB, int NT, bool EXACT>
 int launch(const Args& a, int ctas, cudaStream_t st) {
     using C = Cfg<I8, DB, NT>;
     constexpr int kSmem = C::kWarps * C::kWarpSmem;
@@ -875,20 +884,25 @@ int launch(const Args& a, int ctas, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (set_for != dev) {
-        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
+        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
             cudaSuccess)
             return set_error(WS_ERR_CUDA, "paged_decode: shared memory");
         set_for = dev;
     }
-    const cudaError_t e = launch_dependent(decode_kernel<F16, I8, DB, NT>, dim3(ctas), 32 * C::kWarps, kSmem, st, a);
+    const cudaError_t e = launch_dependent(decode_kernel<F16, I8, DB, NT, EXACT>, dim3(ctas), 32 * C::kWarps, kSmem, st, a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
+}
+
+template <bool F16, bool I8, int DB, int NT>
+int launch_dims(const Args& a, int ctas, cudaStream_t st) {
+    return a.Dk == DB && a.Dv == DB ? launch<F16, I8, DB, NT, true>(a, ctas, st) : launch<F16, I8, DB, NT, false>(a, ctas, st);
 }
 
 template <bool F16, bool I8>
 int launch_any(const Args& a, int DB, int NT, int ctas, cudaStream_t st) {
-    if (DB == 64) return NT == 1 ? launch<F16, I8, 64, 1>(a, ctas, st) : launch<F16, I8, 64, 2>(a, ctas, st);
-    if (DB == 128) return NT == 1 ? launch<F16, I8, 128, 1>(a, ctas, st) : launch<F16, I8, 128, 2>(a, ctas, st);
-    return launch<F16, I8, 256, 1>(a, ctas, st);
+    if (DB == 64) return NT == 1 ? launch_dims<F16, I8, 64, 1>(a, ctas, st) : launch_dims<F16, I8, 64, 2>(a, ctas, st);
+    if (DB == 128) return NT == 1 ? launch_dims<F16, I8, 128, 1>(a, ctas, st) : launch_dims<F16, I8, 128, 2>(a, ctas, st);
+    return launch_dims<F16, I8, 256, 1>(a, ctas, st);
 }
 
 }  // namespace paged

@@ -57,17 +57,20 @@ int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q
     const int64_t strides[6] = {kv->k_stride_page, kv->k_stride_tok, kv->k_stride_head,
                                 kv->v_stride_page, kv->v_stride_tok, kv->v_stride_head};
     uint32_t* const pieces[6] = {&a.kp, &a.kt, &a.kh, &a.vp, &a.vt, &a.vh};
+    const int64_t scale_strides[6] = {kv->ks_stride_page, kv->ks_stride_tok, kv->ks_stride_head,
+                                      kv->vs_stride_page, kv->vs_stride_tok, kv->vs_stride_head};
+    uint32_t* const floats[6] = {&a.ksp, &a.kst, &a.ksh, &a.vsp, &a.vst, &a.vsh};
     for (int i = 0; i < 6; ++i) {
-        if (strides[i] * eb / 16 > UINT32_MAX) return set_error(WS_ERR_UNSUPPORTED, "paged_decode: a pool stride of 64 GB or more");
+        if (strides[i] * eb / 16 > UINT32_MAX || (i8 && (scale_strides[i] > UINT32_MAX || scale_strides[i] < 0)))
+            return set_error(WS_ERR_UNSUPPORTED, "paged_decode: a pool stride of 64 GB or more");
         *pieces[i] = (uint32_t)(strides[i] * eb / 16);
+        *floats[i] = i8 ? (uint32_t)scale_strides[i] : 0;
     }
     a.ks = kv->k_scales, a.vs = kv->v_scales;
-    a.ksp = kv->ks_stride_page, a.kst = kv->ks_stride_tok, a.ksh = kv->ks_stride_head;
-    a.vsp = kv->vs_stride_page, a.vst = kv->vs_stride_tok, a.vsh = kv->vs_stride_head;
     a.table = page_table, a.table_stride = table_stride;
     a.seq_lens = seq_lens;
     a.cap = (int)std::min<int64_t>((int64_t)max_pages * kv->page_size, INT32_MAX - 64);
-    a.whole = kv->page_size % paged::kTok == 0;
+    a.whole = kv->page_size % 16 == 0;
     a.n_pages = (int)kv->n_pages, a.page_size = kv->page_size;
     // t / page_size for t < 2^31 as a multiply and a shift: shift = ceil(log2 P), mul = floor(2^32 (2^shift - P) / P) + 1
     while ((1ull << a.div_shift) < (uint64_t)kv->page_size) ++a.div_shift;
@@ -84,7 +87,7 @@ int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // The kernel counts subtiles in 32 bits: more requests at once than that holds, were every row of the table full,
     // go in several launches.
-    const int64_t most = (std::min<int64_t>(a.cap, window > 0 ? (int64_t)window + paged::kTok : a.cap) / paged::kTok + 1) *
+    const int64_t most = (std::min<int64_t>(a.cap, window > 0 ? (int64_t)window + 32 : a.cap) / 16 + 1) *
                          kv->Hkv * a.hb;
     if (most > INT32_MAX / 2) return set_error(WS_ERR_UNSUPPORTED, "paged_decode: too many tokens times kv heads in one request");
     const int at_once = (int)std::min<int64_t>(B, INT32_MAX / 2 / most);

@@ -6,12 +6,12 @@
 // tile), against G multiply-adds a byte, so the design keeps enough bytes in flight on every SM for any mix of lengths,
 // at few instructions a byte:
 //
-//   * Rows (request, kv head, block of 8*NT query heads) are cut into subtiles of 16 tokens, laid end to end, and the
+//   * Rows (request, kv head, block of 8*NT query heads) are cut into subtiles of 16 or 32 tokens, laid end to end, and the
 //     line is split evenly over the CTAs (one a SM) and again over each CTA's warps.  Every warp runs alone over its
 //     stretch with its own ring of S stages filled by 16-byte cp.async, so no warp ever waits for another and a short
 //     row costs no barrier.  The lengths are read on the device; the host never needs them.
-//   * A subtile is one stage.  With pages of whole subtiles it has one page, and its rows lie at one stride; else each
-//     lane looks up one token's page and the row addresses travel by shuffle.  Entries are fetched a subtile ahead.
+//   * A subtile is one stage.  With pages of whole 16-token tiles a tile has one page, and its rows lie at one stride; else
+//     each lane looks up one token's page and the row addresses travel by shuffle.  Entries are fetched a subtile ahead.
 //     Tokens past the length, before the window or on a page that is none are not read: their shared-memory rows are
 //     zero and their scores -inf.
 //   * Rows in shared memory are an odd number of 16-byte pieces apart, so ldmatrix reads are free of bank conflicts for
@@ -36,12 +36,11 @@
 namespace ws {
 namespace paged {
 
-constexpr int kTok = 16;        // tokens of a subtile
-constexpr int kMinSub = 2;      // subtiles a warp takes before another CTA joins in
-// Rows up to so many subtiles are not cut by a border between two CTAs, or two warps: the border moves to the nearer end
+constexpr int kMinTok = 32;     // tokens a warp takes before another CTA joins in
+// Rows up to so many tokens are not cut by a border between two CTAs, or two warps: the border moves to the nearer end
 // of the row, which unbalances the stretches by half a row at most and saves the joining.
-constexpr int kSnapCta = 40;
-constexpr int kSnapWarp = 4;
+constexpr int kSnapCta = 640;
+constexpr int kSnapWarp = 64;
 constexpr float kSlack = 6.f;   // log2 of how far a probability may pass its bound before the reference moves
 
 struct Args {
@@ -52,12 +51,12 @@ struct Args {
     uint32_t kp, kt, kh, vp, vt, vh;     // strides in 16-byte pieces
     const float* ks;
     const float* vs;
-    int64_t ksp, kst, ksh, vsp, vst, vsh;
+    uint32_t ksp, kst, ksh, vsp, vst, vsh;   // floats
     const int32_t* table;
     int64_t table_stride;
     const int32_t* seq_lens;
     int cap;                             // max_pages * page_size, or less than 2^31
-    int whole;                           // page_size is a multiple of kTok
+    int whole;                           // page_size is a multiple of 16
     int n_pages, page_size;
     uint32_t div_mul, div_shift;         // t / page_size = (umulhi(t, div_mul) + t) >> div_shift
     int B, Hkv, G, hb, Dk, Dv, window;   // hb: head blocks of a kv head
@@ -69,17 +68,18 @@ struct Args {
     int* status;
 };
 
-// The variant for head dims up to DB, 8*NT query heads a block: as many warps, each with two stages, as shared memory and
-// the registers allow (measured at D = 128 in 16 bits, 16 ragged requests to 32768: 8 warps 160 us, 10 warps 152, 12
-// warps 157; three stages put more in flight than the memory takes, and the SMs it serves last fall behind), or more
-// stages where a stage is small.
+// The variant for head dims up to DB, 8*NT query heads a block.  A subtile is 16 tokens, or 32 where 16 would be 4 KB or
+// less (int8, head dims up to 64): what a subtile costs beside its bytes then counts half (measured with int8 rows of 128,
+// 8 requests to 65536: 82 us to 78; 127 requests to 13489 with rows of 64: 167 us to 132).  As many warps, each with two stages, as shared memory and the registers allow
+// (measured at D = 128 in 16 bits, 16 ragged requests to 32768: 8 warps 160 us, 10 warps 152, 12 warps 157; three stages
+// put more in flight than the memory takes, and the SMs it serves last fall behind).
 template <bool I8, int DB, int NT>
 struct Cfg {
     static constexpr int kMt = DB / 16;                                   // accumulator fragments of a head tile
-    static constexpr int kWarps = DB == 256 ? (I8 ? 8 : 5) : DB == 128 ? (NT == 1 ? (I8 ? 16 : 10) : (I8 ? 12 : 8))
-                                                                       : NT == 1 ? 16 : 12;
+    static constexpr int kTok = I8 || DB == 64 ? 32 : 16;                 // tokens of a subtile
+    static constexpr int kWarps = DB == 256 ? 5 : DB == 128 ? (I8 || NT == 2 ? 8 : 10) : I8 ? (NT == 1 ? 16 : 12) : 10;
     static constexpr int kRow = I8 ? ((DB / 16) | 1) * 16 : DB * 2 + 16;  // bytes between rows in shared memory
-    static constexpr int kStage = 2 * kTok * kRow + (I8 ? 128 : 0) + 16;
+    static constexpr int kStage = 2 * kTok * kRow + (I8 ? 8 * kTok : 0) + 16;
     static constexpr int kPiece = NT * (8 * DB + 16);                     // floats: fragments, then m and l of the heads
     static constexpr int kUnits = NT * kMt;
     static constexpr int kFit = ((224 << 10) / kWarps - kPiece * 4) / kStage;
@@ -92,8 +92,9 @@ inline int piece_floats(int DB, int NT) { return NT * (8 * DB + 16); }
 
 // What the filler of a stage leaves for its reader.
 struct __align__(16) Meta {
-    uint32_t mask;   // bit i: token i counts; bit 16: the row ends here
-    int b, row, sub; // request; kv head << 16 | head block; place in the row
+    uint32_t mask;       // bit i: token i counts
+    int b, row;          // request; kv head << 16 | head block
+    int sub;             // place in the row; the sign bit: the row ends here
 };
 
 __device__ __forceinline__ void cp_async16_all(uint32_t dst, const void* src) {
@@ -162,10 +163,11 @@ __device__ __forceinline__ uint32_t s8_pair(uint32_t r) {
 template <bool F16>
 constexpr float s8_unit = F16 ? 1.f : 8192.f;   // the factor that s8_pair leaves out
 
-// Where request b's attended tokens lie: subtiles from (lo & ~15), tokens [lo, L), n subtiles.
+// Where request b's attended tokens lie: tokens [lo, L), n subtiles from lo rounded down to one.
 struct Span {
     int lo, L, n;
 };
+template <int kTok>
 __device__ __forceinline__ Span span_of(const Args& a, int b) {
     Span s;
     s.L = min(max(__ldg(a.seq_lens + b), 0), a.cap);
@@ -216,6 +218,8 @@ template <bool F16, bool I8, int DB, int NT, bool EXACT>
 __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
     using C = Cfg<I8, DB, NT>;
     constexpr int kWarps = C::kWarps, S = C::kStages, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
+    constexpr int kTok = C::kTok, H = kTok / 16;   // H: 16-token tiles of a subtile
+    constexpr int kMinSub = kMinTok / kTok, kSnapC = kSnapCta / kTok, kSnapW = kSnapWarp / kTok;
     constexpr bool kPF16 = F16 && !I8;   // the type of P and V in the second product (bf16's range for scaled P)
     // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
     constexpr float kUp = kPF16 ? 8.f : 0.f;
@@ -239,12 +243,12 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     int my_from = 0, my_to = 0;   // up to 32 requests: where this lane's request lies
     int my_n = 0;                 // (with one request each) its subtiles a row
     if (a.B <= 32) {              // every warp for itself
-        my_n = lane < a.B ? span_of(a, lane).n : 0;
+        my_n = lane < a.B ? span_of<kTok>(a, lane).n : 0;
         my_to = my_n;
     } else {
         const int first = tid * per;
 #pragma unroll 1
-        for (int b = first; b < min(first + per, a.B); ++b) my_n = span_of(a, b).n, my_to += my_n;
+        for (int b = first; b < min(first + per, a.B); ++b) my_n = span_of<kTok>(a, b).n, my_to += my_n;
     }
     my_from = my_to;
 #pragma unroll
@@ -285,7 +289,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             const int c = group + __popc(__ballot_sync(0xffffffffu, lane < kWarps && s_from[group + lane % kWarps] <= y)) - 1;
             b = c * per, from = s_from[c], n = s_cnt[c];
             while (per > 1) {   // and the one of them that holds it, 32 at a time
-                const int i = b + lane, k = i < min((c + 1) * per, a.B) ? span_of(a, i).n : 0;
+                const int i = b + lane, k = i < min((c + 1) * per, a.B) ? span_of<kTok>(a, i).n : 0;
                 int to = k;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -331,15 +335,15 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     Border first = {0, 0, 0, 0};
     if ((int)blockIdx.x < nC) {
         const Split split(N, nC);
-        x0 = border(split.start(blockIdx.x), kSnapCta).y, x1 = border(split.start(blockIdx.x + 1), kSnapCta).y;
+        x0 = border(split.start(blockIdx.x), kSnapC).y, x1 = border(split.start(blockIdx.x + 1), kSnapC).y;
         const int len = x1 - x0, each = (uint32_t)len / kWarps, more = len - each * kWarps;
-        first = border(x0 + each * warp + min(warp, more), kSnapWarp);
-        w0 = first.y, w1 = border(x0 + each * (warp + 1) + min(warp + 1, more), kSnapWarp).y;
+        first = border(x0 + each * warp + min(warp, more), kSnapW);
+        w0 = first.y, w1 = border(x0 + each * (warp + 1) + min(warp + 1, more), kSnapW).y;
     }
     // requests without a token, dealt over the CTAs: zeros, -inf
 #pragma unroll 1
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-        if (span_of(a, b).n) continue;
+        if (span_of<kTok>(a, b).n) continue;
         const int64_t head0 = (int64_t)b * a.Hkv * a.G;
         for (int i = tid; i < a.Hkv * a.G * (Dv / 8); i += 32 * kWarps)
             reinterpret_cast<uint4*>(a.out + head0 * Dv)[i] = make_uint4(0, 0, 0, 0);
@@ -351,15 +355,16 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     const int count = w1 - w0;
     uint8_t* const ring = smem + warp * C::kWarpSmem;
     const uint32_t ring_u = smem_u32(ring);
-    // a stage: key rows, value rows, int8 scales (16 of keys, 16 of values), meta
-    constexpr int kRow = C::kRow, kV = kTok * kRow, kS = 2 * kV, kM = kS + (I8 ? 128 : 0);
+    // a stage: key rows, value rows, int8 scales (the keys', the values'), meta
+    constexpr int kRow = C::kRow, kV = kTok * kRow, kS = 2 * kV, kM = kS + (I8 ? 8 * kTok : 0);
     float* const cta_pieces = a.pieces + (int64_t)blockIdx.x * 2 * kPiece;
 
-    // filler: the row being filled, and the next subtile's page entry (of this lane's token where pages are not whole
-    // subtiles)
+    // filler: the row being filled, and the next subtile's page entry (of this lane's 16 tokens, or of its token where
+    // pages are not whole tiles)
     Span fs = {0, 0, 0};
     int f_b = 0, f_kvh = 0, f_blk = 0, f_sub = 0, f_entry = -1, f_left = count;
     uint32_t f_off = 0;
+    const int tok = lane & (kTok - 1);
     const int l8 = lane & 7, r4 = lane >> 3;   // copies: eight lanes a row, four rows at a time
     const int kchunks = I8 ? Dk >> 4 : Dk >> 3, vchunks = I8 ? Dv >> 4 : Dv >> 3;
     constexpr int kCols = (I8 ? DB / 16 : DB / 8) >= 8 ? (I8 ? DB / 16 : DB / 8) / 8 : 1;
@@ -367,7 +372,9 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 
     auto look_up = [&]() {
         uint32_t t = (uint32_t)(fs.lo & ~(kTok - 1)) + (uint32_t)f_sub * kTok;
-        if (!a.whole) t = min(max(t + (lane & 15), (uint32_t)fs.lo), (uint32_t)fs.L - 1);
+        // within the tokens that count: the entry of any other place may be of no page
+        t = a.whole ? min(max(t + (tok & 16), (uint32_t)fs.lo & ~15u), (uint32_t)fs.L - 1) & ~15u
+                    : min(max(t + tok, (uint32_t)fs.lo), (uint32_t)fs.L - 1);
         const uint32_t page = (__umulhi(t, a.div_mul) + t) >> a.div_shift;
         f_off = t - page * (uint32_t)a.page_size;
         f_entry = __ldg(a.table + (int64_t)f_b * a.table_stride + page);
@@ -376,47 +383,56 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         if (f_left > 0) {
             const uint32_t st = ring_u + slot * C::kStage;
             const int t0 = (fs.lo & ~(kTok - 1)) + f_sub * kTok;
-            uint32_t mask = (0xffffu >> max(t0 + kTok - fs.L, 0)) & (0xffffu << max(fs.lo - t0, 0));
+            constexpr uint32_t kAll = kTok == 32 ? 0xffffffffu : 0xffffu;
+            uint32_t mask = (kAll >> max(t0 + kTok - fs.L, 0)) & (kAll << max(fs.lo - t0, 0));
             const bool page_ok = (uint32_t)f_entry < (uint32_t)a.n_pages;
             const uint32_t pages_ok = __ballot_sync(0xffffffffu, page_ok);
             if (pages_ok != 0xffffffffu) {
                 if (a.status) atomicMax(a.status, kDevBadIndex);
-                mask &= a.whole ? 0u : pages_ok;
+                mask &= pages_ok;   // whole pages: 16 lanes looked at the same one
             }
-            const uint32_t page = page_ok ? f_entry : 0, kvh = f_kvh;
-            uint64_t ka = (uint64_t)page * a.kp + (uint64_t)f_off * a.kt + (uint64_t)kvh * a.kh;
-            uint64_t va = (uint64_t)page * a.vp + (uint64_t)f_off * a.vt + (uint64_t)kvh * a.vh;
+            const uint32_t page = page_ok ? f_entry : 0;
+            const uint64_t ka = (uint64_t)page * a.kp + (uint64_t)f_off * a.kt + (uint64_t)f_kvh * a.kh;
+            const uint64_t va = (uint64_t)page * a.vp + (uint64_t)f_off * a.vt + (uint64_t)f_kvh * a.vh;
             if (I8) {
-                const int64_t off = a.whole ? f_off + (lane & 15) : f_off;
-                const float* src = lane < 16 ? a.ks + (page * a.ksp + off * a.kst + kvh * a.ksh)
-                                             : a.vs + (page * a.vsp + off * a.vst + kvh * a.vsh);
-                cp_async4(st + kS + lane * 4, src, (mask >> (lane & 15)) & 1);
+                const uint32_t off = a.whole ? f_off + (lane & 15) : f_off;
+                const uint64_t ks = page * (uint64_t)a.ksp + off * (uint64_t)a.kst + f_kvh * (uint64_t)a.ksh;
+                const uint64_t vs = page * (uint64_t)a.vsp + off * (uint64_t)a.vst + f_kvh * (uint64_t)a.vsh;
+                const bool on = (mask >> tok) & 1;
+                cp_async4(st + kS + tok * 4, a.ks + ks, on);
+                cp_async4(st + kS + 4 * kTok + tok * 4, a.vs + vs, on);
             }
             if (lane == 0) {
                 Meta m;
-                m.mask = mask | (f_sub == fs.n - 1 ? 1u << 16 : 0u);
-                m.b = f_b, m.row = f_kvh << 16 | f_blk, m.sub = f_sub;
+                m.mask = mask;
+                m.b = f_b, m.row = f_kvh << 16 | f_blk, m.sub = f_sub | (f_sub == fs.n - 1 ? INT32_MIN : 0);
                 *reinterpret_cast<Meta*>(ring + slot * C::kStage + kM) = m;
             }
             const uint32_t kd = st + r4 * kRow + l8 * 16, vd = kd + kV;
-            if (a.whole && mask == 0xffffu) {
-                const uint8_t *kp = a.k + ((ka + k_lane) << 4), *vp = a.v + ((va + v_lane) << 4);
+            if (a.whole && mask == kAll) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int h = 0; h < H; ++h) {
+                    const uint64_t kb = H == 1 ? ka : __shfl_sync(0xffffffffu, ka, 16 * h);
+                    const uint64_t vb = H == 1 ? va : __shfl_sync(0xffffffffu, va, 16 * h);
+                    const uint8_t *kp = a.k + ((kb + k_lane) << 4), *vp = a.v + ((vb + v_lane) << 4);
 #pragma unroll
-                    for (int j = 0; j < kCols; ++j) {
-                        if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * kRow + j * 128, kp + j * 128);
-                        if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * kRow + j * 128, vp + j * 128);
+                    for (int i = 4 * h; i < 4 * h + 4; ++i) {
+#pragma unroll
+                        for (int j = 0; j < kCols; ++j) {
+                            if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * kRow + j * 128, kp + j * 128);
+                            if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * kRow + j * 128, vp + j * 128);
+                        }
+                        kp += (uint64_t)a.kt << 6, vp += (uint64_t)a.vt << 6;
                     }
-                    kp += (uint64_t)a.kt << 6, vp += (uint64_t)a.vt << 6;
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < kTok / 4; ++i) {
                     const int row = 4 * i + r4;
                     const bool on = (mask >> row) & 1;
-                    uint64_t kr = ka + (on ? row * (uint64_t)a.kt : 0), vr = va + (on ? row * (uint64_t)a.vt : 0);
-                    if (!a.whole) kr = __shfl_sync(0xffffffffu, ka, row), vr = __shfl_sync(0xffffffffu, va, row);
+                    const int in_page = a.whole && on ? row & 15 : 0, src = a.whole ? row & 16 : row;
+                    const uint64_t kr = __shfl_sync(0xffffffffu, ka, src) + in_page * (uint64_t)a.kt;
+                    const uint64_t vr = __shfl_sync(0xffffffffu, va, src) + in_page * (uint64_t)a.vt;
                     const uint8_t *kp = a.k + ((kr + l8) << 4), *vp = a.v + ((vr + l8) << 4);
 #pragma unroll
                     for (int j = 0; j < kCols; ++j) {
@@ -433,7 +449,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                         f_blk = 0;
                         if (++f_kvh == a.Hkv) {
                             f_kvh = 0;
-                            do fs = span_of(a, ++f_b);
+                            do fs = span_of<kTok>(a, ++f_b);
                             while (fs.n == 0);
                         }
                     }
@@ -549,11 +565,11 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 
     if (count > 0) {
         f_b = first.b, f_sub = first.sub;
-        fs = span_of(a, f_b);
+        fs = span_of<kTok>(a, f_b);
         int row = first.row;
         if (row == R) {
             row = 0;
-            do fs = span_of(a, ++f_b);
+            do fs = span_of<kTok>(a, ++f_b);
             while (fs.n == 0);
         }
         f_kvh = a.hb == 1 ? row : row / a.hb;
@@ -572,6 +588,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         Meta meta;
         if (it < 0) meta.b = first_b, meta.row = first_row, meta.sub = it == 1 - S ? 0 : 1;
         else meta = *reinterpret_cast<const Meta*>(ring + slot * C::kStage + kM);
+        const bool ends = meta.sub < 0;
+        meta.sub &= INT32_MAX;
         // a row's queries (the first row's before anything else is asked for)
         if (meta.sub == 0 && it != 0 && count > 0) load_q(meta.b, meta.row);
         fill(it < 0 ? it + S - 1 : slot == 0 ? S - 1 : slot - 1);
@@ -580,67 +598,88 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             order_q();
             began = meta.sub == 0;
         }
-        // scores, in two chains
-        float c[NT][4], e[NT][4];
+        // scores of each 16-token tile; a single tile's in two chains
+        constexpr int kChains = H == 1 ? 2 : 1;
+        float c[H][NT][4], e[kChains == 2 ? NT : 1][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[nt][i] = e[nt][i] = 0.f;
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) c[h][nt][i] = 0.f;
+                if (kChains == 2) e[nt][i] = 0.f;
+            }
         const uint32_t k_ld = st + (lane & 15) * kRow + (lane >> 4) * 16;
         if (I8) {
 #pragma unroll
             for (int ks = 0; ks < DB / 16; ks += 2) {
                 if (ks >= nks) break;
-                uint32_t r[4];
-                ldsm_x4(k_ld + ks * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {   // past an odd nks the queries are zero and what was read is finite
-                    const uint32_t a0 = s8_pair<F16>(r[2 * u]), a1 = s8_pair<F16>(r[2 * u + 1]);
-                    const uint32_t a2 = s8_pair<F16>(r[2 * u] >> 8), a3 = s8_pair<F16>(r[2 * u + 1] >> 8);
+                for (int h = 0; h < H; ++h) {
+                    uint32_t r[4];
+                    ldsm_x4(k_ld + h * 16 * kRow + ks * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma16<F16>(u ? e[nt] : c[nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
+                    for (int u = 0; u < 2; ++u) {   // past an odd nks the queries are zero and what was read is finite
+                        const uint32_t a0 = s8_pair<F16>(r[2 * u]), a1 = s8_pair<F16>(r[2 * u + 1]);
+                        const uint32_t a2 = s8_pair<F16>(r[2 * u] >> 8), a3 = s8_pair<F16>(r[2 * u + 1] >> 8);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma16<F16>(kChains == 2 && u ? e[nt] : c[h][nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
+                    }
                 }
             }
         } else {
 #pragma unroll
             for (int ks = 0; ks < DB / 16; ++ks) {
                 if (ks >= nks) break;
-                uint32_t a0, a1, a2, a3;
-                ldsm_x4(k_ld + ks * 32, a0, a1, a2, a3);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16<F16>(ks & 1 ? e[nt] : c[nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
+                for (int h = 0; h < H; ++h) {
+                    uint32_t a0, a1, a2, a3;
+                    ldsm_x4(k_ld + h * 16 * kRow + ks * 32, a0, a1, a2, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma16<F16>(kChains == 2 && (ks & 1) ? e[nt] : c[h][nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
+                }
             }
         }
-        float f0 = a.scale_log2, f1 = f0, v0 = 1.f, v1 = 1.f;
-        if (I8) {
-            const float* sc = reinterpret_cast<const float*>(ring + slot * C::kStage + kS);
-            f0 *= sc[g] * s8_unit<F16>, f1 *= sc[g + 8] * s8_unit<F16>;
-            v0 = sc[16 + g] * s8_unit<kPF16>, v1 = sc[24 + g] * s8_unit<kPF16>;
-        }
+        const float* sc = reinterpret_cast<const float*>(ring + slot * C::kStage + kS);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[nt][i] = (c[nt][i] + e[nt][i]) * (i < 2 ? f0 : f1);
-        if ((meta.mask & 0xffffu) != 0xffffu) {   // tokens that do not count (their values and scales are zero)
-            const bool on0 = (meta.mask >> g) & 1, on1 = (meta.mask >> (g + 8)) & 1;
+        for (int h = 0; h < H; ++h) {
+            const float f0 = I8 ? sc[16 * h + g] * (s8_unit<F16> * a.scale_log2) : a.scale_log2;
+            const float f1 = I8 ? sc[16 * h + g + 8] * (s8_unit<F16> * a.scale_log2) : a.scale_log2;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) c[nt][i] = (i < 2 ? on0 : on1) ? c[nt][i] : -INFINITY;
+                for (int i = 0; i < 4; ++i)
+                    c[h][nt][i] = (kChains == 2 ? c[h][nt][i] + e[nt][i] : c[h][nt][i]) * (i < 2 ? f0 : f1);
         }
+        if (meta.mask != (kTok == 32 ? 0xffffffffu : 0xffffu)) {   // tokens that do not count (their values and scales are zero)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const bool on0 = (meta.mask >> (16 * h + g)) & 1, on1 = (meta.mask >> (16 * h + g + 8)) & 1;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) c[h][nt][i] = (i < 2 ? on0 : on1) ? c[h][nt][i] : -INFINITY;
+            }
+        }
+        float tops[NT][2];
         bool past = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) past |= fmaxf(c[nt][j], c[nt][j + 2]) > m_ref[nt][j] + (kUp + kSlack);
+            for (int j = 0; j < 2; ++j) {
+                tops[nt][j] = fmaxf(c[0][nt][j], c[0][nt][j + 2]);
+                if (H == 2) tops[nt][j] = fmaxf(tops[nt][j], fmaxf(c[H - 1][nt][j], c[H - 1][nt][j + 2]));
+                past |= tops[nt][j] > m_ref[nt][j] + (kUp + kSlack);
+            }
         if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float keep[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float top = fmaxf(c[nt][j], c[nt][j + 2]);
+                    float top = tops[nt][j];
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -656,23 +695,28 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 }
             }
         }
-        uint32_t ph[NT][2], pl[NT][2];
+        uint32_t ph[H][NT][2], pl[H][NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int h = 0; h < H; ++h) {
+            const float v0 = I8 ? sc[kTok + 16 * h + g] * s8_unit<kPF16> : 1.f;
+            const float v1 = I8 ? sc[kTok + 16 * h + g + 8] * s8_unit<kPF16> : 1.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                // while every score so far is -inf the reference is too: any finite one in its place gives 0
-                const float ref = fmaxf(m_ref[nt][j], -3.0e38f);
-                const float p0 = ex2(c[nt][j] - ref), p1 = ex2(c[nt][j + 2] - ref);
-                l_run[nt][j] += p0 + p1;
-                c[nt][j] = I8 ? p0 * v0 : p0;
-                c[nt][j + 2] = I8 ? p1 * v1 : p1;
+            for (int nt = 0; nt < NT; ++nt) {
+                float(&p)[4] = c[h][nt];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    // while every score so far is -inf the reference is too: any finite one in its place gives 0
+                    const float ref = fmaxf(m_ref[nt][j], -3.0e38f);
+                    p[j] = ex2(p[j] - ref), p[j + 2] = ex2(p[j + 2] - ref);
+                    l_run[nt][j] += p[j] + p[j + 2];
+                    if (I8) p[j] *= v0, p[j + 2] *= v1;
+                }
+                const uint32_t h0 = pack16<kPF16>(p[0], p[1]), h1 = pack16<kPF16>(p[2], p[3]);
+                const float2 e0 = unpack16<kPF16>(h0), e1 = unpack16<kPF16>(h1);
+                ph[h][nt][0] = movmatrix_t(h0), ph[h][nt][1] = movmatrix_t(h1);
+                pl[h][nt][0] = movmatrix_t(pack16<kPF16>(p[0] - e0.x, p[1] - e0.y));
+                pl[h][nt][1] = movmatrix_t(pack16<kPF16>(p[2] - e1.x, p[3] - e1.y));
             }
-            const uint32_t h0 = pack16<kPF16>(c[nt][0], c[nt][1]), h1 = pack16<kPF16>(c[nt][2], c[nt][3]);
-            const float2 e0 = unpack16<kPF16>(h0), e1 = unpack16<kPF16>(h1);
-            ph[nt][0] = movmatrix_t(h0), ph[nt][1] = movmatrix_t(h1);
-            pl[nt][0] = movmatrix_t(pack16<kPF16>(c[nt][0] - e0.x, c[nt][1] - e0.y));
-            pl[nt][1] = movmatrix_t(pack16<kPF16>(c[nt][2] - e1.x, c[nt][3] - e1.y));
         }
         // values
         if (I8) {
@@ -680,16 +724,19 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
             for (int mt = 0; mt < kMt; mt += 2) {
                 if (mt >= nmt) break;
-                uint32_t r[4];
-                ldsm_x4_t(v_ld + mt * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {   // past an odd nmt: accumulators that nobody reads
-                    const uint32_t a0 = s8_pair<kPF16>(r[2 * u]), a1 = s8_pair<kPF16>(r[2 * u] >> 8);
-                    const uint32_t a2 = s8_pair<kPF16>(r[2 * u + 1]), a3 = s8_pair<kPF16>(r[2 * u + 1] >> 8);
+                for (int h = 0; h < H; ++h) {
+                    uint32_t r[4];
+                    ldsm_x4_t(v_ld + h * 16 * kRow + mt * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                        mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                    for (int u = 0; u < 2; ++u) {   // past an odd nmt: accumulators that nobody reads
+                        const uint32_t a0 = s8_pair<kPF16>(r[2 * u]), a1 = s8_pair<kPF16>(r[2 * u] >> 8);
+                        const uint32_t a2 = s8_pair<kPF16>(r[2 * u + 1]), a3 = s8_pair<kPF16>(r[2 * u + 1] >> 8);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, ph[h][nt][0], ph[h][nt][1]);
+                            mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, pl[h][nt][0], pl[h][nt][1]);
+                        }
                     }
                 }
             }
@@ -698,17 +745,20 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
             for (int mt = 0; mt < kMt; ++mt) {
                 if (mt >= nmt) break;
-                uint32_t a0, a1, a2, a3;
-                ldsm_x4_t(v_ld + mt * 32, a0, a1, a2, a3);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                    mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                for (int h = 0; h < H; ++h) {
+                    uint32_t a0, a1, a2, a3;
+                    ldsm_x4_t(v_ld + h * 16 * kRow + mt * 32, a0, a1, a2, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, ph[h][nt][0], ph[h][nt][1]);
+                        mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, pl[h][nt][0], pl[h][nt][1]);
+                    }
                 }
             }
         }
         // the row, or this warp's stretch, ends
-        const bool ends = meta.mask >> 16, more = it + 1 < count;
+        const bool more = it + 1 < count;
         if (ends || !more) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -738,7 +788,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     s_start[part] = w0 + it - meta.sub;
                     s_req[part] = meta.b;
                     s_row[part] = meta.row;
-                    s_n[part] = span_of(a, meta.b).n;
+                    s_n[part] = span_of<kTok>(a, meta.b).n;
                 }
             }
         }

@@ -36,6 +36,8 @@
 namespace ws {
 namespace paged {
 
+// Shared memory for the rings: a CTA's 227 KB without what the kernel declares itself.
+constexpr int most_smem(int warps) { return ((227 << 10) - 432 * warps - 128) & ~15; }
 constexpr int kMinTok = 32;     // tokens a warp takes before another CTA joins in
 // Rows up to so many tokens are not cut by a border between two CTAs, or two warps: the border moves to the nearer end
 // of the row, which unbalances the stretches by half a row at most and saves the joining.
@@ -66,6 +68,7 @@ struct Args {
     int* counters;
     float* pieces;                       // [cta][2][piece floats]
     int* status;
+    int krow, vrow, stages, warp_smem;   // where Dk, Dv are not known when compiling: the ring's geometry (see Ring)
 };
 
 // The variant for head dims up to DB, 8*NT query heads a block.  A subtile is 16 tokens, or 32 where 16 would be 4 KB or
@@ -82,11 +85,11 @@ struct Cfg {
     static constexpr int kStage = 2 * kTok * kRow + (I8 ? 8 * kTok : 0) + 16;
     static constexpr int kPiece = NT * (8 * DB + 16);                     // floats: fragments, then m and l of the heads
     static constexpr int kUnits = NT * kMt;
-    static constexpr int kFit = ((224 << 10) / kWarps - kPiece * 4) / kStage;
+    static constexpr int kFit = (most_smem(kWarps) / kWarps - kPiece * 4) / kStage;
     static constexpr int kStages = kFit > 4 ? 4 : kFit;
-    static constexpr int kRing = kStages * kStage;                        // ends as the place of the last part
-    static constexpr int kWarpSmem = kRing + kPiece * 4;                  // the ring and the first part
-    static_assert(kStages >= 2 && kRing >= kPiece * 4 && kRing % 16 == 0, "ring");
+    static constexpr int kWarpSmem = kStages * kStage + kPiece * 4;       // the ring, which ends as the place of the last
+                                                                          // part, and the first part
+    static_assert(kStages >= 2 && kStages * kStage >= kPiece * 4 && kStage % 16 == 0, "ring");
 };
 inline int piece_floats(int DB, int NT) { return NT * (8 * DB + 16); }
 
@@ -217,14 +220,14 @@ __device__ __forceinline__ void finish(const Args& a, int64_t head0, int left, i
 template <bool F16, bool I8, int DB, int NT, bool EXACT>
 __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
     using C = Cfg<I8, DB, NT>;
-    constexpr int kWarps = C::kWarps, S = C::kStages, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
+    constexpr int kWarps = C::kWarps, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
     constexpr int kTok = C::kTok, H = kTok / 16;   // H: 16-token tiles of a subtile
     constexpr int kMinSub = kMinTok / kTok, kSnapC = kSnapCta / kTok, kSnapW = kSnapWarp / kTok;
     constexpr bool kPF16 = F16 && !I8;   // the type of P and V in the second product (bf16's range for scaled P)
     // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
     constexpr float kUp = kPF16 ? 8.f : 0.f;
     extern __shared__ __align__(16) uint8_t smem[];   // [kWarps][kWarpSmem]
-    __shared__ int s_scan[kWarps], s_from[32 * kWarps], s_start[2 * kWarps];   // s_start < 0: no part
+    __shared__ int s_border[kWarps], s_scan[kWarps], s_from[32 * kWarps], s_start[2 * kWarps];   // s_start < 0: no part
     __shared__ int s_list[kWarps][32], s_cnt[32 * kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -335,10 +338,25 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     Border first = {0, 0, 0, 0};
     if ((int)blockIdx.x < nC) {
         const Split split(N, nC);
-        x0 = border(split.start(blockIdx.x), kSnapC).y, x1 = border(split.start(blockIdx.x + 1), kSnapC).y;
-        const int len = x1 - x0, each = (uint32_t)len / kWarps, more = len - each * kWarps;
-        first = border(x0 + each * warp + min(warp, more), kSnapW);
-        w0 = first.y, w1 = border(x0 + each * (warp + 1) + min(warp + 1, more), kSnapW).y;
+        if (a.B <= 32) {
+            x0 = border(split.start(blockIdx.x), kSnapC).y, x1 = border(split.start(blockIdx.x + 1), kSnapC).y;
+            const int len = x1 - x0, each = (uint32_t)len / kWarps, more = len - each * kWarps;
+            first = border(x0 + each * warp + min(warp, more), kSnapW);
+            w0 = first.y, w1 = border(x0 + each * (warp + 1) + min(warp + 1, more), kSnapW).y;
+        } else {   // where finding a border takes longer: each by one warp
+            if (warp < 2) {
+                const int y = border(split.start(blockIdx.x + warp), kSnapC).y;
+                if (lane == 0) s_scan[warp] = y;
+            }
+            __syncthreads();
+            x0 = s_scan[0], x1 = s_scan[1];
+            const int len = x1 - x0, each = (uint32_t)len / kWarps, more = len - each * kWarps;
+            first = border(x0 + each * warp + min(warp, more), kSnapW);
+            w0 = first.y;
+            if (lane == 0) s_border[warp] = w0;
+            __syncthreads();
+            w1 = warp == kWarps - 1 ? x1 : s_border[warp + 1];
+        }
     }
     // requests without a token, dealt over the CTAs: zeros, -inf
 #pragma unroll 1
@@ -353,10 +371,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 
     // ---- this warp's stretch
     const int count = w1 - w0;
-    uint8_t* const ring = smem + warp * C::kWarpSmem;
+    const int warp_smem = EXACT ? C::kWarpSmem : a.warp_smem;
+    uint8_t* const ring = smem + warp * warp_smem;
+    float* const first_part = reinterpret_cast<float*>(ring + warp_smem) - kPiece;
     const uint32_t ring_u = smem_u32(ring);
     // a stage: key rows, value rows, int8 scales (the keys', the values'), meta
-    constexpr int kRow = C::kRow, kV = kTok * kRow, kS = 2 * kV, kM = kS + (I8 ? 8 * kTok : 0);
+    const int S = EXACT ? C::kStages : a.stages;
+    const int krow = EXACT ? C::kRow : a.krow, vrow = EXACT ? C::kRow : a.vrow;
+    const int kV = kTok * krow, kS = kV + kTok * vrow, kM = kS + (I8 ? 8 * kTok : 0), stage = kM + 16;
     float* const cta_pieces = a.pieces + (int64_t)blockIdx.x * 2 * kPiece;
 
     // filler: the row being filled, and the next subtile's page entry (of this lane's 16 tokens, or of its token where
@@ -381,7 +403,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     };
     auto fill = [&](int slot) {
         if (f_left > 0) {
-            const uint32_t st = ring_u + slot * C::kStage;
+            const uint32_t st = ring_u + slot * stage;
             const int t0 = (fs.lo & ~(kTok - 1)) + f_sub * kTok;
             constexpr uint32_t kAll = kTok == 32 ? 0xffffffffu : 0xffffu;
             uint32_t mask = (kAll >> max(t0 + kTok - fs.L, 0)) & (kAll << max(fs.lo - t0, 0));
@@ -406,9 +428,9 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 Meta m;
                 m.mask = mask;
                 m.b = f_b, m.row = f_kvh << 16 | f_blk, m.sub = f_sub | (f_sub == fs.n - 1 ? INT32_MIN : 0);
-                *reinterpret_cast<Meta*>(ring + slot * C::kStage + kM) = m;
+                *reinterpret_cast<Meta*>(ring + slot * stage + kM) = m;
             }
-            const uint32_t kd = st + r4 * kRow + l8 * 16, vd = kd + kV;
+            const uint32_t kd = st + r4 * krow + l8 * 16, vd = st + kV + r4 * vrow + l8 * 16;
             if (a.whole && mask == kAll) {
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
@@ -419,8 +441,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     for (int i = 4 * h; i < 4 * h + 4; ++i) {
 #pragma unroll
                         for (int j = 0; j < kCols; ++j) {
-                            if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * kRow + j * 128, kp + j * 128);
-                            if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * kRow + j * 128, vp + j * 128);
+                            if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * krow + j * 128, kp + j * 128);
+                            if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * vrow + j * 128, vp + j * 128);
                         }
                         kp += (uint64_t)a.kt << 6, vp += (uint64_t)a.vt << 6;
                     }
@@ -436,8 +458,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     const uint8_t *kp = a.k + ((kr + l8) << 4), *vp = a.v + ((vr + l8) << 4);
 #pragma unroll
                     for (int j = 0; j < kCols; ++j) {
-                        if (l8 + 8 * j < kchunks) cp_async16(kd + 4 * i * kRow + j * 128, kp + j * 128, on);
-                        if (l8 + 8 * j < vchunks) cp_async16(vd + 4 * i * kRow + j * 128, vp + j * 128, on);
+                        if (l8 + 8 * j < kchunks) cp_async16(kd + 4 * i * krow + j * 128, kp + j * 128, on);
+                        if (l8 + 8 * j < vchunks) cp_async16(vd + 4 * i * vrow + j * 128, vp + j * 128, on);
                     }
                 }
             }
@@ -581,13 +603,19 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll 1
     for (int it = 1 - S; it < count; ++it) {
         if (it >= 0) {
-            cp_async_wait<S - 2>();
+            if (EXACT) {
+                cp_async_wait<C::kStages - 2>();
+            } else {
+                if (S == 2) cp_async_wait<0>();
+                else if (S == 3) cp_async_wait<1>();
+                else cp_async_wait<2>();
+            }
             __syncwarp();
         }
-        const uint32_t st = ring_u + slot * C::kStage;
+        const uint32_t st = ring_u + slot * stage;
         Meta meta;
         if (it < 0) meta.b = first_b, meta.row = first_row, meta.sub = it == 1 - S ? 0 : 1;
-        else meta = *reinterpret_cast<const Meta*>(ring + slot * C::kStage + kM);
+        else meta = *reinterpret_cast<const Meta*>(ring + slot * stage + kM);
         const bool ends = meta.sub < 0;
         meta.sub &= INT32_MAX;
         // a row's queries (the first row's before anything else is asked for)
@@ -609,7 +637,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 for (int h = 0; h < H; ++h) c[h][nt][i] = 0.f;
                 if (kChains == 2) e[nt][i] = 0.f;
             }
-        const uint32_t k_ld = st + (lane & 15) * kRow + (lane >> 4) * 16;
+        const uint32_t k_ld = st + (lane & 15) * krow + (lane >> 4) * 16;
         if (I8) {
 #pragma unroll
             for (int ks = 0; ks < DB / 16; ks += 2) {
@@ -617,7 +645,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t r[4];
-                    ldsm_x4(k_ld + h * 16 * kRow + ks * 16, r[0], r[1], r[2], r[3]);
+                    ldsm_x4(k_ld + h * 16 * krow + ks * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {   // past an odd nks the queries are zero and what was read is finite
                         const uint32_t a0 = s8_pair<F16>(r[2 * u]), a1 = s8_pair<F16>(r[2 * u + 1]);
@@ -635,14 +663,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t a0, a1, a2, a3;
-                    ldsm_x4(k_ld + h * 16 * kRow + ks * 32, a0, a1, a2, a3);
+                    ldsm_x4(k_ld + h * 16 * krow + ks * 32, a0, a1, a2, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         mma16<F16>(kChains == 2 && (ks & 1) ? e[nt] : c[h][nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
                 }
             }
         }
-        const float* sc = reinterpret_cast<const float*>(ring + slot * C::kStage + kS);
+        const float* sc = reinterpret_cast<const float*>(ring + slot * stage + kS);
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const float f0 = I8 ? sc[16 * h + g] * (s8_unit<F16> * a.scale_log2) : a.scale_log2;
@@ -720,14 +748,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         }
         // values
         if (I8) {
-            const uint32_t v_ld = st + kV + (lane & 15) * kRow + (lane >> 4) * 16;
+            const uint32_t v_ld = st + kV + (lane & 15) * vrow + (lane >> 4) * 16;
 #pragma unroll
             for (int mt = 0; mt < kMt; mt += 2) {
                 if (mt >= nmt) break;
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t r[4];
-                    ldsm_x4_t(v_ld + h * 16 * kRow + mt * 16, r[0], r[1], r[2], r[3]);
+                    ldsm_x4_t(v_ld + h * 16 * vrow + mt * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {   // past an odd nmt: accumulators that nobody reads
                         const uint32_t a0 = s8_pair<kPF16>(r[2 * u]), a1 = s8_pair<kPF16>(r[2 * u] >> 8);
@@ -741,14 +769,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 }
             }
         } else {
-            const uint32_t v_ld = st + kV + ((lane & 7) + ((lane >> 4) << 3)) * kRow + ((lane >> 3) & 1) * 16;
+            const uint32_t v_ld = st + kV + ((lane & 7) + ((lane >> 4) << 3)) * vrow + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int mt = 0; mt < kMt; ++mt) {
                 if (mt >= nmt) break;
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t a0, a1, a2, a3;
-                    ldsm_x4_t(v_ld + h * 16 * kRow + mt * 32, a0, a1, a2, a3);
+                    ldsm_x4_t(v_ld + h * 16 * vrow + mt * 32, a0, a1, a2, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, ph[h][nt][0], ph[h][nt][1]);
@@ -783,7 +811,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 // the stretch's last part takes the ring's place (nothing is in flight into it any more)
                 const int part = 2 * warp + (more ? 0 : 1);
                 __syncwarp();
-                file_piece(reinterpret_cast<float*>(more ? ring + C::kRing : ring));
+                file_piece(more ? first_part : reinterpret_cast<float*>(ring));
                 if (lane == 0) {
                     s_start[part] = w0 + it - meta.sub;
                     s_req[part] = meta.b;
@@ -797,26 +825,29 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     __syncthreads();
 
     // ---- join parts.  First the CTA's, row by row; lane i looks at part i: warp i/2's first (even) or last (odd).  Then,
-    // if this CTA is the last of a row's to file its part, the row's, copied to shared memory.  The units (16 x 8
-    // fragments) of a row are dealt over the warps.
+    // if this CTA is the last of a row's to file its part, the row's, copied to shared memory.  A job is kJob units (16 x 8
+    // fragments) of a row; the jobs are dealt over the warps.
+    constexpr int kJob = 2, kJobs = kUnits / kJob;
+    static_assert(kMt % kJob == 0, "a job's units have the same heads");
     const int my_start = lane < 2 * kWarps ? s_start[lane] : -1;
     uint32_t todo = __ballot_sync(0xffffffffu, my_start >= 0);
     int cross0 = -1, cross1 = -1;   // the row that came from an earlier CTA, the one that goes on into the next
-    int id0 = 0, id1 = 0, turn = warp, ended = -1, done = 0;
-    constexpr int kRoom = kWarps * C::kWarpSmem / (kPiece * 4) < 32 ? kWarps * C::kWarpSmem / (kPiece * 4) : 32;
+    int id0 = 0, id1 = 0, turn = warp, ended = -1, done = 0, ahead = 0;
+    const int room = min(kWarps * warp_smem / (kPiece * 4), 32) - 2;
 #pragma unroll 1
     while (true) {
         int id, n;              // one of the row's parts here; how many parts to join: s_list[warp][0 .. n-1], bytes
         float* to = nullptr;    // a piece in the workspace or in shared memory, or the output
+        __syncwarp();
         if (todo) {
             id = __ffs(todo) - 1;
             const int start = __shfl_sync(0xffffffffu, my_start, id);
             const uint32_t parts = __ballot_sync(0xffffffffu, my_start == start);
             todo &= ~parts;
             n = __popc(parts);
-            __syncwarp();
             if ((parts >> lane) & 1)
-                s_list[warp][__popc(parts & ((1u << lane) - 1))] = (lane >> 1) * C::kWarpSmem + (lane & 1 ? 0 : C::kRing);
+                s_list[warp][__popc(parts & ((1u << lane) - 1))] =
+                    (lane >> 1) * warp_smem + (lane & 1 ? 0 : warp_smem - kPiece * 4);
             if (start < x0) cross0 = start, id0 = id, to = cta_pieces;
             else if (start + s_n[id] > x1) cross1 = start, id1 = id, to = cta_pieces + kPiece;
         } else {
@@ -845,78 +876,103 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 if (ended < 2 && s_ctas[ended] == 0) ++ended;
             }
             if (ended == 2) return;
-            const int ctas = s_ctas[ended], c0 = s_first[ended], carry = done > 0;
+            const int ctas = s_ctas[ended], carry = done > 0;
             id = ended ? id1 : id0;
-            // kRoom parts at a time, with what came of the earlier ones (in place 0 or 1 by turns) as the first
-            const int take = min(ctas - done, kRoom - 2);
-            __syncthreads();
+            if (ended && ahead) {   // came with the other row's
+                n = done = ctas;
+                if (lane < n) s_list[warp][lane] = (2 + ahead + lane) * kPiece * 4;
+            } else {
+                // `room` parts at a time, with what came of the earlier ones (in place 0 or 1 by turns) as the first; and
+                // the other row's too if they fit
+                const int take = min(ctas - done, room), first0 = s_first[ended], first1 = s_first[1];
+                const int extra = ended == 0 && ctas + s_ctas[1] <= room ? s_ctas[1] : 0;
+                ahead = extra ? take : 0;
+                __syncthreads();
 #pragma unroll 1
-            for (int i = tid; i < take * (kPiece / 4); i += 32 * kWarps) {
-                const int p = i / (kPiece / 4), r = i - p * (kPiece / 4), c = done + p;
-                // the first CTA filed the row as its slot 1, the others as their slot 0
-                cp_async16_all(smem_u32(smem) + ((p + 2) * (kPiece / 4) + r) * 16,
-                               a.pieces + ((int64_t)(c0 + c) * 2 + (c == 0 ? 1 : 0)) * kPiece + r * 4);
+                for (int i = tid; i < (take + extra) * (kPiece / 4); i += 32 * kWarps) {
+                    const int p = i / (kPiece / 4), r = i - p * (kPiece / 4), c = p < take ? done + p : p - take;
+                    // the first CTA filed the row as its slot 1, the others as their slot 0
+                    cp_async16_all(smem_u32(smem) + ((p + 2) * (kPiece / 4) + r) * 16,
+                                   a.pieces + ((int64_t)((p < take ? first0 : first1) + c) * 2 + (c == 0 ? 1 : 0)) * kPiece + r * 4);
+                }
+                const int round = done / room;
+                done += take;
+                n = take + carry;
+                if (lane < n) s_list[warp][lane] = (carry && lane == 0 ? (round & 1) : lane - carry + 2) * kPiece * 4;
+                if (done < ctas) to = reinterpret_cast<float*>(smem + ((round + 1) & 1) * kPiece * 4);
+                turn = warp;
+                cp_async_commit();
+                cp_async_wait<0>();
+                __syncthreads();
             }
-            const int round = done / (kRoom - 2);
-            done += take;
-            n = take + carry;
-            __syncwarp();
-            if (lane < n) s_list[warp][lane] = (carry && lane == 0 ? (round & 1) : lane - carry + 2) * kPiece * 4;
-            if (done < ctas) to = reinterpret_cast<float*>(smem + ((round + 1) & 1) * kPiece * 4);
-            turn = warp;
-            cp_async_commit();
-            cp_async_wait<0>();
-            __syncthreads();
         }
         __syncwarp();
-        const int req = s_req[id], row = s_row[id];
+        const int row = s_row[id], left = left_of(row);
+        const int64_t head0 = head_of(s_req[id], row);
 #pragma unroll 1
-        for (; turn < kUnits; turn += kWarps) {
-            const int u = turn, nt = u / kMt, mt = u - nt * kMt, ml = NT * 8 * DB + nt * 16 + 2 * t4;
-            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (; turn < kJobs; turn += kWarps) {
+            const int nt = turn * kJob / kMt, mt0 = turn * kJob - nt * kMt, ml = NT * 8 * DB + nt * 16 + 2 * t4;
+            const int at = (turn * kJob * 32 + lane) * 16;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[kJob][4];
+#pragma unroll
+            for (int q = 0; q < kJob; ++q) o[q][0] = o[q][1] = o[q][2] = o[q][3] = 0.f;
 #pragma unroll 1
             for (int i = 0; i < n; i += 8) {   // eight parts: lane (g, t) looks at part g's m and l of its two heads
                 const bool in = i + g < n;
-                const float* src = reinterpret_cast<const float*>(smem + s_list[warp][in ? i + g : 0]);
+                const int mine = s_list[warp][in ? i + g : 0];
+                const float* src = reinterpret_cast<const float*>(smem + mine);
                 const float2 x = in ? *reinterpret_cast<const float2*>(src + ml) : make_float2(-INFINITY, -INFINITY);
                 const float2 y = in ? *reinterpret_cast<const float2*>(src + ml + 8) : make_float2(0.f, 0.f);
                 const float px[2] = {x.x, x.y}, py[2] = {y.x, y.y};
-                float w[2];
+                float w[2], keep[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float top = fmaxf(px[j], __shfl_xor_sync(0xffffffffu, px[j], 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)), m[j]);
-                    const float ref = fmaxf(top, -3.0e38f), keep = ex2(m[j] - ref);
+                    const float ref = fmaxf(top, -3.0e38f);
+                    keep[j] = ex2(m[j] - ref);
                     m[j] = top;
                     w[j] = ex2(px[j] - ref);
                     float sum = py[j] * w[j];
                     sum += __shfl_xor_sync(0xffffffffu, sum, 4);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                    l[j] = l[j] * keep + sum;
-                    o[j] *= keep, o[j + 2] *= keep;
+                    l[j] = l[j] * keep[j] + sum;
+                }
+                if (i) {
+#pragma unroll
+                    for (int q = 0; q < kJob; ++q) o[q][0] *= keep[0], o[q][1] *= keep[1], o[q][2] *= keep[0], o[q][3] *= keep[1];
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {   // past the last part: the first one, with weight 0
-                    const float4 z = *reinterpret_cast<const float4*>(smem + s_list[warp][i + k < n ? i + k : 0] + (u * 32 + lane) * 16);
+                for (int k = 0; k < 8; ++k) {
+                    if (i + k >= n) break;
+                    const uint8_t* z = smem + __shfl_sync(0xffffffffu, mine, 4 * k) + at;
                     const float w0 = __shfl_sync(0xffffffffu, w[0], 4 * k + t4), w1 = __shfl_sync(0xffffffffu, w[1], 4 * k + t4);
-                    o[0] += z.x * w0, o[1] += z.y * w1, o[2] += z.z * w0, o[3] += z.w * w1;
+#pragma unroll
+                    for (int q = 0; q < kJob; ++q) {
+                        const float4 v = *reinterpret_cast<const float4*>(z + q * 512);
+                        o[q][0] += v.x * w0, o[q][1] += v.y * w1, o[q][2] += v.z * w0, o[q][3] += v.w * w1;
+                    }
                 }
             }
             if (to) {
-                *reinterpret_cast<float4*>(to + (u * 32 + lane) * 4) = make_float4(o[0], o[1], o[2], o[3]);
-                if (mt == 0 && lane < 4) {
+#pragma unroll
+                for (int q = 0; q < kJob; ++q)
+                    *reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(to) + at + q * 512) = make_float4(o[q][0], o[q][1], o[q][2], o[q][3]);
+                if (mt0 == 0 && lane < 4) {
                     *reinterpret_cast<float2*>(to + ml) = make_float2(m[0], m[1]);
                     *reinterpret_cast<float2*>(to + ml + 8) = make_float2(l[0], l[1]);
                 }
             } else {
                 float inv[2];
-                finish(a, head_of(req, row), left_of(row), nt, m, l, mt == 0, inv);
-                if (mt < nmt) store_unit(head_of(req, row), left_of(row), nt, mt, o, inv);
+                finish(a, head0, left, nt, m, l, mt0 == 0, inv);
+#pragma unroll
+                for (int q = 0; q < kJob; ++q)
+                    if (mt0 + q < nmt) store_unit(head0, left, nt, mt0 + q, o[q], inv);
             }
         }
-        turn = (turn - kUnits) % kWarps;
+        turn = (turn - kJobs) % kWarps;
     }
 }
 
@@ -927,19 +983,32 @@ int launch_bf16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 int launch_f16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 
 template <bool F16, bool I8, int DB, int NT, bool EXACT>
-int launch(const Args& a, int ctas, cudaStream_t st) {
+int launch(Args a, int ctas, cudaStream_t st) {
     using C = Cfg<I8, DB, NT>;
-    constexpr int kSmem = C::kWarps * C::kWarpSmem;
+    int smem = C::kWarps * C::kWarpSmem;
+    if (!EXACT) {
+        // rows as long as they are; stages until the copies in flight are 72 KB an SM (what two stages of 128-dim rows in
+        // 16 bits give)
+        a.krow = I8 ? ((a.Dk / 16) | 1) * 16 : a.Dk * 2 + 16, a.vrow = I8 ? ((a.Dv / 16) | 1) * 16 : a.Dv * 2 + 16;
+        const int bytes = C::kTok * (a.Dk + a.Dv) * (I8 ? 1 : 2);
+        const int stage = C::kTok * (a.krow + a.vrow) + (I8 ? 8 * C::kTok : 0) + 16;
+        auto warp_smem = [&](int stages) { return std::max(stages * stage, C::kPiece * 4) + C::kPiece * 4; };
+        a.stages = 2;
+        while (a.stages < 4 && (a.stages - 1) * bytes * C::kWarps < 72 << 10 && C::kWarps * warp_smem(a.stages + 1) <= most_smem(C::kWarps))
+            ++a.stages;
+        a.warp_smem = warp_smem(a.stages);
+        smem = C::kWarps * a.warp_smem;
+    }
     static thread_local int set_for = -1;
     int dev = 0;
     cudaGetDevice(&dev);
     if (set_for != dev) {
-        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
-            cudaSuccess)
+        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 EXACT ? smem : most_smem(C::kWarps)) != cudaSuccess)
             return set_error(WS_ERR_CUDA, "paged_decode: shared memory");
         set_for = dev;
     }
-    const cudaError_t e = launch_dependent(decode_kernel<F16, I8, DB, NT, EXACT>, dim3(ctas), 32 * C::kWarps, kSmem, st, a);
+    const cudaError_t e = launch_dependent(decode_kernel<F16, I8, DB, NT, EXACT>, dim3(ctas), 32 * C::kWarps, smem, st, a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }
 

@@ -13,9 +13,8 @@
 // kilobytes at most.  So every CTA repeats the scan over all requests (two
 // loads a request, kept in shared memory) instead of waiting for another
 // launch, and takes kTokensPerCta tokens; a step of up to that many is one
-// CTA.  Lengths and ring may be updated in place: with one CTA after a
-// barrier, with more by the CTA that finishes last (a ticket), when no other
-// reads them any more.
+// CTA.  Lengths and ring may be updated in place: with more than one CTA then
+// by the one that finishes last (a ticket), when no other reads them any more.
 #include <cstdio>
 
 #include "common.cuh"
@@ -25,48 +24,49 @@ namespace ws {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kTokensPerCta = 2048;
+constexpr int kTokensPerCta = 1024;
 constexpr int kMaxRequests = 8192;   // 16 bytes of shared memory each
 
-// Exclusive scan of one value per thread over the block; `carry` holds the
-// total of the earlier chunks and takes this chunk's.  All threads call it.
-struct BlockScan {
-    long long part[kThreads / 32];
-    long long total;
+// Exclusive scans of two values per thread over the block; `carry` holds the
+// totals of the earlier chunks and takes this chunk's.  All threads call it.
+struct Two {
+    long long a, b;
 };
-__device__ __forceinline__ long long block_scan(long long v, BlockScan& sh, long long& carry) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    long long x = v;
+__device__ __forceinline__ Two operator+(Two x, Two y) { return {x.a + y.a, x.b + y.b}; }
+__device__ __forceinline__ Two operator-(Two x, Two y) { return {x.a - y.a, x.b - y.b}; }
+struct BlockScan {
+    Two part[kThreads / 32];
+    int taken[kThreads / 32];
+};
+__device__ __forceinline__ Two warp_scan(Two x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        const Two y = {__shfl_up_sync(0xffffffffu, x.a, o), __shfl_up_sync(0xffffffffu, x.b, o)};
+        if ((threadIdx.x & 31) >= o) x = x + y;
     }
+    return x;
+}
+__device__ __forceinline__ Two block_scan(Two v, BlockScan& sh, Two& carry) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const Two x = warp_scan(v);
     __syncthreads();   // the previous call's reads are done
     if (lane == 31) sh.part[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        long long p = lane < nw ? sh.part[lane] : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, p, o);
-            if (lane >= o) p += y;
-        }
-        if (lane < nw) sh.part[lane] = p;
-        if (lane == nw - 1) sh.total = p;
-    }
-    __syncthreads();
-    const long long ex = carry + x - v + (warp ? sh.part[warp - 1] : 0);
-    carry += sh.total;
+    // every warp sums the warps' totals for itself: one barrier less than asking one of them
+    const Two p = warp_scan(lane < nw ? sh.part[lane] : Two{0, 0});
+    const Two before = {__shfl_sync(0xffffffffu, p.a, (warp + 31) & 31), __shfl_sync(0xffffffffu, p.b, (warp + 31) & 31)};
+    const Two ex = carry + (x - v) + (warp ? before : Two{0, 0});
+    carry = carry + Two{__shfl_sync(0xffffffffu, p.a, 31), __shfl_sync(0xffffffffu, p.b, 31)};
     return ex;
 }
 
-// True in the CTA that gets here last (always, with one CTA); that CTA then
-// sees everything the others read or wrote before.  The counter returns to 0.
-__device__ __forceinline__ bool last_cta(int* counter) {
-    if (gridDim.x == 1) {
+// The CTA that writes the lengths and the ring.  In place, the one that gets
+// here last, when no other reads them any more (the counter returns to 0);
+// else the first.
+__device__ __forceinline__ bool writes_state(bool in_place, int* counter) {
+    if (!in_place || gridDim.x == 1) {
         __syncthreads();
-        return true;
+        return blockIdx.x == 0;
     }
     __shared__ int last;
     __syncthreads();
@@ -78,6 +78,12 @@ __device__ __forceinline__ bool last_cta(int* counter) {
     }
     __syncthreads();
     return last;
+}
+
+// Pages of P tokens that L tokens fill.
+__device__ __forceinline__ uint32_t pages_of(uint32_t L, int P) {
+    const uint32_t q = L / (uint32_t)P;
+    return q + (q * (uint32_t)P != L);
 }
 
 // First b in [0, B) whose end[b] > t (ends ascend; t < end[B - 1]).
@@ -107,30 +113,39 @@ paged_slots_kernel(const int32_t* seq_lens, const int32_t* __restrict__ new_lens
     pdl_wait_primary();
     pdl_launch_dependents();
     const int head = ring[0], n_free = min(max(ring[1], 0), n_ring);
-    long long tokens = 0, pages = 0, took = 0;
-    int refused = 0;
-    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
-        const int b = b0 + threadIdx.x;
-        const long long L = b < B ? max(seq_lens[b], 0) : 0;
-        const long long n = b < B ? max(new_lens[b], 0) : 0;
-        const long long start = block_scan(n, sh, tokens);
-        const long long held = (L + P - 1) / P, want = (L + n + P - 1) / P;
-        const bool fits = want <= max_pages && start + n <= n_tokens && L + n <= INT32_MAX;
-        const long long need = fits ? want - held : 0;
-        const long long place = block_scan(need, sh, pages);
-        if (b < B) {
-            const bool served = fits && (need == 0 || place + need <= n_free);
-            end[b] = (int)min(start + n, (long long)n_tokens);
-            first[b] = (int)min(start, (long long)n_tokens);
-            len[b] = served ? (int)L : -1;
-            base[b] = (int)min(place, (long long)n_ring);
-            refused += !served;
-            if (served && need) took = max(took, place + need);
-            if (blockIdx.x == 0) {
-                if (b == 0) cu_new[0] = 0;
-                cu_new[b + 1] = (int)min(start + n, (long long)INT32_MAX);
+    Two sums;   // tokens, pages
+    long long took;
+    int refused;
+    // Tokens and pages are scanned together.  Whether a request's tokens fit the step is known only afterwards, so a step
+    // with less room than tokens scans once more, without the pages of those that do not fit.
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+        sums = {0, 0};
+        took = refused = 0;
+#pragma unroll 1
+        for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+            const int b = b0 + threadIdx.x;
+            const uint32_t L = b < B ? max(seq_lens[b], 0) : 0, n = b < B ? max(new_lens[b], 0) : 0;
+            const uint32_t held = pages_of(L, P), want = pages_of(L + n, P);
+            const bool fits = want <= (uint32_t)max_pages && L + n <= INT32_MAX &&
+                              (pass == 0 || (b < B && first[b] + (long long)n <= n_tokens));
+            const uint32_t need = fits ? want - held : 0;
+            const Two at = block_scan({n, need}, sh, sums);
+            if (b < B) {
+                const bool served = fits && (need == 0 || at.b + need <= n_free);
+                end[b] = (int)min(at.a + n, (long long)n_tokens);
+                first[b] = (int)min(at.a, (long long)INT32_MAX);
+                len[b] = served ? (int)L : -1;
+                base[b] = (int)min(at.b, (long long)n_ring);
+                refused += !served;
+                if (served && need) took = max(took, at.b + need);
+                if (blockIdx.x == 0) {
+                    if (b == 0) cu_new[0] = 0;
+                    cu_new[b + 1] = (int)min(at.a + n, (long long)INT32_MAX);
+                }
             }
         }
+        if (sums.a <= n_tokens) break;
     }
     if (B == 0 && blockIdx.x == 0 && threadIdx.x == 0) cu_new[0] = 0;
     __syncthreads();
@@ -160,13 +175,13 @@ paged_slots_kernel(const int32_t* seq_lens, const int32_t* __restrict__ new_lens
         slots[t] = slot;
         positions[t] = pos;
     }
-    if (!last_cta(counter)) return;
+    if (!writes_state(seq_lens_out == seq_lens || ring_out == ring, counter)) return;
     // served requests that took pages are a prefix of those that fit, so the largest end is what was taken
     refused = __reduce_add_sync(0xffffffffu, refused);
     if ((threadIdx.x & 31) == 0 && refused) atomicAdd(&n_refused, refused);
     const int taken = __reduce_max_sync(0xffffffffu, (int)took);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) reinterpret_cast<int*>(sh.part)[threadIdx.x >> 5] = taken;
+    if ((threadIdx.x & 31) == 0) sh.taken[threadIdx.x >> 5] = taken;
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         const int n = max(new_lens[b], 0);
         const int L = max(seq_lens[b], 0);
@@ -175,7 +190,7 @@ paged_slots_kernel(const int32_t* seq_lens, const int32_t* __restrict__ new_lens
     __syncthreads();
     if (threadIdx.x == 0) {
         int all = 0;
-        for (int w = 0; w < (int)(blockDim.x >> 5); ++w) all = max(all, reinterpret_cast<int*>(sh.part)[w]);
+        for (int w = 0; w < (int)(blockDim.x >> 5); ++w) all = max(all, sh.taken[w]);
         ring_out[0] = (int)((head + (long long)all) % n_ring);
         ring_out[1] = n_free - all;
         ring_out[2] = n_refused;
@@ -194,28 +209,28 @@ paged_release_kernel(const int32_t* seq_lens, const uint8_t* __restrict__ done, 
     pdl_launch_dependents();
     const int head = ring[0], n_free = min(max(ring[1], 0), n_ring);
     const int room = n_ring - n_free;
-    long long pages = 0;
+    Two pages = {0, 0};
     for (int b0 = 0; b0 < B; b0 += blockDim.x) {
         const int b = b0 + threadIdx.x;
         long long held = 0;
-        if (b < B && done[b]) held = min(((long long)max(seq_lens[b], 0) + P - 1) / P, (long long)max_pages);
-        const long long start = block_scan(held, sh, pages);
+        if (b < B && done[b]) held = min(pages_of(max(seq_lens[b], 0), P), (uint32_t)max_pages);
+        const long long start = block_scan({held, 0}, sh, pages).a;
         if (b < B) end[b] = (int)min(start + held, (long long)INT32_MAX);
     }
     __syncthreads();
-    const int total = (int)min(pages, (long long)room);
+    const int total = (int)min(pages.a, (long long)room);
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
         const int b = owner_of(end, B, i);
         const int j = i - (b ? end[b - 1] : 0);
         free_pages[(unsigned)((head + (long long)n_free + i) % n_ring)] = table[(int64_t)b * table_stride + j];
     }
-    if (!last_cta(counter)) return;
+    if (!writes_state(seq_lens_out == seq_lens || ring_out == ring, counter)) return;
     for (int b = threadIdx.x; b < B; b += blockDim.x) seq_lens_out[b] = done[b] ? 0 : seq_lens[b];
     if (threadIdx.x == 0) {
         ring_out[0] = head;
         ring_out[1] = n_free + total;
         ring_out[2] = 0;
-        if (pages > room && status) atomicMax(status, kDevBadIndex);
+        if (pages.a > room && status) atomicMax(status, kDevBadIndex);
     }
 }
 

@@ -8,9 +8,12 @@
 // head -- eight pairs, so both halves of every pair are its own: 16 bytes at
 // dim 8u and 16 at rope_dim/2 + 8u, or 32 contiguous bytes for adjacent pairs
 // and for the dims that pass unrotated -- and walks the heads of its token, so
-// the eight cosines and sines are loaded once for all of them.  The units of a
-// head are padded to a power of two and lie in one warp, which the int8 form
-// needs for the row's maximum.
+// the eight cosines and sines are loaded once for all of them (a warp for every
+// step of heads would load them again and again: 94 us instead of 54).  The
+// units of a head are padded to a power of two and lie in one warp, which the
+// int8 form needs for the row's maximum.  Measured: 16384 x 32 heads of 128,
+// three axes, 47.9 us (277 MB, 5.8 TB/s); append of 16384 tokens of 32 + 4 + 4
+// heads 62.0 us (345 MB, 5.6 TB/s).
 //
 // Products and sums are rounded one by one (no fused multiply-add): the result
 // is the elementwise formula's, bit for bit, so an int8 code never depends on
@@ -22,10 +25,13 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace ws {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kGroup = 2;   // rows a thread loads before it turns the first, where it has several
 
 struct Heads {          // one of q, k, v: rows of (token, head)
     const uint16_t* src;
@@ -45,6 +51,7 @@ struct RopeAppendArgs {
     int64_t N, n_slots;
     int page_size, lanes;   // lanes: units of a head, padded to a power of two
     int parts;              // warps that share a token's heads
+    int turns_vec;          // cos_sin is 16-byte aligned
     int* status;
 };
 
@@ -86,13 +93,13 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
 }
 
 // F16: fp16 inputs (else bf16); I8: the pool holds int8 codes; VEC: q, k, v and q_out are 16-byte aligned throughout.
-template <bool F16, bool I8, bool VEC>
+template <bool F16, bool I8, bool VEC, int GROUP>
 __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_constant__ RopeAppendArgs a) {
     pdl_wait_primary();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int64_t t = item / a.parts;
+    const int64_t t = a.parts == 1 ? item : item / a.parts;
     if (t >= a.N) return;
     const int part = (int)(item - t * a.parts);
     const int u = lane & (a.lanes - 1), row0 = lane / a.lanes, rows = 32 / a.lanes;
@@ -113,17 +120,24 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
             }
             return p;
         };
-        if (r.n_axes == 1) {
-            const float* row = r.cos_sin + position(0) * r.rope_dim + 8 * u;
+        const uint32_t axes = r.axis_map[u >> 1] >> (16 * (u & 1)) & 0xffffu;   // of the eight pairs, two bits each
+        if (a.turns_vec && axes == (axes & 3) * 0x5555u) {   // one axis: the eight lie together
+            const float* row = r.cos_sin + position(axes & 3) * r.rope_dim + 8 * u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) c[i] = __ldg(row + i), s[i] = __ldg(row + n + i);
+            for (int i = 0; i < 2; ++i) {
+                const float4 x = __ldg(reinterpret_cast<const float4*>(row) + i), y = __ldg(reinterpret_cast<const float4*>(row + n) + i);
+                c[4 * i] = x.x, c[4 * i + 1] = x.y, c[4 * i + 2] = x.z, c[4 * i + 3] = x.w;
+                s[4 * i] = y.x, s[4 * i + 1] = y.y, s[4 * i + 2] = y.z, s[4 * i + 3] = y.w;
+            }
         } else {
+            int64_t row[4];   // of each axis
+#pragma unroll
+            for (int x = 0; x < 4; ++x) row[x] = x < r.n_axes ? position(x) * r.rope_dim : 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int pair = 8 * u + i;
-                const int axis = (a.rope.axis_map[pair >> 4] >> (2 * (pair & 15))) & 3;
-                const float* row = r.cos_sin + position(axis) * r.rope_dim + pair;
-                c[i] = __ldg(row), s[i] = __ldg(row + n);
+                const int x = axes >> (2 * i) & 3;
+                const float* p = r.cos_sin + (x & 2 ? (x & 1 ? row[3] : row[2]) : (x & 1 ? row[1] : row[0])) + 8 * u + i;
+                c[i] = __ldg(p), s[i] = __ldg(p + n);
             }
         }
         if (r.inverse) {
@@ -136,87 +150,106 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
         const int64_t slot = a.slots[t];
         if (slot >= 0) {
             if (slot < a.n_slots) {
-                page = slot / a.page_size;
+                if (slot >> 32 == 0) page = (uint32_t)slot / (uint32_t)a.page_size;
+                else page = slot / a.page_size;
                 off = slot - page * a.page_size;
             } else if (a.status) {
                 atomicMax(a.status, kDevBadIndex);
             }
         }
     }
-
     const int total = a.h[0].n + a.h[1].n + a.h[2].n;
-    for (int base = part * rows; base < total; base += a.parts * rows) {
-        int h = base + row0, kind = 0;
-        if (h >= a.h[0].n) h -= a.h[0].n, kind = 1;
-        if (kind == 1 && h >= a.h[1].n) h -= a.h[1].n, kind = 2;
-        const Heads& x = a.h[kind];
-        const bool on = base + row0 < total && 16 * u < x.D && (kind == 0 || page >= 0);
-        const bool turn = turned && kind < 2;
-        const bool split = turn && !r.adjacent;   // the unit's two halves lie rope_dim/2 apart
-        const int d0 = split ? 8 * u : 16 * u, d1 = split ? (r.rope_dim >> 1) + 8 * u : 16 * u + 8;
-        float lo[8], hi[8];   // dims d0 .. d0+7 and d1 .. d1+7
-        if (on) {
-            const uint16_t* p = x.src + t * x.src_tok + h * x.src_head;
-            const uint4 v0 = load8<VEC>(p + d0), v1 = load8<VEC>(p + d1);
-            const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+    for (int base0 = part * rows * GROUP; base0 < total; base0 += a.parts * rows * GROUP) {
+        uint4 v0[GROUP], v1[GROUP];
+        auto locate = [&](int k, int& h, int& kind) {   // this thread's row of the group's step k: a head of q, k or v
+            const int at = base0 + k * rows + row0;
+            h = at, kind = 0;
+            if (h >= a.h[0].n) h -= a.h[0].n, kind = 1;
+            if (kind == 1 && h >= a.h[1].n) h -= a.h[1].n, kind = 2;
+            return at < total && 16 * u < a.h[kind].D && (kind == 0 || page >= 0);
+        };
+        auto halves = [&](int kind, int& d0, int& d1) {   // where the unit's two halves lie; true: rope_dim/2 apart
+            const bool split = turned && kind < 2 && !r.adjacent;
+            d0 = split ? 8 * u : 16 * u, d1 = split ? (r.rope_dim >> 1) + 8 * u : 16 * u + 8;
+            return split;
+        };
+        // all the group's loads, then its rows
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = unpack2<F16>(w0[i]), g = unpack2<F16>(w1[i]);
-                lo[2 * i] = f.x, lo[2 * i + 1] = f.y, hi[2 * i] = g.x, hi[2 * i + 1] = g.y;
+        for (int k = 0; k < GROUP; ++k) {
+            int h, kind, d0, d1;
+            if (locate(k, h, kind)) {
+                halves(kind, d0, d1);
+                const Heads& x = a.h[kind];
+                const uint16_t* p = x.src + t * x.src_tok + h * x.src_head;
+                v0[k] = load8<VEC>(p + d0), v1[k] = load8<VEC>(p + d1);
             }
-            auto pair = [](float& x1, float& x2, float cs, float sn) {
-                const float y1 = __fsub_rn(__fmul_rn(x1, cs), __fmul_rn(x2, sn));
-                x2 = __fadd_rn(__fmul_rn(x2, cs), __fmul_rn(x1, sn));
-                x1 = y1;
-            };
-            if (split) {
+        }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) pair(lo[i], hi[i], c[i], s[i]);
-            } else if (turn) {
+        for (int k = 0; k < GROUP; ++k) {
+            int h, kind, d0, d1;
+            const bool on = locate(k, h, kind), split = halves(kind, d0, d1), turn = turned && kind < 2;
+            const Heads& x = a.h[kind];
+            float lo[8], hi[8];   // dims d0 .. d0+7 and d1 .. d1+7
+            if (on) {
+                const uint32_t w0[4] = {v0[k].x, v0[k].y, v0[k].z, v0[k].w}, w1[4] = {v1[k].x, v1[k].y, v1[k].z, v1[k].w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    pair(lo[2 * i], lo[2 * i + 1], c[i], s[i]);
-                    pair(hi[2 * i], hi[2 * i + 1], c[4 + i], s[4 + i]);
+                    const float2 f = unpack2<F16>(w0[i]), g = unpack2<F16>(w1[i]);
+                    lo[2 * i] = f.x, lo[2 * i + 1] = f.y, hi[2 * i] = g.x, hi[2 * i + 1] = g.y;
+                }
+                auto pair = [](float& x1, float& x2, float cs, float sn) {
+                    const float y1 = __fsub_rn(__fmul_rn(x1, cs), __fmul_rn(x2, sn));
+                    x2 = __fadd_rn(__fmul_rn(x2, cs), __fmul_rn(x1, sn));
+                    x1 = y1;
+                };
+                if (split) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) pair(lo[i], hi[i], c[i], s[i]);
+                } else if (turn) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        pair(lo[2 * i], lo[2 * i + 1], c[i], s[i]);
+                        pair(hi[2 * i], hi[2 * i + 1], c[4 + i], s[4 + i]);
+                    }
                 }
             }
-        }
-        if (I8) {
-            float most = 0.f;
-            if (on && kind) {
+            if (I8) {
+                float most = 0.f;
+                if (on && kind) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
-            }
-            for (int o = a.lanes >> 1; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            if (on && kind) {
-                most = fmaxf(most, 1e-6f);
-                const float inv = __fdiv_rn(127.f, most);
-                auto codes = [&](const float* f) {
-                    uint32_t w[2] = {0, 0};
+                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+                }
+                for (int o = a.lanes >> 1; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                if (on && kind) {
+                    most = fmaxf(most, 1e-6f);
+                    const float inv = __fdiv_rn(127.f, most);
+                    auto codes = [&](const float* f) {
+                        uint32_t w[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int q = max(-128, min(127, __float2int_rn(__fmul_rn(f[i], inv))));
-                        w[i >> 2] |= (uint32_t)(q & 0xff) << (8 * (i & 3));
-                    }
-                    return make_uint2(w[0], w[1]);
-                };
-                uint8_t* p = x.dst + page * x.dst_page + off * x.dst_tok + h * x.dst_head;
-                *reinterpret_cast<uint2*>(p + d0) = codes(lo);
-                *reinterpret_cast<uint2*>(p + d1) = codes(hi);
-                if (u == 0) x.scales[page * x.s_page + off * x.s_tok + h * x.s_head] = __fmul_rn(most, 1.0f / 127.0f);
+                        for (int i = 0; i < 8; ++i) {
+                            const int q = max(-128, min(127, __float2int_rn(__fmul_rn(f[i], inv))));
+                            w[i >> 2] |= (uint32_t)(q & 0xff) << (8 * (i & 3));
+                        }
+                        return make_uint2(w[0], w[1]);
+                    };
+                    uint8_t* p = x.dst + page * x.dst_page + off * x.dst_tok + h * x.dst_head;
+                    *reinterpret_cast<uint2*>(p + d0) = codes(lo);
+                    *reinterpret_cast<uint2*>(p + d1) = codes(hi);
+                    if (u == 0) x.scales[page * x.s_page + off * x.s_tok + h * x.s_head] = __fmul_rn(most, 1.0f / 127.0f);
+                }
             }
-            if (kind) continue;
-        }
-        if (on) {
-            uint32_t w0[4], w1[4];
+            if (on && (!I8 || kind == 0)) {
+                uint32_t w0[4], w1[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w0[i] = pack2<F16>(lo[2 * i], lo[2 * i + 1]);
-                w1[i] = pack2<F16>(hi[2 * i], hi[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) {
+                    w0[i] = pack2<F16>(lo[2 * i], lo[2 * i + 1]);
+                    w1[i] = pack2<F16>(hi[2 * i], hi[2 * i + 1]);
+                }
+                const int64_t at = (kind ? page * x.dst_page + off * x.dst_tok : t * x.dst_tok) + h * x.dst_head;
+                uint16_t* p = reinterpret_cast<uint16_t*>(x.dst) + at;
+                store8<VEC>(p + d0, make_uint4(w0[0], w0[1], w0[2], w0[3]));
+                store8<VEC>(p + d1, make_uint4(w1[0], w1[1], w1[2], w1[3]));
             }
-            const int64_t at = kind ? page * x.dst_page + off * x.dst_tok + h * x.dst_head : t * x.dst_tok + h * x.dst_head;
-            uint16_t* p = reinterpret_cast<uint16_t*>(x.dst) + at;
-            store8<VEC>(p + d0, make_uint4(w0[0], w0[1], w0[2], w0[3]));
-            store8<VEC>(p + d1, make_uint4(w1[0], w1[1], w1[2], w1[3]));
         }
     }
 }
@@ -308,6 +341,7 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
             if ((int)((rope->axis_map[i >> 4] >> (2 * (i & 15))) & 3) >= rope->n_axes)
                 return set_error(WS_ERR_INVALID_ARG, "rope_append: a pair's axis has no positions");
         a.rope = *rope;
+        a.turns_vec = reinterpret_cast<uintptr_t>(rope->cos_sin) % 16 == 0;
     }
     a.N = N;
     a.status = device_status_word();
@@ -320,10 +354,17 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
     const int64_t blocks = (N * a.parts + kWarps - 1) / kWarps;
     if (blocks > INT32_MAX) return set_error(WS_ERR_UNSUPPORTED, "rope_append: too many tokens");
     const bool f16 = dtype == WS_DTYPE_F16, i8 = kv && kv->dtype == WS_DTYPE_I8;
-    auto fn = f16 ? (i8 ? (vec ? rope_append_kernel<true, true, true> : rope_append_kernel<true, true, false>)
-                        : (vec ? rope_append_kernel<true, false, true> : rope_append_kernel<true, false, false>))
-                  : (i8 ? (vec ? rope_append_kernel<false, true, true> : rope_append_kernel<false, true, false>)
-                        : (vec ? rope_append_kernel<false, false, true> : rope_append_kernel<false, false, false>));
+    // Two rows in flight a thread where a warp walks many (16384 tokens of 32 heads, us a call with one and two: rotary
+    // alone 51 and 48, append 67 and 62); with few rows, or int8 codes to compute, the registers cost more than that gives
+    // (5212 tokens of 3 heads of 256: 15 and 18; 4097 tokens into int8: 38 and 41).
+    const bool several = a.parts == 1 && steps >= 8 && !i8;
+    auto pick = [&](auto half, auto codes) {
+        constexpr bool F = decltype(half)::value, I = decltype(codes)::value;
+        return !vec ? rope_append_kernel<F, I, false, 1> : several ? rope_append_kernel<F, I, true, kGroup> : rope_append_kernel<F, I, true, 1>;
+    };
+    using yes = std::true_type;
+    using no = std::false_type;
+    auto fn = f16 ? (i8 ? pick(yes{}, yes{}) : pick(yes{}, no{})) : (i8 ? pick(no{}, yes{}) : pick(no{}, no{}));
     const cudaError_t e = launch_dependent(fn, dim3((unsigned)blocks), 32 * kWarps, 0, static_cast<cudaStream_t>(stream), a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -76,7 +76,7 @@ def build_binding(verbose: bool = False, force: bool = False) -> str:
            "-I" + INCLUDE, "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(root, "include"),
            "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-isystem", os.path.join(cuda, "include"), BINDING_SRC, "-o", BINDING + ".tmp",
-           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lc10_cuda", "-lc10"]
     out = subprocess.run(cmd, capture_output=True, text=True)
     if out.returncode != 0:
         raise RuntimeError(f"g++ failed on {BINDING_SRC}:\n{out.stdout}\n{out.stderr}")

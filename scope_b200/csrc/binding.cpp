@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -71,10 +72,14 @@ void want_rows(const char* what, const char* name, const at::Tensor& t, at::Scal
         refuse(what, std::string(name) + " must be " + c10::toString(type) + " [" + std::to_string(N) + ", heads, D] on " +
                          on(dev) + " with unit stride on the head dim");
 }
+// A new contiguous tensor on the current stream's allocator, without the dispatcher's round (0.5 us a tensor).
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Device& dev) {
+    return at::detail::empty_cuda(shape, type, dev, std::nullopt);
+}
 // `given` when it is a tensor of this shape and type, else a new one.
 at::Tensor output(const char* what, const char* name, PyObject* given, at::IntArrayRef shape, at::ScalarType type,
                   const at::Device& dev) {
-    if (given == Py_None) return at::empty(shape, at::TensorOptions().dtype(type).device(dev));
+    if (given == Py_None) return fresh(shape, type, dev);
     const at::Tensor& t = tensor(what, name, given);
     if (t.scalar_type() != type || t.sizes() != shape || !t.is_contiguous() || t.device() != dev)
         refuse(what, std::string(name) + " must be a contiguous " + c10::toString(type) + " tensor of the result's shape on " + on(dev));
@@ -170,9 +175,8 @@ PyObject* paged_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const c10::cuda::OptionalCUDAGuard guard(b.dev);
         const at::Tensor lens_out = output(what, "seq_lens_out", a[7], {b.B}, at::kInt, b.dev);
         const at::Tensor ring_out = output(what, "ring_out", a[8], {3}, at::kInt, b.dev);
-        const auto i32 = at::TensorOptions().dtype(at::kInt).device(b.dev);
-        const at::Tensor slots = at::empty({N}, i32.dtype(at::kLong)), positions = at::empty({N}, i32);
-        const at::Tensor cu = at::empty({b.B + 1}, i32);
+        const at::Tensor slots = fresh({N}, at::kLong, b.dev), positions = fresh({N}, at::kInt, b.dev);
+        const at::Tensor cu = fresh({b.B + 1}, at::kInt, b.dev);
         void* stream = c10::cuda::getCurrentCUDAStream(b.dev.index()).stream();
         const Workspace ws = workspace(g_slots_ws, b.dev, stream);
         check(p_paged_slots(data<int32_t>(lens), data<int32_t>(added), (int)b.B, data<int32_t>(table), table.stride(0),
@@ -269,7 +273,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const c10::cuda::OptionalCUDAGuard guard(dev);
         at::Tensor out;
         if (a[7] == Py_None) {
-            out = at::empty(x.sizes(), at::TensorOptions().dtype(x.scalar_type()).device(dev));
+            out = fresh(x.sizes(), x.scalar_type(), dev);
         } else {
             out = tensor(what, "out", a[7]);
             want_rows(what, "out", out, x.scalar_type(), N, dev);
@@ -351,7 +355,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
             want_rows(what, "q", q, st, N, dev);
             if (q.size(2) != p.Dk) refuse(what, "q must be [N, H, " + std::to_string(p.Dk) + "]");
             if (a[13] == Py_None) {
-                out = at::empty(q.sizes(), at::TensorOptions().dtype(st).device(dev));
+                out = fresh(q.sizes(), st, dev);
             } else {
                 out = tensor(what, "q_out", a[13]);
                 want_rows(what, "q_out", out, st, N, dev);

@@ -130,14 +130,15 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
                 s[4 * i] = y.x, s[4 * i + 1] = y.y, s[4 * i + 2] = y.z, s[4 * i + 3] = y.w;
             }
         } else {
-            int64_t row[4];   // of each axis
+            uint32_t at[4];   // each axis's position
 #pragma unroll
-            for (int x = 0; x < 4; ++x) row[x] = x < r.n_axes ? position(x) * r.rope_dim : 0;
+            for (int x = 0; x < 4; ++x) at[x] = x < r.n_axes ? (uint32_t)position(x) : 0;
+            const float* const unit = r.cos_sin + 8 * u;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int x = axes >> (2 * i) & 3;
-                const float* p = r.cos_sin + (x & 2 ? (x & 1 ? row[3] : row[2]) : (x & 1 ? row[1] : row[0])) + 8 * u + i;
-                c[i] = __ldg(p), s[i] = __ldg(p + n);
+                const float* p = unit + (x & 2 ? (x & 1 ? at[3] : at[2]) : (x & 1 ? at[1] : at[0])) * (uint64_t)(uint32_t)r.rope_dim;
+                c[i] = __ldg(p + i), s[i] = __ldg(p + n + i);
             }
         }
         if (r.inverse) {
@@ -335,7 +336,7 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
         const int Dk = kv ? kv->Dk : D;
         if (rope->rope_dim < 16 || rope->rope_dim % 16 || rope->rope_dim > Dk)
             return set_error(WS_ERR_INVALID_ARG, "rope_append: rope_dim must be a multiple of 16 within the head dim");
-        if (rope->n_axes < 1 || rope->n_axes > 4 || rope->max_pos < 1 || !rope->positions || !rope->cos_sin)
+        if (rope->n_axes < 1 || rope->n_axes > 4 || rope->max_pos < 1 || rope->max_pos > INT32_MAX || !rope->positions || !rope->cos_sin)
             return set_error(WS_ERR_INVALID_ARG, "rope_append: bad rope");
         for (int i = 0; i < rope->rope_dim / 2; ++i)
             if ((int)((rope->axis_map[i >> 4] >> (2 * (i & 15))) & 3) >= rope->n_axes)

@@ -779,3 +779,48 @@ def test_cache_refuses_what_does_not_fit_and_goes_on():
     assert cache.refused() == 0 and cache.free_pages() == 1 and cache.seq_lens.tolist() == [0, 20, 16]
     cache.reset()
     assert cache.free_pages() == 4 and cache.seq_lens.tolist() == [0, 0, 0]
+
+
+def test_decode_more_requests_than_one_launch_counts():
+    """A table so wide that its rows, were they full, pass the kernel's 32-bit count: several launches, one result."""
+    g = gen(30)
+    P, D, B = 1 << 20, 16, 20
+    k, v = (torch.empty(1, P, 1, D, dtype=BF, device=DEV) for _ in range(2))
+    k[0, :100], v[0, :100] = (torch.randn(100, 1, D, generator=g, device=DEV).to(BF) for _ in range(2))
+    lens = [(7 * b) % 101 for b in range(B)]
+    t = torch.zeros(B, 1024, dtype=torch.int32, device=DEV)
+    s = dict(q=torch.randn(B, 2, D, generator=g, device=DEV).to(BF), k=k, v=v, ks=None, vs=None, table=t,
+             lens=torch.tensor(lens, dtype=torch.int32, device=DEV), scale=D ** -0.5,
+             rows=[(torch.zeros(n, dtype=torch.long, device=DEV), torch.arange(n, device=DEV)) for n in lens])
+    agrees(s, *decode(s))
+    wide = torch.zeros(1, 1 << 11, dtype=torch.int32, device=DEV)
+    pool = torch.empty(1, P, 17, D, dtype=BF, device=DEV)
+    with pytest.raises(RuntimeError, match="too many tokens"):
+        paged.paged_decode(torch.zeros(1, 17, D, dtype=BF, device=DEV), pool, pool, wide, s["lens"][:1].contiguous(), 1.0)
+
+
+@pytest.mark.parametrize("dtype,pool", [(BF, BF), (HF, HF), (BF, torch.int8), (HF, torch.int8)])
+@pytest.mark.parametrize("D,Dv", [(64, 64), (128, 128), (256, 256), (192, 128), (80, 80)])
+def test_decode_variants_with_whole_and_split_pages(dtype, pool, D, Dv):
+    """Each compiled variant over lengths that end in every part of a subtile, pages of whole tiles and not."""
+    lens = list(range(1, 34)) + [47, 48, 49, 63, 64, 65, 96, 97, 700]
+    for P in (16, 32, 48, 20):
+        s = make_decode(lens, 12, 2, D, Dv, P, dtype, pool, heads_major=P == 32, seed=D + P)
+        agrees(s, *decode(s))
+        agrees(s, *decode(s, 33), window=33)
+    assert scope_b200.status_take() == 0
+
+
+def test_decode_int8_values_are_exact():
+    """One token: the output is its value row, code * scale, for every code."""
+    codes_ = torch.arange(-128, 128, dtype=torch.int16, device=DEV).to(torch.int8).view(1, 1, 1, 256)
+    for dtype in (BF, HF):
+        scale = torch.tensor([0.0371], device=DEV).view(1, 1, 1)
+        q = torch.randn(1, 1, 256, device=DEV).to(dtype)
+        one = torch.ones(1, dtype=torch.int32, device=DEV)
+        out, lse = paged.paged_decode(q, codes_, codes_, one.view(1, 1) * 0, one, 0.01, k_scales=scale, v_scales=scale)
+        want = codes_.view(-1).double() * scale.double().view(-1)
+        # the probability is 1: its product with the scale as two 16-bit values (2^-16), then one rounding of the result
+        assert ((out.view(-1).double() - want).abs() <= (U[dtype] + 2.0 ** -15) * want.abs()).all()
+        z = 0.01 * 0.0371 * (q.double().view(-1) @ codes_.view(-1).double())
+        assert (lse.double().view(()) - z).abs() <= 260 * 2.0 ** -24 * 0.01 * 0.0371 * (q.double().abs().view(-1) @ codes_.view(-1).double().abs()) + 1e-6

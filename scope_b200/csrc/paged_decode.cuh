@@ -889,11 +889,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 ahead = extra ? take : 0;
                 __syncthreads();
 #pragma unroll 1
-                for (int i = tid; i < (take + extra) * (kPiece / 4); i += 32 * kWarps) {
-                    const int p = i / (kPiece / 4), r = i - p * (kPiece / 4), c = p < take ? done + p : p - take;
+                for (int p = warp; p < take + extra; p += kWarps) {
                     // the first CTA filed the row as its slot 1, the others as their slot 0
-                    cp_async16_all(smem_u32(smem) + ((p + 2) * (kPiece / 4) + r) * 16,
-                                   a.pieces + ((int64_t)((p < take ? first0 : first1) + c) * 2 + (c == 0 ? 1 : 0)) * kPiece + r * 4);
+                    const int c = p < take ? done + p : p - take;
+                    const float* src = a.pieces + ((int64_t)((p < take ? first0 : first1) + c) * 2 + (c == 0 ? 1 : 0)) * kPiece + lane * 4;
+                    const uint32_t dst = smem_u32(smem) + ((p + 2) * kPiece + lane * 4) * 4;
+#pragma unroll
+                    for (int r = 0; r < kPiece / 4; r += 32)
+                        if (r + 32 <= kPiece / 4 || r + lane < kPiece / 4) cp_async16_all(dst + r * 16, src + r * 4);
                 }
                 const int round = done / room;
                 done += take;

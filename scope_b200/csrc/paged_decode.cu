@@ -10,7 +10,7 @@ namespace {
 // Heads a block: 8 (one tensor-core column tile) up to 8 query heads a kv head and at head dims past 128, else 16.  A
 // block reads its keys and values once, so fewer blocks mean fewer bytes, but more accumulators do not fit the registers.
 int tiles_of(int G, int DB) { return G <= 8 || DB > 128 ? 1 : 2; }
-int bound_of(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+int bound_of(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : D <= 192 ? 192 : 256; }
 
 }  // namespace
 }  // namespace ws

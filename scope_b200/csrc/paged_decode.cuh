@@ -80,7 +80,7 @@ template <bool I8, int DB, int NT>
 struct Cfg {
     static constexpr int kMt = DB / 16;                                   // accumulator fragments of a head tile
     static constexpr int kTok = I8 || DB == 64 ? 32 : 16;                 // tokens of a subtile
-    static constexpr int kWarps = DB == 256 ? 5 : DB == 128 ? (I8 || NT == 2 ? 8 : 10) : I8 ? (NT == 1 ? 16 : 12) : 10;
+    static constexpr int kWarps = DB == 256 ? 5 : DB == 192 ? (I8 ? 6 : 7) : DB == 128 ? (I8 || NT == 2 ? 8 : 10) : I8 ? (NT == 1 ? 16 : 12) : 10;
     static constexpr int kRow = I8 ? ((DB / 16) | 1) * 16 : DB * 2 + 16;  // bytes between rows in shared memory
     static constexpr int kStage = 2 * kTok * kRow + (I8 ? 8 * kTok : 0) + 16;
     static constexpr int kPiece = NT * (8 * DB + 16);                     // floats: fragments, then m and l of the heads
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     const int tok = lane & (kTok - 1);
     const int l8 = lane & 7, r4 = lane >> 3;   // copies: eight lanes a row, four rows at a time
     const int kchunks = I8 ? Dk >> 4 : Dk >> 3, vchunks = I8 ? Dv >> 4 : Dv >> 3;
-    constexpr int kCols = (I8 ? DB / 16 : DB / 8) >= 8 ? (I8 ? DB / 16 : DB / 8) / 8 : 1;
+    constexpr int kCols = ((I8 ? DB / 16 : DB / 8) + 7) / 8;
     const uint64_t k_lane = (uint64_t)r4 * a.kt + l8, v_lane = (uint64_t)r4 * a.vt + l8;
 
     auto look_up = [&]() {
@@ -1024,6 +1024,7 @@ template <bool F16, bool I8>
 int launch_any(const Args& a, int DB, int NT, int ctas, cudaStream_t st) {
     if (DB == 64) return NT == 1 ? launch_dims<F16, I8, 64, 1>(a, ctas, st) : launch_dims<F16, I8, 64, 2>(a, ctas, st);
     if (DB == 128) return NT == 1 ? launch_dims<F16, I8, 128, 1>(a, ctas, st) : launch_dims<F16, I8, 128, 2>(a, ctas, st);
+    if (DB == 192) return launch_dims<F16, I8, 192, 1>(a, ctas, st);
     return launch_dims<F16, I8, 256, 1>(a, ctas, st);
 }
 

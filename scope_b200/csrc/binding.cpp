@@ -119,10 +119,6 @@ template <typename T>
 T* data(const at::Tensor& t) {
     return static_cast<T*>(t.data_ptr());
 }
-template <typename T>
-T* data_or_null(PyObject* o) {
-    return o == Py_None ? nullptr : static_cast<T*>(THPVariable_Unpack(o).data_ptr());
-}
 
 // Runs a call: C++ exceptions become Python ones, and none leaves the entry.
 template <typename F>
@@ -159,6 +155,7 @@ Books bookkeeping(const char* what, const at::Tensor& lens, const at::Tensor& ot
     want(what, "ring", ring, at::kInt, 1, b.dev);
     if (other.numel() != b.B || ring.numel() != 3)
         refuse(what, std::string(name) + " must hold one entry per request, and ring three");
+    if (b.B > INT32_MAX || table.size(1) > INT32_MAX || free_pages.numel() > INT32_MAX) refuse(what, "bad shape");
     return b;
 }
 
@@ -269,6 +266,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (x.dim() != 3) refuse(what, "x must be [N, heads, D]");
         const int64_t N = x.size(0);
         want_rows(what, "x", x, x.scalar_type(), N, dev);
+        if (x.size(1) > INT32_MAX || x.size(2) > INT32_MAX) refuse(what, "bad shape");
         const ws_rope r = rope_of(what, a[1], a[2], N, dev, a[3], a[4], a[5], PyObject_IsTrue(a[6]) == 1);
         const c10::cuda::OptionalCUDAGuard guard(dev);
         at::Tensor out;
@@ -353,7 +351,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (a[0] != Py_None) {
             q = tensor(what, "q", a[0]);
             want_rows(what, "q", q, st, N, dev);
-            if (q.size(2) != p.Dk) refuse(what, "q must be [N, H, " + std::to_string(p.Dk) + "]");
+            if (q.size(2) != p.Dk || q.size(1) > INT32_MAX) refuse(what, "q must be [N, H, " + std::to_string(p.Dk) + "]");
             if (a[13] == Py_None) {
                 out = fresh(q.sizes(), st, dev);
             } else {
@@ -392,6 +390,7 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const ws_paged_kv p = pool_of(what, a[1], a[2], a[7], a[8], dev);
         if (p.dtype != type && p.dtype != WS_DTYPE_I8) refuse(what, "the pool must hold q's type or int8");
         if (q.size(2) != p.Dk || p.Hkv < 1 || H < 1 || H % p.Hkv) refuse(what, "q must be [B, Hkv * G, Dk]");
+        if (B > INT32_MAX || H > INT32_MAX) refuse(what, "bad shape");
         want_table(what, table, B, dev);
         want(what, "seq_lens", lens, at::kInt, 1, dev);
         if (lens.numel() != B) refuse(what, "seq_lens must hold one entry per request");

@@ -46,6 +46,9 @@ int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
         workspace_bytes < ws_paged_decode_workspace_size(B, kv->Hkv, G, kv->Dv))
         return set_error(WS_ERR_WORKSPACE, "paged_decode: workspace missing, unaligned or too small");
+    // the kernel keeps a kv head and its block of query heads in one word
+    if (kv->Hkv > INT16_MAX || G > (1 << 18) || (int64_t)kv->Hkv * G > (1 << 24))
+        return set_error(WS_ERR_UNSUPPORTED, "paged_decode: too many heads");
     const bool f16 = q_dtype == WS_DTYPE_F16, i8 = kv->dtype == WS_DTYPE_I8;
     const int64_t eb = i8 ? 1 : 2;
     const int D = std::max(kv->Dk, kv->Dv), DB = bound_of(D), NT = tiles_of(G, DB);

@@ -223,9 +223,9 @@ __device__ __forceinline__ void finish(const Args& a, int64_t head0, int left, i
     const int lane = threadIdx.x & 31, t = lane & 3;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        inv[j] = l[j] > 0.f ? 1.f / l[j] : 0.f;
+        inv[j] = l[j] != 0.f ? 1.f / l[j] : 0.f;   // a NaN stays one
         const int h = nt * 8 + 2 * t + j;
-        if (write && a.lse && lane < 4 && h < left) a.lse[head0 + h] = l[j] > 0.f ? m[j] * kLn2 + logf(l[j]) : -INFINITY;
+        if (write && a.lse && lane < 4 && h < left) a.lse[head0 + h] = l[j] != 0.f ? m[j] * kLn2 + logf(l[j]) : -INFINITY;
     }
 }
 

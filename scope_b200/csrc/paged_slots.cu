@@ -115,7 +115,7 @@ paged_slots_kernel(const int32_t* seq_lens, const int32_t* __restrict__ new_lens
     if (threadIdx.x == 0) n_refused = 0;
     pdl_wait_primary();
     pdl_launch_dependents();
-    const int head = ring[0], n_free = min(max(ring[1], 0), n_ring);
+    const int head = max(ring[0], 0), n_free = min(max(ring[1], 0), n_ring);
     Two sums;   // tokens, pages
     long long took;
     int refused;
@@ -210,7 +210,7 @@ paged_release_kernel(const int32_t* seq_lens, const uint8_t* __restrict__ done, 
     int* end = sm;   // pages of requests 0 .. b that go back
     pdl_wait_primary();
     pdl_launch_dependents();
-    const int head = ring[0], n_free = min(max(ring[1], 0), n_ring);
+    const int head = max(ring[0], 0), n_free = min(max(ring[1], 0), n_ring);
     const int room = n_ring - n_free;
     Two pages = {0, 0};
     for (int b0 = 0; b0 < B; b0 += blockDim.x) {

@@ -824,3 +824,42 @@ def test_decode_int8_values_are_exact():
         assert ((out.view(-1).double() - want).abs() <= (U[dtype] + 2.0 ** -15) * want.abs()).all()
         z = 0.01 * 0.0371 * (q.double().view(-1) @ codes_.view(-1).double())
         assert (lse.double().view(()) - z).abs() <= 260 * 2.0 ** -24 * 0.01 * 0.0371 * (q.double().abs().view(-1) @ codes_.view(-1).double().abs()) + 1e-6
+
+
+@pytest.mark.parametrize("pool", [BF, torch.int8])
+def test_decode_passes_a_nan_on_to_its_rows_alone(pool):
+    """A NaN key gives its request and kv head NaN, in the output and in lse; every other row stays as it was."""
+    s = make_decode([700, 40, 300], 8, 2, 64, 64, 16, BF, pool=pool, seed=53)
+    out, lse = (x.clone() for x in decode(s))
+    page, at = int(s["table"][0, 5]), 3
+    if pool == torch.int8:
+        s["ks"][page, at, 1] = float("nan")
+    else:
+        s["k"][page, at, 1, 0] = float("nan")
+    bad, bad_lse = decode(s)
+    assert bad[0, 4:].isnan().all() and bad_lse[0, 4:].isnan().all()
+    out[0, 4:], lse[0, 4:], bad[0, 4:], bad_lse[0, 4:] = 0, 0, 0, 0
+    assert torch.equal(out, bad) and torch.equal(lse, bad_lse)
+
+
+def test_decode_refuses_more_heads_than_it_counts():
+    k = torch.zeros(1, 16, 1, 16, dtype=BF, device=DEV).expand(1, 16, 40000, 16)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="too many heads"):
+        paged.paged_decode(torch.zeros(1, 40000, 16, dtype=BF, device=DEV), k, k, table, lens, 1.0)
+    k = torch.zeros(1, 16, 1, 16, dtype=BF, device=DEV)
+    with pytest.raises(RuntimeError, match="too many heads"):
+        paged.paged_decode(torch.zeros(1, (1 << 18) + 8, 16, dtype=BF, device=DEV), k, k, table, lens, 1.0)
+
+
+def test_slots_take_a_negative_head_as_the_rings_start():
+    """The ring's words are the caller's memory: whatever they hold, a page comes from within the ring."""
+    free = np.arange(100, 108, dtype=np.int32)
+    lens, new, table = np.zeros(1, np.int32), np.full(1, 20, np.int32), np.full((1, 4), -1, np.int32)
+    for count in (8, 1 << 30):
+        got, d = run_slots(lens, new, table, free, np.array([-5, count, 0], np.int32), 16, 20)
+        assert got[0].tolist() == [1600 + i for i in range(20)] and got[4].tolist() == [2, 6, 0]
+    d[4].copy_(torch.tensor([-5, 6, 0]))
+    lens_out, ring = paged.paged_release(torch.full((1,), 20, dtype=torch.int32, device=DEV),
+                                         torch.ones(1, dtype=torch.bool, device=DEV), d[2], d[3], d[4], 16)
+    assert ring.tolist() == [0, 8, 0] and d[3].tolist() == [100, 101, 102, 103, 104, 105, 100, 101]

@@ -8,14 +8,18 @@
 //
 //   * Rows (request, kv head, block of 8*NT query heads) are cut into subtiles of 16 or 32 tokens, laid end to end, and the
 //     line is split evenly over the CTAs (one a SM) and again over each CTA's warps.  Every warp runs alone over its
-//     stretch with its own ring of S stages filled by 16-byte cp.async, so no warp ever waits for another and a short
-//     row costs no barrier.  The lengths are read on the device; the host never needs them.
+//     stretch with its own ring of S stages, so no warp ever waits for another and a short row costs no barrier.  The
+//     lengths are read on the device; the host never needs them.
+//   * A stage is filled by TMA where the pages are whole 16-token tiles, Dk = Dv is the variant's bound and the pool's
+//     strides are what a tensor map takes; else by 16-byte cp.async (any page size, any head dims).  The memory gives more
+//     to the fewer and larger requests: loads alone run at 7.3 TB/s in blocks of 4 KB by TMA, 6.7 in 16-byte pieces, 6.7
+//     in rows of 256 bytes by bulk copies.  Measured: 32 requests of 131072 tokens 1316 us with cp.async, 1199 with TMA;
+//     16 ragged 141 and 131; 8 in int8 76.7 and 75.6; 1 request of 4096 tokens 11.9 and 11.5.
 //   * A subtile is one stage.  With pages of whole 16-token tiles a tile has one page, and its rows lie at one stride; else
 //     each lane looks up one token's page and the row addresses travel by shuffle.  Entries are fetched a subtile ahead.
-//     Tokens past the length, before the window or on a page that is none are not read: their shared-memory rows are
-//     zero and their scores -inf.
-//   * Rows in shared memory are an odd number of 16-byte pieces apart, so ldmatrix reads are free of bank conflicts for
-//     every head dim without a swizzle.
+//     Of tokens past the length, before the window or on a page that is none, the scores are -inf, and the values in
+//     shared memory zero, whatever the pool holds there.
+//   * ldmatrix reads are free of bank conflicts: TMA swizzles; cp.async puts rows an odd number of 16-byte pieces apart.
 //   * S^T[16 tok x 8 heads] = K . Q^T and O^T[Dv x 8] += V^T . P^T by mma.sync with the heads as the narrow dimension:
 //     at G <= 8 query heads a key there is no 128-row tile for tcgen05 to fill, and the tensor pipe is nearly idle.
 //   * The softmax's reference moves only when a score passes it by 2^kSlack: then, and not every subtile, the lanes
@@ -27,11 +31,11 @@
 //     which the CTA joins in shared memory; what crosses CTAs goes through the workspace and is joined by the CTA that
 //     files the last part (a ticket), always in the same order, so results do not depend on timing.
 //
-// Measured on a B200 (device time): 32 requests of 131072 tokens, 32 query and 4 kv heads of 128, bf16: 1310 us
-// (8.59 GB, 6.55 TB/s, what a copy reaches); 16 ragged to 32768 tokens, 32 and 8 heads: 141 us (852 MB, 6.05 TB/s);
-// 8 of 16384 to 65536 tokens in int8: 77 us (393 MB, 5.1 TB/s).  What is left at those is some 4 us before the first
+// Measured on a B200 (device time): 32 requests of 131072 tokens, 32 query and 4 kv heads of 128, bf16: 1199 us
+// (8.59 GB, 7.17 TB/s; a copy reaches 6.55); 16 ragged to 32768 tokens, 32 and 8 heads: 131 us (852 MB, 6.5 TB/s);
+// 8 of 16384 to 65536 tokens in int8: 76 us (393 MB, 5.2 TB/s).  What is left at those is some 4 us before the first
 // rows arrive (the lengths, the table and the rows come one after the other) and 8 us after the last (join, ticket,
-// join).  Small calls are those latencies alone: 1 request of 4096 tokens 11.9 us, of 100 tokens 6 us.
+// join).  Small calls are those latencies alone: 1 request of 4096 tokens 11.5 us, of 100 tokens 6 us.
 //
 // Why an even split suffices: with 128 KB of copies in flight an SM, 16 of the 148 SMs ended 10% after the others, which
 // the memory serves first; with 80 KB all end within 3% of one another, and the whole sooner.  Built and measured slower:
@@ -48,7 +52,7 @@ namespace ws {
 namespace paged {
 
 // Shared memory for the rings: a CTA's 227 KB without what the kernel declares itself.
-constexpr int most_smem(int warps) { return ((227 << 10) - 432 * warps - 128) & ~15; }
+constexpr int most_smem(int warps) { return ((227 << 10) - 464 * warps - 128) & ~15; }
 constexpr int kMinTok = 32;     // tokens a warp takes before another CTA joins in
 // Rows up to so many tokens are not cut by a border between two CTAs, or two warps: the border moves to the nearer end
 // of the row, which unbalances the stretches by half a row at most and saves the joining (about 5 us; measured with
@@ -58,7 +62,12 @@ constexpr int kSnapCta = 640;
 constexpr int kSnapWarp = 64;
 constexpr float kSlack = 6.f;   // log2 of how far a probability may pass its bound before the reference moves
 
+// Bytes of a row that one TMA box takes, and one span of its swizzle.
+constexpr int inner_of(int row_bytes) { return row_bytes % 128 ? 64 : 128; }
+
 struct Args {
+    CUtensorMap kmap, vmap;              // where tma: boxes of 16 tokens of one head and page
+    int tma, k_head_dim2, v_head_dim2;   // the map's order: dims, tokens, heads, pages; else dims, heads, tokens, pages
     const uint16_t* q;
     int64_t q_b, q_h;                    // elements
     const uint8_t* k;
@@ -86,7 +95,8 @@ struct Args {
 
 // The variant for head dims up to DB, 8*NT query heads a block.  A subtile is 16 tokens, or 32 where 16 would be 4 KB or
 // less (int8, head dims up to 64): what a subtile costs beside its bytes then counts half (measured with int8 rows of 128,
-// 8 requests to 65536: 82 us to 78; 127 requests to 13489 with rows of 64: 167 us to 132).  As many warps, each with two stages, as shared memory and the registers allow
+// 8 requests to 65536: 82 us to 78; 127 requests to 13489 with rows of 64: 167 us to 132).  As many warps, each with two
+// stages, as shared memory and the registers allow
 // (measured at D = 128 in 16 bits, 16 ragged requests to 32768: 8 warps 160 us, 10 warps 152, 12 warps 157; three stages
 // put more in flight than the memory takes, and the SMs it serves last fall behind).
 template <bool I8, int DB, int NT>
@@ -94,15 +104,25 @@ struct Cfg {
     static constexpr int kMt = DB / 16;                                   // accumulator fragments of a head tile
     static constexpr int kTok = I8 || DB == 64 ? 32 : 16;                 // tokens of a subtile
     static constexpr int kWarps = DB == 256 ? 5 : DB == 192 ? (I8 ? 6 : 7) : DB == 128 ? (I8 || NT == 2 ? 8 : 10) : I8 ? (NT == 1 ? 16 : 12) : 10;
-    static constexpr int kRow = I8 ? ((DB / 16) | 1) * 16 : DB * 2 + 16;  // bytes between rows in shared memory
-    static constexpr int kStage = 2 * kTok * kRow + (I8 ? 8 * kTok : 0) + 16;
     static constexpr int kPiece = NT * (8 * DB + 16);                     // floats: fragments, then m and l of the heads
     static constexpr int kUnits = NT * kMt;
-    static constexpr int kFit = (most_smem(kWarps) / kWarps - kPiece * 4) / kStage;
+    // kExact: stages of rows an odd number of 16-byte pieces apart, each with its scales and meta, then the first part (a
+    // stretch's last part takes the ring's place)
+    static constexpr int kGapRow = I8 ? ((DB / 16) | 1) * 16 : DB * 2 + 16;
+    static constexpr int kGapStage = 2 * kTok * kGapRow + (I8 ? 8 * kTok : 0) + 16;
+    static constexpr int kGapFit = (most_smem(kWarps) / kWarps - kPiece * 4) / kGapStage;
+    static constexpr int kGapStages = kGapFit > 4 ? 4 : kGapFit;
+    static constexpr int kGapWarpSmem = kGapStages * kGapStage + kPiece * 4;
+    static_assert(kGapStages >= 2 && kGapStages * kGapStage >= kPiece * 4 && kGapStage % 16 == 0, "ring");
+    // kTma: the stages' rows, swizzled and so without gaps, then their scales and meta, then the first part
+    static constexpr int kRowB = DB * (I8 ? 1 : 2);
+    static constexpr int kInner = inner_of(kRowB), kParts = kRowB / kInner;
+    static constexpr int kTile = 16 * kRowB;                              // 16 tokens' keys, or values
+    static constexpr int kRows = 2 * kTok * kRowB, kMore = (I8 ? 8 * kTok : 0) + 16;
+    static constexpr int kFit = (((most_smem(kWarps) - 1024) / kWarps & ~1023) - kPiece * 4) / (kRows + kMore);
     static constexpr int kStages = kFit > 4 ? 4 : kFit;
-    static constexpr int kWarpSmem = kStages * kStage + kPiece * 4;       // the ring, which ends as the place of the last
-                                                                          // part, and the first part
-    static_assert(kStages >= 2 && kStages * kStage >= kPiece * 4 && kStage % 16 == 0, "ring");
+    static constexpr int kWarpSmem = (kStages * (kRows + kMore) + kPiece * 4 + 1023) & ~1023;
+    static_assert(kStages >= 2 && kStages * kRows >= kPiece * 4 && kRows % 1024 == 0, "ring");
 };
 inline int piece_floats(int DB, int NT) { return NT * (8 * DB + 16); }
 
@@ -229,18 +249,26 @@ __device__ __forceinline__ void finish(const Args& a, int64_t head0, int left, i
     }
 }
 
-// EXACT: Dk = Dv = DB, known when compiling: no bounds on the pieces of a row
-// (358 instructions a subtile to 305 with 16-bit rows, 611 to 518 with int8).
-template <bool F16, bool I8, int DB, int NT, bool EXACT>
+// How rows come, and what is known of them when compiling.
+enum : int {
+    kAny = 0,     // 16-byte cp.async; head dims up to DB
+    kExact = 1,   // 16-byte cp.async; Dk = Dv = DB, so a row's pieces need no bounds (358 instructions a subtile to 305
+                  // with 16-bit rows, 611 to 518 with int8; 2 requests of 100 tokens in pages of 8: 6.4 us to 4.9)
+    kTma = 2,     // TMA; Dk = Dv = DB, pages of whole 16-token tiles
+};
+template <bool F16, bool I8, int DB, int NT, int MODE>
 __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
     using C = Cfg<I8, DB, NT>;
+    constexpr bool EXACT = MODE != kAny, TMA = MODE == kTma;
     constexpr int kWarps = C::kWarps, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
     constexpr int kTok = C::kTok, H = kTok / 16;   // H: 16-token tiles of a subtile
     constexpr int kMinSub = kMinTok / kTok, kSnapC = kSnapCta / kTok, kSnapW = kSnapWarp / kTok;
     constexpr bool kPF16 = F16 && !I8;   // the type of P and V in the second product (bf16's range for scaled P)
     // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
     constexpr float kUp = kPF16 ? 8.f : 0.f;
-    extern __shared__ __align__(16) uint8_t smem[];   // [kWarps][kWarpSmem]
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t* const smem = TMA ? smem_raw + (-smem_u32(smem_raw) & 1023) : smem_raw;   // [kWarps][warp_smem]
+    __shared__ uint64_t s_bar[TMA ? kWarps * 4 : 1];
     __shared__ int s_border[kWarps], s_scan[kWarps], s_from[32 * kWarps], s_start[2 * kWarps];   // s_start < 0: no part
     __shared__ int s_list[kWarps][32], s_cnt[32 * kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
 
@@ -248,6 +276,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     const int g = lane >> 2, t4 = lane & 3;
     const int R = a.Hkv * a.hb;          // rows of a request
     const int Dk = EXACT ? DB : a.Dk, Dv = EXACT ? DB : a.Dv;
+    const int S = TMA ? C::kStages : EXACT ? C::kGapStages : a.stages;
+    const uint32_t bars = smem_u32(s_bar) + warp * 32;
+    if (TMA) {
+        if (lane < S) mbar_init(bars + 8 * lane, 1);
+        if (lane < 2) tma_prefetch_desc(lane ? &a.vmap : &a.kmap);
+        fence_mbar_init();
+        __syncwarp();
+    }
 
     // A programmatic dependent launch: everything before this overlaps the kernel before; its writes are seen after.
     pdl_wait_primary();
@@ -385,18 +421,20 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 
     // ---- this warp's stretch
     const int count = w1 - w0;
-    const int warp_smem = EXACT ? C::kWarpSmem : a.warp_smem;
+    const int warp_smem = TMA ? C::kWarpSmem : EXACT ? C::kGapWarpSmem : a.warp_smem;
     uint8_t* const ring = smem + warp * warp_smem;
     float* const first_part = reinterpret_cast<float*>(ring + warp_smem) - kPiece;
     const uint32_t ring_u = smem_u32(ring);
-    // a stage: key rows, value rows, int8 scales (the keys', the values'), meta
-    const int S = EXACT ? C::kStages : a.stages;
-    const int krow = EXACT ? C::kRow : a.krow, vrow = EXACT ? C::kRow : a.vrow;
-    const int kV = kTok * krow, kS = kV + kTok * vrow, kM = kS + (I8 ? 8 * kTok : 0), stage = kM + 16;
+    // a stage: key rows, value rows; int8 scales (the keys', the values'), meta
+    const int krow = TMA ? C::kRowB : EXACT ? C::kGapRow : a.krow, vrow = TMA ? C::kRowB : EXACT ? C::kGapRow : a.vrow;
+    const int kV = kTok * krow, rows = kV + kTok * vrow, stage = TMA ? rows : rows + C::kMore;
+    auto scales_at = [&](int slot) { return TMA ? S * C::kRows + slot * C::kMore : slot * stage + rows; };
+    auto meta_at = [&](int slot) { return scales_at(slot) + C::kMore - 16; };
     float* const cta_pieces = a.pieces + (int64_t)blockIdx.x * 2 * kPiece;
 
     // filler: the row being filled, and the next subtile's page entry (of this lane's 16 tokens, or of its token where
     // pages are not whole tiles)
+    bool dead = false;   // a copy did not come within its limit: no more are asked for
     Span fs = {0, 0, 0};
     int f_b = 0, f_kvh = 0, f_blk = 0, f_sub = 0, f_entry = -1, f_left = count;
     uint32_t f_off = 0;
@@ -435,45 +473,66 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 const uint64_t ks = page * (uint64_t)a.ksp + off * (uint64_t)a.kst + f_kvh * (uint64_t)a.ksh;
                 const uint64_t vs = page * (uint64_t)a.vsp + off * (uint64_t)a.vst + f_kvh * (uint64_t)a.vsh;
                 const bool on = (mask >> tok) & 1;
-                cp_async4(st + kS + tok * 4, a.ks + ks, on);
-                cp_async4(st + kS + 4 * kTok + tok * 4, a.vs + vs, on);
+                cp_async4(ring_u + scales_at(slot) + tok * 4, a.ks + ks, on);
+                cp_async4(ring_u + scales_at(slot) + 4 * kTok + tok * 4, a.vs + vs, on);
             }
             if (lane == 0) {
                 Meta m;
                 m.mask = mask;
                 m.b = f_b, m.row = f_kvh << 16 | f_blk, m.sub = f_sub | (f_sub == fs.n - 1 ? INT32_MIN : 0);
-                *reinterpret_cast<Meta*>(ring + slot * stage + kM) = m;
+                *reinterpret_cast<Meta*>(ring + meta_at(slot)) = m;
             }
-            const uint32_t kd = st + r4 * krow + l8 * 16, vd = st + kV + r4 * vrow + l8 * 16;
-            if (a.whole && mask == kAll) {
+            if (TMA) {   // a box of each 16-token tile with a token that counts, for keys and values
+                const uint32_t bar = bars + 8 * slot;
+                const int page1 = H == 2 ? __shfl_sync(0xffffffffu, (int)page, 16) : 0;
+                const int off1 = H == 2 ? __shfl_sync(0xffffffffu, (int)f_off, 16) : 0;
+                if (lane == 0 && !dead) {
+                    const int tiles = ((mask & 0xffff) != 0) + (H == 2 && (mask >> 16) != 0);
+                    mbar_arrive_expect_tx(bar, tiles * 2 * C::kTile);
 #pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    const uint64_t kb = H == 1 ? ka : __shfl_sync(0xffffffffu, ka, 16 * h);
-                    const uint64_t vb = H == 1 ? va : __shfl_sync(0xffffffffu, va, 16 * h);
-                    const uint8_t *kp = a.k + ((kb + k_lane) << 4), *vp = a.v + ((vb + v_lane) << 4);
+                    for (int h = 0; h < H; ++h) {
+                        if ((mask >> (16 * h) & 0xffff) == 0) continue;
+                        const int at = h ? off1 : (int)f_off, pg = h ? page1 : (int)page;
 #pragma unroll
-                    for (int i = 4 * h; i < 4 * h + 4; ++i) {
-#pragma unroll
-                        for (int j = 0; j < kCols; ++j) {
-                            if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * krow + j * 128, kp + j * 128);
-                            if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * vrow + j * 128, vp + j * 128);
+                        for (int p = 0; p < C::kParts; ++p) {
+                            const uint32_t to = st + h * C::kTile + p * 16 * C::kInner;
+                            tma_load_4d(to, &a.kmap, bar, p * C::kInner, a.k_head_dim2 ? at : f_kvh, a.k_head_dim2 ? f_kvh : at, pg);
+                            tma_load_4d(to + kV, &a.vmap, bar, p * C::kInner, a.v_head_dim2 ? at : f_kvh, a.v_head_dim2 ? f_kvh : at, pg);
                         }
-                        kp += (uint64_t)a.kt << 6, vp += (uint64_t)a.vt << 6;
                     }
                 }
             } else {
-#pragma unroll
-                for (int i = 0; i < kTok / 4; ++i) {
-                    const int row = 4 * i + r4;
-                    const bool on = (mask >> row) & 1;
-                    const int in_page = a.whole && on ? row & 15 : 0, src = a.whole ? row & 16 : row;
-                    const uint64_t kr = __shfl_sync(0xffffffffu, ka, src) + in_page * (uint64_t)a.kt;
-                    const uint64_t vr = __shfl_sync(0xffffffffu, va, src) + in_page * (uint64_t)a.vt;
-                    const uint8_t *kp = a.k + ((kr + l8) << 4), *vp = a.v + ((vr + l8) << 4);
-#pragma unroll
-                    for (int j = 0; j < kCols; ++j) {
-                        if (l8 + 8 * j < kchunks) cp_async16(kd + 4 * i * krow + j * 128, kp + j * 128, on);
-                        if (l8 + 8 * j < vchunks) cp_async16(vd + 4 * i * vrow + j * 128, vp + j * 128, on);
+                const uint32_t kd = st + r4 * krow + l8 * 16, vd = st + kV + r4 * vrow + l8 * 16;
+                if (a.whole && mask == kAll) {
+    #pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        const uint64_t kb = H == 1 ? ka : __shfl_sync(0xffffffffu, ka, 16 * h);
+                        const uint64_t vb = H == 1 ? va : __shfl_sync(0xffffffffu, va, 16 * h);
+                        const uint8_t *kp = a.k + ((kb + k_lane) << 4), *vp = a.v + ((vb + v_lane) << 4);
+    #pragma unroll
+                        for (int i = 4 * h; i < 4 * h + 4; ++i) {
+    #pragma unroll
+                            for (int j = 0; j < kCols; ++j) {
+                                if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * krow + j * 128, kp + j * 128);
+                                if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * vrow + j * 128, vp + j * 128);
+                            }
+                            kp += (uint64_t)a.kt << 6, vp += (uint64_t)a.vt << 6;
+                        }
+                    }
+                } else {
+    #pragma unroll
+                    for (int i = 0; i < kTok / 4; ++i) {
+                        const int row = 4 * i + r4;
+                        const bool on = (mask >> row) & 1;
+                        const int in_page = a.whole && on ? row & 15 : 0, src = a.whole ? row & 16 : row;
+                        const uint64_t kr = __shfl_sync(0xffffffffu, ka, src) + in_page * (uint64_t)a.kt;
+                        const uint64_t vr = __shfl_sync(0xffffffffu, va, src) + in_page * (uint64_t)a.vt;
+                        const uint8_t *kp = a.k + ((kr + l8) << 4), *vp = a.v + ((vr + l8) << 4);
+    #pragma unroll
+                        for (int j = 0; j < kCols; ++j) {
+                            if (l8 + 8 * j < kchunks) cp_async16(kd + 4 * i * krow + j * 128, kp + j * 128, on);
+                            if (l8 + 8 * j < vchunks) cp_async16(vd + 4 * i * vrow + j * 128, vp + j * 128, on);
+                        }
                     }
                 }
             }
@@ -614,11 +673,20 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     }
     const int first_b = f_b, first_row = f_kvh << 16 | f_blk;
     int slot = 0;   // the stage that iteration `it` reads; the one before it is filled
+    uint32_t phase = 0;
 #pragma unroll 1
     for (int it = 1 - S; it < count; ++it) {
         if (it >= 0) {
-            if (EXACT) {
-                cp_async_wait<C::kStages - 2>();
+            if (TMA) {
+                if (I8) cp_async_wait<C::kStages - 2>();   // the scales
+                if (!dead && !mbar_wait_bounded(bars + 8 * slot, phase)) {
+                    if (a.status) atomicExch(a.status, kDevTimeout);
+                    mbar_wait_bounded(bars + 8 * slot, phase);   // what is in flight
+                    dead = true;
+                }
+                dead = __any_sync(0xffffffffu, dead);
+            } else if (EXACT) {
+                cp_async_wait<C::kGapStages - 2>();
             } else {
                 if (S == 2) cp_async_wait<0>();
                 else if (S == 3) cp_async_wait<1>();
@@ -629,7 +697,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         const uint32_t st = ring_u + slot * stage;
         Meta meta;
         if (it < 0) meta.b = first_b, meta.row = first_row, meta.sub = it == 1 - S ? 0 : 1;
-        else meta = *reinterpret_cast<const Meta*>(ring + slot * stage + kM);
+        else meta = *reinterpret_cast<const Meta*>(ring + meta_at(slot));
         const bool ends = meta.sub < 0;
         meta.sub &= INT32_MAX;
         // a row's queries (the first row's before anything else is asked for)
@@ -651,6 +719,26 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 for (int h = 0; h < H; ++h) c[h][nt][i] = 0.f;
                 if (kChains == 2) e[nt][i] = 0.f;
             }
+        // values of tokens that do not count, which TMA brought with the others: zero (int8 codes are finite)
+        if (TMA && !I8 && meta.mask != (kTok == 32 ? 0xffffffffu : 0xffffu)) {
+            constexpr int kLine = C::kInner / 16;
+            const uint32_t off = ~meta.mask >> lane / kLine;
+#pragma unroll
+            for (int i = 0; i < kTok * C::kRowB / 512; ++i) {   // 32 / kLine tokens at a time
+                constexpr int kStep = 32 / kLine;
+                const int tile = i * 32 / (C::kTile / 16), tok_in = i * kStep & 15;
+                if (off >> (16 * tile + tok_in) & 1)
+                    *reinterpret_cast<uint4*>(ring + slot * stage + kV + (i * 32 + lane) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            if (f_left > 0) fence_proxy_async_smem();   // before TMA writes there again
+            __syncwarp();
+        }
+        // with TMA: 16-byte piece `c` (even) of a lane's row lies where the swizzle puts it
+        constexpr int kLine = C::kInner / 16;
+        const uint32_t turn_of = C::kInner == 128 ? (lane & 7) << 4 : (lane >> 1 & 3) << 4;
+        auto piece = [&](uint32_t base, int row, int hi, int c) {
+            return base + row * C::kInner + ((hi << 4 ^ turn_of) ^ (c % kLine << 4)) + c / kLine * 16 * C::kInner;
+        };
         const uint32_t k_ld = st + (lane & 15) * krow + (lane >> 4) * 16;
         if (I8) {
 #pragma unroll
@@ -659,7 +747,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t r[4];
-                    ldsm_x4(k_ld + h * 16 * krow + ks * 16, r[0], r[1], r[2], r[3]);
+                    ldsm_x4(TMA ? piece(st + h * C::kTile, lane & 15, lane >> 4, ks) : k_ld + h * 16 * krow + ks * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {   // past an odd nks the queries are zero and what was read is finite
                         const uint32_t a0 = s8_pair<F16>(r[2 * u]), a1 = s8_pair<F16>(r[2 * u + 1]);
@@ -677,14 +765,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t a0, a1, a2, a3;
-                    ldsm_x4(k_ld + h * 16 * krow + ks * 32, a0, a1, a2, a3);
+                    ldsm_x4(TMA ? piece(st + h * C::kTile, lane & 15, lane >> 4, 2 * ks) : k_ld + h * 16 * krow + ks * 32, a0, a1, a2, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         mma16<F16>(kChains == 2 && (ks & 1) ? e[nt] : c[h][nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
                 }
             }
         }
-        const float* sc = reinterpret_cast<const float*>(ring + slot * stage + kS);
+        const float* sc = reinterpret_cast<const float*>(ring + scales_at(slot));
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const float f0 = I8 ? sc[16 * h + g] * (s8_unit<F16> * a.scale_log2) : a.scale_log2;
@@ -769,7 +857,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t r[4];
-                    ldsm_x4_t(v_ld + h * 16 * vrow + mt * 16, r[0], r[1], r[2], r[3]);
+                    ldsm_x4_t(TMA ? piece(st + kV + h * C::kTile, lane & 15, lane >> 4, mt) : v_ld + h * 16 * vrow + mt * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {   // past an odd nmt: accumulators that nobody reads
                         const uint32_t a0 = s8_pair<kPF16>(r[2 * u]), a1 = s8_pair<kPF16>(r[2 * u] >> 8);
@@ -790,7 +878,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     uint32_t a0, a1, a2, a3;
-                    ldsm_x4_t(v_ld + h * 16 * vrow + mt * 32, a0, a1, a2, a3);
+                    ldsm_x4_t(TMA ? piece(st + kV + h * C::kTile, (lane & 7) + (lane >> 4 << 3), lane >> 3 & 1, 2 * mt) : v_ld + h * 16 * vrow + mt * 32, a0, a1, a2, a3);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, ph[h][nt][0], ph[h][nt][1]);
@@ -834,7 +922,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 }
             }
         }
-        slot = slot == S - 1 ? 0 : slot + 1;
+        if (++slot == S) slot = 0, phase ^= 1;
     }
     __syncthreads();
 
@@ -999,11 +1087,11 @@ int launch_f16(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 int launch_bf16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 int launch_f16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
 
-template <bool F16, bool I8, int DB, int NT, bool EXACT>
+template <bool F16, bool I8, int DB, int NT, int MODE>
 int launch(Args a, int ctas, cudaStream_t st) {
     using C = Cfg<I8, DB, NT>;
-    int smem = C::kWarps * C::kWarpSmem;
-    if (!EXACT) {
+    int smem = MODE == kTma ? C::kWarps * C::kWarpSmem + 1024 : C::kWarps * C::kGapWarpSmem;
+    if (MODE == kAny) {
         // rows as long as they are; stages until the copies in flight are 72 KB an SM (what two stages of 128-dim rows in
         // 16 bits give)
         a.krow = I8 ? ((a.Dk / 16) | 1) * 16 : a.Dk * 2 + 16, a.vrow = I8 ? ((a.Dv / 16) | 1) * 16 : a.Dv * 2 + 16;
@@ -1020,18 +1108,19 @@ int launch(Args a, int ctas, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (set_for != dev) {
-        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 EXACT ? smem : most_smem(C::kWarps)) != cudaSuccess)
+        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 MODE != kAny ? smem : most_smem(C::kWarps)) != cudaSuccess)
             return set_error(WS_ERR_CUDA, "paged_decode: shared memory");
         set_for = dev;
     }
-    const cudaError_t e = launch_dependent(decode_kernel<F16, I8, DB, NT, EXACT>, dim3(ctas), 32 * C::kWarps, smem, st, a);
+    const cudaError_t e = launch_dependent(decode_kernel<F16, I8, DB, NT, MODE>, dim3(ctas), 32 * C::kWarps, smem, st, a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }
 
 template <bool F16, bool I8, int DB, int NT>
 int launch_dims(const Args& a, int ctas, cudaStream_t st) {
-    return a.Dk == DB && a.Dv == DB ? launch<F16, I8, DB, NT, true>(a, ctas, st) : launch<F16, I8, DB, NT, false>(a, ctas, st);
+    if (a.tma) return launch<F16, I8, DB, NT, kTma>(a, ctas, st);
+    return a.Dk == DB && a.Dv == DB ? launch<F16, I8, DB, NT, kExact>(a, ctas, st) : launch<F16, I8, DB, NT, kAny>(a, ctas, st);
 }
 
 template <bool F16, bool I8>

@@ -863,3 +863,44 @@ def test_slots_take_a_negative_head_as_the_rings_start():
     lens_out, ring = paged.paged_release(torch.full((1,), 20, dtype=torch.int32, device=DEV),
                                          torch.ones(1, dtype=torch.bool, device=DEV), d[2], d[3], d[4], 16)
     assert ring.tolist() == [0, 8, 0] and d[3].tolist() == [100, 101, 102, 103, 104, 105, 100, 101]
+
+
+LONG = [0, 1, 15, 16, 17, 31, 33, 64, 65, 200, 511, 601, 1300, 2000]
+
+
+@pytest.mark.parametrize("heads_major", [False, True])
+@pytest.mark.parametrize("dtype,pool", [(BF, BF), (HF, HF), (BF, torch.int8), (HF, torch.int8)])
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("P,Hkv,G,window", [(16, 2, 4, 0), (64, 1, 12, 600), (48, 3, 1, 0)])
+def test_decode_wide_tables_of_whole_tiles(heads_major, dtype, pool, D, P, Hkv, G, window):
+    """Long rows and short ones in pages of whole 16-token tiles: what lies past a length in a tile is NaN."""
+    s = make_decode(LONG, Hkv * G, Hkv, D, D, P, dtype, pool=pool, heads_major=heads_major, seed=61)
+    agrees(s, *decode(s, window=window), window=window)
+    out, lse = decode(s, window=window)
+    again, lse2 = decode(s, window=window)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    assert scope_b200.status_take() == 0
+
+
+@pytest.mark.parametrize("pool", [BF, torch.int8])
+def test_decode_wide_tables_leave_out_pages_that_are_none(pool):
+    s = make_decode([900, 40, 17, 3000], 8, 2, 128, 128, 16, BF, pool=pool, seed=62)
+    bad = torch.zeros(s["k"].shape[0] + 1, dtype=torch.bool, device=DEV)
+    for b, col, put in ((0, 3, -1), (0, 4, s["k"].shape[0]), (0, 56, 1 << 30), (1, 0, -5), (2, 1, -1), (3, 100, -1)):
+        bad[int(s["table"][b, col])] = True
+        s["table"][b, col] = put
+    agrees(s, *decode(s), leave_out=lambda page: ~bad[page])
+    assert scope_b200.status_take() != 0 and scope_b200.status_take() == 0
+
+
+@pytest.mark.parametrize("head,tok", [(136, 272), (136, 280), (128, 256), (144, 456)])
+def test_decode_wide_tables_of_a_pool_with_gaps(head, tok):
+    """Rows and tokens further apart than they are long, pages that are every other one of a larger buffer."""
+    s = make_decode(LONG, 8, 2, 128, 128, 16, BF, seed=63)
+    n = s["k"].shape[0]
+    for name in ("k", "v"):
+        wide = torch.full((n * 2 * 16 * tok,), float("nan"), dtype=BF, device=DEV)
+        wide = wide.as_strided(s[name].shape, (2 * 16 * tok, tok, head, 1), 16 * tok)
+        wide.copy_(s[name])
+        s[name] = wide
+    agrees(s, *decode(s))

@@ -40,7 +40,8 @@
 // Why an even split suffices: with 128 KB of copies in flight an SM, 16 of the 148 SMs ended 10% after the others, which
 // the memory serves first; with 80 KB all end within 3% of one another, and the whole sooner.  Built and measured slower:
 // rows straight from global memory into fragment registers, no shared memory in the loop (half the instructions, but
-// each warp waits for its own loads: 224 us on the 16 ragged requests, when this design took 160).
+// each warp waits for its own loads: 224 us on the 16 ragged requests, when this design took 160); TMA for head dims not
+// known when compiling (182 requests with keys of 128 and values of 64: 832 us, with cp.async 661; 13 of 112: 88 and 80).
 #pragma once
 
 #include "common.cuh"

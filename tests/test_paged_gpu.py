@@ -904,3 +904,13 @@ def test_decode_wide_tables_of_a_pool_with_gaps(head, tok):
         wide.copy_(s[name])
         s[name] = wide
     agrees(s, *decode(s))
+
+
+@pytest.mark.parametrize("heads_major", [False, True])
+@pytest.mark.parametrize("dtype,pool", [(BF, BF), (HF, HF), (BF, torch.int8), (HF, torch.int8)])
+@pytest.mark.parametrize("Dk,Dv", [(16, 16), (32, 32), (48, 48), (80, 80), (96, 96), (112, 112), (64, 16), (128, 64), (80, 128),
+                                   (96, 192), (192, 128), (160, 160), (224, 64), (256, 80), (144, 240)])
+def test_decode_wide_tables_of_any_head_dims(heads_major, dtype, pool, Dk, Dv):
+    s = make_decode(LONG, 12, 2, Dk, Dv, 32, dtype, pool=pool, heads_major=heads_major, seed=64)
+    agrees(s, *decode(s))
+    assert scope_b200.status_take() == 0

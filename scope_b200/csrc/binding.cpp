@@ -3,7 +3,7 @@
 //
 // A step of a server makes one of these calls per layer, each of a few microseconds on the device, so what the host
 // spends on a call counts as much as the kernel: reading some thirty tensor attributes through Python and converting
-// twenty arguments with ctypes took 15 to 20 us a call, this takes 5 to 6.  The functions take positional arguments
+// twenty arguments with ctypes took 15 to 20 us a call, this takes 5 to 8.  The functions take positional arguments
 // only; scope_b200/paged.py has their signatures and documentation.  The C ABI's functions are handed over by address
 // (setup), so this module serves whichever build of the library the package loaded.
 #include <Python.h>

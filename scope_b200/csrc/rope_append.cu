@@ -12,8 +12,9 @@
 // step of heads would load them again and again: 94 us instead of 54).  The
 // units of a head are padded to a power of two and lie in one warp, which the
 // int8 form needs for the row's maximum.  Measured: 16384 x 32 heads of 128,
-// three axes, 47.9 us (277 MB, 5.8 TB/s); append of 16384 tokens of 32 + 4 + 4
-// heads 62.0 us (345 MB, 5.6 TB/s).
+// three axes, 47.0 us (277 MB, 5.9 TB/s); append of 16384 tokens of 32 + 4 + 4
+// heads 60.0 us (345 MB, 5.7 TB/s).  The first rows are asked for before the position is known, whose turns would else
+// delay them by two latencies (47.9 and 61.9 us; 1202 tokens of 40 + 8 + 8 heads 11.9 to 10.8; 64 tokens 2.65 to 2.47).
 //
 // Products and sums are rounded one by one (no fused multiply-add): the result
 // is the elementwise formula's, bit for bit, so an int8 code never depends on
@@ -104,9 +105,40 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
     const int part = (int)(item - t * a.parts);
     const int u = lane & (a.lanes - 1), row0 = lane / a.lanes, rows = 32 / a.lanes;
 
-    // this unit's eight turns, shared by all of the token's q and k heads
     const ws_rope& r = a.rope;
     const bool turned = 16 * u < r.rope_dim;
+    const int total = a.h[0].n + a.h[1].n + a.h[2].n;
+    auto locate = [&](int at, int& h, int& kind) {   // row `at` of the token: a head of q, k or v
+        h = at, kind = 0;
+        if (h >= a.h[0].n) h -= a.h[0].n, kind = 1;
+        if (kind == 1 && h >= a.h[1].n) h -= a.h[1].n, kind = 2;
+        return at < total && 16 * u < a.h[kind].D;
+    };
+    auto halves = [&](int kind, int& d0, int& d1) {   // where the unit's two halves lie; true: rope_dim/2 apart
+        const bool split = turned && kind < 2 && !r.adjacent;
+        d0 = split ? 8 * u : 16 * u, d1 = split ? (r.rope_dim >> 1) + 8 * u : 16 * u + 8;
+        return split;
+    };
+    // All loads of a group of rows.  The first group's are on their way before the turns, which wait for the position, and
+    // before the slot.
+    uint4 v0[GROUP], v1[GROUP];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int k = 0; k < GROUP; ++k) {
+            int h, kind, d0, d1;
+            if (locate(base + k * rows + row0, h, kind)) {
+                halves(kind, d0, d1);
+                const Heads& x = a.h[kind];
+                const uint16_t* p = x.src + t * x.src_tok + h * x.src_head;
+                v0[k] = load8<VEC>(p + d0), v1[k] = load8<VEC>(p + d1);
+            }
+        }
+    };
+    const int64_t slot = a.slots ? a.slots[t] : -1;
+    int base0 = part * rows * GROUP;
+    load(base0);
+
+    // this unit's eight turns, shared by all of the token's q and k heads
     float c[8], s[8];
     if (turned) {
         const int n = r.rope_dim >> 1;
@@ -147,48 +179,21 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
         }
     }
     int64_t page = -1, off = 0;
-    if (a.slots) {
-        const int64_t slot = a.slots[t];
-        if (slot >= 0) {
-            if (slot < a.n_slots) {
-                if (slot >> 32 == 0) page = (uint32_t)slot / (uint32_t)a.page_size;
-                else page = slot / a.page_size;
-                off = slot - page * a.page_size;
-            } else if (a.status) {
-                atomicMax(a.status, kDevBadIndex);
-            }
+    if (slot >= 0) {
+        if (slot < a.n_slots) {
+            if (slot >> 32 == 0) page = (uint32_t)slot / (uint32_t)a.page_size;
+            else page = slot / a.page_size;
+            off = slot - page * a.page_size;
+        } else if (a.status) {
+            atomicMax(a.status, kDevBadIndex);
         }
     }
-    const int total = a.h[0].n + a.h[1].n + a.h[2].n;
-    for (int base0 = part * rows * GROUP; base0 < total; base0 += a.parts * rows * GROUP) {
-        uint4 v0[GROUP], v1[GROUP];
-        auto locate = [&](int k, int& h, int& kind) {   // this thread's row of the group's step k: a head of q, k or v
-            const int at = base0 + k * rows + row0;
-            h = at, kind = 0;
-            if (h >= a.h[0].n) h -= a.h[0].n, kind = 1;
-            if (kind == 1 && h >= a.h[1].n) h -= a.h[1].n, kind = 2;
-            return at < total && 16 * u < a.h[kind].D && (kind == 0 || page >= 0);
-        };
-        auto halves = [&](int kind, int& d0, int& d1) {   // where the unit's two halves lie; true: rope_dim/2 apart
-            const bool split = turned && kind < 2 && !r.adjacent;
-            d0 = split ? 8 * u : 16 * u, d1 = split ? (r.rope_dim >> 1) + 8 * u : 16 * u + 8;
-            return split;
-        };
-        // all the group's loads, then its rows
+#pragma unroll 1
+    while (base0 < total) {
 #pragma unroll
         for (int k = 0; k < GROUP; ++k) {
             int h, kind, d0, d1;
-            if (locate(k, h, kind)) {
-                halves(kind, d0, d1);
-                const Heads& x = a.h[kind];
-                const uint16_t* p = x.src + t * x.src_tok + h * x.src_head;
-                v0[k] = load8<VEC>(p + d0), v1[k] = load8<VEC>(p + d1);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < GROUP; ++k) {
-            int h, kind, d0, d1;
-            const bool on = locate(k, h, kind), split = halves(kind, d0, d1), turn = turned && kind < 2;
+            const bool on = locate(base0 + k * rows + row0, h, kind) && (kind == 0 || page >= 0), split = halves(kind, d0, d1), turn = turned && kind < 2;
             const Heads& x = a.h[kind];
             float lo[8], hi[8];   // dims d0 .. d0+7 and d1 .. d1+7
             if (on) {
@@ -252,6 +257,8 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
                 store8<VEC>(p + d1, make_uint4(w1[0], w1[1], w1[2], w1[3]));
             }
         }
+        base0 += a.parts * rows * GROUP;
+        if (base0 < total) load(base0);
     }
 }
 

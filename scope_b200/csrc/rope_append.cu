@@ -355,13 +355,15 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
     a.status = device_status_word();
     a.lanes = 1;
     while (a.lanes * 16 < Dmax) a.lanes *= 2;
-    // One warp walks all heads of a token when there are tokens for every SM; with fewer, its rows are shared out.
+    // One warp walks all heads of a token when there are tokens for every SM; with fewer, its rows are shared out.  Into
+    // int8, where a row takes longer, that pays with half as many tokens only (4097 tokens of 20 + 5 + 5 heads, us with 16,
+    // 32, 64 and 128 warps wanted an SM: 14.5, 15.5, 17.2, 20.4).
+    const bool f16 = dtype == WS_DTYPE_F16, i8 = kv && kv->dtype == WS_DTYPE_I8;
     const int rows = 32 / a.lanes, steps = (H + (kv ? 2 * kv->Hkv : 0) + rows - 1) / rows;
-    const int64_t want = (int64_t)device_sm_count() * 32;
+    const int64_t want = (int64_t)device_sm_count() * (i8 ? 16 : 32);
     a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps, (want + N - 1) / N));
     const int64_t blocks = (N * a.parts + kWarps - 1) / kWarps;
     if (blocks > INT32_MAX) return set_error(WS_ERR_UNSUPPORTED, "rope_append: too many tokens");
-    const bool f16 = dtype == WS_DTYPE_F16, i8 = kv && kv->dtype == WS_DTYPE_I8;
     // Two rows in flight a thread where a warp walks many (16384 tokens of 32 heads, us a call with one and two: rotary
     // alone 51 and 48, append 67 and 62); with few rows, or int8 codes to compute, the registers cost more than that gives
     // (5212 tokens of 3 heads of 256: 15 and 18; 4097 tokens into int8: 38 and 41).

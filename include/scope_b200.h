@@ -14,11 +14,12 @@
  * the one allocating entry, for the multi-GPU exchange): callers pass a 16-byte
  * aligned workspace whose size the matching *_workspace_size() returns.  A workspace must be zeroed
  * once when it is allocated (its counters reset themselves after every
- * launch) and must not be shared by launches that may overlap in time.
- * Exception: when ws_status_take() returns WS_ERR_DEVICE, a launch may have
- * given up between taking and returning a merge counter, so every workspace
- * used since the previous ws_status_take() must be zeroed again before its
- * next use.
+ * launch) and must not be shared by launches that may overlap in time; a
+ * captured graph holds its address, so it must outlive the graph.
+ * Exception: when ws_status_read() reports WS_STATUS_TIMEOUT, a launch may
+ * have given up between taking and returning a merge counter, so every
+ * workspace used since the status was last read must be zeroed again before
+ * its next use.  (WS_STATUS_BAD_INDEX leaves the counters at zero.)
  *
  * bf16 tensors are passed as their 16-bit storage.  The reference interfaces
  * each entry replaces are cited as path:line of the reference checkout.
@@ -56,9 +57,14 @@ const char* ws_last_error(void);
 int ws_version(void);
 
 /* Device-side status word: kernels whose bounded waits give up (they never
- * spin forever) record WS_ERR_DEVICE there.  Returns the word for the current
- * device and clears it (synchronises the given stream). */
+ * spin forever), and kernels that leave out an index outside its range, record
+ * it there.  Both read and clear the current device's word (and synchronise
+ * the given stream) and return WS_OK, or WS_ERR_DEVICE where something was
+ * recorded; ws_status_read also says what (NULL: not wanted). */
+#define WS_STATUS_TIMEOUT 1     /* a bounded wait gave up */
+#define WS_STATUS_BAD_INDEX 2   /* an id, page, slot or position outside its range was left out or clamped */
 int ws_status_take(void* stream);
+int ws_status_read(void* stream, int* what);
 
 /*
  * GQA / MLA decode over one strided KV share.

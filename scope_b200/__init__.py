@@ -59,15 +59,18 @@ def build_csa_attn():
 def status_take(device=None) -> int:
     """Read and clear the device status word of ``device`` (synchronises its
     current stream): 0 when no kernel reported a problem since the last call,
-    else WS_ERR_DEVICE (5): a bounded wait gave up, or a CSA id outside the
-    KV buffer was skipped.  On WS_ERR_DEVICE the device's pooled workspaces
-    are dropped, so the next launch runs on a freshly zeroed one (a launch
-    that gave up may have left a merge counter set)."""
+    else WS_ERR_DEVICE (5): a bounded wait gave up, or an id, page, slot or
+    position outside its range was left out.  After a wait that gave up the
+    device's pooled workspaces are zeroed where they lie (that launch may have
+    left a merge counter set; waits for the whole device); captured graphs
+    stay valid."""
+    import ctypes
     import torch
-    from ._lib import workspaces
+    from ._lib import WS_STATUS_TIMEOUT, workspaces
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(dev):
-        rc = int(lib().ws_status_take(torch.cuda.current_stream(dev).cuda_stream))
-    if rc != 0:
-        workspaces.drop_device(dev.index if dev.index is not None else torch.cuda.current_device())
+        what = ctypes.c_int(0)
+        rc = int(lib().ws_status_read(torch.cuda.current_stream(dev).cuda_stream, ctypes.byref(what)))
+    if what.value & WS_STATUS_TIMEOUT:
+        workspaces.rezero(dev.index if dev.index is not None else torch.cuda.current_device())
     return rc

@@ -24,6 +24,9 @@ WS_ERR_CUDA = 3
 WS_ERR_WORKSPACE = 4
 WS_ERR_DEVICE = 5
 
+WS_STATUS_TIMEOUT = 1     # bits of ws_status_read
+WS_STATUS_BAD_INDEX = 2
+
 WS_DTYPE_BF16 = 0
 WS_DTYPE_F32 = 1
 WS_DTYPE_I8 = 2
@@ -59,6 +62,7 @@ SIGNATURES = {
     "ws_last_error": (ctypes.c_char_p, []),
     "ws_version": (_i, []),
     "ws_status_take": (_i, [_V]),
+    "ws_status_read": (_i, [_V, ctypes.POINTER(_i)]),
     "ws_gqa_decode": (_i, [_V, _V, _V, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _i, _f, _i, _i,
                            _V, _V, _V, _V, _V, _sz, _V]),
     "ws_gqa_decode_workspace_size": (_sz, [_i, _i, _i, _i]),
@@ -195,30 +199,47 @@ class _WorkspacePool:
     The kernels reset their counters after every launch, so a workspace is
     zeroed only when it is (re)allocated.  Keyed by stream because launches on
     different streams may overlap and must not share counters.
+
+    A captured CUDA graph holds the address of the workspace of the stream it
+    was captured on, and nothing tells the pool for how long.  So a workspace
+    is never given back: one that was outgrown is kept beside the larger one,
+    and one whose counters are in doubt is zeroed where it lies.  A workspace
+    that is first asked for inside a capture is made and zeroed outside of it
+    (a recorded zeroing would happen at each replay of that graph only, and
+    the buffer serves every launch on the stream).  Graphs captured on one
+    stream share its workspace: their replays must not overlap, nor overlap
+    with launches on that stream.
     """
+
+    # most operators' size, and the paged decode's: a stream that starts with small calls does not outgrow this at once
+    MIN_BYTES = 4 << 20
 
     def __init__(self):
         self._bufs: dict[tuple[int, int], torch.Tensor] = {}
+        self._outgrown: list[tuple[int, torch.Tensor]] = []   # (device, buffer)
 
     def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
         key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device))
         buf = self._bufs.get(key)
         if buf is None or buf.numel() < nbytes:
-            size = max(nbytes, 1 << 20, 0 if buf is None else 2 * buf.numel())
-            buf = torch.zeros(size, dtype=torch.uint8, device=device)
+            size = max(nbytes, self.MIN_BYTES, 0 if buf is None else 2 * buf.numel())
+            if buf is not None:
+                self._outgrown.append((key[0], buf))
+            if torch.cuda.is_current_stream_capturing():
+                buf = binding().zeros_outside_capture(size, key[0])
+            else:
+                buf = torch.zeros(size, dtype=torch.uint8, device=device)
             self._bufs[key] = buf
         return buf
 
-    def clear(self) -> None:
-        self._bufs.clear()
-
-    def drop_device(self, index: int) -> None:
-        """Forget every workspace of device ``index``; the next launch there
-        allocates a freshly zeroed one.  Called after a kernel reported a
-        device-side failure: a launch that gave up may leave a merge counter
-        of its workspace non-zero."""
-        for key in [k for k in self._bufs if k[0] == index]:
-            del self._bufs[key]
+    def rezero(self, index: int) -> None:
+        """Zero every workspace of device ``index`` in place, once nothing
+        runs there.  Called after a bounded wait gave up: that launch may have
+        left a merge counter of its workspace non-zero."""
+        torch.cuda.synchronize(index)
+        for buf in [b for k, b in self._bufs.items() if k[0] == index] + [b for d, b in self._outgrown if d == index]:
+            buf.zero_()
+        torch.cuda.synchronize(index)
 
 
 workspaces = _WorkspacePool()

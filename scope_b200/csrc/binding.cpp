@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Device.h>
@@ -86,7 +87,8 @@ at::Tensor output(const char* what, const char* name, PyObject* given, at::IntAr
     return t;
 }
 
-// The workspace of this device and stream, from the package's pool.
+// The workspace of this device and stream, from the package's pool, which never frees one: a captured launch keeps the
+// address.
 struct Workspace {
     void* ptr;
     size_t bytes;
@@ -416,6 +418,28 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// bytes, device index: a zeroed buffer made while the current stream is being captured, but outside of the capture: on
+// another stream, and with the capture's ban on allocations lifted for this thread meanwhile.
+PyObject* zeros_outside_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 2, [&]() -> PyObject* {
+        const int64_t bytes = integer(a[0]), index = integer(a[1]);
+        const at::Device dev(at::kCUDA, (c10::DeviceIndex)index);
+        const c10::cuda::OptionalCUDAGuard guard(dev);
+        const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+        c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, dev.index());
+        for (int i = 0; i < 64; ++i) {   // the captured stream may be of the pool too
+            const c10::cuda::CUDAStreamGuard on_side(side);
+            if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) {
+                const at::Tensor t = at::zeros({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+                side.synchronize();
+                return THPVariable_Wrap(t);
+            }
+            side = c10::cuda::getStreamFromPool(false, dev.index());
+        }
+        refuse("workspace", "no stream that is not being captured");
+    });
+}
+
 // (addresses of ws_last_error, ws_paged_slots, ws_paged_release, ws_rope_append, ws_paged_decode; the two workspace
 // sizes; ScopeError, workspaces.get, the pool's dict, PagedStep)
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -438,7 +462,7 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ENTRY(setup), ENTRY(paged_slots), ENTRY(paged_release), ENTRY(rope), ENTRY(rope_append),
+PyMethodDef methods[] = {ENTRY(setup), ENTRY(zeros_outside_capture), ENTRY(paged_slots), ENTRY(paged_release), ENTRY(rope), ENTRY(rope_append),
                          ENTRY(paged_decode), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods};
 

@@ -133,7 +133,10 @@ const char* ws_last_error(void) { return g_err; }
 
 int ws_version(void) { return 100; }
 
-int ws_status_take(void* stream) {
+int ws_status_take(void* stream) { return ws_status_read(stream, nullptr); }
+
+int ws_status_read(void* stream, int* what) {
+    if (what) *what = 0;
     int* w = device_status_word();
     if (!w) return set_error(WS_ERR_CUDA, "status word unavailable");
     int h = 0;
@@ -141,6 +144,8 @@ int ws_status_take(void* stream) {
     if (cudaMemcpyAsync(&h, w, sizeof(int), cudaMemcpyDeviceToHost, st) != cudaSuccess ||
         cudaMemsetAsync(w, 0, sizeof(int), st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess)
         return set_error(WS_ERR_CUDA, "status word read failed");
+    static_assert(kDevTimeout == WS_STATUS_TIMEOUT && kDevBadIndex == WS_STATUS_BAD_INDEX, "the word is these bits");
+    if (what) *what = h;
     return h == 0 ? WS_OK : WS_ERR_DEVICE;
 }
 

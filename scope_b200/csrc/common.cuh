@@ -16,6 +16,7 @@ constexpr float kLn2 = 0.6931471805599453f;     // ln(2)
 
 // Status word written by kernels whose bounded waits gave up.  Read (and
 // cleared) by ws_status_take() in capi.cu.
+// Bits: kDevBadIndex is or-ed in, so that it never hides a timeout.
 enum : int { kDevOk = 0, kDevTimeout = 1, kDevBadIndex = 2 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) csa_decode_kernel(const Params p)
             row[u] = -1;
             if (id[u] != INT64_MIN) {
                 if (id[u] >= p.shard_lo && id[u] < p.shard_hi) row[u] = (int)(id[u] - p.shard_lo);
-                else if (p.window == WS_CSA_IDX_ALL) atomicExch(p.status, kDevBadIndex);   // skipped, and reported
+                else if (p.window == WS_CSA_IDX_ALL) atomicOr(p.status, kDevBadIndex);   // skipped, and reported
             }
         }
 #pragma unroll

@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             const bool page_ok = (uint32_t)f_entry < (uint32_t)a.n_pages;
             const uint32_t pages_ok = __ballot_sync(0xffffffffu, page_ok);
             if (pages_ok != 0xffffffffu) {
-                if (a.status) atomicMax(a.status, kDevBadIndex);
+                if (a.status) atomicOr(a.status, kDevBadIndex);
                 mask &= pages_ok;   // whole pages: 16 lanes looked at the same one
             }
             const uint32_t page = page_ok ? f_entry : 0;
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             if (TMA) {
                 if (I8) cp_async_wait<C::kStages - 2>();   // the scales
                 if (!dead && !mbar_wait_bounded(bars + 8 * slot, phase)) {
-                    if (a.status) atomicExch(a.status, kDevTimeout);
+                    if (a.status) atomicOr(a.status, kDevTimeout);
                     mbar_wait_bounded(bars + 8 * slot, phase);   // what is in flight
                     dead = true;
                 }

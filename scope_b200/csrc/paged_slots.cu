@@ -233,7 +233,7 @@ paged_release_kernel(const int32_t* seq_lens, const uint8_t* __restrict__ done, 
         ring_out[0] = head;
         ring_out[1] = n_free + total;
         ring_out[2] = 0;
-        if (pages.a > room && status) atomicMax(status, kDevBadIndex);
+        if (pages.a > room && status) atomicOr(status, kDevBadIndex);
     }
 }
 

@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
             int64_t p = r.positions_i64 ? static_cast<const int64_t*>(r.positions)[at]
                                         : static_cast<const int32_t*>(r.positions)[at];
             if ((uint64_t)p >= (uint64_t)r.max_pos) {
-                if (a.status) atomicMax(a.status, kDevBadIndex);
+                if (a.status) atomicOr(a.status, kDevBadIndex);
                 p = p < 0 ? 0 : r.max_pos - 1;
             }
             return p;
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
             else page = slot / a.page_size;
             off = slot - page * a.page_size;
         } else if (a.status) {
-            atomicMax(a.status, kDevBadIndex);
+            atomicOr(a.status, kDevBadIndex);
         }
     }
 #pragma unroll 1

@@ -57,9 +57,20 @@ class OneLayer:
 
 def serve(model: OneLayer, prompts, n_new: int, batch: int, num_pages: int, page_size: int = 16, graph: bool = True,
           on_step=None):
-    """Greedy continuations of ``n_new`` tokens for every prompt (lists of token ids), ``batch`` requests at a time."""
+    """Greedy continuations of ``n_new`` tokens for every prompt (lists of token ids), ``batch`` requests at a time.  A
+    prompt is admitted when the pool holds every page that it and the running requests can still come to need."""
+    def pages_of(tokens):
+        return -(-tokens // page_size)
+
+    def need_of(prompt):                        # the last token is emitted and never cached
+        return pages_of(len(prompt) + n_new - 1)
+
+    if n_new < 1 or not all(prompts):
+        raise ValueError("serve: at least one new token, and one in every prompt")
+    if any(need_of(p) > num_pages for p in prompts):
+        raise ValueError("serve: a prompt and its continuation take more pages than the pool has")
     dev = model.embed.device
-    longest = max(len(p) for p in prompts) + n_new
+    longest = max((len(p) for p in prompts), default=0) + n_new
     cache = PagedKVCache(1, num_pages, page_size, model.Hkv, model.D, batch, longest, device=dev)
     waiting, done = list(range(len(prompts))), {}
     slot_of, text = [None] * batch, {}          # which prompt each row of the batch serves; its tokens so far
@@ -70,11 +81,11 @@ def serve(model: OneLayer, prompts, n_new: int, batch: int, num_pages: int, page
     while waiting or any(s is not None for s in slot_of):
         new, joining = [0] * batch, []
         free = cache.free_pages()
-        owed = sum(-(-(len(prompts[s]) + n_new) // page_size) - -(-len(text[s]) // page_size)
-                   for s in slot_of if s is not None)
+        # the cache holds a running text without its last token, which the next step appends
+        owed = sum(need_of(prompts[s]) - pages_of(len(text[s]) - 1) for s in slot_of if s is not None)
         for b in range(batch):
             if slot_of[b] is None and waiting:
-                need = -(-(len(prompts[waiting[0]]) + n_new) // page_size)
+                need = need_of(prompts[waiting[0]])
                 if owed + need > free:          # it waits until pages come back
                     break
                 owed += need
@@ -113,6 +124,8 @@ def serve(model: OneLayer, prompts, n_new: int, batch: int, num_pages: int, page
         else:
             got = model.step(cache, torch.tensor(packed, device=dev), torch.tensor(new, dtype=torch.int32, device=dev),
                              torch.tensor(last, device=dev))
+        if cache.refused():
+            raise RuntimeError("serve: a request found no page")
         if on_step is not None:
             on_step([text[s] if s is not None else None for s in slot_of], got)
         choice, leaving = got.argmax(1).tolist(), [False] * batch

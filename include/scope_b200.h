@@ -480,7 +480,8 @@ typedef struct ws_rope {
  *   (t, h, d) at base + t*stride_tok + h*stride_head + d; dtype WS_DTYPE_BF16 or
  *   WS_DTYPE_F16.  The pool holds that type, or int8 codes:
  *   scale = max(max|x|, 1e-6) / 127, code = rne(x * 127 / max) per row (the rule
- *   of ws_csa_kv_quantize_s8), taken from the rotated fp32 row.
+ *   of ws_csa_kv_quantize_s8), taken from the rotated fp32 row.  A NaN in a row
+ *   makes its scale NaN, an infinity makes it infinite; the codes are 0 then.
  *   slots int64 [N]: token t's keys and values go to slot slots[t]; a negative
  *   slot drops them, one past the pool drops them and records WS_ERR_DEVICE.
  * rope NULL: no rotation.  H = 0: no queries.  kv NULL: queries only (k, v,

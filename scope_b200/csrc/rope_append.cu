@@ -70,6 +70,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return pack_bf16(a, b);
 }
 
+// The larger of two, or NaN where either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 // Eight 16-bit values from p; without VEC the address need not be aligned.
 template <bool VEC>
 __device__ __forceinline__ uint4 load8(const uint16_t* p) {
@@ -220,14 +227,14 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
                 }
             }
             if (I8) {
-                float most = 0.f;
+                float most = 0.f;   // a NaN in the row makes its scale one, and so all that is read back of it
                 if (on && kind) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+                    for (int i = 0; i < 8; ++i) most = max_nan(most, max_nan(fabsf(lo[i]), fabsf(hi[i])));
                 }
-                for (int o = a.lanes >> 1; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                for (int o = a.lanes >> 1; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
                 if (on && kind) {
-                    most = fmaxf(most, 1e-6f);
+                    most = max_nan(most, 1e-6f);
                     const float inv = __fdiv_rn(127.f, most);
                     auto codes = [&](const float* f) {
                         uint32_t w[2] = {0, 0};

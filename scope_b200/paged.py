@@ -136,7 +136,8 @@ def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positi
     q [N, H, Dk] (or None), k [N, Hkv, Dk], v [N, Hkv, Dv]: bf16 or fp16, any strides with a unit head dim (views of a
     packed projection are read in place).  slots int64 [N] (``PagedStep.slots``): token t's key and value rows go to
     slot slots[t]; a negative slot drops them.  An int8 pool gets codes and one scale per row, taken from the rotated
-    row in fp32 (the rule of ``kv_quantize_bf16_to_int8``).  ``cos_sin`` None: no rotation.  Rotary arguments as in
+    row in fp32 (the rule of ``kv_quantize_bf16_to_int8``); a NaN in a row makes the row's scale NaN, an infinity makes it
+    infinite over codes of 0, so either row reads back as NaN.  ``cos_sin`` None: no rotation.  Rotary arguments as in
     ``rope``.  Returns the rotated queries (``q_out``, which may be q), or None without q.
     """
     axis_map, axes = (None, 1) if cos_sin is None else _axes(cos_sin, sections, cyclic)

@@ -1,0 +1,62 @@
+"""GPU checks of the paged operators on values that are no numbers, or no finite ones, and of how exactly values come
+through."""
+import pytest
+import torch
+
+from scope_b200 import paged
+from test_paged_gpu import BF, DEV, HF, codes, gen, table_of, turned
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ append into int8 pools
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("H,Hkv,D,Dv,rot", [(4, 2, 128, 128, 128), (6, 3, 80, 48, 64), (2, 1, 16, 256, 16), (0, 2, 192, 16, 64)])
+@pytest.mark.parametrize("pairs", ["half", "adjacent"])
+def test_append_into_int8_keeps_what_is_no_number(dtype, H, Hkv, D, Dv, rot, pairs):
+    """A row with a NaN or an infinity anywhere reads back as NaN; every other row has its own codes and scale."""
+    g = gen(D + Dv)
+    bad = [float("nan"), float("inf"), float("-inf")]
+    N = 3 * (D + Dv) + 5   # one token for every place and value, and a few sound ones
+    k = torch.randn(N, Hkv, D, generator=g, device=DEV).to(dtype)
+    v = torch.randn(N, Hkv, Dv, generator=g, device=DEV).to(dtype)
+    at = 0
+    for x, width in ((k, D), (v, Dv)):
+        for d in range(width):
+            for value in bad:
+                x[at, (at // 7) % Hkv, d] = value
+                at += 1
+    table, pos = table_of(300, rot), torch.randint(0, 300, (N,), generator=g, device=DEV, dtype=torch.int32)
+    q = torch.randn(N, H, D, generator=g, device=DEV).to(dtype) if H else None
+    P = 16
+    n_pages = -(-N // P)
+    kp, vp = (torch.full((n_pages, P, Hkv, w), 99, dtype=torch.int8, device=DEV) for w in (D, Dv))
+    ks, vs = (torch.zeros(n_pages, P, Hkv, device=DEV) for _ in range(2))
+    slots = torch.randperm(n_pages * P, generator=g, device=DEV)[:N].contiguous()
+    paged.rope_append(q, k, v, pos, table, slots, kp, vp, k_scales=ks, v_scales=vs, pairs=pairs)
+    rows = ((kp, ks, turned(k, pos[None], table, [0] * (rot // 2), pairs)), (vp, vs, v.float()))
+    for pool, scales, x in rows:
+        got, scale = pool.view(-1, Hkv, x.shape[-1])[slots], scales.view(-1, Hkv)[slots]
+        want, most = codes(x)
+        sound = torch.isfinite(x).all(-1)
+        assert torch.equal(torch.isfinite(scale), sound) and torch.equal(scale.isnan(), x.isnan().any(-1))
+        assert torch.equal(got[sound], want[sound]) and torch.equal(scale[sound], most[sound])
+        assert (got[~sound] == 0).all() and (got.float() * scale[..., None])[~sound].isnan().all()
+        assert 0 < int((~sound).sum()) < sound.numel()
+
+
+def test_a_nan_key_appended_into_int8_reaches_the_output():
+    g = gen(2)
+    Hkv, D, P = 2, 64, 16
+    kp, vp = (torch.zeros(4, P, Hkv, D, dtype=torch.int8, device=DEV) for _ in range(2))
+    ks, vs = (torch.zeros(4, P, Hkv, device=DEV) for _ in range(2))
+    k, v = (torch.randn(40, Hkv, D, generator=g, device=DEV).to(BF) for _ in range(2))
+    k[7, 1, 30] = float("nan")
+    paged.rope_append(None, k, v, None, None, torch.arange(40, device=DEV), kp, vp, k_scales=ks, v_scales=vs)
+    q = torch.randn(1, 4, D, generator=g, device=DEV).to(BF)
+    out, lse = paged.paged_decode(q, kp, vp, torch.arange(4, dtype=torch.int32, device=DEV)[None],
+                                  torch.tensor([40], dtype=torch.int32, device=DEV), 0.1, k_scales=ks, v_scales=vs)
+    assert torch.isfinite(out[0, :2]).all() and torch.isfinite(lse[0, :2]).all()
+    assert out[0, 2:].isnan().all() and lse[0, 2:].isnan().all()

@@ -50,6 +50,12 @@ int64_t integer(PyObject* o) {
     return v;
 }
 
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw PythonError();
+    return v;
+}
+
 bool unit(const at::Tensor& t, int d) { return t.size(d) <= 1 || t.stride(d) == 1; }
 std::string on(const at::Device& dev) { return dev.str(); }
 
@@ -269,7 +275,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t N = x.size(0);
         want_rows(what, "x", x, x.scalar_type(), N, dev);
         if (x.size(1) > INT32_MAX || x.size(2) > INT32_MAX) refuse(what, "bad shape");
-        const ws_rope r = rope_of(what, a[1], a[2], N, dev, a[3], a[4], a[5], PyObject_IsTrue(a[6]) == 1);
+        const ws_rope r = rope_of(what, a[1], a[2], N, dev, a[3], a[4], a[5], truth(a[6]));
         const c10::cuda::OptionalCUDAGuard guard(dev);
         at::Tensor out;
         if (a[7] == Py_None) {

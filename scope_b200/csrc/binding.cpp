@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -91,6 +92,15 @@ at::Tensor output(const char* what, const char* name, PyObject* given, at::IntAr
     if (t.scalar_type() != type || t.sizes() != shape || !t.is_contiguous() || t.device() != dev)
         refuse(what, std::string(name) + " must be a contiguous " + c10::toString(type) + " tensor of the result's shape on " + on(dev));
     return t;
+}
+
+// A given output may be the input that it replaces (`same`), whole, and shares no memory with the others: the kernels read
+// those while they write it.
+void want_apart(const at::Tensor& out, const at::Tensor& same, std::initializer_list<const at::Tensor*> others) {
+    at::assert_no_internal_overlap(out);
+    at::assert_no_partial_overlap(out, same);
+    for (const at::Tensor* t : others)
+        if (t->defined()) at::assert_no_overlap(out, *t);
 }
 
 // The workspace of this device and stream, from the package's pool, which never frees one: a captured launch keeps the
@@ -180,6 +190,8 @@ PyObject* paged_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const c10::cuda::OptionalCUDAGuard guard(b.dev);
         const at::Tensor lens_out = output(what, "seq_lens_out", a[7], {b.B}, at::kInt, b.dev);
         const at::Tensor ring_out = output(what, "ring_out", a[8], {3}, at::kInt, b.dev);
+        if (a[7] != Py_None) want_apart(lens_out, lens, {&added, &table, &pages, &ring, &ring_out});
+        if (a[8] != Py_None) want_apart(ring_out, ring, {&lens, &added, &table, &pages});
         const at::Tensor slots = fresh({N}, at::kLong, b.dev), positions = fresh({N}, at::kInt, b.dev);
         const at::Tensor cu = fresh({b.B + 1}, at::kInt, b.dev);
         void* stream = c10::cuda::getCurrentCUDAStream(b.dev.index()).stream();
@@ -215,6 +227,8 @@ PyObject* paged_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const c10::cuda::OptionalCUDAGuard guard(b.dev);
         const at::Tensor lens_out = output(what, "seq_lens_out", a[6], {b.B}, at::kInt, b.dev);
         const at::Tensor ring_out = output(what, "ring_out", a[7], {3}, at::kInt, b.dev);
+        if (a[6] != Py_None) want_apart(lens_out, lens, {&done, &table, &pages, &ring, &ring_out});
+        if (a[7] != Py_None) want_apart(ring_out, ring, {&lens, &done, &table, &pages});
         void* stream = c10::cuda::getCurrentCUDAStream(b.dev.index()).stream();
         const Workspace ws = workspace(g_slots_ws, b.dev, stream);
         check(p_paged_release(data<int32_t>(lens), static_cast<uint8_t*>(done.data_ptr()), (int)b.B, data<int32_t>(table),
@@ -284,6 +298,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
             out = tensor(what, "out", a[7]);
             want_rows(what, "out", out, x.scalar_type(), N, dev);
             if (out.sizes() != x.sizes()) refuse(what, "out must have x's shape");
+            want_apart(out, x, {});
         }
         void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
         check(p_rope_append(&r, x.data_ptr(), x.stride(0), x.stride(1), (int)x.size(1), (int)x.size(2), out.data_ptr(),
@@ -345,6 +360,8 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         want_rows(what, "k", k, st, N, dev);
         want_rows(what, "v", v, st, N, dev);
         const ws_paged_kv p = pool_of(what, a[6], a[7], a[8], a[9], dev);
+        for (int i = 6; i < 10; ++i)
+            if (a[i] != Py_None) at::assert_no_internal_overlap(THPVariable_Unpack(a[i]));
         if (k.size(1) != p.Hkv || v.size(1) != p.Hkv || k.size(2) != p.Dk || v.size(2) != p.Dv)
             refuse(what, "k, v must be [N, " + std::to_string(p.Hkv) + ", " + std::to_string(p.Dk) + "] and [N, " +
                              std::to_string(p.Hkv) + ", " + std::to_string(p.Dv) + "] as the pool is");
@@ -366,6 +383,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 out = tensor(what, "q_out", a[13]);
                 want_rows(what, "q_out", out, st, N, dev);
                 if (out.sizes() != q.sizes()) refuse(what, "q_out must have q's shape");
+                want_apart(out, q, {&k, &v});
             }
         } else if (a[13] != Py_None) {
             refuse(what, "q_out without q");
@@ -409,6 +427,10 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const c10::cuda::OptionalCUDAGuard guard(dev);
         const at::Tensor out = output(what, "out", a[9], {B, H, p.Dv}, st, dev);
         const at::Tensor lse = output(what, "lse", a[10], {B, H}, at::kFloat, dev);
+        for (const at::Tensor* t : {&q, &table, &lens}) {
+            if (a[9] != Py_None) at::assert_no_overlap(out, *t);
+            if (a[10] != Py_None) at::assert_no_overlap(lse, *t);
+        }
         void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
         const Workspace ws = workspace(g_decode_ws, dev, stream);
         check(p_paged_decode(q.data_ptr(), q.stride(0), q.stride(1), type, (int)B, (int)(H / p.Hkv), &p, data<int32_t>(table),

@@ -57,7 +57,7 @@ def paged_slots(seq_lens: torch.Tensor, new_lens: torch.Tensor, page_table: torc
 
     A request is refused whole -- its length, row and the ring unchanged, its tokens' slots -1 -- when its pages would
     pass the table's width, its tokens would pass n_tokens, or too few pages are free; ``ring[2]`` counts them.
-    ``seq_lens_out`` / ``ring_out`` may be the inputs, which a captured step wants.
+    ``seq_lens_out`` / ``ring_out`` may be the inputs, which a captured step wants, and share no memory with the others.
     """
     return (_c or _load()).paged_slots(seq_lens, new_lens, page_table, free_pages, ring, page_size, n_tokens, seq_lens_out,
                                        ring_out)
@@ -116,7 +116,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, *, sec
     cos_sin fp32 [max_pos, rope_dim]: the cosines of a position's rope_dim / 2 pairs, then the sines.  ``pairs``:
     'half' pairs dims (i, rope_dim/2 + i), 'adjacent' dims (2i, 2i+1).  positions int32 / int64 [N], or [A, N] with
     ``sections`` (the pairs of each of A <= 4 axes, see ``rope_axis_map``): time, height and width of images and
-    video.  ``inverse`` turns back, which is also the gradient.  ``out`` may be x.  Products and sums are rounded to
+    video.  ``inverse`` turns back, which is also the gradient.  ``out`` may be x, whole.  Products and sums are rounded to
     fp32 one by one and the result once more to x's type.
     """
     axis_map, axes = _axes(cos_sin, sections, cyclic)

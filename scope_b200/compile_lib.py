@@ -11,6 +11,7 @@ that the process has loaded.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import contextlib
 import os
 import shutil
 import subprocess
@@ -23,6 +24,7 @@ BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libscope_b200.so")
 BINDING_SRC = os.path.join(CSRC, "binding.cpp")
 BINDING = os.path.join(PKG, "_binding.so")
+BINDING_STAMP = os.path.join(BUILD, "binding.stamp")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -60,11 +62,22 @@ def _compile(src: str, verbose: bool) -> tuple[str, str]:
     return obj, out.stderr if verbose else ""
 
 
+def binding_stamp() -> str:
+    """What the binding is compiled against beside its sources: it holds PyTorch's and Python's C++ layouts."""
+    import torch
+    return "\n".join([torch.__version__, str(torch.version.git_version), os.path.dirname(torch.__file__),
+                      f"cxx11 abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}", sys.version, sysconfig.get_paths()["include"]])
+
+
 def build_binding(verbose: bool = False, force: bool = False) -> str:
-    """Build the binding if its source is newer than it; return its path."""
+    """Build the binding if its source is newer than it, or if it was built against another PyTorch or Python; return its
+    path."""
     newest = max(os.path.getmtime(BINDING_SRC), _headers_mtime())
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest:
-        return BINDING
+    stamp = binding_stamp()
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest and os.path.exists(BINDING_STAMP):
+        with open(BINDING_STAMP) as f:
+            if f.read() == stamp:
+                return BINDING
     import torch
     root = os.path.dirname(torch.__file__)
     cxx = shutil.which("g++")
@@ -82,7 +95,12 @@ def build_binding(verbose: bool = False, force: bool = False) -> str:
         raise RuntimeError(f"g++ failed on {BINDING_SRC}:\n{out.stdout}\n{out.stderr}")
     if verbose:
         sys.stdout.write(out.stderr)
+    os.makedirs(BUILD, exist_ok=True)
+    with contextlib.suppress(FileNotFoundError):
+        os.remove(BINDING_STAMP)
     os.replace(BINDING + ".tmp", BINDING)
+    with open(BINDING_STAMP, "w") as f:
+        f.write(stamp)
     return BINDING
 
 

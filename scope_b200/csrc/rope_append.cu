@@ -377,7 +377,10 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
     const bool several = a.parts == 1 && steps >= 8 && !i8;
     auto pick = [&](auto half, auto codes) {
         constexpr bool F = decltype(half)::value, I = decltype(codes)::value;
-        return !vec ? rope_append_kernel<F, I, false, 1> : several ? rope_append_kernel<F, I, true, kGroup> : rope_append_kernel<F, I, true, 1>;
+        if (!vec) return rope_append_kernel<F, I, false, 1>;
+        if constexpr (!I)
+            if (several) return rope_append_kernel<F, I, true, kGroup>;
+        return rope_append_kernel<F, I, true, 1>;
     };
     using yes = std::true_type;
     using no = std::false_type;

@@ -23,7 +23,9 @@
 //   * S^T[16 tok x 8 heads] = K . Q^T and O^T[Dv x 8] += V^T . P^T by mma.sync with the heads as the narrow dimension:
 //     at G <= 8 query heads a key there is no 128-row tile for tcgen05 to fill, and the tensor pipe is nearly idle.
 //   * The softmax's reference moves only when a score passes it by 2^kSlack: then, and not every subtile, the lanes
-//     agree on a new maximum and the accumulators are rescaled.  Sums are fp32; P enters the second product as the sum
+//     agree on a new maximum and the accumulators are rescaled.  Sums are fp32, and only a subtile's own is left to the
+//     tensor cores, which cut partial sums off instead of rounding them (over 11 thousand tokens a warp that came to
+//     2^-14 of the sum, always the same way; the additions cost nothing to 2 %).  P enters the second product as the sum
 //     of two 16-bit values (the rounded one and the rest), which keeps its error below the output's own rounding.
 //   * int8 rows go from shared memory to bf16 (fp16) fragments by bit operations, exactly; the row's scale multiplies
 //     the score, or the probability.
@@ -160,6 +162,23 @@ __device__ __forceinline__ void mma16(float* d, uint32_t a0, uint32_t a1, uint32
     if (F16) mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
     else mma_bf16_16816(d, a0, a1, a2, a3, b0, b1);
 }
+// d = A B, or d + A B.
+template <bool F16, bool FIRST>
+__device__ __forceinline__ void mma16_part(float* d, const uint32_t* a, const uint32_t* b) {
+    if (!FIRST) {
+        mma16<F16>(d, a[0], a[1], a[2], a[3], b[0], b[1]);
+    } else if (F16) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+    }
+}
 template <bool F16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     if (F16) {
@@ -174,6 +193,14 @@ __device__ __forceinline__ float2 unpack16(uint32_t v) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
+// Two sums in one instruction: x += a, y += b.
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+    uint64_t v, w;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(a), "f"(b));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(w));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
 // (r & m) ^ x in one instruction.
 __device__ __forceinline__ uint32_t and_xor(uint32_t r, uint32_t m, uint32_t x) {
     uint32_t d;
@@ -265,6 +292,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     constexpr int kTok = C::kTok, H = kTok / 16;   // H: 16-token tiles of a subtile
     constexpr int kMinSub = kMinTok / kTok, kSnapC = kSnapCta / kTok, kSnapW = kSnapWarp / kTok;
     constexpr bool kPF16 = F16 && !I8;   // the type of P and V in the second product (bf16's range for scaled P)
+    constexpr int kParts = 2;        // the 16-bit floats that a probability enters it as
     // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
     constexpr float kUp = kPF16 ? 8.f : 0.f;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -826,7 +854,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 }
             }
         }
-        uint32_t ph[H][NT][2], pl[H][NT][2];
+        uint32_t ps[H][NT][2][kParts];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const float v0 = I8 ? sc[kTok + 16 * h + g] * s8_unit<kPF16> : 1.f;
@@ -842,51 +870,58 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     l_run[nt][j] += p[j] + p[j + 2];
                     if (I8) p[j] *= v0, p[j + 2] *= v1;
                 }
-                const uint32_t h0 = pack16<kPF16>(p[0], p[1]), h1 = pack16<kPF16>(p[2], p[3]);
-                const float2 e0 = unpack16<kPF16>(h0), e1 = unpack16<kPF16>(h1);
-                ph[h][nt][0] = movmatrix_t(h0), ph[h][nt][1] = movmatrix_t(h1);
-                pl[h][nt][0] = movmatrix_t(pack16<kPF16>(p[0] - e0.x, p[1] - e0.y));
-                pl[h][nt][1] = movmatrix_t(pack16<kPF16>(p[2] - e1.x, p[3] - e1.y));
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t top = pack16<kPF16>(p[2 * j], p[2 * j + 1]);
+                    const float2 e = unpack16<kPF16>(top);
+                    ps[h][nt][j][0] = top, ps[h][nt][j][1] = pack16<kPF16>(p[2 * j] - e.x, p[2 * j + 1] - e.y);
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i) ps[h][nt][j][i] = movmatrix_t(ps[h][nt][j][i]);
+                }
             }
         }
-        // values
-        if (I8) {
-            const uint32_t v_ld = st + kV + (lane & 15) * vrow + (lane >> 4) * 16;
+        // values, two fragments at a time: the subtile's own sum on the tensor cores, added to the row's in fp32
+        const uint32_t v_ld = st + kV + (I8 ? (lane & 15) * vrow + (lane >> 4) * 16 : ((lane & 7) + ((lane >> 4) << 3)) * vrow + ((lane >> 3) & 1) * 16);
 #pragma unroll
-            for (int mt = 0; mt < kMt; mt += 2) {
-                if (mt >= nmt) break;
+        for (int mt = 0; mt < kMt; mt += 2) {
+            if (mt >= nmt) break;
+            float sum[2][NT][4];
 #pragma unroll
-                for (int h = 0; h < H; ++h) {
+            for (int h = 0; h < H; ++h) {
+                uint32_t v[2][4];   // past an odd nmt: sums that nobody reads
+                if (I8) {
                     uint32_t r[4];
                     ldsm_x4_t(TMA ? piece(st + kV + h * C::kTile, lane & 15, lane >> 4, mt) : v_ld + h * 16 * vrow + mt * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {   // past an odd nmt: accumulators that nobody reads
-                        const uint32_t a0 = s8_pair<kPF16>(r[2 * u]), a1 = s8_pair<kPF16>(r[2 * u] >> 8);
-                        const uint32_t a2 = s8_pair<kPF16>(r[2 * u + 1]), a3 = s8_pair<kPF16>(r[2 * u + 1] >> 8);
+                    for (int u = 0; u < 2; ++u) {
+                        v[u][0] = s8_pair<kPF16>(r[2 * u]), v[u][1] = s8_pair<kPF16>(r[2 * u] >> 8);
+                        v[u][2] = s8_pair<kPF16>(r[2 * u + 1]), v[u][3] = s8_pair<kPF16>(r[2 * u + 1] >> 8);
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        ldsm_x4_t(TMA ? piece(st + kV + h * C::kTile, (lane & 7) + (lane >> 4 << 3), lane >> 3 & 1, 2 * (mt + u)) : v_ld + h * 16 * vrow + (mt + u) * 32, v[u][0], v[u][1], v[u][2], v[u][3]);
+                }
+#pragma unroll
+                for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, ph[h][nt][0], ph[h][nt][1]);
-                            mma16<kPF16>(acc[nt][mt + u], a0, a1, a2, a3, pl[h][nt][0], pl[h][nt][1]);
+                            const uint32_t p[2] = {ps[h][nt][0][i], ps[h][nt][1][i]};
+                            if (h == 0 && i == 0) mma16_part<kPF16, true>(sum[u][nt], v[u], p);
+                            else mma16_part<kPF16, false>(sum[u][nt], v[u], p);
                         }
-                    }
-                }
             }
-        } else {
-            const uint32_t v_ld = st + kV + ((lane & 7) + ((lane >> 4) << 3)) * vrow + ((lane >> 3) & 1) * 16;
 #pragma unroll
-            for (int mt = 0; mt < kMt; ++mt) {
-                if (mt >= nmt) break;
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    uint32_t a0, a1, a2, a3;
-                    ldsm_x4_t(TMA ? piece(st + kV + h * C::kTile, (lane & 7) + (lane >> 4 << 3), lane >> 3 & 1, 2 * mt) : v_ld + h * 16 * vrow + mt * 32, a0, a1, a2, a3);
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, ph[h][nt][0], ph[h][nt][1]);
-                        mma16<kPF16>(acc[nt][mt], a0, a1, a2, a3, pl[h][nt][0], pl[h][nt][1]);
+                    for (int i = 0; i < 4; i += 2) {
+                        float* const o = acc[nt][mt + u] + i;
+                        add2(o[0], o[1], sum[u][nt][i], sum[u][nt][i + 1]);
                     }
-                }
-            }
         }
         // the row, or this warp's stretch, ends
         const bool more = it + 1 < count;

@@ -60,3 +60,35 @@ def test_a_nan_key_appended_into_int8_reaches_the_output():
                                   torch.tensor([40], dtype=torch.int32, device=DEV), 0.1, k_scales=ks, v_scales=vs)
     assert torch.isfinite(out[0, :2]).all() and torch.isfinite(lse[0, :2]).all()
     assert out[0, 2:].isnan().all() and lse[0, 2:].isnan().all()
+
+
+# ------------------------------------------------------------------ how exactly the decode adds up
+
+
+@pytest.mark.parametrize("pool", [HF, torch.int8])
+def test_decode_long_sums_are_rounded_to_nearest(pool):
+    """Rows of values 1 and then -1: a sum that rises to half of the weights and falls back to about nothing.
+
+    Adding in fp32 rounds up to m = 8192 / 16 partial sums of at most l / 2 (l: the weights' sum) to nearest, each by at
+    most 2^-25 l, either way: six standard deviations of a row's are below 6 sqrt(m / 3) 2^-25 l = 2.4e-6 l, and what is
+    left at other places (scores, products, the subtiles' own sums) has no side that it prefers: 0.6e-6 for its mean.
+    Sums that are cut off at every step lose half a unit each time, always the same way: 1024 / 2 2^-24 / 4 = 7.6e-6.
+    """
+    g = gen(71)
+    n, D, P, B = 8192, 64, 16, 2960
+    k = torch.randn(n // P, P, 1, D, generator=g, device=DEV).to(HF)
+    v = torch.ones(n // P, P, 1, D, dtype=HF, device=DEV)
+    v[n // P // 2:] = -1
+    q = torch.randn(B, 1, D, generator=g, device=DEV).to(HF)
+    table = torch.arange(n // P, dtype=torch.int32, device=DEV).expand(B, -1).contiguous()   # all read the same pages
+    lens = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    scale, kw, kd = D ** -0.5, {}, k.double().view(n, D)
+    if pool == torch.int8:
+        one = torch.full((n // P, P, 1), 0.03, device=DEV)
+        k, kw = (k.float() * 32).round().clamp(-127, 127).to(torch.int8), dict(k_scales=one, v_scales=torch.ones_like(one))
+        v, kd = v.to(torch.int8), k.double().view(n, D) * one.double().view(n, 1)
+    out, _ = paged.paged_decode(q, k, v, table, lens, scale, **kw)
+    p = torch.softmax(q.double().view(B, D) @ kd.t() * scale, 1)
+    exact = p[:, :n // 2].sum(1) - p[:, n // 2:].sum(1)
+    off = out.double().view(B, D) - exact[:, None]
+    assert off.mean().abs() <= 3e-6

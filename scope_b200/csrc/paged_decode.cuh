@@ -25,10 +25,13 @@
 //   * The softmax's reference moves only when a score passes it by 2^kSlack: then, and not every subtile, the lanes
 //     agree on a new maximum and the accumulators are rescaled.  Sums are fp32, and only a subtile's own is left to the
 //     tensor cores, which cut partial sums off instead of rounding them (over 11 thousand tokens a warp that came to
-//     2^-14 of the sum, always the same way; the additions cost nothing to 2 %).  P enters the second product as the sum
-//     of two 16-bit values (the rounded one and the rest), which keeps its error below the output's own rounding.
+//     2^-14 of the sum, always the same way; the additions cost nothing to 2 %).  A probability enters the second
+//     product exactly, as the sum of three bf16 values, or to 2^-22 as two in fp16.  (As two bf16 values: 0.15 to 0.3 %
+//     of the 16-bit outputs not the nearest ones; so 0.02 to 0.05 %, the plain form in fp32 0.07 to 0.3 %; 1 request of
+//     4096 tokens 11.7 us and 11.9, the others within 1 %.)  No part is 0 where values may be infinite, so an infinite
+//     value gives an infinite output.
 //   * int8 rows go from shared memory to bf16 (fp16) fragments by bit operations, exactly; the row's scale multiplies
-//     the score, or the probability.
+//     the score, or the probability, which then enters as two fp16 values (three bf16 values: 85 us to 78).
 //   * A row that ends inside one warp's stretch is written at once.  The others leave a state (o, m, l) per warp,
 //     which the CTA joins in shared memory; what crosses CTAs goes through the workspace and is joined by the CTA that
 //     files the last part (a ticket), always in the same order, so results do not depend on timing.
@@ -201,6 +204,43 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(w));
     asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
 }
+// Two floats' leading bits as a pair of 16-bit floats, towards zero: what is left has the sign of the whole.
+template <bool F16>
+__device__ __forceinline__ uint32_t top16(float lo, float hi) {
+    uint32_t d;
+    if (F16) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    else d = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+    return d;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t max16(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if (F16) asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t min16(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if (F16) asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// Two probabilities as PARTS pairs of 16-bit floats that sum to them: in bf16 three, exactly; in fp16 two, to 2^-22 of the
+// larger ones.  Where values may be infinite (not I8), no part of a probability above 0 is 0, else 0 * inf would make a NaN
+// of what is infinite: it is the type's least number at least (2^-133; 2^-24 of probabilities kept 2^8 larger).
+template <bool F16, bool I8, int PARTS>
+__device__ __forceinline__ void split16(float x, float y, uint32_t* part) {
+    const uint32_t least = F16 ? __byte_perm(x > 0.f, y > 0.f, 0x5410) : min16<F16>(top16<F16>(x, y), 0x00010001u);
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        part[i] = F16 && i + 1 == PARTS ? pack16<F16>(x, y) : top16<F16>(x, y);
+        const float2 e = unpack16<F16>(part[i]);
+        add2(x, y, -e.x, -e.y);
+        if (!I8 && (F16 || i)) part[i] = max16<F16>(part[i], least);
+    }
+}
+
 // (r & m) ^ x in one instruction.
 __device__ __forceinline__ uint32_t and_xor(uint32_t r, uint32_t m, uint32_t x) {
     uint32_t d;
@@ -291,8 +331,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     constexpr int kWarps = C::kWarps, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
     constexpr int kTok = C::kTok, H = kTok / 16;   // H: 16-token tiles of a subtile
     constexpr int kMinSub = kMinTok / kTok, kSnapC = kSnapCta / kTok, kSnapW = kSnapWarp / kTok;
-    constexpr bool kPF16 = F16 && !I8;   // the type of P and V in the second product (bf16's range for scaled P)
-    constexpr int kParts = 2;        // the 16-bit floats that a probability enters it as
+    constexpr bool kPF16 = F16 || I8;        // the type of P and V in the second product
+    constexpr int kParts = kPF16 ? 2 : 3;    // the 16-bit floats that a probability enters it as
     // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
     constexpr float kUp = kPF16 ? 8.f : 0.f;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -855,10 +895,18 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             }
         }
         uint32_t ps[H][NT][2][kParts];
+        // int8: the values' scales over the power of two below the subtile's largest, so that fp16 holds their products with
+        // probabilities; what is left out of them is 2^-32 of the largest scale at most
+        float down = 1.f, back = 1.f;
+        if (I8) {
+            static_assert(!I8 || kTok == 32, "a scale a lane");
+            const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(sc[kTok + lane]) & INT32_MAX) >> 23, 1u), 253u);
+            down = __uint_as_float((254 - e) << 23), back = __uint_as_float(e << 23);
+        }
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            const float v0 = I8 ? sc[kTok + 16 * h + g] * s8_unit<kPF16> : 1.f;
-            const float v1 = I8 ? sc[kTok + 16 * h + g + 8] * s8_unit<kPF16> : 1.f;
+            const float v0 = I8 ? sc[kTok + 16 * h + g] * down : 1.f;
+            const float v1 = I8 ? sc[kTok + 16 * h + g + 8] * down : 1.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float(&p)[4] = c[h][nt];
@@ -872,9 +920,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const uint32_t top = pack16<kPF16>(p[2 * j], p[2 * j + 1]);
-                    const float2 e = unpack16<kPF16>(top);
-                    ps[h][nt][j][0] = top, ps[h][nt][j][1] = pack16<kPF16>(p[2 * j] - e.x, p[2 * j + 1] - e.y);
+                    split16<kPF16, I8, kParts>(p[2 * j], p[2 * j + 1], ps[h][nt][j]);
 #pragma unroll
                     for (int i = 0; i < kParts; ++i) ps[h][nt][j][i] = movmatrix_t(ps[h][nt][j][i]);
                 }
@@ -920,7 +966,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                     for (int i = 0; i < 4; i += 2) {
                         float* const o = acc[nt][mt + u] + i;
-                        add2(o[0], o[1], sum[u][nt][i], sum[u][nt][i + 1]);
+                        if (I8) o[0] = fmaf(sum[u][nt][i], back, o[0]), o[1] = fmaf(sum[u][nt][i + 1], back, o[1]);
+                        else add2(o[0], o[1], sum[u][nt][i], sum[u][nt][i + 1]);
                     }
         }
         // the row, or this warp's stretch, ends

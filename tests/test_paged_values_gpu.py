@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from scope_b200 import paged
-from test_paged_gpu import BF, DEV, HF, codes, gen, table_of, turned
+from test_paged_gpu import BF, DEV, HF, U, codes, decode, gen, make_decode, reference, table_of, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,93 @@ def test_decode_long_sums_are_rounded_to_nearest(pool):
     exact = p[:, :n // 2].sum(1) - p[:, n // 2:].sum(1)
     off = out.double().view(B, D) - exact[:, None]
     assert off.mean().abs() <= 3e-6
+
+
+VARIANTS = [  # D, page size, query heads a kv head, width of the table: every compiled head dim, by TMA and by cp.async
+    (64, 16, 4, 200), (128, 16, 4, 200), (128, 24, 4, 100), (128, 16, 12, 200), (192, 32, 4, 100), (256, 16, 2, 200),
+    (80, 16, 4, 200), (112, 7, 9, 300)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D,P,G,width", VARIANTS)
+@pytest.mark.parametrize("spread", [0.0, 1.0, 4.0])
+def test_decode_passes_infinite_values_on(dtype, D, P, G, width, spread):
+    """One infinite value gives every head of its request and kv head that infinity in its dim, both signs in a dim give
+    NaN, and every other output is what it was."""
+    lens = [1, 2, 40, 300, 1300]
+    s = make_decode(lens, 2 * G, 2, D, D, P, dtype, width=width, seed=81, spread=spread)
+    want, want_lse = (x.clone() for x in decode(s))
+    inf = float("inf")
+    # with P = 16 the places are in a request's first, second and last subtile
+    for b, n in enumerate(lens):
+        for t, h, d, value in ((0, 0, 0, inf), (min(17, n - 1), 0, 3, -inf), (n - 1, 1, D - 1, inf), (n // 2, 0, 9, inf),
+                               (0, 1, 16, inf), (n - 1, 1, 16, -inf if n > 1 else inf)):
+            page, off = s["rows"][b]
+            s["v"][page[t], off[t], h, d] = value
+            want[b, h * G:(h + 1) * G, d] = value if (h, d) != (1, 16) or n == 1 else float("nan")
+    out, lse = decode(s)
+    assert torch.equal(lse, want_lse)
+    odd = ~torch.isfinite(want)
+    assert torch.equal(out[~odd], want[~odd])
+    assert torch.equal(out[odd].nan_to_num(nan=7.0), want[odd].nan_to_num(nan=7.0))
+
+
+def test_decode_of_one_token_gives_its_value_row():
+    """Probability 1, nothing to round: whatever the row holds comes out, infinities too."""
+    for dtype in (BF, HF):
+        v = torch.cat([torch.linspace(-8, 8, 61, device=DEV), torch.tensor([float("inf"), float("-inf"), 0.0], device=DEV)]).to(dtype)
+        k = torch.randn(1, 16, 1, 64, device=DEV).to(dtype)
+        pages = torch.full((1, 16, 1, 64), float("nan"), dtype=dtype, device=DEV)
+        pages[0, 0, 0] = v
+        one = torch.ones(1, dtype=torch.int32, device=DEV)
+        out, _ = paged.paged_decode(torch.randn(1, 3, 64, device=DEV).to(dtype), k, pages, one.view(1, 1) * 0, one, 1.0)
+        assert torch.equal(out, v.expand(1, 3, 64))
+
+
+@pytest.mark.parametrize("dtype,pool", [(BF, BF), (HF, HF), (BF, torch.int8), (HF, torch.int8)])
+@pytest.mark.parametrize("D,P,G,width", VARIANTS)
+def test_decode_keeps_all_bits_of_a_probability(dtype, pool, D, P, G, width):
+    """Values that cancel: tokens of probability 1 (times l) and value 1, and as many of just below 1 and value -1, which
+    a probability rounded once would make equal.
+
+    Probabilities enter exactly or to 2^-22, so what is left is a score's error (exact here: one product), exp2's 2^-22,
+    the sums' (n + 64) 2^-24 and the result's rounding."""
+    n, step = 96, 2.0 ** (-10 if dtype == BF else -13)
+    s = make_decode([n, 5 * n], 2 * G, 2, D, D, P, dtype, pool, width=width, seed=82)
+    s["q"].zero_()
+    s["q"][..., 0] = 1
+    s["scale"] = 1.0
+    for page, off in s["rows"]:
+        low = (torch.arange(len(page), device=DEV) % 2).bool()
+        for name in ("k", "v"):
+            s[name][page, off] = 0
+        if pool == torch.int8:
+            s["k"][page[low], off[low], :, 0], s["ks"][page, off] = -1, step
+            s["v"][page, off], s["vs"][page, off] = 64, 1 / 64
+            s["v"][page[low], off[low]] = -64
+        else:
+            s["k"][page[low], off[low], :, 0] = -step
+            s["v"][page, off] = 1
+            s["v"][page[low], off[low]] = -1
+    out, lse = decode(s)
+    exact, exact_lse, _, _ = reference(s)
+    total = (2.0 ** -22 + 2.0 ** -22 + (5 * n + 64) * 2.0 ** -24)
+    assert (1 - U[dtype]) * exact.min() > total   # of the inputs: a probability rounded once would be seen
+    assert ((out.double() - exact).abs() <= U[dtype] * exact.abs() + total).all()
+    assert ((lse.double() - exact_lse).abs() <= 1e-5).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_int8_scales_of_every_size(dtype):
+    """Scales from 1e-30 to 1e30 within a request, and the largest on a token that does not count or counts for nothing."""
+    s = make_decode([600, 64, 33], 8, 2, 128, 128, 16, dtype, torch.int8, seed=83)
+    g = gen(84)
+    for (page, off), low, high in zip(s["rows"], (-3.0, -30.0, 20.0), (0.0, -27.0, 24.0)):
+        s["vs"][page, off] = 10 ** (torch.rand(len(page), 2, generator=g, device=DEV) * (high - low) + low)
+    out, lse = decode(s)
+    exact, exact_lse, room, lse_room = reference(s)
+    exact = exact.clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max) if dtype == HF else exact
+    ok = exact.abs() < torch.finfo(dtype).max
+    least = 2.0 ** -133 if dtype == BF else 2.0 ** -25   # half of the type's least step
+    assert ((out.double() - exact).abs() <= room + least)[ok].all()
+    assert ((lse.double() - exact_lse).abs() <= lse_room).all()

@@ -274,7 +274,7 @@ struct Span {
 template <int kTok>
 __device__ __forceinline__ Span span_of(const Args& a, int b) {
     Span s;
-    s.L = min(max(__ldg(a.seq_lens + b), 0), a.cap);
+    s.L = min(max(a.seq_lens[b], 0), a.cap);
     s.lo = a.window > 0 ? max(s.L - a.window, 0) : 0;
     s.n = (s.L - (s.lo & ~(kTok - 1)) + kTok - 1) / kTok;   // lo = 0 without a token
     return s;
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     : min(max(t + tok, (uint32_t)fs.lo), (uint32_t)fs.L - 1);
         const uint32_t page = (__umulhi(t, a.div_mul) + t) >> a.div_shift;
         f_off = t - page * (uint32_t)a.page_size;
-        f_entry = __ldg(a.table + (int64_t)f_b * a.table_stride + page);
+        f_entry = a.table[(int64_t)f_b * a.table_stride + page];
     };
     auto fill = [&](int slot) {
         if (f_left > 0) {
@@ -645,14 +645,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                 for (int ks = 0; ks < DB / 16; ++ks) {   // dims 16ks + 4t .. 4t + 3
                     uint2 w = make_uint2(0, 0);
-                    if (ks < nks && h < a.G) w = __ldg(reinterpret_cast<const uint2*>(q + 16 * ks));
+                    if (ks < nks && h < a.G) w = *reinterpret_cast<const uint2*>(q + 16 * ks);
                     bq[nt][ks][0] = w.x, bq[nt][ks][1] = w.y;
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < DB / 32; ++i) {      // dims 32i + 8t .. 8t + 7
                     uint4 w = make_uint4(0, 0, 0, 0);
-                    if (32 * i + 8 * t4 < Dk && h < a.G) w = __ldg(reinterpret_cast<const uint4*>(q + 32 * i));
+                    if (32 * i + 8 * t4 < Dk && h < a.G) w = *reinterpret_cast<const uint4*>(q + 32 * i);
                     bq[nt][2 * i][0] = w.x, bq[nt][2 * i][1] = w.y, bq[nt][2 * i + 1][0] = w.z, bq[nt][2 * i + 1][1] = w.w;
                 }
             }

@@ -100,8 +100,8 @@ __device__ __forceinline__ int owner_of(const int* end, int B, int t) {
 }
 
 __global__ void __launch_bounds__(kThreads)
-paged_slots_kernel(const int32_t* seq_lens, const int32_t* __restrict__ new_lens, int B, int32_t* table,
-                   int64_t table_stride, int max_pages, const int32_t* __restrict__ free_pages, int n_ring,
+paged_slots_kernel(const int32_t* seq_lens, const int32_t* new_lens, int B, int32_t* table,
+                   int64_t table_stride, int max_pages, const int32_t* free_pages, int n_ring,
                    const int32_t* ring, int P, int64_t n_tokens, int64_t* __restrict__ slots,
                    int32_t* __restrict__ positions, int32_t* __restrict__ cu_new, int32_t* seq_lens_out,
                    int32_t* ring_out, int* counter) {
@@ -201,8 +201,8 @@ paged_slots_kernel(const int32_t* seq_lens, const int32_t* __restrict__ new_lens
 }
 
 __global__ void __launch_bounds__(kThreads)
-paged_release_kernel(const int32_t* seq_lens, const uint8_t* __restrict__ done, int B,
-                     const int32_t* __restrict__ table, int64_t table_stride, int max_pages, int32_t* free_pages,
+paged_release_kernel(const int32_t* seq_lens, const uint8_t* done, int B,
+                     const int32_t* table, int64_t table_stride, int max_pages, int32_t* free_pages,
                      int n_ring, const int32_t* ring, int P, int32_t* seq_lens_out, int32_t* ring_out, int* counter,
                      int* status) {
     extern __shared__ int sm[];

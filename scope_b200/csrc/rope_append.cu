@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
             const float* row = r.cos_sin + position(axes & 3) * r.rope_dim + 8 * u;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float4 x = __ldg(reinterpret_cast<const float4*>(row) + i), y = __ldg(reinterpret_cast<const float4*>(row + n) + i);
+                const float4 x = reinterpret_cast<const float4*>(row)[i], y = reinterpret_cast<const float4*>(row + n)[i];
                 c[4 * i] = x.x, c[4 * i + 1] = x.y, c[4 * i + 2] = x.z, c[4 * i + 3] = x.w;
                 s[4 * i] = y.x, s[4 * i + 1] = y.y, s[4 * i + 2] = y.z, s[4 * i + 3] = y.w;
             }
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_c
             for (int i = 0; i < 8; ++i) {
                 const int x = axes >> (2 * i) & 3;
                 const float* p = unit + (x & 2 ? (x & 1 ? at[3] : at[2]) : (x & 1 ? at[1] : at[0])) * (uint64_t)(uint32_t)r.rope_dim;
-                c[i] = __ldg(p + i), s[i] = __ldg(p + n + i);
+                c[i] = p[i], s[i] = p[n + i];
             }
         }
         if (r.inverse) {

@@ -37,7 +37,8 @@ bool make_page_map(CUtensorMap* map, const void* base, int64_t row, int64_t page
                    int64_t stride_tok, int64_t stride_head, int64_t stride_page, int inner, int* head_in_dim2);
 
 // Launch as a programmatic dependent of the previous grid on the stream: the kernel calls griddepcontrol.wait before it
-// reads or writes global memory.
+// reads or writes global memory, and reads with plain loads.  The read-only path (__ldg, const __restrict__) promises that
+// nobody writes there while the kernel runs, and it runs from before that wait on.
 template <typename... P, typename... A>
 cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A&&... args) {
     cudaLaunchAttribute attr;

@@ -750,7 +750,9 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 if (I8) cp_async_wait<C::kStages - 2>();   // the scales
                 if (!dead && !mbar_wait_bounded(bars + 8 * slot, phase)) {
                     if (a.status) atomicOr(a.status, kDevTimeout);
-                    mbar_wait_bounded(bars + 8 * slot, phase);   // what is in flight
+                    // whatever is in flight lands before the ring is used for anything else, or the kernel ends
+                    for (int i = 0; i < S - 1 && it + i < count; ++i)
+                        mbar_wait_bounded(bars + 8 * ((slot + i) % S), phase ^ (slot + i >= S));
                     dead = true;
                 }
                 dead = __any_sync(0xffffffffu, dead);

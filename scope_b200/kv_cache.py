@@ -226,8 +226,9 @@ class PagedKVCache:
         """Every request empty, every page free."""
         self.page_table.fill_(-1)
         self.seq_lens.zero_()
-        self._free.copy_(torch.arange(self.num_pages, dtype=torch.int32))
-        self._ring.copy_(torch.tensor([0, self.num_pages, 0], dtype=torch.int32))
+        torch.arange(self.num_pages, out=self._free)
+        self._ring.zero_()
+        self._ring[1].fill_(self.num_pages)
 
     def begin_step(self, new_lens, n_tokens):
         """new_lens int32 [max_requests] on the device: the tokens each request adds (0: none); n_tokens: the rows of

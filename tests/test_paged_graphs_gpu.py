@@ -156,3 +156,18 @@ def test_workspaces_are_zeroed_where_they_lie():
     buf[:64] = 1
     _lib.workspaces.rezero(torch.cuda.current_device())
     assert _lib.workspaces.get(1 << 20, torch.device(DEV)) is buf and not buf.any()
+
+
+def test_a_cache_is_reset_without_waiting():
+    """Nothing of it touches the host's memory, so it can be captured."""
+    cache = scope_b200.PagedKVCache(1, 9, 16, 1, 32, 3, 64, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph, _ = capture(side, cache.reset)
+        cache.begin_step(torch.tensor([40, 20, 70], dtype=torch.int32, device=DEV), 130)
+        assert cache.free_pages() == 4 and cache.refused() == 1 and cache.seq_lens.tolist() == [40, 20, 0]
+        graph.replay()
+        side.synchronize()
+    assert cache.free_pages() == 9 and cache.refused() == 0 and cache.seq_lens.tolist() == [0, 0, 0]
+    assert cache._free.tolist() == list(range(9)) and (cache.page_table == -1).all()

@@ -504,6 +504,10 @@ int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stride_tok, int
  * A request without tokens gives out = 0, lse = -inf.  A page id outside the
  * pool leaves its tokens out and records WS_ERR_DEVICE.  Nothing past a
  * request's length is used, whatever the pages hold there.
+ * WS_ERR_UNSUPPORTED where one request's table is too wide to count in 32 bits:
+ * (min(max_pages * page_size, window + 32 with a window) / 16 + 1) * Hkv * hb
+ * of 2^30 or more (hb = G / 8 rounded up, or G / 16 past 8 heads and up to 128 dims),
+ * whatever its length; and above 32767 kv heads, 2^18 heads a kv head, 2^24 in all.
  */
 int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q_dtype, int B, int G,
                     const ws_paged_kv* kv, const int32_t* page_table, int64_t table_stride, int max_pages,

@@ -202,7 +202,9 @@ class PagedKVCache:
         cache.release(done)                               # finished requests' pages go back
 
     Nothing here waits for the device; ``free_pages()`` and ``refused()`` do.  The table, lengths and ring are updated
-    in place, so the calls can be captured in a CUDA graph.
+    in place, so the calls can be captured in a CUDA graph.  ``begin_step`` serves requests in order and refuses whole what
+    does not fit; a request that lacks pages also keeps those behind it from new ones (``paged.paged_slots``), so admit
+    only what the pool can hold to its end.
     """
 
     def __init__(self, num_layers, num_pages, page_size, num_kv_heads, head_dim, max_requests, max_seq,
@@ -264,5 +266,6 @@ class PagedKVCache:
         return int(self._ring[1])
 
     def refused(self) -> int:
-        """Requests the last begin_step refused (waits for the device)."""
+        """How many requests the last begin_step refused (waits for the device).  Their lengths did not grow; their
+        tokens were not written."""
         return int(self._ring[2])

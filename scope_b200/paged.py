@@ -9,8 +9,12 @@ with unit stride on the head dim, so a head-major ``[n_pages, Hkv, page_size, D]
 ``[n_pages, page_size, Hkv]``).  ``scope_b200.kv_cache.PagedKVCache`` holds the pools of a model's layers and the
 requests' tables.
 
-A step's calls, all asynchronous on the current stream and free of host synchronisation (so they can be captured in a
-CUDA graph):
+The operators are outside autograd: inputs that require gradients are read as they are, and results require none
+(``rope`` with ``inverse`` is the rotation's gradient, for a caller's own ``torch.autograd.Function``).
+
+A step's calls, all asynchronous on the current stream and free of host synchronisation, so they can be captured in a
+CUDA graph (graphs captured on one stream share its workspace: replay them one after the other, and not beside launches
+on that stream):
 
     step = paged_slots(seq_lens, new_lens, page_table, free_pages, ring, page_size, n_tokens)
     q = rope_append(q, k, v, step.positions, cos_sin, step.slots, k_pages, v_pages)       # per layer
@@ -56,7 +60,11 @@ def paged_slots(seq_lens: torch.Tensor, new_lens: torch.Tensor, page_table: torc
     token get slot -1).
 
     A request is refused whole -- its length, row and the ring unchanged, its tokens' slots -1 -- when its pages would
-    pass the table's width, its tokens would pass n_tokens, or too few pages are free; ``ring[2]`` counts them.
+    pass the table's width, its tokens would pass n_tokens, or the pages it lacks, added to those that the requests before
+    it lack, are more than are free.  Requests are served in order: those refused for want of pages count against all
+    later ones, so behind one that does not fit no later request gets a page in this step, even while some are free.
+    ``ring[2]`` counts the refused; which they are shows in the lengths that did not grow.  Refused tokens have no place:
+    the caller repeats them, or admits only what fits.
     ``seq_lens_out`` / ``ring_out`` may be the inputs, which a captured step wants, and share no memory with the others.
     """
     return (_c or _load()).paged_slots(seq_lens, new_lens, page_table, free_pages, ring, page_size, n_tokens, seq_lens_out,
@@ -156,7 +164,8 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     (the new one included), with ``window`` > 0 the last ``window`` of them.  Returns (out [B, H, Dv] in q's type,
     normalised; lse fp32 [B, H]).  A request without tokens gives out = 0, lse = -inf.  What pages hold past a
     request's length is never used.  A page id outside the pool leaves its tokens out and is reported by
-    ``scope_b200.status_take``.
+    ``scope_b200.status_take``.  How rows are fetched follows the table's width, as the lengths stay on the device: for
+    requests known to be of 512 tokens or less, their part ``page_table[:, :n]`` is the faster argument.
     """
     return (_c or _load()).paged_decode(q, k_pages, v_pages, page_table, seq_lens, scale, window, k_scales, v_scales, out,
                                         lse)

@@ -76,8 +76,8 @@ int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q
     a.whole = kv->page_size % 16 == 0;
     const int inner = paged::inner_of(DB * (int)eb);
     // Rows short by the table's width, or the window, are faster with cp.async, whose first bytes are there sooner and
-    // whose last subtile costs less (us with TMA and with cp.async: 204 requests of up to 101 tokens 24.8 and 23.4, 64 of
-    // up to 2 9.3 and 8.5; 1 of 4096 11.5 and 11.9, 16 of up to 32768 131 and 141).
+    // whose last subtile costs less (us with TMA and with cp.async: 204 requests of up to 101 tokens 12.9 and 12.5, 64 of
+    // up to 2 8.8 and 8.3; 1 of 4096 11.9 and 12.1, 16 of up to 32768 136 and 146).
     const bool whole_rows = kv->page_size % 16 == 0 && kv->Dk == DB && kv->Dv == DB && kv->n_pages > 0;
     a.tma = whole_rows && (window > 0 ? std::min(a.cap, window) : a.cap) > 512 &&
             make_page_map(&a.kmap, kv->k, DB * eb, kv->page_size, kv->Hkv, kv->n_pages, kv->k_stride_tok * eb,

@@ -13,8 +13,8 @@
 //   * A stage is filled by TMA where the pages are whole 16-token tiles, Dk = Dv is the variant's bound and the pool's
 //     strides are what a tensor map takes; else by 16-byte cp.async (any page size, any head dims).  The memory gives more
 //     to the fewer and larger requests: loads alone run at 7.3 TB/s in blocks of 4 KB by TMA, 6.7 in 16-byte pieces, 6.7
-//     in rows of 256 bytes by bulk copies.  Measured: 32 requests of 131072 tokens 1316 us with cp.async, 1199 with TMA;
-//     16 ragged 141 and 131; 8 in int8 76.7 and 75.6; 1 request of 4096 tokens 11.9 and 11.5.
+//     in rows of 256 bytes by bulk copies.  Measured under lasting load: 32 requests of 131072 tokens 1365 us with
+//     cp.async, 1274 with TMA; 16 ragged 146 and 136; 8 in int8 87 and 84; 1 request of 4096 tokens 12.1 and 11.9.
 //   * A subtile is one stage.  With pages of whole 16-token tiles a tile has one page, and its rows lie at one stride; else
 //     each lane looks up one token's page and the row addresses travel by shuffle.  Entries are fetched a subtile ahead.
 //     Of tokens past the length, before the window or on a page that is none, the scores are -inf, and the values in
@@ -36,11 +36,11 @@
 //     which the CTA joins in shared memory; what crosses CTAs goes through the workspace and is joined by the CTA that
 //     files the last part (a ticket), always in the same order, so results do not depend on timing.
 //
-// Measured on a B200 (device time): 32 requests of 131072 tokens, 32 query and 4 kv heads of 128, bf16: 1199 us
-// (8.59 GB, 7.17 TB/s; a copy reaches 6.55); 16 ragged to 32768 tokens, 32 and 8 heads: 131 us (852 MB, 6.5 TB/s);
-// 8 of 16384 to 65536 tokens in int8: 76 us (393 MB, 5.2 TB/s).  What is left at those is some 4 us before the first
-// rows arrive (the lengths, the table and the rows come one after the other) and 8 us after the last (join, ticket,
-// join).  Small calls are those latencies alone: 1 request of 4096 tokens 11.5 us, of 100 tokens 6 us.
+// Measured on a B200 (device time, a few replays on a cool card): 32 requests of 131072 tokens, 32 query and 4 kv heads of
+// 128, bf16: 1207 us (8.59 GB, 7.1 TB/s; a copy reaches 6.55); 16 ragged to 32768 tokens, 32 and 8 heads: 131.7 us
+// (852 MB, 6.5 TB/s); 8 of 16384 to 65536 tokens in int8: 78 us (393 MB, 5.0 TB/s).  What is left at those is some 4 us
+// before the first rows arrive (the lengths, the table and the rows come one after the other) and 8 us after the last
+// (join, ticket, join).  Small calls are those latencies alone: 1 request of 4096 tokens 12.0 us, of 100 9.8.
 //
 // Why an even split suffices: with 128 KB of copies in flight an SM, 16 of the 148 SMs ended 10% after the others, which
 // the memory serves first; with 80 KB all end within 3% of one another, and the whole sooner.  Built and measured slower:
@@ -62,8 +62,9 @@ constexpr int most_smem(int warps) { return ((227 << 10) - 464 * warps - 128) & 
 constexpr int kMinTok = 32;     // tokens a warp takes before another CTA joins in
 // Rows up to so many tokens are not cut by a border between two CTAs, or two warps: the border moves to the nearer end
 // of the row, which unbalances the stretches by half a row at most and saves the joining (about 5 us; measured with
-// 640, 320, 160 and 0 tokens: 78 requests of 26 to 377 tokens 12.9, 15.7, 16.0, 16.1 us; 128 of up to 700, 29.0, 29.8,
-// 31.1, 31.1 us; longer rows the same).
+// 640, 320, 160 and 0 tokens: 78 requests of 26 to 377 tokens 14.0, 15.1, 15.8, 16.6 us; 128 of up to 700, 26.8, 29.2,
+// 27.9, 27.9 us; longer rows the same.  The price is balance: 116 subtiles in the longest CTA of the latter's like, 96 on
+// average).
 constexpr int kSnapCta = 640;
 constexpr int kSnapWarp = 64;
 constexpr float kSlack = 6.f;   // log2 of how far a probability may pass its bound before the reference moves
@@ -104,7 +105,8 @@ struct Args {
 // 8 requests to 65536: 82 us to 78; 127 requests to 13489 with rows of 64: 167 us to 132).  As many warps, each with two
 // stages, as shared memory and the registers allow
 // (measured at D = 128 in 16 bits, 16 ragged requests to 32768: 8 warps 160 us, 10 warps 152, 12 warps 157; three stages
-// put more in flight than the memory takes, and the SMs it serves last fall behind).
+// put more in flight than the memory takes, and the SMs it serves last fall behind).  These figures are of when the choice
+// was made, with cp.async and each probability in two parts.
 template <bool I8, int DB, int NT>
 struct Cfg {
     static constexpr int kMt = DB / 16;                                   // accumulator fragments of a head tile
@@ -320,8 +322,8 @@ __device__ __forceinline__ void finish(const Args& a, int64_t head0, int left, i
 // How rows come, and what is known of them when compiling.
 enum : int {
     kAny = 0,     // 16-byte cp.async; head dims up to DB
-    kExact = 1,   // 16-byte cp.async; Dk = Dv = DB, so a row's pieces need no bounds (358 instructions a subtile to 305
-                  // with 16-bit rows, 611 to 518 with int8; 2 requests of 100 tokens in pages of 8: 6.4 us to 4.9)
+    kExact = 1,   // 16-byte cp.async; Dk = Dv = DB, so a row's pieces need no bounds (8 requests to 65536
+                  // tokens in int8 99 us to 87, 204 of up to 101 tokens 14.5 to 12.5, 2 of 100 in pages of 8 11.5 to 10.2)
     kTma = 2,     // TMA; Dk = Dv = DB, pages of whole 16-token tiles
 };
 template <bool F16, bool I8, int DB, int NT, int MODE>

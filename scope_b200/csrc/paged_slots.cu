@@ -15,9 +15,10 @@
 // launch, and takes kTokensPerCta tokens; a step of up to that many is one
 // CTA.  Lengths and ring may be updated in place: with more than one CTA then
 // by the one that finishes last (a ticket), when no other reads them any more.
-// Measured: 64 requests of one token each 3.2 us; 512 requests, half of them
-// prompts of up to 1024 tokens (130 thousand slots), 5.4 us, 7.9 with one scan
-// after the other and a ticket in every call.
+// Measured: 64 requests of one token each 3.3 us (3.4 in place); 512 requests,
+// half of them prompts of up to 1024 tokens (129 thousand slots), 5.2 us, and
+// 7.2 in place, where 126 CTAs take a ticket.  Release: 5 of the 64 requests
+// (781 pages) 3.3 us, 512 at once (182 thousand pages) 10.7.
 #include <cstdio>
 
 #include "common.cuh"

@@ -13,8 +13,10 @@
 // units of a head are padded to a power of two and lie in one warp, which the
 // int8 form needs for the row's maximum.  Measured: 16384 x 32 heads of 128,
 // three axes, 47.3 us (277 MB, 5.9 TB/s); append of 16384 tokens of 32 + 4 + 4
-// heads 60.3 us (345 MB, 5.7 TB/s); 4097 tokens of 20 + 5 + 5 heads of 80 into int8 15.0 us.  The first rows are asked for before the position is known, whose turns would else
-// delay them by two latencies (47.9 and 61.9 us; 1202 tokens of 40 + 8 + 8 heads 11.9 to 10.8; 64 tokens 2.65 to 2.47).
+// heads 60.3 us (345 MB, 5.7 TB/s); 4097 tokens of 20 + 5 + 5 heads of 80 into
+// int8 15.0 us.  The first rows are asked for before the position is known,
+// whose turns would else delay them by two latencies (47.9 and 61.9 us; 1202
+// tokens of 40 + 8 + 8 heads 11.9 to 10.8; 64 tokens 2.65 to 2.47).
 //
 // Products and sums are rounded one by one (no fused multiply-add): the result
 // is the elementwise formula's, bit for bit, so an int8 code never depends on

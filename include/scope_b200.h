@@ -47,6 +47,7 @@ extern "C" {
 #define WS_DTYPE_F32 1
 #define WS_DTYPE_I8 2
 #define WS_DTYPE_F16 3     /* the paged entries only */
+#define WS_DTYPE_E4M3 4    /* 8-bit floats of 4 and 3 bits, no infinities: pools of pages only */
 
 /* ---- GQA output modes (what the reference wrappers return) */
 #define WS_OUT_NORM_BF16 0   /* out bf16 normalised, max/sum bf16: fused_cpu_attn on bf16 (kernel/cpu_attn.cpp:631-634) */
@@ -396,23 +397,25 @@ int ws_lse_merge_strided(const float* o_parts, int64_t o_part_stride, const floa
  * Keys and values of slot s = page * page_size + offset, kv head h:
  *   k (page, offset, h, d) at k + page*k_stride_page + offset*k_stride_tok + h*k_stride_head + d   (Dk wide)
  *   v the same with v_stride_* and Dv.
- * dtype WS_DTYPE_BF16, WS_DTYPE_F16, or WS_DTYPE_I8 with one fp32 scale per
- * row (value = code * scale) at k_scales + page*ks_stride_page +
- * offset*ks_stride_tok + h*ks_stride_head, likewise v_scales.
+ * dtype WS_DTYPE_BF16, WS_DTYPE_F16, or WS_DTYPE_I8 or WS_DTYPE_E4M3 with one
+ * fp32 scale per block of scale_block tokens (0 counts as 1: a scale per row;
+ * it divides page_size) and head: value = code * scale, the scale at k_scales +
+ * page*ks_stride_page + (offset / scale_block)*ks_stride_tok + h*ks_stride_head,
+ * likewise v_scales.
  * Constraints: Dk, Dv multiples of 16, at most 256; page_size >= 1; k, v
  * 16-byte aligned with strides of whole 16 bytes.
  */
 typedef struct ws_paged_kv {
     void* k;
     void* v;
-    float* k_scales;   /* WS_DTYPE_I8 only */
+    float* k_scales;   /* 8-bit types only */
     float* v_scales;
     int64_t n_pages;
     int64_t k_stride_page, k_stride_tok, k_stride_head;
     int64_t v_stride_page, v_stride_tok, v_stride_head;
     int64_t ks_stride_page, ks_stride_tok, ks_stride_head;
     int64_t vs_stride_page, vs_stride_tok, vs_stride_head;
-    int32_t page_size, Hkv, Dk, Dv, dtype, reserved;
+    int32_t page_size, Hkv, Dk, Dv, dtype, scale_block;
 } ws_paged_kv;
 
 /*
@@ -478,10 +481,20 @@ typedef struct ws_rope {
  * values into the paged cache, in one launch.
  *   q [N, H, Dk] -> q_out (may be q); k [N, Hkv, Dk], v [N, Hkv, Dv]: element
  *   (t, h, d) at base + t*stride_tok + h*stride_head + d; dtype WS_DTYPE_BF16 or
- *   WS_DTYPE_F16.  The pool holds that type, or int8 codes:
+ *   WS_DTYPE_F16.  The pool holds that type, or int8 codes with a scale per row:
  *   scale = max(max|x|, 1e-6) / 127, code = rne(x * 127 / max) per row (the rule
  *   of ws_csa_kv_quantize_s8), taken from the rotated fp32 row.  A NaN in a row
  *   makes its scale NaN, an infinity makes it infinite; the codes are 0 then.
+ *   With a scale per block of tokens (scale_block > 1, or any with e4m3) a block
+ *   is filled from its front.  Of its rows in this call, the first at offset o:
+ *     s_new = max(max|x|, 1e-6) / 127 (int8), or the least power of two with
+ *             max(max|x|, 1e-6) <= 448 s_new (e4m3);
+ *     s = max(s_old, s_new) where o > 0 (s_old: the scale that lies there), else s_new;
+ *     code = rne(x * (1 / s)), within 127 or 448; rows before o whose s_old < s get
+ *     rne(code * (s_old * (1 / s))), and rows behind the last written are nobody's.
+ *   s NaN or infinite: all these codes are 0, so the block reads back as NaN.
+ *   A block's tokens follow one another in the call, dropped ones aside, in the
+ *   order of their slots; ws_paged_slots lays them so.
  *   slots int64 [N]: token t's keys and values go to slot slots[t]; a negative
  *   slot drops them, one past the pool drops them and records WS_ERR_DEVICE.
  * rope NULL: no rotation.  H = 0: no queries.  kv NULL: queries only (k, v,
@@ -495,7 +508,7 @@ int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stride_tok, int
 /*
  * Attention of one new token per request over the paged cache.
  *   q [B, Hkv*G, Dk] in q_dtype (WS_DTYPE_BF16 or WS_DTYPE_F16; the pool holds
- *   that type or int8): head (b, h) at q + b*q_stride_b + h*q_stride_h,
+ *   that type, int8 or e4m3): head (b, h) at q + b*q_stride_b + h*q_stride_h,
  *   h = kvh * G + g, 16-byte aligned rows;
  *   page_table int32 [B, max_pages], row b at page_table + b*table_stride;
  *   seq_lens int32 [B]: tokens [0, seq_lens[b]) are attended (clipped to
@@ -514,6 +527,41 @@ int ws_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q
                     const int32_t* seq_lens, int window, float scale, void* out, float* out_lse, void* workspace,
                     size_t workspace_bytes, void* stream);
 size_t ws_paged_decode_workspace_size(int B, int Hkv, int G, int Dv);
+
+/*
+ * Differential attention of one new token per request over the paged cache:
+ *   o = softmax(scale q1 k1) v - lam softmax(scale q2 k2) v,
+ *   out = o, or with norm_weight  o * rsqrt(mean(o^2) + norm_eps) * norm_weight.
+ * The pool's heads come in pairs g: the keys of heads 2g and 2g + 1 are the two
+ * maps', the values of head 2g are the first Dv dims of the pair's values and
+ * those of head 2g + 1 the last.  G query heads share a pair:
+ *   q [B, 2*H, Dk], H = Hkv/2 * G: map m of head h at q + b*q_stride_b + (2*h + m)*q_stride_h;
+ *   lam fp32, head h's at lam + h*lam_stride (0: one for all); norm_weight fp32 [2*Dv] or NULL;
+ *   out [B, H, 2*Dv] contiguous in q_dtype; out_lse [B, 2*H] fp32, of each map (NULL: none).
+ * Dk, Dv at most 128; everything else, the workspace too, as in ws_paged_decode
+ * (whose limits hold with Hkv/2 heads of 2*G queries, 2*Dk and 2*Dv dims).
+ */
+int ws_paged_diff_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, int q_dtype, int B, int G,
+                         const ws_paged_kv* kv, const int32_t* page_table, int64_t table_stride, int max_pages,
+                         const int32_t* seq_lens, int window, float scale, const float* lam, int lam_stride,
+                         const float* norm_weight, float norm_eps, void* out, float* out_lse, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * Requests' rows read back from the paged cache, packed one after the other:
+ * row r of the outputs, cu[b] <= r < cu[b+1], is token starts[b] + r - cu[b] of
+ * request b (starts NULL: from the first).
+ *   cu int32 [B+1], ascending; starts int32 [B];
+ *   k_out [n_tokens, Hkv, Dk], v_out [n_tokens, Hkv, Dv] contiguous, 16-byte
+ *   aligned, in out_dtype (WS_DTYPE_BF16 or WS_DTYPE_F16): code * scale rounded
+ *   to fp32 and once more to out_dtype; a 16-bit pool is read in its own type.
+ * Rows before cu[0] and from cu[B] on stay as they were.  A token before the
+ * first, past the table's width or on a page outside the pool gives zeros and
+ * records WS_ERR_DEVICE.  One launch.
+ */
+int ws_paged_read(const ws_paged_kv* kv, const int32_t* page_table, int64_t table_stride, int max_pages, int B,
+                  const int32_t* cu, const int32_t* starts, int64_t n_tokens, int out_dtype, void* k_out, void* v_out,
+                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -31,6 +31,7 @@ WS_DTYPE_BF16 = 0
 WS_DTYPE_F32 = 1
 WS_DTYPE_I8 = 2
 WS_DTYPE_F16 = 3   # the paged entries only
+WS_DTYPE_E4M3 = 4  # pools of pages only
 
 WS_OUT_NORM_BF16 = 0
 WS_OUT_UNNORM_F32 = 1
@@ -98,6 +99,9 @@ SIGNATURES = {
                             _V]),
     "ws_paged_decode": (_i, [_V, _i64, _i64, _i, _i, _i, _V, _V, _i64, _i, _V, _i, _f, _V, _V, _V, _sz, _V]),
     "ws_paged_decode_workspace_size": (_sz, [_i, _i, _i, _i]),
+    "ws_paged_diff_decode": (_i, [_V, _i64, _i64, _i, _i, _i, _V, _V, _i64, _i, _V, _i, _f, _V, _i, _V, _f, _V, _V, _V, _sz,
+                                  _V]),
+    "ws_paged_read": (_i, [_V, _V, _i64, _i, _i, _V, _V, _i64, _i, _V, _V, _V]),
     "ws_peer_exchange_bytes": (_sz, [_i, _i64, _i]),
     "ws_peer_slot_offset": (_sz, [_i, _i64, _i, _i]),
     "ws_peer_buffer_create": (_i, [_sz, ctypes.POINTER(_V), _V]),
@@ -163,7 +167,8 @@ def binding():
                 spec.loader.exec_module(mod)
                 from .paged import PagedStep
                 address = [ctypes.cast(getattr(L, n), _V).value for n in (
-                    "ws_last_error", "ws_paged_slots", "ws_paged_release", "ws_rope_append", "ws_paged_decode")]
+                    "ws_last_error", "ws_paged_slots", "ws_paged_release", "ws_rope_append", "ws_paged_decode",
+                    "ws_paged_diff_decode", "ws_paged_read")]
                 mod.setup(*address, L.ws_paged_slots_workspace_size(), L.ws_paged_decode_workspace_size(1, 1, 1, 16),
                           ScopeError, workspaces.get, workspaces._bufs, PagedStep)
                 _binding = mod

@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Device.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -30,6 +31,8 @@ decltype(&ws_paged_slots) p_paged_slots;
 decltype(&ws_paged_release) p_paged_release;
 decltype(&ws_rope_append) p_rope_append;
 decltype(&ws_paged_decode) p_paged_decode;
+decltype(&ws_paged_diff_decode) p_paged_diff_decode;
+decltype(&ws_paged_read) p_paged_read;
 size_t g_slots_ws, g_decode_ws;   // workspace sizes (they do not depend on the call)
 PyObject *g_error, *g_pool_get, *g_pool_bufs, *g_step;   // ScopeError, workspaces.get, its dict, PagedStep
 
@@ -313,8 +316,8 @@ ws_paged_kv pool_of(const char* what, PyObject* k_pages, PyObject* v_pages, PyOb
                     const at::Device& dev) {
     const at::Tensor &k = tensor(what, "k_pages", k_pages), &v = tensor(what, "v_pages", v_pages);
     const at::ScalarType type = k.scalar_type();
-    const bool i8 = type == at::kChar;
-    if (!i8 && half_of(type) < 0) refuse(what, "the pool must be bf16, fp16 or int8");
+    const bool e4 = type == at::kFloat8_e4m3fn, eight = type == at::kChar || e4;
+    if (!eight && half_of(type) < 0) refuse(what, "the pool must be bf16, fp16 or int8, or float8_e4m3fn");
     if (k.dim() != 4 || v.dim() != 4 || k.size(0) != v.size(0) || k.size(1) != v.size(1) || k.size(2) != v.size(2) ||
         v.scalar_type() != type || k.device() != dev || v.device() != dev)
         refuse(what, "k_pages, v_pages must be [n_pages, page_size, Hkv, D] of one type on " + on(dev));
@@ -323,25 +326,28 @@ ws_paged_kv pool_of(const char* what, PyObject* k_pages, PyObject* v_pages, PyOb
     memset(&p, 0, sizeof(p));
     for (int d = 1; d < 4; ++d)
         if (k.size(d) > INT32_MAX || v.size(d) > INT32_MAX) refuse(what, "bad pool shape");
-    if (i8) {
-        if (k_scales == Py_None || v_scales == Py_None) refuse(what, "an int8 pool needs k_scales and v_scales");
+    if (eight) {
+        if (k_scales == Py_None || v_scales == Py_None)
+            refuse(what, std::string(e4 ? "a float8_e4m3fn" : "an int8") + " pool needs k_scales and v_scales");
         const at::Tensor &ks = tensor(what, "k_scales", k_scales), &vs = tensor(what, "v_scales", v_scales);
         for (const at::Tensor* s : {&ks, &vs})
-            if (s->scalar_type() != at::kFloat || s->dim() != 3 || s->size(0) != k.size(0) || s->size(1) != k.size(1) ||
-                s->size(2) != k.size(2) || s->device() != dev)
-                refuse(what, "scales must be fp32 [n_pages, page_size, Hkv] on " + on(dev));
+            if (s->scalar_type() != at::kFloat || s->dim() != 3 || s->size(0) != k.size(0) || s->size(2) != k.size(2) ||
+                s->device() != dev || s->size(1) != ks.size(1) || (s->size(1) < 1 ? k.size(1) > 0 : k.size(1) % s->size(1) != 0))
+                refuse(what, "scales must be fp32 [n_pages, page_size, Hkv], or [n_pages, blocks, Hkv] with pages of whole blocks, on " +
+                                 on(dev));
+        p.scale_block = ks.size(1) ? (int)(k.size(1) / ks.size(1)) : 1;
         p.k_scales = data<float>(ks), p.v_scales = data<float>(vs);
         p.ks_stride_page = ks.stride(0), p.ks_stride_tok = ks.stride(1), p.ks_stride_head = ks.stride(2);
         p.vs_stride_page = vs.stride(0), p.vs_stride_tok = vs.stride(1), p.vs_stride_head = vs.stride(2);
     } else if (k_scales != Py_None || v_scales != Py_None) {
-        refuse(what, "scales belong to an int8 pool");
+        refuse(what, "scales belong to an int8 or float8_e4m3fn pool");
     }
     p.k = k.data_ptr(), p.v = v.data_ptr();
     p.n_pages = k.size(0);
     p.k_stride_page = k.stride(0), p.k_stride_tok = k.stride(1), p.k_stride_head = k.stride(2);
     p.v_stride_page = v.stride(0), p.v_stride_tok = v.stride(1), p.v_stride_head = v.stride(2);
     p.page_size = (int)k.size(1), p.Hkv = (int)k.size(2), p.Dk = (int)k.size(3), p.Dv = (int)v.size(3);
-    p.dtype = i8 ? WS_DTYPE_I8 : half_of(type);
+    p.dtype = e4 ? WS_DTYPE_E4M3 : eight ? WS_DTYPE_I8 : half_of(type);
     return p;
 }
 
@@ -400,48 +406,149 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// What the two decodes share: checks, outputs, the call.  a: q, k_pages, v_pages, page_table, seq_lens, scale, window,
+// k_scales, v_scales, out, lse.  maps: 2 where heads come in pairs.
+template <typename F>
+PyObject* decode(const char* what, PyObject* const* a, int maps, F&& call) {
+    const at::Tensor &q = tensor(what, "q", a[0]), &table = tensor(what, "page_table", a[3]),
+                     &lens = tensor(what, "seq_lens", a[4]);
+    if (!q.is_cuda()) refuse(what, "CUDA tensors required (there is no CPU path)");
+    const at::Device dev = q.device();
+    const at::ScalarType st = q.scalar_type();
+    const int type = half_of(st);
+    if (type < 0 || q.dim() != 3 || !unit(q, 2))
+        refuse(what, "q must be bf16 or fp16 [B, H, Dk] with unit stride on the head dim");
+    const int64_t B = q.size(0), H = q.size(1);
+    const ws_paged_kv p = pool_of(what, a[1], a[2], a[7], a[8], dev);
+    if (p.dtype != type && p.dtype != WS_DTYPE_I8 && p.dtype != WS_DTYPE_E4M3)
+        refuse(what, "the pool must hold q's type or int8 or float8_e4m3fn");
+    if (p.Hkv % maps) refuse(what, "the pool's heads must come in pairs");
+    if (q.size(2) != p.Dk || p.Hkv < 1 || H < 1 || H % p.Hkv)
+        refuse(what, maps == 1 ? "q must be [B, Hkv * G, Dk]" : "q must be [B, 2 * H, Dk], with H a multiple of the pool's pairs");
+    if (B > INT32_MAX || H > INT32_MAX) refuse(what, "bad shape");
+    want_table(what, table, B, dev);
+    want(what, "seq_lens", lens, at::kInt, 1, dev);
+    if (lens.numel() != B) refuse(what, "seq_lens must hold one entry per request");
+    const double scale = PyFloat_AsDouble(a[5]);
+    if (scale == -1.0 && PyErr_Occurred()) throw PythonError();
+    const int64_t window = integer(a[6]);
+    if (window < 0) refuse(what, "window must not be negative");
+    const c10::cuda::OptionalCUDAGuard guard(dev);
+    const at::Tensor out = output(what, "out", a[9], {B, H / maps, maps * p.Dv}, st, dev);
+    const at::Tensor lse = output(what, "lse", a[10], {B, H}, at::kFloat, dev);
+    for (const at::Tensor* t : {&q, &table, &lens}) {
+        if (a[9] != Py_None) at::assert_no_overlap(out, *t);
+        if (a[10] != Py_None) at::assert_no_overlap(lse, *t);
+    }
+    void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const Workspace ws = workspace(g_decode_ws, dev, stream);
+    call(q, type, (int)B, (int)(H / p.Hkv), p, table, lens, (int)std::min<int64_t>(window, INT32_MAX), (float)scale, out, lse, ws,
+         stream);
+    PyObject* r = PyTuple_New(2);
+    if (!r) return nullptr;
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(lse));
+    return r;
+}
+int pages_of(const at::Tensor& table) { return (int)std::min<int64_t>(table.size(1), INT32_MAX); }
+
 // q, k_pages, v_pages, page_table, seq_lens, scale, window, k_scales, v_scales, out, lse
 PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 11, [&]() -> PyObject* {
-        const char* what = "paged_decode";
-        const at::Tensor &q = tensor(what, "q", a[0]), &table = tensor(what, "page_table", a[3]),
-                         &lens = tensor(what, "seq_lens", a[4]);
-        if (!q.is_cuda()) refuse(what, "CUDA tensors required (there is no CPU path)");
-        const at::Device dev = q.device();
-        const at::ScalarType st = q.scalar_type();
-        const int type = half_of(st);
-        if (type < 0 || q.dim() != 3 || !unit(q, 2))
-            refuse(what, "q must be bf16 or fp16 [B, H, Dk] with unit stride on the head dim");
-        const int64_t B = q.size(0), H = q.size(1);
-        const ws_paged_kv p = pool_of(what, a[1], a[2], a[7], a[8], dev);
-        if (p.dtype != type && p.dtype != WS_DTYPE_I8) refuse(what, "the pool must hold q's type or int8");
-        if (q.size(2) != p.Dk || p.Hkv < 1 || H < 1 || H % p.Hkv) refuse(what, "q must be [B, Hkv * G, Dk]");
-        if (B > INT32_MAX || H > INT32_MAX) refuse(what, "bad shape");
+        return decode("paged_decode", a, 1, [&](const at::Tensor& q, int type, int B, int G, const ws_paged_kv& p, const at::Tensor& table,
+                                                const at::Tensor& lens, int window, float scale, const at::Tensor& out,
+                                                const at::Tensor& lse, const Workspace& ws, void* stream) {
+            check(p_paged_decode(q.data_ptr(), q.stride(0), q.stride(1), type, B, G, &p, data<int32_t>(table), table.stride(0),
+                                 pages_of(table), data<int32_t>(lens), window, scale, out.data_ptr(), data<float>(lse), ws.ptr,
+                                 ws.bytes, stream),
+                  "ws_paged_decode");
+        });
+    });
+}
+
+// q, k_pages, v_pages, page_table, seq_lens, scale, window, k_scales, v_scales, out, lse, lam, norm_weight, norm_eps
+PyObject* paged_diff_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 14, [&]() -> PyObject* {
+        const char* what = "paged_diff_decode";
+        return decode(what, a, 2, [&](const at::Tensor& q, int type, int B, int G, const ws_paged_kv& p, const at::Tensor& table,
+                                      const at::Tensor& lens, int window, float scale, const at::Tensor& out, const at::Tensor& lse,
+                                      const Workspace& ws, void* stream) {
+            const at::Device dev = q.device();
+            const int64_t H = q.size(1) / 2;
+            const at::Tensor& lam = tensor(what, "lam", a[11]);
+            if (lam.scalar_type() != at::kFloat || lam.device() != dev || lam.dim() > 1 || (lam.numel() != H && lam.numel() != 1))
+                refuse(what, "lam must be fp32 [" + std::to_string(H) + "], or one value, on " + on(dev));
+            const int64_t lam_stride = lam.numel() == 1 ? 0 : lam.stride(0);
+            if (lam_stride > INT32_MAX) refuse(what, "bad stride of lam");
+            const float* weight = nullptr;
+            if (a[12] != Py_None) {
+                const at::Tensor& w = tensor(what, "norm_weight", a[12]);
+                want(what, "norm_weight", w, at::kFloat, 1, dev);
+                if (w.numel() != 2 * p.Dv) refuse(what, "norm_weight must hold " + std::to_string(2 * p.Dv) + " values");
+                weight = data<float>(w);
+            }
+            const double eps = PyFloat_AsDouble(a[13]);
+            if (eps == -1.0 && PyErr_Occurred()) throw PythonError();
+            if (!(eps >= 0)) refuse(what, "norm_eps must not be negative");
+            for (const int i : {11, 12}) {
+                if (a[i] == Py_None) continue;
+                if (a[9] != Py_None) at::assert_no_overlap(out, THPVariable_Unpack(a[i]));
+                if (a[10] != Py_None) at::assert_no_overlap(lse, THPVariable_Unpack(a[i]));
+            }
+            check(p_paged_diff_decode(q.data_ptr(), q.stride(0), q.stride(1), type, B, G, &p, data<int32_t>(table), table.stride(0),
+                                      pages_of(table), data<int32_t>(lens), window, scale, data<float>(lam), (int)lam_stride, weight,
+                                      (float)eps, out.data_ptr(), data<float>(lse), ws.ptr, ws.bytes, stream),
+                  "ws_paged_diff_decode");
+        });
+    });
+}
+
+// k_pages, v_pages, page_table, cu_seqlens, n_tokens, starts, k_scales, v_scales, dtype, k_out, v_out
+PyObject* paged_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 11, [&]() -> PyObject* {
+        const char* what = "paged_read";
+        const at::Tensor &k = tensor(what, "k_pages", a[0]), &table = tensor(what, "page_table", a[2]),
+                         &cu = tensor(what, "cu_seqlens", a[3]);
+        if (!k.is_cuda()) refuse(what, "CUDA tensors required (there is no CPU path)");
+        const at::Device dev = k.device();
+        const ws_paged_kv p = pool_of(what, a[0], a[1], a[6], a[7], dev);
+        want(what, "cu_seqlens", cu, at::kInt, 1, dev);
+        const int64_t B = cu.numel() - 1, N = integer(a[4]);
+        if (B < 0 || B > INT32_MAX || N < 0) refuse(what, "cu_seqlens must hold one entry more than requests, n_tokens not be negative");
         want_table(what, table, B, dev);
-        want(what, "seq_lens", lens, at::kInt, 1, dev);
-        if (lens.numel() != B) refuse(what, "seq_lens must hold one entry per request");
-        const double scale = PyFloat_AsDouble(a[5]);
-        if (scale == -1.0 && PyErr_Occurred()) throw PythonError();
-        const int64_t window = integer(a[6]);
-        if (window < 0) refuse(what, "window must not be negative");
-        const c10::cuda::OptionalCUDAGuard guard(dev);
-        const at::Tensor out = output(what, "out", a[9], {B, H, p.Dv}, st, dev);
-        const at::Tensor lse = output(what, "lse", a[10], {B, H}, at::kFloat, dev);
-        for (const at::Tensor* t : {&q, &table, &lens}) {
-            if (a[9] != Py_None) at::assert_no_overlap(out, *t);
-            if (a[10] != Py_None) at::assert_no_overlap(lse, *t);
+        const int32_t* starts = nullptr;
+        if (a[5] != Py_None) {
+            const at::Tensor& s = tensor(what, "starts", a[5]);
+            want(what, "starts", s, at::kInt, 1, dev);
+            if (s.numel() != B) refuse(what, "starts must hold one entry per request");
+            starts = data<int32_t>(s);
         }
+        const bool eight = p.dtype == WS_DTYPE_I8 || p.dtype == WS_DTYPE_E4M3;
+        at::ScalarType type = eight ? at::kBFloat16 : k.scalar_type();
+        if (a[8] != Py_None) {
+            if (!THPDtype_Check(a[8])) refuse(what, "dtype must be a torch.dtype");
+            type = reinterpret_cast<THPDtype*>(a[8])->scalar_type;
+        }
+        if (half_of(type) < 0) refuse(what, "the output must be bf16 or fp16");
+        if (!eight && type != k.scalar_type()) refuse(what, "a 16-bit pool is read in its own type");
+        const c10::cuda::OptionalCUDAGuard guard(dev);
+        const at::Tensor k_out = output(what, "k_out", a[9], {N, p.Hkv, p.Dk}, type, dev);
+        const at::Tensor v_out = output(what, "v_out", a[10], {N, p.Hkv, p.Dv}, type, dev);
+        for (const int i : {9, 10}) {
+            if (a[i] == Py_None) continue;
+            const at::Tensor& t = i == 9 ? k_out : v_out;
+            for (const int j : {0, 1, 2, 3, 5, 6, 7})
+                if (a[j] != Py_None) at::assert_no_overlap(t, THPVariable_Unpack(a[j]));
+        }
+        if (a[9] != Py_None && a[10] != Py_None) at::assert_no_overlap(k_out, v_out);
         void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-        const Workspace ws = workspace(g_decode_ws, dev, stream);
-        check(p_paged_decode(q.data_ptr(), q.stride(0), q.stride(1), type, (int)B, (int)(H / p.Hkv), &p, data<int32_t>(table),
-                             table.stride(0), (int)std::min<int64_t>(table.size(1), INT32_MAX), data<int32_t>(lens),
-                             (int)std::min<int64_t>(window, INT32_MAX), (float)scale, out.data_ptr(), data<float>(lse), ws.ptr,
-                             ws.bytes, stream),
-              "ws_paged_decode");
+        check(p_paged_read(&p, data<int32_t>(table), table.stride(0), pages_of(table), (int)B, data<int32_t>(cu), starts, N,
+                           half_of(type), k_out.data_ptr(), v_out.data_ptr(), stream),
+              "ws_paged_read");
         PyObject* r = PyTuple_New(2);
         if (!r) return nullptr;
-        PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));
-        PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(lse));
+        PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(k_out));
+        PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(v_out));
         return r;
     });
 }
@@ -468,22 +575,24 @@ PyObject* zeros_outside_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// (addresses of ws_last_error, ws_paged_slots, ws_paged_release, ws_rope_append, ws_paged_decode; the two workspace
-// sizes; ScopeError, workspaces.get, the pool's dict, PagedStep)
+// (addresses of ws_last_error, ws_paged_slots, ws_paged_release, ws_rope_append, ws_paged_decode, ws_paged_diff_decode,
+// ws_paged_read; the two workspace sizes; ScopeError, workspaces.get, the pool's dict, PagedStep)
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded(n, 11, [&]() -> PyObject* {
+    return guarded(n, 13, [&]() -> PyObject* {
         auto address = [&](int i) { return reinterpret_cast<void*>((uintptr_t)integer(a[i])); };
         p_last_error = reinterpret_cast<decltype(p_last_error)>(address(0));
         p_paged_slots = reinterpret_cast<decltype(p_paged_slots)>(address(1));
         p_paged_release = reinterpret_cast<decltype(p_paged_release)>(address(2));
         p_rope_append = reinterpret_cast<decltype(p_rope_append)>(address(3));
         p_paged_decode = reinterpret_cast<decltype(p_paged_decode)>(address(4));
-        g_slots_ws = (size_t)integer(a[5]), g_decode_ws = (size_t)integer(a[6]);
+        p_paged_diff_decode = reinterpret_cast<decltype(p_paged_diff_decode)>(address(5));
+        p_paged_read = reinterpret_cast<decltype(p_paged_read)>(address(6));
+        g_slots_ws = (size_t)integer(a[7]), g_decode_ws = (size_t)integer(a[8]);
         PyObject** keep[4] = {&g_error, &g_pool_get, &g_pool_bufs, &g_step};
         for (int i = 0; i < 4; ++i) {
-            Py_INCREF(a[7 + i]);
+            Py_INCREF(a[9 + i]);
             Py_XDECREF(*keep[i]);
-            *keep[i] = a[7 + i];
+            *keep[i] = a[9 + i];
         }
         Py_RETURN_NONE;
     });
@@ -491,7 +600,7 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(setup), ENTRY(zeros_outside_capture), ENTRY(paged_slots), ENTRY(paged_release), ENTRY(rope), ENTRY(rope_append),
-                         ENTRY(paged_decode), {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(paged_decode), ENTRY(paged_diff_decode), ENTRY(paged_read), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods};
 
 }  // namespace

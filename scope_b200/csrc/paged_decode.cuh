@@ -58,7 +58,7 @@ namespace ws {
 namespace paged {
 
 // Shared memory for the rings: a CTA's 227 KB without what the kernel declares itself.
-constexpr int most_smem(int warps) { return ((227 << 10) - 464 * warps - 128) & ~15; }
+constexpr int most_smem(int warps, bool diff) { return ((227 << 10) - 464 * warps - (diff ? 640 : 128)) & ~15; }
 constexpr int kMinTok = 32;     // tokens a warp takes before another CTA joins in
 // Rows up to so many tokens are not cut by a border between two CTAs, or two warps: the border moves to the nearer end
 // of the row, which unbalances the stretches by half a row at most and saves the joining (about 5 us; measured with
@@ -82,7 +82,8 @@ struct Args {
     uint32_t kp, kt, kh, vp, vt, vh;     // strides in 16-byte pieces
     const float* ks;
     const float* vs;
-    uint32_t ksp, kst, ksh, vsp, vst, vsh;   // floats
+    uint32_t ksp, kst, ksh, vsp, vst, vsh;   // floats; kst, vst: from block to block
+    uint32_t blk_mul, blk_shift;         // t / (tokens of a scale), as div_mul and div_shift below
     const int32_t* table;
     int64_t table_stride;
     const int32_t* seq_lens;
@@ -98,7 +99,16 @@ struct Args {
     float* pieces;                       // [cta][2][piece floats]
     int* status;
     int krow, vrow, stages, warp_smem;   // where Dk, Dv are not known when compiling: the ring's geometry (launch)
+    // DIFF (kh and vh lead from pair to pair, ksh and vsh from pool head to pool head)
+    int64_t kjump, vjump;                // bytes from where a pair's second head would follow its first to where it lies
+    const float* lam;                    // of head h at h * lam_stride
+    int lam_stride;
+    float eps;
+    const float* weight;                 // null: no norm
 };
+
+// What a pool holds.
+enum : int { k16 = 0, kS8 = 1, kE4M3 = 2 };
 
 // The variant for head dims up to DB, 8*NT query heads a block.  A subtile is 16 tokens, or 32 where 16 would be 4 KB or
 // less (int8, head dims up to 64): what a subtile costs beside its bytes then counts half (measured with int8 rows of 128,
@@ -107,7 +117,7 @@ struct Args {
 // (measured at D = 128 in 16 bits, 16 ragged requests to 32768: 8 warps 160 us, 10 warps 152, 12 warps 157; three stages
 // put more in flight than the memory takes, and the SMs it serves last fall behind).  These figures are of when the choice
 // was made, with cp.async and each probability in two parts.
-template <bool I8, int DB, int NT>
+template <bool I8, bool DIFF, int DB, int NT>
 struct Cfg {
     static constexpr int kMt = DB / 16;                                   // accumulator fragments of a head tile
     static constexpr int kTok = I8 || DB == 64 ? 32 : 16;                 // tokens of a subtile
@@ -117,17 +127,20 @@ struct Cfg {
     // kExact: stages of rows an odd number of 16-byte pieces apart, each with its scales and meta, then the first part (a
     // stretch's last part takes the ring's place)
     static constexpr int kGapRow = I8 ? ((DB / 16) | 1) * 16 : DB * 2 + 16;
-    static constexpr int kGapStage = 2 * kTok * kGapRow + (I8 ? 8 * kTok : 0) + 16;
-    static constexpr int kGapFit = (most_smem(kWarps) / kWarps - kPiece * 4) / kGapStage;
+    static constexpr int kMore = (I8 ? (DIFF ? 16 : 8) * kTok : 0) + 16;
+    static constexpr int kGapStage = 2 * kTok * kGapRow + kMore;
+    static constexpr int kGapFit = (most_smem(kWarps, DIFF) / kWarps - kPiece * 4) / kGapStage;
     static constexpr int kGapStages = kGapFit > 4 ? 4 : kGapFit;
     static constexpr int kGapWarpSmem = kGapStages * kGapStage + kPiece * 4;
     static_assert(kGapStages >= 2 && kGapStages * kGapStage >= kPiece * 4 && kGapStage % 16 == 0, "ring");
     // kTma: the stages' rows, swizzled and so without gaps, then their scales and meta, then the first part
     static constexpr int kRowB = DB * (I8 ? 1 : 2);
-    static constexpr int kInner = inner_of(kRowB), kParts = kRowB / kInner;
+    static constexpr int kHeadB = DIFF ? kRowB / 2 : kRowB;               // bytes of a pool head's row
+    static constexpr bool kCanTma = kHeadB % 64 == 0;
+    static constexpr int kInner = inner_of(kHeadB), kParts = kRowB / kInner;
     static constexpr int kTile = 16 * kRowB;                              // 16 tokens' keys, or values
-    static constexpr int kRows = 2 * kTok * kRowB, kMore = (I8 ? 8 * kTok : 0) + 16;
-    static constexpr int kFit = (((most_smem(kWarps) - 1024) / kWarps & ~1023) - kPiece * 4) / (kRows + kMore);
+    static constexpr int kRows = 2 * kTok * kRowB;
+    static constexpr int kFit = (((most_smem(kWarps, DIFF) - 1024) / kWarps & ~1023) - kPiece * 4) / (kRows + kMore);
     static constexpr int kStages = kFit > 4 ? 4 : kFit;
     static constexpr int kWarpSmem = (kStages * (kRows + kMore) + kPiece * 4 + 1023) & ~1023;
     static_assert(kStages >= 2 && kStages * kRows >= kPiece * 4 && kRows % 1024 == 0, "ring");
@@ -269,6 +282,15 @@ __device__ __forceinline__ uint32_t s8_pair(uint32_t r) {
 template <bool F16>
 constexpr float s8_unit = F16 ? 1.f : 8192.f;   // the factor that s8_pair leaves out
 
+// The lower, or the upper, two e4m3 bytes of r as a pair of fp16, exactly.
+template <bool UP>
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t r) {
+    uint32_t d;
+    if (UP) asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h;}" : "=r"(d) : "r"(r));
+    else asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(d) : "r"(r));
+    return d;
+}
+
 // Where request b's attended tokens lie: tokens [lo, L), n subtiles from lo rounded down to one.
 struct Span {
     int lo, L, n;
@@ -326,14 +348,17 @@ enum : int {
                   // tokens in int8 99 us to 87, 204 of up to 101 tokens 14.5 to 12.5, 2 of 100 in pages of 8 11.5 to 10.2)
     kTma = 2,     // TMA; Dk = Dv = DB, pages of whole 16-token tiles
 };
-template <bool F16, bool I8, int DB, int NT, int MODE>
-__global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
-    using C = Cfg<I8, DB, NT>;
+template <bool F16, int CODE, bool DIFF, int DB, int NT, int MODE>
+__global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
+    constexpr bool I8 = CODE != k16, E4M3 = CODE == kE4M3;   // I8: codes of 8 bits
+    using C = Cfg<I8, DIFF, DB, NT>;
     constexpr bool EXACT = MODE != kAny, TMA = MODE == kTma;
     constexpr int kWarps = C::kWarps, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
     constexpr int kTok = C::kTok, H = kTok / 16;   // H: 16-token tiles of a subtile
     constexpr int kMinSub = kMinTok / kTok, kSnapC = kSnapCta / kTok, kSnapW = kSnapWarp / kTok;
+    constexpr bool kKF16 = F16 || E4M3;      // the type of Q and K in the first product
     constexpr bool kPF16 = F16 || I8;        // the type of P and V in the second product
+    constexpr int kMaps = DIFF ? 2 : 1;      // scales of a token's keys, and values
     constexpr int kParts = kPF16 ? 2 : 3;    // the 16-bit floats that a probability enters it as
     // fp16 probabilities are kept 2^8 larger, so that the sum of many small ones is not lost below fp16's least value
     constexpr float kUp = kPF16 ? 8.f : 0.f;
@@ -341,6 +366,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     uint8_t* const smem = TMA ? smem_raw + (-smem_u32(smem_raw) & 1023) : smem_raw;   // [kWarps][warp_smem]
     __shared__ uint64_t s_bar[TMA ? kWarps * 4 : 1];
     __shared__ int s_border[kWarps], s_scan[kWarps], s_from[32 * kWarps], s_start[2 * kWarps];   // s_start < 0: no part
+    __shared__ float s_sq[DIFF ? 2 : 1][DIFF ? kUnits / 2 : 1][4];   // joining: sums of squares by job and head
     __shared__ int s_list[kWarps][32], s_cnt[32 * kWarps], s_req[2 * kWarps], s_row[2 * kWarps], s_n[2 * kWarps], s_first[2], s_ctas[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -484,8 +510,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
         if (span_of<kTok>(a, b).n) continue;
         const int64_t head0 = (int64_t)b * a.Hkv * a.G;
-        for (int i = tid; i < a.Hkv * a.G * (Dv / 8); i += 32 * kWarps)
-            reinterpret_cast<uint4*>(a.out + head0 * Dv)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < a.Hkv * a.G / kMaps * (Dv / 8); i += 32 * kWarps)
+            reinterpret_cast<uint4*>(a.out + head0 / kMaps * Dv)[i] = make_uint4(0, 0, 0, 0);
         for (int i = tid; a.lse && i < a.Hkv * a.G; i += 32 * kWarps) a.lse[head0 + i] = -INFINITY;
     }
     if (x0 == x1) return;
@@ -514,6 +540,9 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     const int kchunks = I8 ? Dk >> 4 : Dk >> 3, vchunks = I8 ? Dv >> 4 : Dv >> 3;
     constexpr int kCols = ((I8 ? DB / 16 : DB / 8) + 7) / 8;
     const uint64_t k_lane = (uint64_t)r4 * a.kt + l8, v_lane = (uint64_t)r4 * a.vt + l8;
+    // a pair's second head
+    auto k_jump = [&](int j) { return DIFF && 2 * (l8 + 8 * j) >= kchunks ? a.kjump : 0; };
+    auto v_jump = [&](int j) { return DIFF && 2 * (l8 + 8 * j) >= vchunks ? a.vjump : 0; };
 
     auto look_up = [&]() {
         uint32_t t = (uint32_t)(fs.lo & ~(kTok - 1)) + (uint32_t)f_sub * kTok;
@@ -541,11 +570,17 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             const uint64_t va = (uint64_t)page * a.vp + (uint64_t)f_off * a.vt + (uint64_t)f_kvh * a.vh;
             if (I8) {
                 const uint32_t off = a.whole ? f_off + (lane & 15) : f_off;
-                const uint64_t ks = page * (uint64_t)a.ksp + off * (uint64_t)a.kst + f_kvh * (uint64_t)a.ksh;
-                const uint64_t vs = page * (uint64_t)a.vsp + off * (uint64_t)a.vst + f_kvh * (uint64_t)a.vsh;
+                const uint32_t blk = (__umulhi(off, a.blk_mul) + off) >> a.blk_shift;
+                const uint64_t ks = page * (uint64_t)a.ksp + blk * (uint64_t)a.kst + f_kvh * kMaps * (uint64_t)a.ksh;
+                const uint64_t vs = page * (uint64_t)a.vsp + blk * (uint64_t)a.vst + f_kvh * kMaps * (uint64_t)a.vsh;
                 const bool on = (mask >> tok) & 1;
-                cp_async4(ring_u + scales_at(slot) + tok * 4, a.ks + ks, on);
-                cp_async4(ring_u + scales_at(slot) + 4 * kTok + tok * 4, a.vs + vs, on);
+                const uint32_t to = ring_u + scales_at(slot) + tok * 4;
+                cp_async4(to, a.ks + ks, on);
+                cp_async4(to + 4 * kMaps * kTok, a.vs + vs, on);
+                if (DIFF) {
+                    cp_async4(to + 4 * kTok, a.ks + ks + a.ksh, on);
+                    cp_async4(to + 12 * kTok, a.vs + vs + a.vsh, on);
+                }
             }
             if (lane == 0) {
                 Meta m;
@@ -567,8 +602,9 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                         for (int p = 0; p < C::kParts; ++p) {
                             const uint32_t to = st + h * C::kTile + p * 16 * C::kInner;
-                            tma_load_4d(to, &a.kmap, bar, p * C::kInner, a.k_head_dim2 ? at : f_kvh, a.k_head_dim2 ? f_kvh : at, pg);
-                            tma_load_4d(to + kV, &a.vmap, bar, p * C::kInner, a.v_head_dim2 ? at : f_kvh, a.v_head_dim2 ? f_kvh : at, pg);
+                            const int x = p * C::kInner % C::kHeadB, hd = DIFF ? 2 * f_kvh + p * C::kInner / C::kHeadB : f_kvh;
+                            tma_load_4d(to, &a.kmap, bar, x, a.k_head_dim2 ? at : hd, a.k_head_dim2 ? hd : at, pg);
+                            tma_load_4d(to + kV, &a.vmap, bar, x, a.v_head_dim2 ? at : hd, a.v_head_dim2 ? hd : at, pg);
                         }
                     }
                 }
@@ -584,8 +620,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                         for (int i = 4 * h; i < 4 * h + 4; ++i) {
     #pragma unroll
                             for (int j = 0; j < kCols; ++j) {
-                                if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * krow + j * 128, kp + j * 128);
-                                if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * vrow + j * 128, vp + j * 128);
+                                if (l8 + 8 * j < kchunks) cp_async16_all(kd + 4 * i * krow + j * 128, kp + j * 128 + k_jump(j));
+                                if (l8 + 8 * j < vchunks) cp_async16_all(vd + 4 * i * vrow + j * 128, vp + j * 128 + v_jump(j));
                             }
                             kp += (uint64_t)a.kt << 6, vp += (uint64_t)a.vt << 6;
                         }
@@ -601,8 +637,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                         const uint8_t *kp = a.k + ((kr + l8) << 4), *vp = a.v + ((vr + l8) << 4);
     #pragma unroll
                         for (int j = 0; j < kCols; ++j) {
-                            if (l8 + 8 * j < kchunks) cp_async16(kd + 4 * i * krow + j * 128, kp + j * 128, on);
-                            if (l8 + 8 * j < vchunks) cp_async16(vd + 4 * i * vrow + j * 128, vp + j * 128, on);
+                            if (l8 + 8 * j < kchunks) cp_async16(kd + 4 * i * krow + j * 128, kp + j * 128 + k_jump(j), on);
+                            if (l8 + 8 * j < vchunks) cp_async16(vd + 4 * i * vrow + j * 128, vp + j * 128 + v_jump(j), on);
                         }
                     }
                 }
@@ -628,6 +664,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 
     float m_ref[NT][2], l_run[NT][2], acc[NT][kMt][4];
     uint32_t bq[NT][DB / 16][2];
+    float q_scale[E4M3 ? NT : 1][2];   // what scores are times where queries went to fp16
     bool began = false;                // the row's first subtile was this warp's
 
     const int nks = Dk >> 4, nmt = Dv >> 4;
@@ -642,19 +679,21 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int h = h0 + nt * 8 + g;
-            const uint16_t* q = a.q + b * a.q_b + ((int64_t)kvh * a.G + h) * a.q_h + (I8 ? 4 : 8) * t4;
+            // DIFF: heads 2i and 2i + 1 are a head's two maps, the first half of the dims belongs to the one, the second to the other
+            const int from = DIFF ? (g & 1) * (Dk >> 1) : 0, to = DIFF ? from + (Dk >> 1) : Dk;
+            const uint16_t* q = a.q + b * a.q_b + ((int64_t)kvh * a.G + h) * a.q_h + (I8 ? 4 : 8) * t4 - from;
             if (I8) {
 #pragma unroll
                 for (int ks = 0; ks < DB / 16; ++ks) {   // dims 16ks + 4t .. 4t + 3
                     uint2 w = make_uint2(0, 0);
-                    if (ks < nks && h < a.G) w = *reinterpret_cast<const uint2*>(q + 16 * ks);
+                    if (16 * ks < to && (!DIFF || 16 * ks >= from) && h < a.G) w = *reinterpret_cast<const uint2*>(q + 16 * ks);
                     bq[nt][ks][0] = w.x, bq[nt][ks][1] = w.y;
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < DB / 32; ++i) {      // dims 32i + 8t .. 8t + 7
                     uint4 w = make_uint4(0, 0, 0, 0);
-                    if (32 * i + 8 * t4 < Dk && h < a.G) w = *reinterpret_cast<const uint4*>(q + 32 * i);
+                    if (32 * i + 8 * t4 < to && (!DIFF || 32 * i + 8 * t4 >= from) && h < a.G) w = *reinterpret_cast<const uint4*>(q + 32 * i);
                     bq[nt][2 * i][0] = w.x, bq[nt][2 * i][1] = w.y, bq[nt][2 * i + 1][0] = w.z, bq[nt][2 * i + 1][1] = w.w;
                 }
             }
@@ -663,7 +702,29 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     auto order_q = [&]() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            if (I8) {   // the order in which s8_pair gives the dims: (0, 2), (1, 3) of each four
+            if (E4M3) {   // e4m3_pair leaves the dims in order
+                // bf16 to fp16: times the power of two that brings the head's largest to [2^14, 2^15)
+                q_scale[nt][0] = q_scale[nt][1] = 1.f;
+                if (!F16) {
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int ks = 0; ks < DB / 16; ++ks)
+                        most = max16<false>(most, max16<false>(bq[nt][ks][0] & 0x7fff7fffu, bq[nt][ks][1] & 0x7fff7fffu));
+                    most = max(most & 0xffffu, most >> 16);
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    const uint32_t e = max(most >> 7, 20u);   // infinite: 255
+                    const float up = __uint_as_float((268 - e) << 23), down = __uint_as_float((e - 14) << 23);
+#pragma unroll
+                    for (int ks = 0; ks < DB / 16; ++ks)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float2 f = unpack16<false>(bq[nt][ks][i]);
+                            bq[nt][ks][i] = pack16<true>(f.x * up, f.y * up);
+                        }
+                    q_scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t4), q_scale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t4 + 4);
+                }
+            } else if (I8) {   // the order in which s8_pair gives the dims: (0, 2), (1, 3) of each four
 #pragma unroll
                 for (int ks = 0; ks < DB / 16; ++ks) {
                     const uint32_t x = bq[nt][ks][0], y = bq[nt][ks][1];
@@ -727,6 +788,30 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 *reinterpret_cast<uint32_t*>(base + (int64_t)h * Dv + 8 + 2 * t4) = hi;
             }
         }
+    };
+
+    // DIFF: head t4 of tile nt has its maps in columns 2t and 2t + 1, so a lane holds both.
+    auto lam_of = [&](int row, int left, int nt) {
+        const int h = nt * 8 + 2 * t4;
+        return h < left ? a.lam[(((row >> 16) * a.G + (row & 0xffff) * 8 * NT + h) >> 1) * a.lam_stride] : 0.f;
+    };
+    auto difference = [&](const float* o, const float* inv, float lam) {   // lam: with the second map's 1/l
+        return make_float2(o[0] * inv[0] - o[1] * lam, o[2] * inv[0] - o[3] * lam);
+    };
+    // Two dims of the head in fragment mt, times r and the norm's weights.
+    auto store_pair = [&](int64_t head0, int left, int nt, int mt, float2 x, float r) {
+        const int h = nt * 8 + 2 * t4, d0 = 16 * mt + (I8 ? 2 * g : g), d1 = I8 ? d0 + 1 : d0 + 8;
+        if (h >= left) return;
+        if (a.weight) x.x *= r * a.weight[d0], x.y *= r * a.weight[d1];
+        uint16_t* const o = a.out + ((head0 + h) >> 1) * Dv;
+        const uint32_t w = pack16<F16>(x.x, x.y);
+        if (I8) *reinterpret_cast<uint32_t*>(o + d0) = w;
+        else o[d0] = (uint16_t)w, o[d1] = (uint16_t)(w >> 16);
+    };
+    auto over_dims = [&](float sq) {   // the lanes of a head's dims
+        sq += __shfl_xor_sync(0xffffffffu, sq, 4);
+        sq += __shfl_xor_sync(0xffffffffu, sq, 8);
+        return sq + __shfl_xor_sync(0xffffffffu, sq, 16);
     };
 
     if (count > 0) {
@@ -793,7 +878,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 if (kChains == 2) e[nt][i] = 0.f;
             }
         // values of tokens that do not count, which TMA brought with the others: zero (int8 codes are finite)
-        if (TMA && !I8 && meta.mask != (kTok == 32 ? 0xffffffffu : 0xffffu)) {
+        if (TMA && CODE != kS8 && meta.mask != (kTok == 32 ? 0xffffffffu : 0xffffu)) {
             constexpr int kLine = C::kInner / 16;
             const uint32_t off = ~meta.mask >> lane / kLine;
 #pragma unroll
@@ -823,11 +908,13 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     ldsm_x4(TMA ? piece(st + h * C::kTile, lane & 15, lane >> 4, ks) : k_ld + h * 16 * krow + ks * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {   // past an odd nks the queries are zero and what was read is finite
-                        const uint32_t a0 = s8_pair<F16>(r[2 * u]), a1 = s8_pair<F16>(r[2 * u + 1]);
-                        const uint32_t a2 = s8_pair<F16>(r[2 * u] >> 8), a3 = s8_pair<F16>(r[2 * u + 1] >> 8);
+                        const uint32_t a0 = E4M3 ? e4m3_pair<false>(r[2 * u]) : s8_pair<F16>(r[2 * u]);
+                        const uint32_t a1 = E4M3 ? e4m3_pair<false>(r[2 * u + 1]) : s8_pair<F16>(r[2 * u + 1]);
+                        const uint32_t a2 = E4M3 ? e4m3_pair<true>(r[2 * u]) : s8_pair<F16>(r[2 * u] >> 8);
+                        const uint32_t a3 = E4M3 ? e4m3_pair<true>(r[2 * u + 1]) : s8_pair<F16>(r[2 * u + 1] >> 8);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
-                            mma16<F16>(kChains == 2 && u ? e[nt] : c[h][nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
+                            mma16<kKF16>(kChains == 2 && u ? e[nt] : c[h][nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
                     }
                 }
             }
@@ -848,13 +935,20 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         const float* sc = reinterpret_cast<const float*>(ring + scales_at(slot));
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            const float f0 = I8 ? sc[16 * h + g] * (s8_unit<F16> * a.scale_log2) : a.scale_log2;
-            const float f1 = I8 ? sc[16 * h + g + 8] * (s8_unit<F16> * a.scale_log2) : a.scale_log2;
+            float f[kMaps][2];   // of tokens g and g + 8
+#pragma unroll
+            for (int m = 0; m < kMaps; ++m)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    f[m][i] = I8 ? sc[m * kTok + 16 * h + g + 8 * i] * (s8_unit<kKF16> * a.scale_log2) : a.scale_log2;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    c[h][nt][i] = (kChains == 2 ? c[h][nt][i] + e[nt][i] : c[h][nt][i]) * (i < 2 ? f0 : f1);
+                for (int i = 0; i < 4; ++i) {
+                    float by = f[DIFF ? i & 1 : 0][i >> 1];
+                    if (E4M3 && !F16) by *= q_scale[nt][i & 1];
+                    c[h][nt][i] = (kChains == 2 ? c[h][nt][i] + e[nt][i] : c[h][nt][i]) * by;
+                }
         }
         if (meta.mask != (kTok == 32 ? 0xffffffffu : 0xffffu)) {   // tokens that do not count (their values and scales are zero)
 #pragma unroll
@@ -898,19 +992,26 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 }
             }
         }
-        uint32_t ps[H][NT][2][kParts];
+        constexpr int kV2 = DIFF && I8 ? 2 : 1;   // a pair's two value heads have scales of their own
+        uint32_t ps[kV2][H][NT][2][kParts];
         // int8: the values' scales over the power of two below the subtile's largest, so that fp16 holds their products with
         // probabilities; what is left out of them is 2^-32 of the largest scale at most
-        float down = 1.f, back = 1.f;
+        float down[kV2], back[kV2];
         if (I8) {
             static_assert(!I8 || kTok == 32, "a scale a lane");
-            const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(sc[kTok + lane]) & INT32_MAX) >> 23, 1u), 253u);
-            down = __uint_as_float((254 - e) << 23), back = __uint_as_float(e << 23);
+#pragma unroll
+            for (int m = 0; m < kV2; ++m) {
+                const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(sc[(kMaps + m) * kTok + lane]) & INT32_MAX) >> 23, 1u), 253u);
+                down[m] = __uint_as_float((254 - e) << 23), back[m] = __uint_as_float(e << 23);
+            }
         }
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            const float v0 = I8 ? sc[kTok + 16 * h + g] * down : 1.f;
-            const float v1 = I8 ? sc[kTok + 16 * h + g + 8] * down : 1.f;
+            float v[kV2][2];
+#pragma unroll
+            for (int m = 0; m < kV2; ++m)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) v[m][i] = I8 ? sc[(kMaps + m) * kTok + 16 * h + g + 8 * i] * down[m] : 1.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float(&p)[4] = c[h][nt];
@@ -920,14 +1021,16 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     const float ref = fmaxf(m_ref[nt][j], -3.0e38f);
                     p[j] = ex2(p[j] - ref), p[j + 2] = ex2(p[j + 2] - ref);
                     l_run[nt][j] += p[j] + p[j + 2];
-                    if (I8) p[j] *= v0, p[j + 2] *= v1;
                 }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    split16<kPF16, I8, kParts>(p[2 * j], p[2 * j + 1], ps[h][nt][j]);
+                for (int m = 0; m < kV2; ++m)
 #pragma unroll
-                    for (int i = 0; i < kParts; ++i) ps[h][nt][j][i] = movmatrix_t(ps[h][nt][j][i]);
-                }
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t* const part = ps[m][h][nt][j];
+                        split16<kPF16, I8, kParts>(I8 ? p[2 * j] * v[m][j] : p[2 * j], I8 ? p[2 * j + 1] * v[m][j] : p[2 * j + 1], part);
+#pragma unroll
+                        for (int i = 0; i < kParts; ++i) part[i] = movmatrix_t(part[i]);
+                    }
             }
         }
         // values, two fragments at a time: the subtile's own sum on the tensor cores, added to the row's in fp32
@@ -944,8 +1047,14 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     ldsm_x4_t(TMA ? piece(st + kV + h * C::kTile, lane & 15, lane >> 4, mt) : v_ld + h * 16 * vrow + mt * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        v[u][0] = s8_pair<kPF16>(r[2 * u]), v[u][1] = s8_pair<kPF16>(r[2 * u] >> 8);
-                        v[u][2] = s8_pair<kPF16>(r[2 * u + 1]), v[u][3] = s8_pair<kPF16>(r[2 * u + 1] >> 8);
+                        if (E4M3) {   // a dim's two tokens side by side
+                            const uint32_t x = __byte_perm(r[2 * u], 0, 0x3120), y = __byte_perm(r[2 * u + 1], 0, 0x3120);
+                            v[u][0] = e4m3_pair<false>(x), v[u][1] = e4m3_pair<true>(x);
+                            v[u][2] = e4m3_pair<false>(y), v[u][3] = e4m3_pair<true>(y);
+                        } else {
+                            v[u][0] = s8_pair<kPF16>(r[2 * u]), v[u][1] = s8_pair<kPF16>(r[2 * u] >> 8);
+                            v[u][2] = s8_pair<kPF16>(r[2 * u + 1]), v[u][3] = s8_pair<kPF16>(r[2 * u + 1] >> 8);
+                        }
                     }
                 } else {
 #pragma unroll
@@ -958,7 +1067,9 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const uint32_t p[2] = {ps[h][nt][0][i], ps[h][nt][1][i]};
+                            const bool up = kV2 == 2 && 2 * (mt + u) >= nmt;
+                            const uint32_t p[2] = {up ? ps[kV2 - 1][h][nt][0][i] : ps[0][h][nt][0][i],
+                                                   up ? ps[kV2 - 1][h][nt][1][i] : ps[0][h][nt][1][i]};
                             if (h == 0 && i == 0) mma16_part<kPF16, true>(sum[u][nt], v[u], p);
                             else mma16_part<kPF16, false>(sum[u][nt], v[u], p);
                         }
@@ -970,7 +1081,8 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
 #pragma unroll
                     for (int i = 0; i < 4; i += 2) {
                         float* const o = acc[nt][mt + u] + i;
-                        if (I8) o[0] = fmaf(sum[u][nt][i], back, o[0]), o[1] = fmaf(sum[u][nt][i + 1], back, o[1]);
+                        const float by = I8 ? (kV2 == 2 && 2 * (mt + u) >= nmt ? back[kV2 - 1] : back[0]) : 1.f;
+                        if (I8) o[0] = fmaf(sum[u][nt][i], by, o[0]), o[1] = fmaf(sum[u][nt][i + 1], by, o[1]);
                         else add2(o[0], o[1], sum[u][nt][i], sum[u][nt][i + 1]);
                     }
         }
@@ -992,9 +1104,24 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
                 for (int nt = 0; nt < NT; ++nt) {
                     float inv[2];
                     finish(a, head0, left, nt, m_ref[nt], l_run[nt], true, inv);
+                    if (DIFF) {
+                        const float lam = lam_of(meta.row, left, nt) * inv[1];
+                        float sq = 0.f;
 #pragma unroll
-                    for (int mt = 0; mt < kMt; ++mt)
-                        if (mt < nmt) store_unit(head0, left, nt, mt, acc[nt][mt], inv);
+                        for (int mt = 0; mt < kMt; ++mt) {
+                            if (mt >= nmt) break;
+                            const float2 x = difference(acc[nt][mt], inv, lam);
+                            sq += x.x * x.x + x.y * x.y;
+                        }
+                        const float r = __frsqrt_rn(over_dims(sq) / Dv + a.eps);
+#pragma unroll
+                        for (int mt = 0; mt < kMt; ++mt)
+                            if (mt < nmt) store_pair(head0, left, nt, mt, difference(acc[nt][mt], inv, lam), r);
+                    } else {
+#pragma unroll
+                        for (int mt = 0; mt < kMt; ++mt)
+                            if (mt < nmt) store_unit(head0, left, nt, mt, acc[nt][mt], inv);
+                    }
                 }
             } else {
                 // the stretch's last part takes the ring's place (nothing is in flight into it any more)
@@ -1021,7 +1148,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
     const int my_start = lane < 2 * kWarps ? s_start[lane] : -1;
     uint32_t todo = __ballot_sync(0xffffffffu, my_start >= 0);
     int cross0 = -1, cross1 = -1;   // the row that came from an earlier CTA, the one that goes on into the next
-    int id0 = 0, id1 = 0, turn = warp, ended = -1, done = 0, ahead = 0;
+    int id0 = 0, id1 = 0, turn = warp, ended = -1, done = 0, ahead = 0, parity = 0;
     const int room = min(kWarps * warp_smem / (kPiece * 4), 32) - 2;
 #pragma unroll 1
     while (true) {
@@ -1101,6 +1228,7 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
         __syncwarp();
         const int row = s_row[id], left = left_of(row);
         const int64_t head0 = head_of(s_req[id], row);
+        const int turn0 = turn;
 #pragma unroll 1
         for (; turn < kJobs; turn += kWarps) {
             const int nt = turn * kJob / kMt, mt0 = turn * kJob - nt * kMt, ml = NT * 8 * DB + nt * 16 + 2 * t4;
@@ -1159,34 +1287,70 @@ __global__ void __launch_bounds__(32 * Cfg<I8, DB, NT>::kWarps, 1) decode_kernel
             } else {
                 float inv[2];
                 finish(a, head0, left, nt, m, l, mt0 == 0, inv);
+                if (DIFF) {   // kept in the place of the first part's sums, which nobody else reads, until all jobs' squares are known
+                    const float lam = lam_of(row, left, nt) * inv[1];
+                    float sq = 0.f;
+#pragma unroll
+                    for (int q = 0; q < kJob; ++q) {
+                        const float2 x = difference(o[q], inv, lam);
+                        *reinterpret_cast<float2*>(smem + s_list[warp][0] + at + q * 512) = x;
+                        if (mt0 + q < nmt) sq += x.x * x.x + x.y * x.y;
+                    }
+                    sq = over_dims(sq);
+                    if (lane < 4) s_sq[parity][turn][lane] = sq;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < kJob; ++q)
+                        if (mt0 + q < nmt) store_unit(head0, left, nt, mt0 + q, o[q], inv);
+                }
+            }
+        }
+        if (DIFF && !to) {   // every warp is here with the same row
+            __syncthreads();
+#pragma unroll 1
+            for (int i = turn0; i < kJobs; i += kWarps) {
+                const int nt = i * kJob / kMt, mt0 = i * kJob - nt * kMt;
+                float sq = 0.f;
+#pragma unroll
+                for (int k = 0; k < kMt / kJob; ++k) sq += s_sq[parity][nt * (kMt / kJob) + k][t4];
+                const float r = __frsqrt_rn(sq / Dv + a.eps);
 #pragma unroll
                 for (int q = 0; q < kJob; ++q)
-                    if (mt0 + q < nmt) store_unit(head0, left, nt, mt0 + q, o[q], inv);
+                    if (mt0 + q < nmt)
+                        store_pair(head0, left, nt, mt0 + q, *reinterpret_cast<const float2*>(smem + s_list[warp][0] + (i * kJob * 32 + lane) * 16 + q * 512), r);
             }
+            parity ^= 1;
         }
         turn = (turn - kJobs) % kWarps;
     }
 }
 
-// Host: the variants of one pair of types, by head-dim bound and heads a block (paged_decode_*.cu).
-int launch_bf16(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
-int launch_f16(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
-int launch_bf16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
-int launch_f16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
+// Host: the variants of one pair of types, by head-dim bound and heads a block (paged_decode_*.cu, paged_diff_*.cu).
+#define WS_PAGED_LAUNCHES(of)                                                  \
+    int of##_bf16(const Args& a, int DB, int NT, int ctas, cudaStream_t st);     \
+    int of##_f16(const Args& a, int DB, int NT, int ctas, cudaStream_t st);      \
+    int of##_bf16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);  \
+    int of##_f16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st);   \
+    int of##_bf16_e4(const Args& a, int DB, int NT, int ctas, cudaStream_t st);  \
+    int of##_f16_e4(const Args& a, int DB, int NT, int ctas, cudaStream_t st);
+WS_PAGED_LAUNCHES(launch)
+WS_PAGED_LAUNCHES(launch_diff)
+#undef WS_PAGED_LAUNCHES
 
-template <bool F16, bool I8, int DB, int NT, int MODE>
+template <bool F16, int CODE, bool DIFF, int DB, int NT, int MODE>
 int launch(Args a, int ctas, cudaStream_t st) {
-    using C = Cfg<I8, DB, NT>;
+    constexpr bool I8 = CODE != k16;
+    using C = Cfg<I8, DIFF, DB, NT>;
     int smem = MODE == kTma ? C::kWarps * C::kWarpSmem + 1024 : C::kWarps * C::kGapWarpSmem;
     if (MODE == kAny) {
         // rows as long as they are; stages until the copies in flight are 72 KB an SM (what two stages of 128-dim rows in
         // 16 bits give)
         a.krow = I8 ? ((a.Dk / 16) | 1) * 16 : a.Dk * 2 + 16, a.vrow = I8 ? ((a.Dv / 16) | 1) * 16 : a.Dv * 2 + 16;
         const int bytes = C::kTok * (a.Dk + a.Dv) * (I8 ? 1 : 2);
-        const int stage = C::kTok * (a.krow + a.vrow) + (I8 ? 8 * C::kTok : 0) + 16;
+        const int stage = C::kTok * (a.krow + a.vrow) + C::kMore;
         auto warp_smem = [&](int stages) { return std::max(stages * stage, C::kPiece * 4) + C::kPiece * 4; };
         a.stages = 2;
-        while (a.stages < 4 && (a.stages - 1) * bytes * C::kWarps < 72 << 10 && C::kWarps * warp_smem(a.stages + 1) <= most_smem(C::kWarps))
+        while (a.stages < 4 && (a.stages - 1) * bytes * C::kWarps < 72 << 10 && C::kWarps * warp_smem(a.stages + 1) <= most_smem(C::kWarps, DIFF))
             ++a.stages;
         a.warp_smem = warp_smem(a.stages);
         smem = C::kWarps * a.warp_smem;
@@ -1195,27 +1359,29 @@ int launch(Args a, int ctas, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (set_for != dev) {
-        if (cudaFuncSetAttribute(decode_kernel<F16, I8, DB, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 MODE != kAny ? smem : most_smem(C::kWarps)) != cudaSuccess)
+        if (cudaFuncSetAttribute(decode_kernel<F16, CODE, DIFF, DB, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 MODE != kAny ? smem : most_smem(C::kWarps, DIFF)) != cudaSuccess)
             return set_error(WS_ERR_CUDA, "paged_decode: shared memory");
         set_for = dev;
     }
-    const cudaError_t e = launch_dependent(decode_kernel<F16, I8, DB, NT, MODE>, dim3(ctas), 32 * C::kWarps, smem, st, a);
+    const cudaError_t e = launch_dependent(decode_kernel<F16, CODE, DIFF, DB, NT, MODE>, dim3(ctas), 32 * C::kWarps, smem, st, a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }
 
-template <bool F16, bool I8, int DB, int NT>
+template <bool F16, int CODE, bool DIFF, int DB, int NT>
 int launch_dims(const Args& a, int ctas, cudaStream_t st) {
-    if (a.tma) return launch<F16, I8, DB, NT, kTma>(a, ctas, st);
-    return a.Dk == DB && a.Dv == DB ? launch<F16, I8, DB, NT, kExact>(a, ctas, st) : launch<F16, I8, DB, NT, kAny>(a, ctas, st);
+    if constexpr (Cfg<CODE != k16, DIFF, DB, NT>::kCanTma)
+        if (a.tma) return launch<F16, CODE, DIFF, DB, NT, kTma>(a, ctas, st);
+    return a.Dk == DB && a.Dv == DB ? launch<F16, CODE, DIFF, DB, NT, kExact>(a, ctas, st)
+                                    : launch<F16, CODE, DIFF, DB, NT, kAny>(a, ctas, st);
 }
 
-template <bool F16, bool I8>
+template <bool F16, int CODE, bool DIFF>
 int launch_any(const Args& a, int DB, int NT, int ctas, cudaStream_t st) {
-    if (DB == 64) return NT == 1 ? launch_dims<F16, I8, 64, 1>(a, ctas, st) : launch_dims<F16, I8, 64, 2>(a, ctas, st);
-    if (DB == 128) return NT == 1 ? launch_dims<F16, I8, 128, 1>(a, ctas, st) : launch_dims<F16, I8, 128, 2>(a, ctas, st);
-    if (DB == 192) return launch_dims<F16, I8, 192, 1>(a, ctas, st);
-    return launch_dims<F16, I8, 256, 1>(a, ctas, st);
+    if (DB == 64) return NT == 1 ? launch_dims<F16, CODE, DIFF, 64, 1>(a, ctas, st) : launch_dims<F16, CODE, DIFF, 64, 2>(a, ctas, st);
+    if (DB == 128) return NT == 1 ? launch_dims<F16, CODE, DIFF, 128, 1>(a, ctas, st) : launch_dims<F16, CODE, DIFF, 128, 2>(a, ctas, st);
+    if (DB == 192) return launch_dims<F16, CODE, DIFF, 192, 1>(a, ctas, st);
+    return launch_dims<F16, CODE, DIFF, 256, 1>(a, ctas, st);
 }
 
 }  // namespace paged

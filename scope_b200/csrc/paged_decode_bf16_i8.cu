@@ -5,7 +5,7 @@ namespace ws {
 namespace paged {
 
 int launch_bf16_i8(const Args& a, int DB, int NT, int ctas, cudaStream_t st) {
-    return launch_any<false, true>(a, DB, NT, ctas, st);
+    return launch_any<false, kS8, false>(a, DB, NT, ctas, st);
 }
 
 }  // namespace paged

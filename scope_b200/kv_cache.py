@@ -193,13 +193,16 @@ class PagedKVCache:
     ring of free pages that the layers share.
 
     Where ``ShardedKVCache`` reserves max_seq tokens for every row, a request here holds only the pages its tokens
-    fill, so ``num_pages * page_size`` bounds the requests' summed length.  ``dtype`` bf16, fp16 or int8 (codes with
-    one fp32 scale per row).  Per step:
+    fill, so ``num_pages * page_size`` bounds the requests' summed length.  ``dtype`` bf16, fp16, int8 or
+    float8_e4m3fn (codes with one fp32 scale for each head and ``scale_block`` tokens of a page, which it divides; 1: one
+    per row).  Per step:
 
         step = cache.begin_step(new_lens, n_tokens)       # pages, slots, positions; lengths advance
         q = cache.append(li, q, k, v, step, cos_sin)      # each layer: rotate, write keys and values
         out, lse = cache.decode(li, q_last, scale)        # each layer: one query per request
         cache.release(done)                               # finished requests' pages go back
+
+    ``read`` gives rows back, and ``diff_decode`` is differential attention, with the cache's heads in pairs.
 
     Nothing here waits for the device; ``free_pages()`` and ``refused()`` do.  The table, lengths and ring are updated
     in place, so the calls can be captured in a CUDA graph.  ``begin_step`` serves requests in order and refuses whole what
@@ -208,16 +211,19 @@ class PagedKVCache:
     """
 
     def __init__(self, num_layers, num_pages, page_size, num_kv_heads, head_dim, max_requests, max_seq,
-                 v_head_dim=None, dtype=torch.bfloat16, device=None):
+                 v_head_dim=None, dtype=torch.bfloat16, device=None, scale_block=1):
+        quantised = dtype in (torch.int8, torch.float8_e4m3fn)
+        if scale_block < 1 or page_size % scale_block or (scale_block > 1 and not quantised):
+            raise RuntimeError("PagedKVCache: scale_block must divide page_size, and belongs to an 8-bit cache")
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         self.device, self.page_size, self.num_pages, self.max_requests = dev, page_size, num_pages, max_requests
         vd = head_dim if v_head_dim is None else v_head_dim
         pool = (num_pages, page_size, num_kv_heads)
         self.k_pages = [torch.empty(*pool, head_dim, dtype=dtype, device=dev) for _ in range(num_layers)]
         self.v_pages = [torch.empty(*pool, vd, dtype=dtype, device=dev) for _ in range(num_layers)]
-        quantised = dtype == torch.int8
-        self.k_scales = [torch.empty(pool, device=dev) if quantised else None for _ in range(num_layers)]
-        self.v_scales = [torch.empty(pool, device=dev) if quantised else None for _ in range(num_layers)]
+        blocks = (num_pages, page_size // scale_block, num_kv_heads)
+        self.k_scales = [torch.empty(blocks, device=dev) if quantised else None for _ in range(num_layers)]
+        self.v_scales = [torch.empty(blocks, device=dev) if quantised else None for _ in range(num_layers)]
         self.page_table = torch.empty(max_requests, -(-max_seq // page_size), dtype=torch.int32, device=dev)
         self.seq_lens = torch.empty(max_requests, dtype=torch.int32, device=dev)
         self._free = torch.empty(num_pages, dtype=torch.int32, device=dev)
@@ -254,6 +260,21 @@ class PagedKVCache:
         from .paged import paged_decode
         return paged_decode(q, self.k_pages[li], self.v_pages[li], self.page_table, self.seq_lens, scale,
                             window=window, k_scales=self.k_scales[li], v_scales=self.v_scales[li], out=out, lse=lse)
+
+    def diff_decode(self, li, q, scale, lam, norm_weight=None, norm_eps=1e-5, window=0, out=None, lse=None):
+        """Differential attention, pool heads 2g and 2g + 1 a pair: q [max_requests, 2 * H, D] -> (out [max_requests, H,
+        2 * v_head_dim], lse of each map); ``paged.paged_diff_decode``."""
+        from .paged import paged_diff_decode
+        return paged_diff_decode(q, self.k_pages[li], self.v_pages[li], self.page_table, self.seq_lens, scale, lam,
+                                 norm_weight=norm_weight, norm_eps=norm_eps, window=window, k_scales=self.k_scales[li],
+                                 v_scales=self.v_scales[li], out=out, lse=lse)
+
+    def read(self, li, cu_seqlens, n_tokens, starts=None, dtype=None, k_out=None, v_out=None):
+        """Rows of layer li, request b's at [cu_seqlens[b], cu_seqlens[b + 1]) from its token starts[b] on (default: the
+        first) -> (k [n_tokens, kv heads, D], v); ``paged.paged_read``."""
+        from .paged import paged_read
+        return paged_read(self.k_pages[li], self.v_pages[li], self.page_table, cu_seqlens, n_tokens, starts=starts,
+                          k_scales=self.k_scales[li], v_scales=self.v_scales[li], dtype=dtype, k_out=k_out, v_out=v_out)
 
     def release(self, done):
         """done bool [max_requests] on the device: these requests' pages go back and their lengths become 0."""

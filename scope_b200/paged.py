@@ -1,13 +1,15 @@
 """Operators of a paged key-value cache: page tables and slot maps from request lengths, rotary positions with
-several axes, the append of rotated keys and values into pages, and the decode attention that reads them.
+several axes, the append of rotated keys and values into pages, the decode attention that reads them, softmax or
+differential, and the way back from pages to rows.
 
 The reference reserves one row of ``max_seq`` tokens for every request (``InplaceKVCache``,
 system/qwenoffload.py:59-141); a paged pool bounds the requests' summed length instead.  A pool is a pair of tensors
 ``k_pages [n_pages, page_size, Hkv, Dk]`` and ``v_pages [n_pages, page_size, Hkv, Dv]`` (any strides of whole 16 bytes
 with unit stride on the head dim, so a head-major ``[n_pages, Hkv, page_size, D]`` buffer is passed as its
-``transpose(1, 2)``) in bf16, fp16, or int8 with one fp32 scale per row (``k_scales``, ``v_scales``
-``[n_pages, page_size, Hkv]``).  ``scope_b200.kv_cache.PagedKVCache`` holds the pools of a model's layers and the
-requests' tables.
+``transpose(1, 2)``) in bf16, fp16, or in 8 bits (int8, float8_e4m3fn) with fp32 scales: ``k_scales``, ``v_scales``
+``[n_pages, page_size, Hkv]``, one per row, or ``[n_pages, blocks, Hkv]``, one for each block of page_size / blocks tokens
+and head (any strides; ``value = code * scale``).  ``scope_b200.kv_cache.PagedKVCache`` holds the pools of a model's layers
+and the requests' tables.
 
 The operators are outside autograd: inputs that require gradients are read as they are, and results require none
 (``rope`` with ``inverse`` is the rotation's gradient, for a caller's own ``torch.autograd.Function``).
@@ -19,6 +21,7 @@ on that stream):
     step = paged_slots(seq_lens, new_lens, page_table, free_pages, ring, page_size, n_tokens)
     q = rope_append(q, k, v, step.positions, cos_sin, step.slots, k_pages, v_pages)       # per layer
     out, lse = paged_decode(q_last, k_pages, v_pages, page_table, step.seq_lens, scale)    # per layer
+    k, v = paged_read(k_pages, v_pages, page_table, cu_seqlens, n_tokens)                  # where rows are wanted back
     seq_lens, ring = paged_release(step.seq_lens, done, page_table, free_pages, step.ring, page_size)
 """
 from __future__ import annotations
@@ -147,6 +150,16 @@ def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positi
     row in fp32 (the rule of ``kv_quantize_bf16_to_int8``); a NaN in a row makes the row's scale NaN, an infinity makes it
     infinite over codes of 0, so either row reads back as NaN.  ``cos_sin`` None: no rotation.  Rotary arguments as in
     ``rope``.  Returns the rotated queries (``q_out``, which may be q), or None without q.
+
+    With a scale for each block of tokens (int8), and with float8_e4m3fn always, blocks are quantised as they fill, front
+    to back.  Of a block's rows in this call, the first at offset o:
+        s_new = max(max|x|, 1e-6) / 127,  for e4m3 the least power of two with max(max|x|, 1e-6) <= 448 s_new
+        s = max(s_old, s_new) where o > 0, s_old being the scale that lies there, else s_new
+        code = rne(x * (1 / s)),  and the rows before o, where s > s_old:  code = rne(code * (s_old * (1 / s)))
+    so an open block's earlier int8 rows move by up to half a step each time it grows; e4m3 rows, by powers of two, only
+    where they leave the normal range.  Rows behind the last one written are nobody's.  A NaN or an infinity makes the
+    whole block read back as NaN.  A block's tokens follow one another in the call in the order of their slots, as
+    ``paged_slots`` lays them; dropped ones may lie between.
     """
     axis_map, axes = (None, 1) if cos_sin is None else _axes(cos_sin, sections, cyclic)
     return (_c or _load()).rope_append(q, k, v, positions, cos_sin, slots, k_pages, v_pages, k_scales, v_scales, axis_map,
@@ -160,7 +173,7 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     """Attention of one new token per request over a paged cache.
 
     q [B, H, Dk] bf16 or fp16 with H = Hkv * G (head h = kvh * G + g; any strides of whole 16 bytes); the pool holds
-    q's type or int8.  page_table int32 [B, pages]; seq_lens int32 [B]: request b attends its first seq_lens[b] tokens
+    q's type, int8 or float8_e4m3fn.  page_table int32 [B, pages]; seq_lens int32 [B]: request b attends its first seq_lens[b] tokens
     (the new one included), with ``window`` > 0 the last ``window`` of them.  Returns (out [B, H, Dv] in q's type,
     normalised; lse fp32 [B, H]).  A request without tokens gives out = 0, lse = -inf.  What pages hold past a
     request's length is never used.  A page id outside the pool leaves its tokens out and is reported by
@@ -169,3 +182,41 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     """
     return (_c or _load()).paged_decode(q, k_pages, v_pages, page_table, seq_lens, scale, window, k_scales, v_scales, out,
                                         lse)
+
+
+def paged_diff_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                      seq_lens: torch.Tensor, scale: float, lam: torch.Tensor, *, norm_weight: torch.Tensor | None = None,
+                      norm_eps: float = 1e-5, window: int = 0, k_scales: torch.Tensor | None = None,
+                      v_scales: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                      lse: torch.Tensor | None = None):
+    """Differential attention of one new token per request over a paged cache:
+
+        o = softmax(scale q1 k1) v - lam softmax(scale q2 k2) v,    out = o, or o * rsqrt(mean(o^2) + norm_eps) * norm_weight
+
+    The pool's heads come in pairs: keys of heads 2g and 2g + 1 are pair g's two maps (Dk dims each), values of the two,
+    one after the other, its 2 * Dv values.  q [B, 2 * H, Dk]: map m of head h is q[:, 2 * h + m]; H is a multiple of the
+    pairs, heads of a pair side by side.  lam fp32 [H] or one value: exp(lq1 . lk1) - exp(lq2 . lk2) + lam_init of the
+    layer's learned vectors.  norm_weight fp32 [2 * Dv] (a factor 1 - lam_init goes into it).  Returns (out [B, H, 2 * Dv]
+    in q's type, lse fp32 [B, 2 * H] of each map).  Dk, Dv at most 128.  Pools, page_table, seq_lens, window and what is
+    left out as in ``paged_decode``; ``rope_append`` writes such a pool with k [N, 2 * pairs, Dk] and
+    v.view(N, 2 * pairs, Dv).
+    """
+    return (_c or _load()).paged_diff_decode(q, k_pages, v_pages, page_table, seq_lens, scale, window, k_scales, v_scales, out,
+                                             lse, lam, norm_weight, norm_eps)
+
+
+def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor, n_tokens: int,
+               *, starts: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
+               v_scales: torch.Tensor | None = None, dtype: torch.dtype | None = None, k_out: torch.Tensor | None = None,
+               v_out: torch.Tensor | None = None):
+    """Requests' keys and values as packed rows: (k [n_tokens, Hkv, Dk], v [n_tokens, Hkv, Dv]), in one launch.
+
+    cu_seqlens int32 [B + 1], ascending: request b's rows are [cu_seqlens[b], cu_seqlens[b + 1]), its tokens from
+    starts[b] (int32 [B]; None: from the first) on.  ``n_tokens`` is the number of rows there is room for (the host's
+    cu_seqlens[B], or any bound of it); rows from cu_seqlens[B] on stay as they were.  8-bit pools give code * scale,
+    rounded to fp32 and once more to ``dtype`` (bf16, the default, or fp16); a 16-bit pool is read in its own type.  A
+    token before the first, past the table's width or on a page outside the pool gives zeros and is reported by
+    ``scope_b200.status_take``.
+    """
+    return (_c or _load()).paged_read(k_pages, v_pages, page_table, cu_seqlens, n_tokens, starts, k_scales, v_scales, dtype,
+                                      k_out, v_out)

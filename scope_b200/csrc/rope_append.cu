@@ -137,7 +137,14 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
     a.lanes = 1;
     while (a.lanes * 16 < Dmax) a.lanes *= 2;
     const int block = kv ? std::max(kv->scale_block, 1) : 1;
-    if (kv && (kv->dtype == WS_DTYPE_E4M3 || (kv->dtype == WS_DTYPE_I8 && block > 1)))
+    const bool blocks8 = kv && (kv->dtype == WS_DTYPE_E4M3 || (kv->dtype == WS_DTYPE_I8 && block > 1));
+    if (blocks8 && H > 0 && !block_append_small(N, kv->Hkv)) {
+        if (const int rc = ws_rope_append(rope, q, q_stride_tok, q_stride_head, H, D, q_out, qo_stride_tok, qo_stride_head, nullptr, 0,
+                                          0, nullptr, 0, 0, dtype, N, nullptr, nullptr, stream))
+            return rc;
+        a.h[0].n = 0;
+    }
+    if (blocks8)
         return block_append_launch(a, dtype == WS_DTYPE_F16, kv->dtype == WS_DTYPE_E4M3, vec, block, static_cast<cudaStream_t>(stream));
     // One warp walks all heads of a token when there are tokens for every SM; with fewer, its rows are shared out.  Into
     // int8, where a row takes longer, that pays with half as many tokens only (4097 tokens of 20 + 5 + 5 heads, us with 16,

@@ -102,7 +102,7 @@ int make_kv_map(CUtensorMap* map, const void* base, int64_t stride_tok, int64_t 
 }
 
 bool make_page_map(CUtensorMap* map, const void* base, int64_t row, int64_t page_size, int64_t heads, int64_t pages,
-                   int64_t stride_tok, int64_t stride_head, int64_t stride_page, int inner, int* head_in_dim2) {
+                   int64_t stride_tok, int64_t stride_head, int64_t stride_page, int inner, int box_tok, int* head_in_dim2) {
     auto fn = encode_fn();
     if (!fn) return false;
     // the strides of axes of one are irrelevant
@@ -116,7 +116,7 @@ bool make_page_map(CUtensorMap* map, const void* base, int64_t row, int64_t page
     const cuuint64_t strides[3] = {(cuuint64_t)s[0], (cuuint64_t)s[1], (cuuint64_t)stride_page};
     cuuint32_t box[4] = {(cuuint32_t)inner, 1, 1, 1};
     dims[*head_in_dim2 ? 2 : 1] = heads;
-    dims[*head_in_dim2 ? 1 : 2] = page_size, box[*head_in_dim2 ? 1 : 2] = 16;
+    dims[*head_in_dim2 ? 1 : 2] = page_size, box[*head_in_dim2 ? 1 : 2] = box_tok;
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, es,
               CU_TENSOR_MAP_INTERLEAVE_NONE, inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
               row >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,

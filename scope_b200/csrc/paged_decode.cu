@@ -82,15 +82,18 @@ int decode(const char* what, const Diff* diff, const void* q, int64_t q_stride_b
     a.cap = (int)std::min<int64_t>((int64_t)max_pages * kv->page_size, INT32_MAX - 64);
     a.whole = kv->page_size % 16 == 0;
     const int head_bytes = DB / maps * (int)eb, inner = paged::inner_of(head_bytes);
+    const int code = i8 ? paged::kS8 : e4 ? paged::kE4M3 : paged::k16, tok = paged::tok_of(code, diff != nullptr, DB);
+    a.flat = eight && kv->page_size % tok == 0 && std::max(kv->scale_block, 1) % tok == 0;
+    const int box = a.flat && paged::one_box(code, diff != nullptr, DB) ? 32 : 16;
     // Rows short by the table's width, or the window, are faster with cp.async, whose first bytes are there sooner and
     // whose last subtile costs less (us with TMA and with cp.async: 204 requests of up to 101 tokens 12.9 and 12.5, 64 of
     // up to 2 8.8 and 8.3; 1 of 4096 11.9 and 12.1, 16 of up to 32768 136 and 146).
     const bool whole_rows = kv->page_size % 16 == 0 && Dk == DB && Dv == DB && head_bytes % 64 == 0 && kv->n_pages > 0;
     a.tma = whole_rows && (window > 0 ? std::min(a.cap, window) : a.cap) > 512 &&
             make_page_map(&a.kmap, kv->k, head_bytes, kv->page_size, kv->Hkv, kv->n_pages, kv->k_stride_tok * eb,
-                          kv->k_stride_head * eb, kv->k_stride_page * eb, inner, &a.k_head_dim2) &&
+                          kv->k_stride_head * eb, kv->k_stride_page * eb, inner, box, &a.k_head_dim2) &&
             make_page_map(&a.vmap, kv->v, head_bytes, kv->page_size, kv->Hkv, kv->n_pages, kv->v_stride_tok * eb,
-                          kv->v_stride_head * eb, kv->v_stride_page * eb, inner, &a.v_head_dim2);
+                          kv->v_stride_head * eb, kv->v_stride_page * eb, inner, box, &a.v_head_dim2);
     a.n_pages = (int)kv->n_pages, a.page_size = kv->page_size;
     // t / P for t < 2^31 as a multiply and a shift: shift = ceil(log2 P), mul = floor(2^32 (2^shift - P) / P) + 1
     auto divide_by = [](int P, uint32_t& mul, uint32_t& shift) {

@@ -73,7 +73,8 @@ constexpr float kSlack = 6.f;   // log2 of how far a probability may pass its bo
 constexpr int inner_of(int row_bytes) { return row_bytes % 128 ? 64 : 128; }
 
 struct Args {
-    CUtensorMap kmap, vmap;              // where tma: boxes of 16 tokens of one head and page
+    CUtensorMap kmap, vmap;              // where tma: boxes of 16 (32: one_box) tokens of one head and page
+    int flat;                            // 8 bits: pages and scales' blocks are whole subtiles
     int tma, k_head_dim2, v_head_dim2;   // the map's order: dims, tokens, heads, pages; else dims, heads, tokens, pages
     const uint16_t* q;
     int64_t q_b, q_h;                    // elements
@@ -117,11 +118,19 @@ enum : int { k16 = 0, kS8 = 1, kE4M3 = 2 };
 // (measured at D = 128 in 16 bits, 16 ragged requests to 32768: 8 warps 160 us, 10 warps 152, 12 warps 157; three stages
 // put more in flight than the memory takes, and the SMs it serves last fall behind).  These figures are of when the choice
 // was made, with cp.async and each probability in two parts.
-template <bool I8, bool DIFF, int DB, int NT>
+constexpr int tok_of(int code, bool diff, int DB) {
+    return code == k16 ? (DB == 64 ? 32 : 16) : DB >= 192 && (diff || code == kE4M3) ? 16 : 32;
+}
+// Whether one box holds a subtile's keys, or values, where pages are whole subtiles.
+constexpr bool one_box(int code, bool diff, int DB) {
+    return tok_of(code, diff, DB) == 32 && DB * (code == k16 ? 2 : 1) == inner_of(DB * (code == k16 ? 2 : 1) / (diff ? 2 : 1));
+}
+template <int CODE, bool DIFF, int DB, int NT>
 struct Cfg {
+    static constexpr bool I8 = CODE != k16;
     static constexpr int kMt = DB / 16;                                   // accumulator fragments of a head tile
-    static constexpr int kTok = I8 || DB == 64 ? 32 : 16;                 // tokens of a subtile
-    static constexpr int kWarps = DB == 256 ? 5 : DB == 192 ? (I8 ? 6 : 7) : DB == 128 ? (I8 || NT == 2 ? 8 : 10) : I8 ? (NT == 1 ? 16 : 12) : 10;
+    static constexpr int kTok = tok_of(CODE, DIFF, DB);                   // tokens of a subtile
+    static constexpr int kWarps = I8 && kTok == 16 ? 8 : DB == 256 ? 5 : DB == 192 ? (I8 ? 6 : 7) : DB == 128 ? (I8 || NT == 2 ? 8 : 10) : I8 ? (NT == 1 ? 16 : 12) : 10;
     static constexpr int kPiece = NT * (8 * DB + 16);                     // floats: fragments, then m and l of the heads
     static constexpr int kUnits = NT * kMt;
     // kExact: stages of rows an odd number of 16-byte pieces apart, each with its scales and meta, then the first part (a
@@ -347,12 +356,13 @@ enum : int {
     kExact = 1,   // 16-byte cp.async; Dk = Dv = DB, so a row's pieces need no bounds (8 requests to 65536
                   // tokens in int8 99 us to 87, 204 of up to 101 tokens 14.5 to 12.5, 2 of 100 in pages of 8 11.5 to 10.2)
     kTma = 2,     // TMA; Dk = Dv = DB, pages of whole 16-token tiles
+    kFlat = 3,    // TMA; 8 bits, and pages and the scales' blocks of whole subtiles: a subtile has one page and one scale
 };
 template <bool F16, int CODE, bool DIFF, int DB, int NT, int MODE>
-__global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decode_kernel(const __grid_constant__ Args a) {
     constexpr bool I8 = CODE != k16, E4M3 = CODE == kE4M3;   // I8: codes of 8 bits
-    using C = Cfg<I8, DIFF, DB, NT>;
-    constexpr bool EXACT = MODE != kAny, TMA = MODE == kTma;
+    using C = Cfg<CODE, DIFF, DB, NT>;
+    constexpr bool EXACT = MODE != kAny, TMA = MODE >= kTma, FLAT = MODE == kFlat, BOX = FLAT && one_box(CODE, DIFF, DB);
     constexpr int kWarps = C::kWarps, kMt = C::kMt, kUnits = C::kUnits, kPiece = C::kPiece;
     constexpr int kTok = C::kTok, H = kTok / 16;   // H: 16-token tiles of a subtile
     constexpr int kMinSub = kMinTok / kTok, kSnapC = kSnapCta / kTok, kSnapW = kSnapWarp / kTok;
@@ -547,8 +557,9 @@ __global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1
     auto look_up = [&]() {
         uint32_t t = (uint32_t)(fs.lo & ~(kTok - 1)) + (uint32_t)f_sub * kTok;
         // within the tokens that count: the entry of any other place may be of no page
-        t = a.whole ? min(max(t + (tok & 16), (uint32_t)fs.lo & ~15u), (uint32_t)fs.L - 1) & ~15u
-                    : min(max(t + tok, (uint32_t)fs.lo), (uint32_t)fs.L - 1);
+        if (!FLAT)
+            t = a.whole ? min(max(t + (tok & 16), (uint32_t)fs.lo & ~15u), (uint32_t)fs.L - 1) & ~15u
+                        : min(max(t + tok, (uint32_t)fs.lo), (uint32_t)fs.L - 1);
         const uint32_t page = (__umulhi(t, a.div_mul) + t) >> a.div_shift;
         f_off = t - page * (uint32_t)a.page_size;
         f_entry = a.table[(int64_t)f_b * a.table_stride + page];
@@ -568,7 +579,14 @@ __global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1
             const uint32_t page = page_ok ? f_entry : 0;
             const uint64_t ka = (uint64_t)page * a.kp + (uint64_t)f_off * a.kt + (uint64_t)f_kvh * a.kh;
             const uint64_t va = (uint64_t)page * a.vp + (uint64_t)f_off * a.vt + (uint64_t)f_kvh * a.vh;
-            if (I8) {
+            if (FLAT) {   // lane 0: the keys' scale, lane 1: the values' (DIFF: two of each)
+                const uint32_t blk = (__umulhi(f_off, a.blk_mul) + f_off) >> a.blk_shift;
+                const bool of_v = lane >= kMaps;
+                const uint32_t head = f_kvh * kMaps + (lane & (kMaps - 1));
+                const uint64_t at = page * (uint64_t)(of_v ? a.vsp : a.ksp) + blk * (uint64_t)(of_v ? a.vst : a.kst) +
+                                    head * (uint64_t)(of_v ? a.vsh : a.ksh);
+                if (lane < 2 * kMaps) cp_async4(ring_u + scales_at(slot) + lane * 4, (of_v ? a.vs : a.ks) + at, page_ok);
+            } else if (I8) {
                 const uint32_t off = a.whole ? f_off + (lane & 15) : f_off;
                 const uint32_t blk = (__umulhi(off, a.blk_mul) + off) >> a.blk_shift;
                 const uint64_t ks = page * (uint64_t)a.ksp + blk * (uint64_t)a.kst + f_kvh * kMaps * (uint64_t)a.ksh;
@@ -590,14 +608,15 @@ __global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1
             }
             if (TMA) {   // a box of each 16-token tile with a token that counts, for keys and values
                 const uint32_t bar = bars + 8 * slot;
-                const int page1 = H == 2 ? __shfl_sync(0xffffffffu, (int)page, 16) : 0;
-                const int off1 = H == 2 ? __shfl_sync(0xffffffffu, (int)f_off, 16) : 0;
+                const int page1 = H == 2 && !FLAT ? __shfl_sync(0xffffffffu, (int)page, 16) : (int)page;
+                const int off1 = H == 2 && !FLAT ? __shfl_sync(0xffffffffu, (int)f_off, 16) : (int)f_off + 16;
                 if (lane == 0 && !dead) {
-                    const int tiles = ((mask & 0xffff) != 0) + (H == 2 && (mask >> 16) != 0);
+                    constexpr int kBoxes = BOX ? 1 : H;
+                    const int tiles = BOX ? (mask != 0 ? 2 : 0) : ((mask & 0xffff) != 0) + (H == 2 && (mask >> 16) != 0);
                     mbar_arrive_expect_tx(bar, tiles * 2 * C::kTile);
 #pragma unroll
-                    for (int h = 0; h < H; ++h) {
-                        if ((mask >> (16 * h) & 0xffff) == 0) continue;
+                    for (int h = 0; h < kBoxes; ++h) {
+                        if (BOX ? mask == 0 : (mask >> (16 * h) & 0xffff) == 0) continue;
                         const int at = h ? off1 : (int)f_off, pg = h ? page1 : (int)page;
 #pragma unroll
                         for (int p = 0; p < C::kParts; ++p) {
@@ -940,7 +959,7 @@ __global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1
             for (int m = 0; m < kMaps; ++m)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    f[m][i] = I8 ? sc[m * kTok + 16 * h + g + 8 * i] * (s8_unit<kKF16> * a.scale_log2) : a.scale_log2;
+                    f[m][i] = I8 ? sc[FLAT ? m : m * kTok + 16 * h + g + 8 * i] * (s8_unit<kKF16> * a.scale_log2) : a.scale_log2;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -993,25 +1012,28 @@ __global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1
             }
         }
         constexpr int kV2 = DIFF && I8 ? 2 : 1;   // a pair's two value heads have scales of their own
-        uint32_t ps[kV2][H][NT][2][kParts];
+        constexpr int kP2 = FLAT ? 1 : kV2;       // and probabilities, which a scale a token goes into
+        uint32_t ps[kP2][H][NT][2][kParts];
         // int8: the values' scales over the power of two below the subtile's largest, so that fp16 holds their products with
         // probabilities; what is left out of them is 2^-32 of the largest scale at most
         float down[kV2], back[kV2];
-        if (I8) {
-            static_assert(!I8 || kTok == 32, "a scale a lane");
+        if (FLAT) {
+#pragma unroll
+            for (int m = 0; m < kV2; ++m) back[m] = sc[kMaps + m];
+        } else if (I8) {
 #pragma unroll
             for (int m = 0; m < kV2; ++m) {
-                const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(sc[(kMaps + m) * kTok + lane]) & INT32_MAX) >> 23, 1u), 253u);
+                const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(sc[(kMaps + m) * kTok + tok]) & INT32_MAX) >> 23, 1u), 253u);
                 down[m] = __uint_as_float((254 - e) << 23), back[m] = __uint_as_float(e << 23);
             }
         }
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            float v[kV2][2];
+            float v[kP2][2];
 #pragma unroll
-            for (int m = 0; m < kV2; ++m)
+            for (int m = 0; m < kP2; ++m)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) v[m][i] = I8 ? sc[(kMaps + m) * kTok + 16 * h + g + 8 * i] * down[m] : 1.f;
+                for (int i = 0; i < 2; ++i) v[m][i] = I8 && !FLAT ? sc[(kMaps + m) * kTok + 16 * h + g + 8 * i] * down[m] : 1.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float(&p)[4] = c[h][nt];
@@ -1023,11 +1045,12 @@ __global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1
                     l_run[nt][j] += p[j] + p[j + 2];
                 }
 #pragma unroll
-                for (int m = 0; m < kV2; ++m)
+                for (int m = 0; m < kP2; ++m)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
+                        constexpr bool kScaled = I8 && !FLAT;
                         uint32_t* const part = ps[m][h][nt][j];
-                        split16<kPF16, I8, kParts>(I8 ? p[2 * j] * v[m][j] : p[2 * j], I8 ? p[2 * j + 1] * v[m][j] : p[2 * j + 1], part);
+                        split16<kPF16, I8, kParts>(kScaled ? p[2 * j] * v[m][j] : p[2 * j], kScaled ? p[2 * j + 1] * v[m][j] : p[2 * j + 1], part);
 #pragma unroll
                         for (int i = 0; i < kParts; ++i) part[i] = movmatrix_t(part[i]);
                     }
@@ -1067,9 +1090,9 @@ __global__ void __launch_bounds__(32 * Cfg<CODE != k16, DIFF, DB, NT>::kWarps, 1
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const bool up = kV2 == 2 && 2 * (mt + u) >= nmt;
-                            const uint32_t p[2] = {up ? ps[kV2 - 1][h][nt][0][i] : ps[0][h][nt][0][i],
-                                                   up ? ps[kV2 - 1][h][nt][1][i] : ps[0][h][nt][1][i]};
+                            const bool up = kP2 == 2 && 2 * (mt + u) >= nmt;
+                            const uint32_t p[2] = {up ? ps[kP2 - 1][h][nt][0][i] : ps[0][h][nt][0][i],
+                                                   up ? ps[kP2 - 1][h][nt][1][i] : ps[0][h][nt][1][i]};
                             if (h == 0 && i == 0) mma16_part<kPF16, true>(sum[u][nt], v[u], p);
                             else mma16_part<kPF16, false>(sum[u][nt], v[u], p);
                         }
@@ -1340,8 +1363,8 @@ WS_PAGED_LAUNCHES(launch_diff)
 template <bool F16, int CODE, bool DIFF, int DB, int NT, int MODE>
 int launch(Args a, int ctas, cudaStream_t st) {
     constexpr bool I8 = CODE != k16;
-    using C = Cfg<I8, DIFF, DB, NT>;
-    int smem = MODE == kTma ? C::kWarps * C::kWarpSmem + 1024 : C::kWarps * C::kGapWarpSmem;
+    using C = Cfg<CODE, DIFF, DB, NT>;
+    int smem = MODE >= kTma ? C::kWarps * C::kWarpSmem + 1024 : C::kWarps * C::kGapWarpSmem;
     if (MODE == kAny) {
         // rows as long as they are; stages until the copies in flight are 72 KB an SM (what two stages of 128-dim rows in
         // 16 bits give)
@@ -1370,8 +1393,11 @@ int launch(Args a, int ctas, cudaStream_t st) {
 
 template <bool F16, int CODE, bool DIFF, int DB, int NT>
 int launch_dims(const Args& a, int ctas, cudaStream_t st) {
-    if constexpr (Cfg<CODE != k16, DIFF, DB, NT>::kCanTma)
+    if constexpr (Cfg<CODE, DIFF, DB, NT>::kCanTma) {
+        if constexpr (CODE != k16)
+            if (a.tma && a.flat) return launch<F16, CODE, DIFF, DB, NT, kFlat>(a, ctas, st);
         if (a.tma) return launch<F16, CODE, DIFF, DB, NT, kTma>(a, ctas, st);
+    }
     return a.Dk == DB && a.Dv == DB ? launch<F16, CODE, DIFF, DB, NT, kExact>(a, ctas, st)
                                     : launch<F16, CODE, DIFF, DB, NT, kAny>(a, ctas, st);
 }

@@ -30,11 +30,11 @@ constexpr size_t kCounterHeaderBytes = size_t(256) << 10;
 constexpr int kMaxGroupsPerLaunch = int(kCounterHeaderBytes / 4);
 constexpr int kMaxHeadsPerLaunch = 16;   // query heads per kv row one GQA launch takes (two MMA column tiles)
 
-// TMA map of a pool of pages, as bytes: boxes of `inner` (64 or 128, swizzled over as much) bytes of 16 tokens of one head
+// TMA map of a pool of pages, as bytes: boxes of `inner` (64 or 128, swizzled over as much) bytes of `box_tok` tokens of one head
 // and page, from the axes (row, head, token, page), or (row, token, head, page) with *head_in_dim2.  False where the
 // strides are not what a map takes: ascending, each a multiple of the one before.
 bool make_page_map(CUtensorMap* map, const void* base, int64_t row, int64_t page_size, int64_t heads, int64_t pages,
-                   int64_t stride_tok, int64_t stride_head, int64_t stride_page, int inner, int* head_in_dim2);
+                   int64_t stride_tok, int64_t stride_head, int64_t stride_page, int inner, int box_tok, int* head_in_dim2);
 
 // Launch as a programmatic dependent of the previous grid on the stream: the kernel calls griddepcontrol.wait before it
 // reads or writes global memory, and reads with plain loads.  The read-only path (__ldg, const __restrict__) promises that

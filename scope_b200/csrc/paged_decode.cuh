@@ -818,10 +818,14 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
         return make_float2(o[0] * inv[0] - o[1] * lam, o[2] * inv[0] - o[3] * lam);
     };
     // Two dims of the head in fragment mt, times r and the norm's weights.
-    auto store_pair = [&](int64_t head0, int left, int nt, int mt, float2 x, float r) {
+    auto weights = [&](int mt) {
+        const int d0 = 16 * mt + (I8 ? 2 * g : g);
+        return a.weight && mt < nmt ? make_float2(a.weight[d0], a.weight[I8 ? d0 + 1 : d0 + 8]) : make_float2(1.f, 1.f);
+    };
+    auto store_pair = [&](int64_t head0, int left, int nt, int mt, float2 x, float r, float2 by) {
         const int h = nt * 8 + 2 * t4, d0 = 16 * mt + (I8 ? 2 * g : g), d1 = I8 ? d0 + 1 : d0 + 8;
         if (h >= left) return;
-        if (a.weight) x.x *= r * a.weight[d0], x.y *= r * a.weight[d1];
+        if (a.weight) x.x *= r * by.x, x.y *= r * by.y;
         uint16_t* const o = a.out + ((head0 + h) >> 1) * Dv;
         const uint32_t w = pack16<F16>(x.x, x.y);
         if (I8) *reinterpret_cast<uint32_t*>(o + d0) = w;
@@ -1139,7 +1143,7 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                         const float r = __frsqrt_rn(over_dims(sq) / Dv + a.eps);
 #pragma unroll
                         for (int mt = 0; mt < kMt; ++mt)
-                            if (mt < nmt) store_pair(head0, left, nt, mt, difference(acc[nt][mt], inv, lam), r);
+                            if (mt < nmt) store_pair(head0, left, nt, mt, difference(acc[nt][mt], inv, lam), r, weights(mt));
                     } else {
 #pragma unroll
                         for (int mt = 0; mt < kMt; ++mt)
@@ -1257,6 +1261,7 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
             const int nt = turn * kJob / kMt, mt0 = turn * kJob - nt * kMt, ml = NT * 8 * DB + nt * 16 + 2 * t4;
             const int at = (turn * kJob * 32 + lane) * 16;
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[kJob][4];
+            const float lam0 = DIFF && !to ? lam_of(row, left, nt) : 0.f;   // asked for before it is needed
 #pragma unroll
             for (int q = 0; q < kJob; ++q) o[q][0] = o[q][1] = o[q][2] = o[q][3] = 0.f;
 #pragma unroll 1
@@ -1311,7 +1316,7 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                 float inv[2];
                 finish(a, head0, left, nt, m, l, mt0 == 0, inv);
                 if (DIFF) {   // kept in the place of the first part's sums, which nobody else reads, until all jobs' squares are known
-                    const float lam = lam_of(row, left, nt) * inv[1];
+                    const float lam = lam0 * inv[1];
                     float sq = 0.f;
 #pragma unroll
                     for (int q = 0; q < kJob; ++q) {
@@ -1329,6 +1334,12 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
             }
         }
         if (DIFF && !to) {   // every warp is here with the same row
+            float2 w0[kJob];   // the first job's weights, before the others are waited for
+#pragma unroll
+            for (int q = 0; q < kJob; ++q) {
+                const int nt = turn0 * kJob / kMt;
+                w0[q] = turn0 < kJobs ? weights(turn0 * kJob - nt * kMt + q) : make_float2(0.f, 0.f);
+            }
             __syncthreads();
 #pragma unroll 1
             for (int i = turn0; i < kJobs; i += kWarps) {
@@ -1340,7 +1351,8 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
 #pragma unroll
                 for (int q = 0; q < kJob; ++q)
                     if (mt0 + q < nmt)
-                        store_pair(head0, left, nt, mt0 + q, *reinterpret_cast<const float2*>(smem + s_list[warp][0] + (i * kJob * 32 + lane) * 16 + q * 512), r);
+                        store_pair(head0, left, nt, mt0 + q, *reinterpret_cast<const float2*>(smem + s_list[warp][0] + (i * kJob * 32 + lane) * 16 + q * 512),
+                                   r, i == turn0 ? w0[q] : weights(mt0 + q));
             }
             parity ^= 1;
         }

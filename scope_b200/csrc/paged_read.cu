@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostTok = 32;   // tokens of a CTA
-constexpr int kAhead = 4;
+constexpr int kAhead = 2;
 
 struct Side {   // keys or values
     const uint8_t* src;                  // bytes

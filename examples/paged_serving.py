@@ -1,6 +1,6 @@
 """Serve prompts of any length from one paged cache, with requests joining and leaving while others run.
 
-    python examples/paged_serving.py [--requests 40] [--batch 16]
+    python examples/paged_serving.py [--requests 40] [--batch 16] [--cache bf16|int8|e4m3]
 
 A model of one attention layer with random weights, so that a prompt needs the attention of its last token only.  Every
 step packs the tokens that the running requests add -- a whole prompt for a request that joins, one token for the others
@@ -56,9 +56,10 @@ class OneLayer:
 
 
 def serve(model: OneLayer, prompts, n_new: int, batch: int, num_pages: int, page_size: int = 16, graph: bool = True,
-          on_step=None):
+          on_step=None, dtype=None, scale_block=1):
     """Greedy continuations of ``n_new`` tokens for every prompt (lists of token ids), ``batch`` requests at a time.  A
-    prompt is admitted when the pool holds every page that it and the running requests can still come to need."""
+    prompt is admitted when the pool holds every page that it and the running requests can still come to need.  ``dtype``
+    and ``scale_block``: the cache's, for one in 8 bits."""
     def pages_of(tokens):
         return -(-tokens // page_size)
 
@@ -71,7 +72,8 @@ def serve(model: OneLayer, prompts, n_new: int, batch: int, num_pages: int, page
         raise ValueError("serve: a prompt and its continuation take more pages than the pool has")
     dev = model.embed.device
     longest = max((len(p) for p in prompts), default=0) + n_new
-    cache = PagedKVCache(1, num_pages, page_size, model.Hkv, model.D, batch, longest, device=dev)
+    held_as = {} if dtype is None else dict(dtype=dtype, scale_block=scale_block)
+    cache = PagedKVCache(1, num_pages, page_size, model.Hkv, model.D, batch, longest, device=dev, **held_as)
     waiting, done = list(range(len(prompts))), {}
     slot_of, text = [None] * batch, {}          # which prompt each row of the batch serves; its tokens so far
     # the decode step's fixed buffers, and its graph
@@ -146,13 +148,15 @@ def main():
     ap.add_argument("--requests", type=int, default=40)
     ap.add_argument("--batch", type=int, default=16)
     ap.add_argument("--new", type=int, default=64)
+    ap.add_argument("--cache", choices=["bf16", "int8", "e4m3"], default="bf16", help="8 bits: a scale a page and head")
     a = ap.parse_args()
     model = OneLayer()
     g = torch.Generator().manual_seed(1)
     prompts = [torch.randint(0, 512, (int(n),), generator=g).tolist() for n in torch.randint(1, 1500, (a.requests,), generator=g)]
     pages = 16 * a.batch + 200
     t = time.perf_counter()
-    texts = serve(model, prompts, a.new, a.batch, pages)
+    held_as = {"bf16": {}, "int8": dict(dtype=torch.int8, scale_block=16), "e4m3": dict(dtype=torch.float8_e4m3fn, scale_block=16)}
+    texts = serve(model, prompts, a.new, a.batch, pages, **held_as[a.cache])
     torch.cuda.synchronize()
     t = time.perf_counter() - t
     held = sum(len(x) for x in texts)

@@ -218,9 +218,17 @@ class PagedKVCache:
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         self.device, self.page_size, self.num_pages, self.max_requests = dev, page_size, num_pages, max_requests
         vd = head_dim if v_head_dim is None else v_head_dim
-        pool = (num_pages, page_size, num_kv_heads)
-        self.k_pages = [torch.empty(*pool, head_dim, dtype=dtype, device=dev) for _ in range(num_layers)]
-        self.v_pages = [torch.empty(*pool, vd, dtype=dtype, device=dev) for _ in range(num_layers)]
+        # A head's rows of a page lie together where there is a scale a block: rows of 8 bits are short pieces otherwise
+        # (32 requests of 65536 tokens, 8 heads of 128 in e4m3: 650 us, with a token's heads together 731).
+        heads_major = quantised and (scale_block > 1 or dtype != torch.int8)
+
+        def pages(D):
+            if heads_major:
+                return torch.empty(num_pages, num_kv_heads, page_size, D, dtype=dtype, device=dev).transpose(1, 2)
+            return torch.empty(num_pages, page_size, num_kv_heads, D, dtype=dtype, device=dev)
+
+        self.k_pages = [pages(head_dim) for _ in range(num_layers)]
+        self.v_pages = [pages(vd) for _ in range(num_layers)]
         blocks = (num_pages, page_size // scale_block, num_kv_heads)
         self.k_scales = [torch.empty(blocks, device=dev) if quantised else None for _ in range(num_layers)]
         self.v_scales = [torch.empty(blocks, device=dev) if quantised else None for _ in range(num_layers)]

@@ -219,6 +219,72 @@ def test_append_scale_limits():
             assert ks[2, 0, 0] == 1 and ks[3, 0, 0] == 2 and ks[0, 0, 0] == 2.0 ** -28
 
 
+@pytest.mark.parametrize("sections,cyclic", [((12, 10, 10), False), ((12, 10, 10), True), (None, False)])
+@pytest.mark.parametrize("i64,odd", [(False, False), (True, True)])
+@pytest.mark.parametrize("N", [30, 3000])
+def test_append_turns_by_axes_positions_out_of_range_and_unaligned_turns(sections, cyclic, i64, odd, N):
+    g, Hkv, D, P, block = gen(8), 2, 80, 32, 16
+    A = 1 if sections is None else 3
+    table = table_of(50, 64)
+    if odd:   # 4 bytes past a boundary
+        table = torch.cat([table.new_zeros(1), table.flatten()])[1:].view(50, 64)
+    pos = torch.randint(0, 50, (A, N), generator=g, device=DEV, dtype=torch.int64 if i64 else torch.int32)
+    given = pos.clone()
+    given[:, 3], pos[:, 3] = -7, 0
+    given[:, 9], pos[:, 9] = (1 << 40) if i64 else (1 << 30), 49
+    axes = [0] * 32
+    if sections and cyclic:
+        axes = [i % 3 if i // 3 < sections[i % 3] else 0 for i in range(32)]
+    elif sections:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    q, k, v = (torch.randn(N, h, D, generator=g, device=DEV).to(HF) for h in (4, Hkv, Hkv))
+    kp, ks = make_pool(g, 100, P, block, Hkv, D, E4)
+    vp, vs = make_pool(g, 100, P, block, Hkv, D, E4)
+    slots = torch.arange(N, device=DEV) + 5
+    rk = turned(k, pos, table, axes, "half")
+    wk, wks = append_reference(rk, slots, kp, ks, block)
+    got = paged.rope_append(q, k, v, given[0] if A == 1 else given, table, slots, kp, vp, k_scales=ks, v_scales=vs, sections=sections,
+                            cyclic=cyclic)
+    assert torch.equal(got, turned(q, pos, table, axes, "half").to(HF))
+    assert torch.equal(ks, wks) and torch.equal(raw(kp), raw(wk))
+    assert scope_b200.status_take() == 5
+
+
+def test_append_of_a_slot_beside_others_and_in_place():
+    """Queries turned in place in the packed projection that keys and values are read from; a call without a token."""
+    g, N, H, Hkv, D = gen(12), 70, 4, 2, 64
+    for n in (N, 4000):
+        qkv = torch.randn(n, (H + 2 * Hkv) * D, generator=g, device=DEV).to(BF)
+        q, k, v = (x.view(n, h, D) for x, h in zip(qkv.split([H * D, Hkv * D, Hkv * D], 1), (H, Hkv, Hkv)))
+        table, pos = table_of(100, D), torch.randint(0, 100, (n,), generator=g, device=DEV)
+        kp, ks = make_pool(g, 260, 16, 16, Hkv, D, I8)
+        vp, vs = make_pool(g, 260, 16, 16, Hkv, D, I8)
+        slots = torch.arange(n, device=DEV)
+        want = turned(q, pos[None], table, [0] * 32, "half").to(BF)
+        wk, wks = append_reference(turned(k, pos[None], table, [0] * 32, "half"), slots, kp, ks, 16)
+        wv, wvs = append_reference(v.float(), slots, vp, vs, 16)
+        assert paged.rope_append(q, k, v, pos, table, slots, kp, vp, k_scales=ks, v_scales=vs, q_out=q) is q
+        assert torch.equal(q, want)
+        assert torch.equal(raw(kp), raw(wk)) and torch.equal(raw(vp), raw(wv)) and torch.equal(ks, wks) and torch.equal(vs, wvs)
+    none = torch.empty(0, Hkv, D, dtype=BF, device=DEV)
+    paged.rope_append(None, none, none, None, None, slots[:0], kp, vp, k_scales=ks, v_scales=vs)
+    assert torch.equal(raw(kp), raw(wk))
+
+
+def test_append_behind_many_dropped_tokens():
+    """A block that goes on behind thousands of dropped tokens, in a call that ends in as many."""
+    g, P, block = gen(13), 64, 64
+    kp, ks = make_pool(g, 3, P, block, 1, 32, I8)
+    vp, vs = make_pool(g, 3, P, block, 1, 32, I8)
+    slots = torch.full((9000,), -1, dtype=torch.int64, device=DEV)
+    slots[10], slots[4000], slots[4100], slots[4101] = 70, 72, 71 + 5, 128
+    k, v = (torch.randn(9000, 1, 32, generator=g, device=DEV).to(BF) for _ in range(2))
+    wk, wks = append_reference(k.float(), slots, kp, ks, block)
+    wv, wvs = append_reference(v.float(), slots, vp, vs, block)
+    paged.rope_append(None, k, v, None, None, slots, kp, vp, k_scales=ks, v_scales=vs)
+    assert torch.equal(ks, wks) and torch.equal(vs, wvs) and torch.equal(raw(kp), raw(wk)) and torch.equal(raw(vp), raw(wv))
+
+
 def test_append_slots_past_the_pool_and_unaligned_rows():
     pool, scales = torch.zeros(2, 2, 16, 1, 32, dtype=I8, device=DEV), torch.zeros(2, 2, 2, 1, device=DEV)
     flat = torch.ones(4 * 32 + 3, device=DEV).to(BF)
@@ -388,6 +454,36 @@ def test_decode_head_dims(Dk, Dv, dtype, pool):
     wide = dict(s, table=torch.cat([s["table"], torch.full((5, 40), 1 << 20, dtype=torch.int32, device=DEV)], 1))
     agrees(s, *decode(wide))
     assert scope_b200.status_take() == 0
+
+
+def widened(s, n=60):
+    """The same requests behind a table too wide for the form that short tables take."""
+    B = s["table"].shape[0]
+    return dict(s, table=torch.cat([s["table"], torch.full((B, n), 1 << 20, dtype=torch.int32, device=DEV)], 1))
+
+
+@pytest.mark.parametrize("P,block", [(32, 32), (64, 32), (64, 64), (96, 96), (96, 32), (16, 16), (48, 48), (256, 128), (64, 8)])
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("dtype,pool", [(BF, I8), (HF, E4), (BF, E4)])
+def test_decode_where_a_subtile_has_one_scale_and_where_not(P, block, D, dtype, pool):
+    """Lengths at every border of pages, blocks and subtiles, rows by TMA; e4m3 codes behind a length are NaN."""
+    lens = [0, 1, 15, 16, 17, 31, 32, 33, 47, 63, 64, 65, 95, 96, 97, 700, 1500]
+    s = widened(make_decode(lens, 6, 2, D, D, P, block, dtype, pool, heads_major=P == 64, seed=P + block + D))
+    agrees(s, *decode(s))
+    agrees(s, *decode(s, window=601), window=601)
+    assert scope_b200.status_take() == 0
+
+
+def test_decode_leaves_bad_pages_out():
+    for pool, P, block in ((I8, 64, 64), (E4, 64, 64), (E4, 16, 16)):
+        s = widened(make_decode([700, 90], 4, 2, 128, 128, P, block, BF, pool, seed=9))
+        s["table"][0, 1], s["table"][0, 3] = -1, s["k"].shape[0]
+        page, off = s["rows"][0]
+        t = torch.arange(700, device=DEV) // P
+        keep = (t != 1) & (t != 3)
+        s["rows"][0] = (page[keep], off[keep])
+        agrees(s, *decode(s))
+        assert scope_b200.status_take() == 5
 
 
 @pytest.mark.parametrize("G", [1, 3, 8, 9, 16, 20])

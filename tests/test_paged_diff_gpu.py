@@ -126,6 +126,18 @@ def test_head_dims(Dk, Dv, dtype, pool, block):
     agrees(s, *diff(wide, False), norm=False)
 
 
+@pytest.mark.parametrize("P,block", [(16, 16), (32, 32), (64, 64), (64, 32), (96, 48), (64, 8)])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("dtype,pool", [(BF, I8), (HF, E4)])
+def test_where_a_subtile_has_one_scale_and_where_not(P, block, D, dtype, pool):
+    lens = [0, 1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 700, 1500]
+    s = make(lens, 4, 2, D, D, P, dtype, pool, block, heads_major=P == 64, seed=P + block + D)
+    s["table"] = torch.cat([s["table"], torch.full((len(lens), 60), 1 << 20, dtype=torch.int32, device=DEV)], 1)
+    agrees(s, *diff(s))
+    agrees(s, *diff(s, False, window=601), norm=False, window=601)
+    assert scope_b200.status_take() == 0
+
+
 @pytest.mark.parametrize("G", [1, 2, 4, 5, 8, 9])
 @pytest.mark.parametrize("D", [32, 64, 128])
 @pytest.mark.parametrize("dtype,pool,block", [(BF, BF, 1), (HF, I8, 16)])

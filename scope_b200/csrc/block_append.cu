@@ -61,31 +61,6 @@ __device__ __forceinline__ float warp_most(float x) {
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x) & INT32_MAX));
 }
 
-// The scale that rows up to `most` ask for; NaN and infinity stay.
-template <bool E4M3>
-__device__ __forceinline__ float own_scale(float most) {
-    most = max_nan(most, 1e-6f);
-    if (!E4M3) return __fmul_rn(most, 1.0f / 127.0f);
-    const uint32_t bits = __float_as_uint(most);
-    if (!(most < INFINITY)) return most;
-    // most = 1.m 2^e, 448 = 1.75 2^8
-    return __uint_as_float(((bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000)) << 23);
-}
-
-// Four values times inv as codes.
-template <bool E4M3>
-__device__ __forceinline__ uint32_t codes4(float2 x, float2 y, float inv) {
-    x = make_float2(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv)), y = make_float2(__fmul_rn(y.x, inv), __fmul_rn(y.y, inv));
-    uint32_t w;
-    if (E4M3) {
-        asm("{.reg .b16 l, h; cvt.rn.satfinite.e4m3x2.f32 l, %2, %1; cvt.rn.satfinite.e4m3x2.f32 h, %4, %3; mov.b32 %0, {l, h};}"
-            : "=r"(w) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
-    } else {   // within 127 by clamping first: rounding keeps the order
-        auto code = [](float f) { return (uint32_t)__float2int_rn(fminf(fmaxf(f, -127.f), 127.f)); };
-        w = __byte_perm(__byte_perm(code(x.x), code(x.y), 0x0040), __byte_perm(code(y.x), code(y.y), 0x0040), 0x5410);
-    }
-    return w;
-}
 // Four codes times `ratio` as codes again.
 template <bool E4M3>
 __device__ __forceinline__ uint32_t again4(uint32_t w, float ratio) {
@@ -116,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, WARPS == 1 ? 4 : 5) block_append_ker
     // CTAs for keys and values are spread evenly among those for queries: the ones wait, the others stream
     const uint32_t nth = a.all_jobs ? blockIdx.x : __umulhi(blockIdx.x, a.job_rate);
     if (!a.all_jobs && nth == __umulhi(blockIdx.x + 1, a.job_rate)) {
-        rope_rows<F16, false, VEC, 2>(a.q, (int64_t)(blockIdx.x - nth) * kWarps + warp);
+        rope_rows<F16, kRows16, VEC, 2>(a.q, (int64_t)(blockIdx.x - nth) * kWarps + warp);
         return;
     }
     const uint32_t id = WARPS == 1 ? nth * kWarps + warp : nth;

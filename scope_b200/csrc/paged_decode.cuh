@@ -32,13 +32,28 @@
 //     value gives an infinite output.
 //   * int8 rows go from shared memory to bf16 (fp16) fragments by bit operations, exactly; the row's scale multiplies
 //     the score, or the probability, which then enters as two fp16 values (three bf16 values: 85 us to 78).
+//   * Codes have one scale a row, or a block of tokens and head.  In general each token's scale is fetched beside its row.
+//     Where pages and blocks are whole subtiles (kFlat), a subtile has one page and two scales: one TMA box each for keys and
+//     values, the keys' scale on the scores, the values' on the subtile's sums instead of the probabilities (8 requests of
+//     16384 to 65536 tokens in int8: 78.8 us, 71.6; two value heads of a pair no longer take two sets of probabilities:
+//     164 us to 127).  e4m3 codes become fp16 in one conversion a pair and enter both products as such; bf16 queries go to
+//     fp16 with them, times the power of two that brings a head's largest value to 2^14, exact to 2^-38 of it (8 requests:
+//     69.2 us).  Their bytes may be NaN, so values that do not count are zeroed as in 16 bits.
+//   * DIFF: o = softmax(q1 k1) v - lam softmax(q2 k2) v over pairs of pool heads.  A pair is one row: its keys lie side by
+//     side, and the queries of the two maps are two columns, each zero over the other's dims, so one pass over keys and
+//     values serves both maps and the products are the ones above.  A lane then holds both maps' sums of a head and takes
+//     the difference, and the norm over a head's dims, before it writes; joined rows keep the difference in shared memory
+//     until all jobs' sums of squares are known.
 //   * A row that ends inside one warp's stretch is written at once.  The others leave a state (o, m, l) per warp,
 //     which the CTA joins in shared memory; what crosses CTAs goes through the workspace and is joined by the CTA that
 //     files the last part (a ticket), always in the same order, so results do not depend on timing.
 //
 // Measured on a B200 (device time, a few replays on a cool card): 32 requests of 131072 tokens, 32 query and 4 kv heads of
 // 128, bf16: 1207 us (8.59 GB, 7.1 TB/s; a copy reaches 6.55); 16 ragged to 32768 tokens, 32 and 8 heads: 131.7 us
-// (852 MB, 6.5 TB/s); 8 of 16384 to 65536 tokens in int8: 78 us (393 MB, 5.0 TB/s).  What is left at those is some 4 us
+// (852 MB, 6.5 TB/s); 8 of 16384 to 65536 tokens in int8: 78 us (393 MB, 5.0 TB/s).  In e4m3 with a scale for 64 tokens, 32
+// requests of 65536 tokens, 64 and 8 heads of 128: 731 us (4.30 GB, 5.9 TB/s; rows of 128 bytes a kilobyte apart; with a
+// head's rows of a page together 650 us, 6.6 TB/s).  Differential, 16 ragged to 32768 tokens, 16 heads of 2 x 64, 8 pairs:
+// 121 us (738 MB, 6.1 TB/s); 24 of up to 16384 in int8, 32 heads of 2 x 128, 8 pairs, window 8000: 127 us (629 MB, 5.0 TB/s).  What is left at those is some 4 us
 // before the first rows arrive (the lengths, the table and the rows come one after the other) and 8 us after the last
 // (join, ticket, join).  Small calls are those latencies alone: 1 request of 4096 tokens 12.0 us, of 100 9.8.
 //
@@ -112,7 +127,8 @@ struct Args {
 enum : int { k16 = 0, kS8 = 1, kE4M3 = 2 };
 
 // The variant for head dims up to DB, 8*NT query heads a block.  A subtile is 16 tokens, or 32 where 16 would be 4 KB or
-// less (int8, head dims up to 64): what a subtile costs beside its bytes then counts half (measured with int8 rows of 128,
+// less (8 bits, head dims up to 64; of rows of 192 and 256 in 8 bits e4m3 and DIFF take 16: 8 warps then fit instead of 5,
+// which with flat scales took 24 requests of 256-byte rows from 164 us to 127): what a subtile costs beside its bytes then counts half (measured with int8 rows of 128,
 // 8 requests to 65536: 82 us to 78; 127 requests to 13489 with rows of 64: 167 us to 132).  As many warps, each with two
 // stages, as shared memory and the registers allow
 // (measured at D = 128 in 16 bits, 16 ragged requests to 32768: 8 warps 160 us, 10 warps 152, 12 warps 157; three stages
@@ -812,7 +828,7 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
     // DIFF: head t4 of tile nt has its maps in columns 2t and 2t + 1, so a lane holds both.
     auto lam_of = [&](int row, int left, int nt) {
         const int h = nt * 8 + 2 * t4;
-        return h < left ? a.lam[(((row >> 16) * a.G + (row & 0xffff) * 8 * NT + h) >> 1) * a.lam_stride] : 0.f;
+        return h < left ? a.lam[(((row >> 16) * a.G + (row & 0xffff) * 8 * NT + h) >> 1) * (int64_t)a.lam_stride] : 0.f;
     };
     auto difference = [&](const float* o, const float* inv, float lam) {   // lam: with the second map's 1/l
         return make_float2(o[0] * inv[0] - o[1] * lam, o[2] * inv[0] - o[3] * lam);

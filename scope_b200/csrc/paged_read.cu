@@ -5,6 +5,9 @@
 // What bounds it: memory, each code read once and two bytes written for it.  A thread owns a unit of 16 dims of a head (16
 // bytes of codes, 32 of output; 16-bit pools: 8 dims) and walks its CTA's tokens, kAhead loads in flight.  The tokens'
 // places are looked up once for a CTA.
+// Measured: 16 requests of up to 32768 tokens from the first sixteenth on, 8 heads of 128 in e4m3, 169 us (1.04 GB, 6.15
+// TB/s, 0.94 of a copy's rate); 1000 tokens of 4 heads 2.8 us.  Loads ahead: 1 took 182 us, 2 169, 4 178, 8 236 (registers);
+// CTAs of 16 tokens 163 us there but 6.1 us for 4.1 where heads are few; of 64 tokens 183; 128 threads 181, 512 threads 194.
 #include <cstdio>
 
 #include "common.cuh"

@@ -33,11 +33,11 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kGroup = 2;   // rows a thread loads before it turns the first, where it has several
 
-template <bool F16, bool I8, bool VEC, int GROUP>
+template <bool F16, int CODE, bool VEC, int GROUP>
 __global__ void __launch_bounds__(32 * kWarps) rope_append_kernel(const __grid_constant__ RopeAppendArgs a) {
     pdl_wait_primary();
     pdl_launch_dependents();
-    rope_rows<F16, I8, VEC, GROUP>(a, (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5));
+    rope_rows<F16, CODE, VEC, GROUP>(a, (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5));
 }
 
 }  // namespace
@@ -137,7 +137,7 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
     a.lanes = 1;
     while (a.lanes * 16 < Dmax) a.lanes *= 2;
     const int block = kv ? std::max(kv->scale_block, 1) : 1;
-    const bool blocks8 = kv && (kv->dtype == WS_DTYPE_E4M3 || (kv->dtype == WS_DTYPE_I8 && block > 1));
+    const bool e4 = kv && kv->dtype == WS_DTYPE_E4M3, blocks8 = kv && block > 1 && (e4 || kv->dtype == WS_DTYPE_I8);
     if (blocks8 && H > 0 && !block_append_small(N, kv->Hkv)) {
         if (const int rc = ws_rope_append(rope, q, q_stride_tok, q_stride_head, H, D, q_out, qo_stride_tok, qo_stride_head, nullptr, 0,
                                           0, nullptr, 0, 0, dtype, N, nullptr, nullptr, stream))
@@ -149,7 +149,7 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
     // One warp walks all heads of a token when there are tokens for every SM; with fewer, its rows are shared out.  Into
     // int8, where a row takes longer, that pays with half as many tokens only (4097 tokens of 20 + 5 + 5 heads, us with 16,
     // 32, 64 and 128 warps wanted an SM: 14.5, 15.5, 17.2, 20.4).
-    const bool f16 = dtype == WS_DTYPE_F16, i8 = kv && kv->dtype == WS_DTYPE_I8;
+    const bool f16 = dtype == WS_DTYPE_F16, i8 = e4 || (kv && kv->dtype == WS_DTYPE_I8);
     const int rows = 32 / a.lanes, steps = (H + (kv ? 2 * kv->Hkv : 0) + rows - 1) / rows;
     const int64_t want = (int64_t)device_sm_count() * (i8 ? 16 : 32);
     a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps, (want + N - 1) / N));
@@ -160,15 +160,18 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
     // (5212 tokens of 3 heads of 256: 15 and 18; 4097 tokens into int8: 38 and 41).
     const bool several = a.parts == 1 && steps >= 8 && !i8;
     auto pick = [&](auto half, auto codes) {
-        constexpr bool F = decltype(half)::value, I = decltype(codes)::value;
-        if (!vec) return rope_append_kernel<F, I, false, 1>;
-        if constexpr (!I)
-            if (several) return rope_append_kernel<F, I, true, kGroup>;
-        return rope_append_kernel<F, I, true, 1>;
+        constexpr bool F = decltype(half)::value;
+        constexpr int C = decltype(codes)::value;
+        if (!vec) return rope_append_kernel<F, C, false, 1>;
+        if constexpr (C == kRows16)
+            if (several) return rope_append_kernel<F, C, true, kGroup>;
+        return rope_append_kernel<F, C, true, 1>;
     };
-    using yes = std::true_type;
-    using no = std::false_type;
-    auto fn = f16 ? (i8 ? pick(yes{}, yes{}) : pick(yes{}, no{})) : (i8 ? pick(no{}, yes{}) : pick(no{}, no{}));
+    auto by = [&](auto half) {
+        if (e4) return pick(half, std::integral_constant<int, kRowsE4M3>{});
+        return i8 ? pick(half, std::integral_constant<int, kRowsS8>{}) : pick(half, std::integral_constant<int, kRows16>{});
+    };
+    auto fn = f16 ? by(std::true_type{}) : by(std::false_type{});
     const cudaError_t e = launch_dependent(fn, dim3((unsigned)blocks), 32 * kWarps, 0, static_cast<cudaStream_t>(stream), a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));
 }

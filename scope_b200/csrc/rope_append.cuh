@@ -122,10 +122,38 @@ __device__ __forceinline__ void turn_pair(float& x1, float& x2, float c, float s
     x1 = y1;
 }
 
-// A warp's rows: item = token * parts + part.  F16: fp16 inputs (else bf16); I8: the pool holds int8 codes; VEC: q, k, v
-// and q_out are 16-byte aligned throughout.
-template <bool F16, bool I8, bool VEC, int GROUP>
+// The scale that rows up to `most` ask for; NaN and infinity stay.
+template <bool E4M3>
+__device__ __forceinline__ float own_scale(float most) {
+    most = max_nan(most, 1e-6f);
+    if (!E4M3) return __fmul_rn(most, 1.0f / 127.0f);
+    const uint32_t bits = __float_as_uint(most);
+    if (!(most < INFINITY)) return most;
+    // most = 1.m 2^e, 448 = 1.75 2^8
+    return __uint_as_float(((bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000)) << 23);
+}
+
+// Four values times inv as codes.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t codes4(float2 x, float2 y, float inv) {
+    x = make_float2(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv)), y = make_float2(__fmul_rn(y.x, inv), __fmul_rn(y.y, inv));
+    uint32_t w;
+    if (E4M3) {
+        asm("{.reg .b16 l, h; cvt.rn.satfinite.e4m3x2.f32 l, %2, %1; cvt.rn.satfinite.e4m3x2.f32 h, %4, %3; mov.b32 %0, {l, h};}"
+            : "=r"(w) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+    } else {   // within 127 by clamping first: rounding keeps the order
+        auto code = [](float f) { return (uint32_t)__float2int_rn(fminf(fmaxf(f, -127.f), 127.f)); };
+        w = __byte_perm(__byte_perm(code(x.x), code(x.y), 0x0040), __byte_perm(code(y.x), code(y.y), 0x0040), 0x5410);
+    }
+    return w;
+}
+enum : int { kRows16 = 0, kRowsS8 = 1, kRowsE4M3 = 2 };   // how rows are held: as they are, or as codes with a scale a row
+
+// A warp's rows: item = token * parts + part.  F16: fp16 inputs (else bf16); CODE: what the pool holds; VEC: q, k, v and
+// q_out are 16-byte aligned throughout.
+template <bool F16, int CODE, bool VEC, int GROUP>
 __device__ __forceinline__ void rope_rows(const RopeAppendArgs& a, int64_t item) {
+    constexpr bool I8 = CODE != kRows16;
     const int lane = threadIdx.x & 31;
     const int64_t t = a.parts == 1 ? item : item / a.parts;
     if (t >= a.N) return;
@@ -213,8 +241,14 @@ __device__ __forceinline__ void rope_rows(const RopeAppendArgs& a, int64_t item)
                 for (int o = a.lanes >> 1; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
                 if (on && kind) {
                     most = max_nan(most, 1e-6f);
-                    const float inv = __fdiv_rn(127.f, most);
+                    const float scale = CODE == kRowsE4M3 ? own_scale<true>(most) : __fmul_rn(most, 1.0f / 127.0f);
+                    const float inv = CODE == kRowsE4M3 ? (scale < INFINITY ? __fdiv_rn(1.f, scale) : 0.f) : __fdiv_rn(127.f, most);
                     auto codes = [&](const float* f) {
+                        if (CODE == kRowsE4M3) {   // 0 where the scale is not finite
+                            if (!(inv > 0.f)) return make_uint2(0, 0);
+                            return make_uint2(codes4<true>(make_float2(f[0], f[1]), make_float2(f[2], f[3]), inv),
+                                              codes4<true>(make_float2(f[4], f[5]), make_float2(f[6], f[7]), inv));
+                        }
                         uint32_t w[2] = {0, 0};
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
@@ -226,7 +260,7 @@ __device__ __forceinline__ void rope_rows(const RopeAppendArgs& a, int64_t item)
                     uint8_t* p = x.dst + page * x.dst_page + off * x.dst_tok + h * x.dst_head;
                     *reinterpret_cast<uint2*>(p + d0) = codes(lo);
                     *reinterpret_cast<uint2*>(p + d1) = codes(hi);
-                    if (u == 0) x.scales[page * x.s_page + off * x.s_tok + h * x.s_head] = __fmul_rn(most, 1.0f / 127.0f);
+                    if (u == 0) x.scales[page * x.s_page + off * x.s_tok + h * x.s_head] = scale;
                 }
             }
             if (on && (!I8 || kind == 0)) {

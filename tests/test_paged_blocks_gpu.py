@@ -250,6 +250,37 @@ def test_append_turns_by_axes_positions_out_of_range_and_unaligned_turns(section
     assert scope_b200.status_take() == 5
 
 
+@pytest.mark.parametrize("N,H,Hkv,D,Dv,rot,P", [(1, 8, 2, 128, 128, 128, 16), (513, 12, 3, 80, 80, 64, 24), (3000, 8, 4, 64, 192, 64, 1)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("pairs", ["half", "adjacent"])
+def test_append_e4m3_rows_in_any_order(N, H, Hkv, D, Dv, rot, P, dtype, pairs):
+    """A scale a row: rows of zeros, of one NaN and of one infinity among them, slots in any order."""
+    g = gen(N)
+    table, pos = table_of(400, rot), torch.randint(0, 400, (1, N), generator=g, device=DEV)
+    q, k, v = (torch.randn(N, h, d, generator=g, device=DEV).to(dtype) for h, d in ((H, D), (Hkv, D), (Hkv, Dv)))
+    if N > 5:
+        k[2], v[3, 0, 5], v[4, 1, 0] = 0, float("nan"), float("-inf")
+    n_pages = -(-N // P) + 5
+    (kp, ks), (vp, vs) = (make_pool(g, n_pages, P, 1, Hkv, d, E4, heads_major=D == 80) for d in (D, Dv))
+    slots = torch.randperm(n_pages * P, generator=g, device=DEV)[:N].contiguous()
+    slots[torch.rand(N, generator=g, device=DEV) < 0.1] = -1
+    wk, wks, wv, wvs = kp.clone(), ks.clone(), vp.clone(), vs.clone()
+    rk = turned(k, pos, table, [0] * (rot // 2), pairs)
+    at = torch.nonzero(slots >= 0)[:, 0]
+    page, off = slots[at] // P, slots[at] % P
+    for x, pages, scales in ((rk, wk, wks), (v.float(), wv, wvs)):
+        most = x.abs().amax(-1).clamp(min=1e-6)      # clamp keeps a NaN
+        part, up = torch.frexp(most)
+        s = torch.where(most.isfinite(), torch.exp2((up - 9 + (part > 0.875).int()).float()), most)
+        codes = torch.where(most.isfinite()[..., None], (x * (torch.ones_like(s) / s)[..., None]).clamp(-448, 448), 0.0).to(E4)
+        raw(pages)[page, off], scales[page, off] = raw(codes)[at], s[at]
+    got = paged.rope_append(q, k, v, pos, table, slots, kp, vp, k_scales=ks, v_scales=vs, pairs=pairs)
+    assert torch.equal(got, turned(q, pos, table, [0] * (rot // 2), pairs).to(dtype))
+    assert torch.equal(raw(kp), raw(wk)) and torch.equal(raw(vp), raw(wv))
+    assert torch.equal(ks, wks) and torch.equal(vs.nan_to_num(nan=-3.0), wvs.nan_to_num(nan=-3.0))
+    assert scope_b200.status_take() == 0
+
+
 def test_append_of_a_slot_beside_others_and_in_place():
     """Queries turned in place in the packed projection that keys and values are read from; a call without a token."""
     g, N, H, Hkv, D = gen(12), 70, 4, 2, 64

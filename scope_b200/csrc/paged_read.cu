@@ -3,11 +3,12 @@
 //   row cu[b] + i  =  token starts[b] + i of request b, its codes times their scale, rounded once.
 //
 // What bounds it: memory, each code read once and two bytes written for it.  A thread owns a unit of 16 dims of a head (16
-// bytes of codes, 32 of output; 16-bit pools: 8 dims) and walks its CTA's tokens, kAhead loads in flight.  The tokens'
+// bytes of codes, 32 of output; 16-bit pools: 8 dims) and walks its CTA's tokens, two or four loads in flight.  The tokens'
 // places are looked up once for a CTA.
-// Measured: 16 requests of up to 32768 tokens from the first sixteenth on, 8 heads of 128 in e4m3, 169 us (1.04 GB, 6.15
-// TB/s, 0.94 of a copy's rate); 1000 tokens of 4 heads 2.8 us.  Loads ahead: 1 took 182 us, 2 169, 4 178, 8 236 (registers);
-// CTAs of 16 tokens 163 us there but 6.1 us for 4.1 where heads are few; of 64 tokens 183; 128 threads 181, 512 threads 194.
+// Measured: 16 requests of up to 32768 tokens from the first sixteenth on, 8 heads of 128 in e4m3, 168 us (1.04 GB, 6.2 TB/s,
+// 0.94 of a copy's rate); 1000 tokens of 4 heads 2.8 us.  Loads in flight: 1 took 182 us, 2 169, 4 178, 8 236 (registers,
+// so fewer warps); but where all may lie in L2 (18 thousand tokens of 4 heads just written) 2 took 16.6 us and 4 14.0.  CTAs
+// of 16 tokens took 163 us there, but 6.1 us for 4.1 where heads are few; of 64 tokens 183; of 128 threads 181, 512 194.
 #include <cstdio>
 
 #include "common.cuh"
@@ -15,12 +16,13 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace ws {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostTok = 32;   // tokens of a CTA
-constexpr int kAhead = 2;
 
 struct Side {   // keys or values
     const uint8_t* src;                  // bytes
@@ -69,8 +71,8 @@ __device__ __forceinline__ void values16(const uint4& w, float s, uint32_t* y) {
     }
 }
 
-// KIND: 0 16-bit values, 1 int8, 2 e4m3.
-template <bool F16, int KIND>
+// KIND: 0 16-bit values, 1 int8, 2 e4m3.  AHEAD: loads in flight a thread.
+template <bool F16, int KIND, int AHEAD>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadArgs a) {
     __shared__ int s_page[kMostTok], s_off[kMostTok];   // page < 0: -1 zeros, -2 nothing
     pdl_wait_primary();
@@ -115,11 +117,11 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
     uint16_t* const dst = x.dst + ((row0 * a.Hkv + head) * x.D + d);
     const int64_t row_elems = (int64_t)a.Hkv * x.D;
 #pragma unroll 1
-    for (int t = tok0; t < a.tok; t += step * kAhead) {
-        uint4 w[kAhead];
-        float s[kAhead];
+    for (int t = tok0; t < a.tok; t += step * AHEAD) {
+        uint4 w[AHEAD];
+        float s[AHEAD];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < AHEAD; ++i) {
             const int tk = t + i * step;
             w[i] = make_uint4(0, 0, 0, 0), s[i] = 0.f;
             if (tk < a.tok && s_page[tk] >= 0) {
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
             }
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < AHEAD; ++i) {
             const int tk = t + i * step;
             if (tk >= a.tok || s_page[tk] == -2) continue;
             uint4* const p = reinterpret_cast<uint4*>(dst + tk * row_elems);
@@ -185,9 +187,16 @@ extern "C" int ws_paged_read(const ws_paged_kv* kv, const int32_t* page_table, i
     if (blocks > INT32_MAX) return set_error(WS_ERR_UNSUPPORTED, "paged_read: too many tokens");
     a.status = device_status_word();
     const bool f16 = out_dtype == WS_DTYPE_F16, i8 = kv->dtype == WS_DTYPE_I8;
-    auto fn = !eight ? read_kernel<false, 0>
-              : f16  ? (i8 ? read_kernel<true, 1> : read_kernel<true, 2>)
-                     : (i8 ? read_kernel<false, 1> : read_kernel<false, 2>);
+    // four loads in flight where what is read and written may lie in L2 and a thread has more than two tokens (31 requests
+    // of one head, two tokens a thread: 5.4 us with four, 4.1 with two)
+    const bool small = a.tok * std::min<int64_t>(units, kThreads) > 2 * kThreads && n_tokens * kv->Hkv * (kv->Dk + kv->Dv) <= 48 << 20;
+    auto pick = [&](auto ahead) {
+        constexpr int A = decltype(ahead)::value;
+        return !eight ? read_kernel<false, 0, A>
+               : f16  ? (i8 ? read_kernel<true, 1, A> : read_kernel<true, 2, A>)
+                      : (i8 ? read_kernel<false, 1, A> : read_kernel<false, 2, A>);
+    };
+    auto fn = small ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 2>{});
     const cudaError_t e = launch_dependent(fn, dim3((unsigned)blocks, (unsigned)slices), kThreads, 0,
                                            static_cast<cudaStream_t>(stream), a);
     return e == cudaSuccess ? WS_OK : set_error(WS_ERR_CUDA, cudaGetErrorString(e));

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, WARPS == 1 ? 4 : 5) block_append_ker
         float* const scale = x.scales + page * x.s_page + (uint64_t)(uint32_t)j * x.s_tok + (uint64_t)(uint32_t)head * x.s_head;
         auto place_of = [&](int64_t s) { return (uint64_t)(s - base) < (uint64_t)block ? (int)(s - base) : -1; };
         // As many tokens as the block has room for are looked at: those of this block have their place by their slots.
-        int end = min(i + block - front, N);
+        int end = (int)min((int64_t)i + block - front, (int64_t)N);
         const float held = *scale;   // what lies there, used only with rows before the first
         uint4 old = make_uint4(0, 0, 0, 0);   // the first of this thread's earlier rows, in case the scale grows
         if (in && row < front) old = *reinterpret_cast<const uint4*>(dst + (uint64_t)(uint32_t)row * x.dst_tok + 16 * u);

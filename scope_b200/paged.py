@@ -145,7 +145,7 @@ def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positi
     """Rotate a step's queries and keys and write its keys and values into the pool, in one launch.
 
     q [N, H, Dk] (or None), k [N, Hkv, Dk], v [N, Hkv, Dv]: bf16 or fp16, any strides with a unit head dim (views of a
-    packed projection are read in place).  slots int64 [N] (``PagedStep.slots``): token t's key and value rows go to
+    packed projection are read in place).  slots int64 [N] (``PagedStep.slots``, each at most once): token t's key and value rows go to
     slot slots[t]; a negative slot drops them.  An int8 pool gets codes and one scale per row, taken from the rotated
     row in fp32 (the rule of ``kv_quantize_bf16_to_int8``); a NaN in a row makes the row's scale NaN, an infinity makes it
     infinite over codes of 0, so either row reads back as NaN.  ``cos_sin`` None: no rotation.  Rotary arguments as in

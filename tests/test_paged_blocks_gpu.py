@@ -542,6 +542,44 @@ def test_decode_queries_of_any_size_over_e4m3(size):
     agrees(s, *decode(s))
 
 
+@pytest.mark.parametrize("pool,block", [(I8, 64), (E4, 64), (I8, 16)])
+def test_decode_past_32_bits(pool, block):
+    """A pool of more than 2^32 bytes, its first and last pages, as one cache and as pairs of heads."""
+    n_pages, P, Hkv, D = 70000, 64, 8, 128
+    codes = torch.zeros(n_pages, P, Hkv, D, dtype=I8, device=DEV)
+    scales = torch.full((n_pages, P // block, Hkv), float("nan"), device=DEV)
+    g, at = gen(21), torch.tensor([n_pages - 1, 3, n_pages - 2], device=DEV)
+    x, sc = make_pool(g, 3, P, block, Hkv, D, pool)
+    raw(codes)[at], scales[at] = raw(x), sc
+    pages = codes.view(pool)
+    s = dict(q=torch.randn(2, 32, D, generator=g, device=DEV).to(BF), k=pages, v=pages, ks=scales, vs=scales, block=block,
+             table=torch.full((2, 20), -1, dtype=torch.int32, device=DEV), scale=D ** -0.5,
+             lens=torch.tensor([180, 64], dtype=torch.int32, device=DEV))
+    s["table"][0, :3], s["table"][1, :1] = at.int(), at[:1].int()
+    t = torch.arange(180, device=DEV)
+    s["rows"] = [(at[t // P], t % P), (at[:1].expand(64), t[:64])]
+    agrees(s, *decode(s))
+    lam = torch.full((1,), 0.3, device=DEV)
+    out, lse = paged.paged_diff_decode(s["q"], pages, pages, s["table"], s["lens"], s["scale"], lam, k_scales=scales, v_scales=scales)
+    small = torch.tensor([[0, 1, 2], [0, 0, 0]], dtype=torch.int32, device=DEV)   # the same pages in a pool of three
+    table = torch.cat([small, torch.full((2, 17), -1, dtype=torch.int32, device=DEV)], 1)
+    out2, lse2 = paged.paged_diff_decode(s["q"], x, x, table, s["lens"], s["scale"], lam, k_scales=sc, v_scales=sc)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2) and scope_b200.status_take() == 0
+
+
+def test_decode_queries_in_a_packed_projection_and_lengths_past_the_table():
+    s = make_decode([100, 64], 8, 2, 64, 64, 16, 16, BF, E4, seed=14)
+    wide = torch.randn(2, 8, 96, device=DEV).to(BF)
+    wide[:, :, 16:80] = s["q"]
+    more = s["lens"].clone()
+    more[0] += 1000     # the table ends at 112 tokens: what lies there counts
+    raw(s["k"])[s["table"][0, 6].long(), 4:], raw(s["v"])[s["table"][0, 6].long(), 4:] = 0, 0
+    t = torch.arange(112, device=DEV)
+    s["rows"][0] = (s["table"][0].long()[t // 16], t % 16)
+    out, lse = paged.paged_decode(wide[:, :, 16:80], s["k"], s["v"], s["table"], more, s["scale"], k_scales=s["ks"], v_scales=s["vs"])
+    agrees(s, out, lse)
+
+
 def test_decode_values_that_are_nan():
     """A NaN code of a token that counts reaches its dim only; one past the length, nobody."""
     s = make_decode([50, 700], 4, 2, 128, 128, 16, 16, HF, E4, seed=3)

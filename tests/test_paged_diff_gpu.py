@@ -238,6 +238,37 @@ def test_through_a_cache_and_a_graph():
     assert scope_b200.status_take() == 0
 
 
+def test_queries_in_a_packed_projection_and_another_stream():
+    s = make([100, 700], 4, 2, 64, 64, 16, BF, I8, 16, seed=15)
+    wide = torch.randn(2, 8, 96, device=DEV).to(BF)
+    wide[:, :, 16:80] = s["q"]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = diff(dict(s, q=wide[:, :, 16:80]))
+    side.synchronize()
+    agrees(s, *got)
+
+
+def test_two_captured_graphs_replayed_in_turn():
+    """Graphs of one stream share its workspace; replayed one after the other each gives what it gave alone."""
+    a, b = make([3000, 40], 4, 2, 64, 64, 16, BF, BF, seed=16), make([10, 5000], 8, 2, 64, 64, 64, BF, E4, 64, seed=17)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, held = [], []
+    with torch.cuda.stream(side):
+        for s in (a, b):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                held.append(diff(s))
+        for _ in range(3):
+            for graph in graphs:
+                graph.replay()
+    side.synchronize()
+    agrees(a, *held[0])
+    agrees(b, *held[1])
+
+
 def test_outputs_given_and_refusals():
     s = make([100, 30], 4, 2, 64, 64, 16, BF, BF, seed=7)
     out, lse = torch.empty(2, 4, 128, dtype=BF, device=DEV), torch.empty(2, 8, device=DEV)

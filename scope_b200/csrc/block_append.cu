@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, WARPS == 1 ? 4 : 5) block_append_ker
             most = warp_most(most);
             first = __reduce_min_sync(0xffffffffu, first);
             dropped = __any_sync(0xffffffffu, dropped);
-            if (WARPS == 1) return;
+            if (WARPS == 1) return __syncwarp();   // all have read the scale that one is about to write
             const int buf = turns++ & 1;
             if (lane == 0) s_most[buf][warp] = most, s_more[buf][warp] = make_int2(first, dropped);
             __syncthreads();

@@ -44,7 +44,7 @@ struct BlockAppendArgs {
     int block, chunk;       // tokens of a block, of a job
     uint32_t blk_mul, blk_shift;   // s / block = (umulhi(s, mul) + s) >> shift for s < 2^31
     int Hkv;
-    int one_axis;           // all pairs turn by one axis, their turns 16-byte aligned
+    int one_axis;           // all pairs turn by one axis, forward, their turns 16-byte aligned
     uint32_t jobs;          // stretches of tokens times keys and values times heads
     uint32_t job_rate;      // of 2^32 CTAs, how many are theirs
     int all_jobs;           // there are no others
@@ -365,7 +365,7 @@ int block_append_launch(const RopeAppendArgs& q, bool f16, bool e4m3, bool vec, 
     a.block = block;
     while ((1ull << a.blk_shift) < (uint64_t)block) ++a.blk_shift;
     a.blk_mul = (uint32_t)((((1ull << a.blk_shift) - block) << 32) / block + 1);
-    a.one_axis = q.turns_vec && q.rope.n_axes == 1;
+    a.one_axis = q.turns_vec && q.rope.n_axes == 1 && !q.rope.inverse;   // turning back is rare: unit_turns does it
     if (q.N > INT32_MAX - 4096) return set_error(WS_ERR_UNSUPPORTED, "rope_append: too many tokens");
     // A job is the block of one token where there are few, else those of up to a block of tokens, as long as every SM has 16
     // warps.  A warp takes it, or a CTA where blocks are large and tokens many (17 thousand tokens of 4 + 4 heads of 128 in

@@ -946,7 +946,10 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                     uint32_t r[4];
                     ldsm_x4(TMA ? piece(st + h * C::kTile, lane & 15, lane >> 4, ks) : k_ld + h * 16 * krow + ks * 16, r[0], r[1], r[2], r[3]);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {   // past an odd nks the queries are zero and what was read is finite
+                    for (int u = 0; u < 2; ++u) {
+                        // past an odd nks lies the next row, against queries of zero: int8 codes are finite, but an e4m3
+                        // code may be NaN
+                        if (E4M3 && ks + u >= nks) break;
                         const uint32_t a0 = E4M3 ? e4m3_pair<false>(r[2 * u]) : s8_pair<F16>(r[2 * u]);
                         const uint32_t a1 = E4M3 ? e4m3_pair<false>(r[2 * u + 1]) : s8_pair<F16>(r[2 * u + 1]);
                         const uint32_t a2 = E4M3 ? e4m3_pair<true>(r[2 * u]) : s8_pair<F16>(r[2 * u] >> 8);

@@ -40,7 +40,8 @@
 //     fp16 with them, times the power of two that brings a head's largest value to 2^14, exact to 2^-38 of it (8 requests:
 //     69.2 us).  Their bytes may be NaN, so values that do not count are zeroed as in 16 bits.
 //   * DIFF: o = softmax(q1 k1) v - lam softmax(q2 k2) v over pairs of pool heads.  A pair is one row: its keys lie side by
-//     side, and the queries of the two maps are two columns, each zero over the other's dims, so one pass over keys and
+//     side, and the queries of the two maps are two columns, each against its own half of the dims (the products with the
+//     other half go into sums that nobody reads: one that is not finite stays in its map), so one pass over keys and
 //     values serves both maps and the products are the ones above.  A lane then holds both maps' sums of a head and takes
 //     the difference, and the norm over a head's dims, before it writes; joined rows keep the difference in shared memory
 //     until all jobs' sums of squares are known.
@@ -905,17 +906,22 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
             order_q();
             began = meta.sub == 0;
         }
-        // scores of each 16-token tile; a single tile's in two chains
-        constexpr int kChains = H == 1 ? 2 : 1;
-        float c[H][NT][4], e[kChains == 2 ? NT : 1][4];
+        // scores of each 16-token tile; a single tile's in two chains.  DIFF: c is the first map's and e the second's, so that a
+        // key that is not finite meets no other map's zeros (193 requests of up to 11054 tokens, 6 pairs of 2 x 48 dims in int8:
+        // 400 us, 395 with the sums in common; 64 of 4000, 16-dim maps of 8 heads a pair: 58.9 and 55.7; nothing where rows
+        // come by TMA)
+        constexpr int kChains = DIFF || H == 1 ? 2 : 1, kE = kChains == 2 ? H : 1;
+        float c[H][NT][4], e[kE][NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
                 for (int h = 0; h < H; ++h) c[h][nt][i] = 0.f;
-                if (kChains == 2) e[nt][i] = 0.f;
+#pragma unroll
+                for (int h = 0; h < kE; ++h) e[h][nt][i] = 0.f;
             }
+        auto in_e = [&](int ks) { return kChains == 2 && (DIFF ? 2 * ks >= nks : ks & 1); };
         // values of tokens that do not count, which TMA brought with the others: zero (int8 codes are finite)
         if (TMA && CODE != kS8 && meta.mask != (kTok == 32 ? 0xffffffffu : 0xffffu)) {
             constexpr int kLine = C::kInner / 16;
@@ -955,8 +961,10 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                         const uint32_t a2 = E4M3 ? e4m3_pair<true>(r[2 * u]) : s8_pair<F16>(r[2 * u] >> 8);
                         const uint32_t a3 = E4M3 ? e4m3_pair<true>(r[2 * u + 1]) : s8_pair<F16>(r[2 * u + 1] >> 8);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            mma16<kKF16>(kChains == 2 && u ? e[nt] : c[h][nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if (in_e(ks + u)) mma16<kKF16>(e[h % kE][nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
+                            else mma16<kKF16>(c[h][nt], a0, a1, a2, a3, bq[nt][ks + u][0], bq[nt][ks + u][1]);
+                        }
                     }
                 }
             }
@@ -969,8 +977,10 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                     uint32_t a0, a1, a2, a3;
                     ldsm_x4(TMA ? piece(st + h * C::kTile, lane & 15, lane >> 4, 2 * ks) : k_ld + h * 16 * krow + ks * 32, a0, a1, a2, a3);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma16<F16>(kChains == 2 && (ks & 1) ? e[nt] : c[h][nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (in_e(ks)) mma16<F16>(e[h % kE][nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
+                        else mma16<F16>(c[h][nt], a0, a1, a2, a3, bq[nt][ks][0], bq[nt][ks][1]);
+                    }
                 }
             }
         }
@@ -989,7 +999,9 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                 for (int i = 0; i < 4; ++i) {
                     float by = f[DIFF ? i & 1 : 0][i >> 1];
                     if (E4M3 && !F16) by *= q_scale[nt][i & 1];
-                    c[h][nt][i] = (kChains == 2 ? c[h][nt][i] + e[nt][i] : c[h][nt][i]) * by;
+                    float z = c[h][nt][i];
+                    if (kChains == 2) z = !DIFF ? z + e[h % kE][nt][i] : i & 1 ? e[h % kE][nt][i] : z;
+                    c[h][nt][i] = z * by;
                 }
         }
         if (meta.mask != (kTok == 32 ? 0xffffffffu : 0xffffu)) {   // tokens that do not count (their values and scales are zero)

@@ -4,6 +4,7 @@ import torch
 
 import scope_b200
 from test_paged_blocks_gpu import E4, decode, make_decode, raw, widened
+from test_paged_diff_gpu import diff, make
 from test_paged_gpu import BF, DEV, HF
 
 pytestmark = pytest.mark.gpu
@@ -31,3 +32,52 @@ def test_a_nan_value_in_e4m3_reaches_its_dim_only(Dk, Dv, dtype, P, block):
         assert torch.equal(out.isnan(), nan) and torch.equal(lse, want_lse)
         assert torch.equal(out[~nan], want[~nan])
     assert scope_b200.status_take() == 0
+
+
+def far(s, n=600):
+    """The same requests behind a table of more than n tokens: rows by TMA, where they can come so."""
+    return dict(s, table=torch.cat([s["table"], s["table"].new_full((s["table"].shape[0], n // s["k"].shape[1] + 1), 1 << 20)], 1))
+
+
+@pytest.mark.parametrize("Dk,Dv", [(16, 16), (32, 32), (48, 48), (64, 64), (80, 80), (96, 96), (112, 16), (128, 128)])
+@pytest.mark.parametrize("dtype,pool,block", [(BF, BF, 1), (HF, HF, 1), (BF, E4, 16), (HF, E4, 64), (BF, E4, 8)])
+@pytest.mark.parametrize("heads", [4, 12])
+@pytest.mark.parametrize("m", [0, 1])
+def test_a_key_of_one_map_does_not_reach_the_other(Dk, Dv, dtype, pool, block, heads, m):
+    """A NaN key of one head of a pair, in every row of a subtile and every group of dims, a request each: that map's heads
+    have a NaN lse and outputs; the other map's lse, and the other pair, are bit for bit what they were."""
+    B, pairs = 131, 2
+    G = heads // pairs
+    s = make([70] * B, heads, pairs, Dk, Dv, 64, dtype, pool, block, seed=Dk + heads)
+    b = torch.arange(B, device=DEV)
+    t, dim = b % 67, 5 * b % Dk
+    page, off = s["table"].long()[b, t // 64], t % 64
+    want, want_lse = diff(s)
+    assert want.isfinite().all() and want_lse.isfinite().all()
+    if pool == E4:
+        raw(s["k"])[page, off, 2 + m, dim] = 0xff
+    else:
+        s["k"][page, off, 2 + m, dim] = float("nan")
+    for x in (s, far(s)):
+        out, lse = diff(x)
+        assert lse[:, 2 * G + m::2].isnan().all() and out[:, G:].isnan().all()
+        assert torch.equal(lse[:, :2 * G], want_lse[:, :2 * G]) and torch.equal(out[:, :G], want[:, :G])
+        assert torch.equal(lse[:, 2 * G + 1 - m::2], want_lse[:, 2 * G + 1 - m::2])
+    assert scope_b200.status_take() == 0
+
+
+@pytest.mark.parametrize("Dk", [32, 48, 64, 96, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m", [0, 1])
+def test_a_score_of_minus_infinity_leaves_a_token_out_of_its_map(Dk, dtype, m):
+    """Keys of -inf against positive queries weigh nothing in their map, as ones do whose score is finite and far below."""
+    s = make([70, 700, 33], 4, 2, Dk, Dk, 64, dtype, dtype, seed=Dk)
+    s["q"][:, :, 7] = 32.0
+    got = []
+    for x in (torch.finfo(dtype).min, float("-inf")):   # times 32 and the scale: far below any other score
+        for b, t in ((0, 3), (0, 69), (1, 0), (1, 511), (2, 32)):
+            s["k"][s["table"][b, t // 64].long(), t % 64, 2 + m, 7] = x
+        got += [diff(s), diff(far(s))]
+    for out, lse in got:
+        assert out.isfinite().all() and lse.isfinite().all()
+        assert torch.equal(out, got[0][0]) and torch.equal(lse, got[0][1])

@@ -6,7 +6,7 @@ A model of one attention layer with random weights, so that a prompt needs the a
 step packs the tokens that the running requests add -- a whole prompt for a request that joins, one token for the others
 -- and runs
     begin_step   pages, slots and positions from the lengths       (one launch)
-    append       rotate q and k, write k and v into the pages      (one launch)
+    append       rotate q and k, write k and v into the pages      (one launch; long prompts into 8-bit blocks: two)
     decode       each request's last token over its pages          (one launch)
     release      the pages of requests that are done go back       (one launch)
 A step without prompts has one shape, so its launches are captured in a CUDA graph once and replayed.

@@ -478,7 +478,8 @@ typedef struct ws_rope {
 
 /*
  * Rotation of a step's queries and keys, and the scatter of its keys and
- * values into the paged cache, in one launch.
+ * values into the paged cache: one launch, or two where many tokens go into blocks
+ * that share a scale (the queries first, after every check of the call).
  *   q [N, H, Dk] -> q_out (may be q); k [N, Hkv, Dk], v [N, Hkv, Dv]: element
  *   (t, h, d) at base + t*stride_tok + h*stride_head + d; dtype WS_DTYPE_BF16 or
  *   WS_DTYPE_F16.  The pool holds that type, or int8 codes with a scale per row:

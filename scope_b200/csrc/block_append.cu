@@ -350,8 +350,10 @@ __global__ void __launch_bounds__(kThreads, WARPS == 1 ? 4 : 5) block_append_ker
 
 bool block_append_small(int64_t N, int Hkv) { return N * 2 * Hkv <= (int64_t)device_sm_count() * 16; }
 
-int block_append_launch(const RopeAppendArgs& q, bool f16, bool e4m3, bool vec, int block, cudaStream_t st) {
-    BlockAppendArgs a;
+namespace {
+
+// What a call refuses, and how it is cut: into `blocks` CTAs, a job taken by `warps` warps.
+int plan(const RopeAppendArgs& q, int block, BlockAppendArgs& a, int& warps, int64_t& blocks) {
     memset(&a, 0, sizeof(a));
     a.q = q;
     for (int i = 0; i < 2; ++i) {
@@ -372,12 +374,12 @@ int block_append_launch(const RopeAppendArgs& q, bool f16, bool e4m3, bool vec, 
     // blocks of 64, us by warps and by CTAs: 59 and 29; 4.6 thousand of 5 + 5 heads of 80 in blocks of 8: 13 and 20).
     const int Hkv = a.Hkv = a.kv[0].n, sms = device_sm_count();
     const int64_t each = q.N * 2 * Hkv, units = (int64_t)block * q.lanes;
-    const int warps = units > kThreads && !block_append_small(q.N, Hkv) ? kWarps : 1;
+    warps = units > kThreads && !block_append_small(q.N, Hkv) ? kWarps : 1;
     const int64_t room = (int64_t)sms * 16 / warps;
     a.chunk = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(block, 4096), (each + room - 1) / room));
     const int64_t parts = (q.N + a.chunk - 1) / a.chunk;
     const int64_t jobs = parts * 2 * Hkv, job_ctas = warps == 1 ? (jobs + kWarps - 1) / kWarps : jobs;
-    int64_t blocks = job_ctas;
+    blocks = job_ctas;
     if (q.h[0].n) {   // the queries: as in rope_append_kernel, two rows a turn
         const int rows = 32 / q.lanes, steps = (q.h[0].n + 2 * rows - 1) / (2 * rows);
         a.q.parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps, ((int64_t)sms * 32 + q.N - 1) / q.N));
@@ -388,6 +390,23 @@ int block_append_launch(const RopeAppendArgs& q, bool f16, bool e4m3, bool vec, 
     // CTA b is the n-th for jobs where n = floor(b rate / 2^32) is below floor((b + 1) rate / 2^32)
     a.all_jobs = job_ctas == blocks;
     a.job_rate = a.all_jobs ? 0 : (uint32_t)((((uint64_t)job_ctas << 32) + blocks - 1) / blocks);
+    return WS_OK;
+}
+
+}  // namespace
+
+int block_append_check(const RopeAppendArgs& q, int block) {
+    BlockAppendArgs a;
+    int warps;
+    int64_t blocks;
+    return plan(q, block, a, warps, blocks);
+}
+
+int block_append_launch(const RopeAppendArgs& q, bool f16, bool e4m3, bool vec, int block, cudaStream_t st) {
+    BlockAppendArgs a;
+    int warps;
+    int64_t blocks;
+    if (const int rc = plan(q, block, a, warps, blocks)) return rc;
     auto pick = [&](auto half, auto eight) {
         constexpr bool F = decltype(half)::value, E = decltype(eight)::value;
         if (warps == 1) return vec ? block_append_kernel<F, E, true, 1> : block_append_kernel<F, E, false, 1>;

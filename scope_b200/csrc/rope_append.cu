@@ -140,10 +140,11 @@ extern "C" int ws_rope_append(const ws_rope* rope, const void* q, int64_t q_stri
     const int block = kv ? std::max(kv->scale_block, 1) : 1;
     const bool e4 = kv && kv->dtype == WS_DTYPE_E4M3, blocks8 = kv && block > 1 && (e4 || kv->dtype == WS_DTYPE_I8);
     if (blocks8 && H > 0 && !block_append_small(N, kv->Hkv)) {
+        a.h[0].n = 0;
+        if (const int rc = block_append_check(a, block)) return rc;   // before q_out, which may be q, is written
         if (const int rc = ws_rope_append(rope, q, q_stride_tok, q_stride_head, H, D, q_out, qo_stride_tok, qo_stride_head, nullptr, 0,
                                           0, nullptr, 0, 0, dtype, N, nullptr, nullptr, stream))
             return rc;
-        a.h[0].n = 0;
     }
     if (blocks8)
         return block_append_launch(a, dtype == WS_DTYPE_F16, kv->dtype == WS_DTYPE_E4M3, vec, block, static_cast<cudaStream_t>(stream));

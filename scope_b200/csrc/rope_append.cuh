@@ -282,8 +282,9 @@ __device__ __forceinline__ void rope_rows(const RopeAppendArgs& a, int64_t item)
 }
 
 // The append into blocks of `block` tokens that share a scale (block_append.cu).  The queries go with it where the call is
-// small, else by themselves.
+// small, else by themselves, ahead of it and after its check.
 bool block_append_small(int64_t N, int Hkv);
+int block_append_check(const RopeAppendArgs& args, int block);
 int block_append_launch(const RopeAppendArgs& args, bool f16, bool e4m3, bool vec, int block, cudaStream_t st);
 
 }  // namespace ws

@@ -142,7 +142,8 @@ def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positi
                 k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
                 sections: Sequence[int] | None = None, cyclic: bool = False, pairs: str = "half",
                 q_out: torch.Tensor | None = None):
-    """Rotate a step's queries and keys and write its keys and values into the pool, in one launch.
+    """Rotate a step's queries and keys and write its keys and values into the pool: one launch, or two where many tokens go
+    into blocks that share a scale.
 
     q [N, H, Dk] (or None), k [N, Hkv, Dk], v [N, Hkv, Dv]: bf16 or fp16, any strides with a unit head dim (views of a
     packed projection are read in place).  slots int64 [N] (``PagedStep.slots``, each at most once): token t's key and value rows go to

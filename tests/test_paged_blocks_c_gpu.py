@@ -61,3 +61,22 @@ def test_append_turned_back(pool, block, N, aligned, adjacent, axes):
     assert torch.equal(ks, wks) and torch.equal(vs, wvs)
     assert torch.equal(raw(kp), raw(wk)) and torch.equal(raw(vp), raw(wv))
     assert scope_b200.status_take() == 0
+
+
+@pytest.mark.parametrize("N", [20, 3000])
+def test_a_refused_append_leaves_the_queries(N):
+    """In place, so a caller who falls back after the refusal does not turn them twice."""
+    g, H, Hkv, D = gen(N), 4, 2, 64
+    q, k, v = (torch.randn(N, h, D, generator=g, device=DEV).to(BF) for h in (H, Hkv, Hkv))
+    (kp, ks), (vp, vs) = (make_pool(g, 200, 16, 16, Hkv, D, I8) for _ in range(2))
+    table, pos = table_of(100, D), torch.randint(1, 100, (N,), generator=g, device=DEV, dtype=torch.int32)
+    rope = rope_pack(pos.data_ptr(), table.data_ptr(), 0, 100, 0, 1, D, 0, 0, 0, b"")
+    was, pages = q.clone(), kp.clone()
+    kv = kv_of(kp, vp, ks, vs)
+    L, s = _lib.lib(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    slots = torch.arange(N, device=DEV)
+    rc = L.ws_rope_append(rope, q.data_ptr(), q.stride(0), q.stride(1), H, D, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+                          1 << 33, D, v.data_ptr(), v.stride(0), v.stride(1), DTYPE[BF], N, slots.data_ptr(), kv, s)
+    assert rc == _lib.WS_ERR_UNSUPPORTED
+    torch.cuda.synchronize()
+    assert torch.equal(q, was) and torch.equal(raw(kp), raw(pages))

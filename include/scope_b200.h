@@ -495,7 +495,8 @@ typedef struct ws_rope {
  *     rne(code * (s_old * (1 / s))), and rows behind the last written are nobody's.
  *   s NaN or infinite: all these codes are 0, so the block reads back as NaN.
  *   A block's tokens follow one another in the call, dropped ones aside, in the
- *   order of their slots; ws_paged_slots lays them so.
+ *   order of their slots; ws_paged_slots lays them so.  Strides from token to
+   token and from block to block stay below 2^32 elements there.
  *   slots int64 [N]: token t's keys and values go to slot slots[t]; a negative
  *   slot drops them, one past the pool drops them and records WS_ERR_DEVICE.
  * rope NULL: no rotation.  H = 0: no queries.  kv NULL: queries only (k, v,

@@ -30,12 +30,12 @@ namespace {
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kHeld = 4;    // rows of a block that a thread keeps; those behind them are read twice
 
-struct Side {           // keys or values: Heads with strides that fit 32 bits
+struct Side {           // keys or values: Heads with strides of tokens and blocks that fit 32 bits
     const uint16_t* src;
     uint8_t* dst;
     float* scales;
-    int64_t dst_page, s_page;
-    uint32_t src_tok, src_head, dst_tok, dst_head, s_tok, s_head;
+    int64_t dst_page, s_page, src_head, dst_head, s_head;
+    uint32_t src_tok, dst_tok, s_tok;
     int n, D;
 };
 struct BlockAppendArgs {
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, WARPS == 1 ? 4 : 5) block_append_ker
     const bool in = 16 * u < x.D, turn = kind == 0 && 16 * u < r.rope_dim, split = turn && !r.adjacent;
     const int d0 = split ? 8 * u : 16 * u, d1 = split ? (r.rope_dim >> 1) + 8 * u : 16 * u + 8;
     const int N = (int)a.q.N, block = a.block;
-    const uint16_t* const src = x.src + (uint64_t)(uint32_t)head * x.src_head;
+    const uint16_t* const src = x.src + head * x.src_head;
     int* const s_place = reinterpret_cast<int*>(s_row + kHeld * 4 * kThreads);
 
     auto slot_of = [&](int t) -> int64_t {   // -1: dropped, or none
@@ -189,8 +189,8 @@ __global__ void __launch_bounds__(kThreads, WARPS == 1 ? 4 : 5) block_append_ker
         const int front = offset_of(s_i);
         const int64_t base = s_i - front, page = base >> 31 == 0 ? (int64_t)((uint32_t)base / (uint32_t)a.q.page_size) : base / a.q.page_size;
         const int at = (int)(base - page * a.q.page_size), j = (int)((__umulhi((uint32_t)at, a.blk_mul) + (uint32_t)at) >> a.blk_shift);
-        uint8_t* const dst = x.dst + page * x.dst_page + (uint64_t)(uint32_t)at * x.dst_tok + (uint64_t)(uint32_t)head * x.dst_head;
-        float* const scale = x.scales + page * x.s_page + (uint64_t)(uint32_t)j * x.s_tok + (uint64_t)(uint32_t)head * x.s_head;
+        uint8_t* const dst = x.dst + page * x.dst_page + (uint64_t)(uint32_t)at * x.dst_tok + head * x.dst_head;
+        float* const scale = x.scales + page * x.s_page + (uint64_t)(uint32_t)j * x.s_tok + head * x.s_head;
         auto place_of = [&](int64_t s) { return (uint64_t)(s - base) < (uint64_t)block ? (int)(s - base) : -1; };
         // As many tokens as the block has room for are looked at: those of this block have their place by their slots.
         int end = (int)min((int64_t)i + block - front, (int64_t)N);
@@ -358,10 +358,10 @@ int plan(const RopeAppendArgs& q, int block, BlockAppendArgs& a, int& warps, int
     a.q = q;
     for (int i = 0; i < 2; ++i) {
         const Heads& h = q.h[1 + i];
-        for (const int64_t stride : {h.src_tok, h.src_head, h.dst_tok, h.dst_head, h.s_tok, h.s_head})
-            if (stride < 0 || stride > UINT32_MAX) return set_error(WS_ERR_UNSUPPORTED, "rope_append: a stride past 32 bits");
-        a.kv[i] = {h.src, h.dst, h.scales, h.dst_page, h.s_page, (uint32_t)h.src_tok, (uint32_t)h.src_head, (uint32_t)h.dst_tok,
-                   (uint32_t)h.dst_head, (uint32_t)h.s_tok, (uint32_t)h.s_head, h.n, h.D};
+        for (const int64_t stride : {h.src_tok, h.dst_tok, h.s_tok})
+            if (stride < 0 || stride > UINT32_MAX) return set_error(WS_ERR_UNSUPPORTED, "rope_append: a stride of tokens or blocks past 32 bits");
+        a.kv[i] = {h.src, h.dst, h.scales, h.dst_page, h.s_page, h.src_head, h.dst_head, h.s_head,
+                   (uint32_t)h.src_tok, (uint32_t)h.dst_tok, (uint32_t)h.s_tok, h.n, h.D};
     }
     a.q.h[1].n = a.q.h[2].n = 0;
     a.block = block;

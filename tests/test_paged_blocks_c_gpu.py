@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import scope_b200
-from scope_b200 import _lib
+from scope_b200 import _lib, paged
 from test_paged import paged_kv_pack, rope_pack
 from test_paged_blocks_gpu import E4, I8, append_reference, make_pool, raw
 from test_paged_gpu import BF, DEV, HF, gen, table_of, turned
@@ -80,3 +80,19 @@ def test_a_refused_append_leaves_the_queries(N):
     assert rc == _lib.WS_ERR_UNSUPPORTED
     torch.cuda.synchronize()
     assert torch.equal(q, was) and torch.equal(raw(kp), raw(pages))
+
+
+def test_append_where_heads_lie_past_32_bits():
+    """A pool with its heads outermost, each of more than 2^32 codes: its last pages."""
+    n_pages, P, Hkv, D, block = 270000, 128, 2, 128, 16
+    kp = torch.zeros(Hkv, n_pages, P, D, dtype=I8, device=DEV).permute(1, 2, 0, 3)
+    vp = torch.zeros(n_pages, P, Hkv, 16, dtype=I8, device=DEV)
+    ks, vs = (torch.zeros(n_pages, P // block, Hkv, device=DEV) for _ in range(2))
+    assert kp.stride(2) > 1 << 32
+    for N in (3, 1000):
+        k = torch.randn(N, Hkv, D, generator=gen(N), device=DEV).to(BF)
+        near = torch.arange(N, device=DEV) + 5     # in the last nine pages
+        want = append_reference(k.float(), near, kp[-9:], ks[-9:], block)
+        paged.rope_append(None, k, k[..., :16], None, None, near + (n_pages - 9) * P, kp, vp, k_scales=ks, v_scales=vs)
+        assert torch.equal(raw(kp[-9:]), raw(want[0])) and torch.equal(ks[-9:], want[1])
+    assert scope_b200.status_take() == 0

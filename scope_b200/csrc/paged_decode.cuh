@@ -906,11 +906,13 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
             order_q();
             began = meta.sub == 0;
         }
-        // scores of each 16-token tile; a single tile's in two chains.  DIFF: c is the first map's and e the second's, so that a
-        // key that is not finite meets no other map's zeros (193 requests of up to 11054 tokens, 6 pairs of 2 x 48 dims in int8:
-        // 400 us, 395 with the sums in common; 64 of 4000, 16-dim maps of 8 heads a pair: 58.9 and 55.7; nothing where rows
-        // come by TMA)
-        constexpr int kChains = DIFF || H == 1 ? 2 : 1, kE = kChains == 2 ? H : 1;
+        // scores of each 16-token tile; a single tile's in two chains.  DIFF: the maps apart, so that a key that is not finite
+        // meets no other map's zeros: of two tiles c is the first map's and e the second's; of one, and where the registers do
+        // not hold both (16-dim maps of more than four heads a pair: 58.9 us so, 57.2 this way), the first map's columns are put
+        // by where its steps end.  (Against the maps in common, by cp.async: 193 requests of up to 11054 tokens, 6 pairs of
+        // 2 x 48 dims in int8, 402 us and 396; 24 of up to 86, 2 x 80 in bf16, 19.0 and 18.5; by TMA the same.)
+        constexpr bool kApart = DIFF && H == 2 && (EXACT || NT == 1), kPutBy = DIFF && !kApart;
+        constexpr int kChains = kApart || H == 1 ? 2 : 1, kE = kChains == 2 ? H : 1;
         float c[H][NT][4], e[kE][NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -921,7 +923,19 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
 #pragma unroll
                 for (int h = 0; h < kE; ++h) e[h][nt][i] = 0.f;
             }
-        auto in_e = [&](int ks) { return kChains == 2 && (DIFF ? 2 * ks >= nks : ks & 1); };
+        auto in_e = [&](int ks) { return kChains == 2 && (kApart ? 2 * ks >= nks : ks & 1); };
+        float first_map[kPutBy ? H : 1][kPutBy ? NT : 1][2];
+        auto put_by = [&](int ks, int h) {
+            if (!kPutBy || 2 * ks != nks) return;
+#pragma unroll
+            for (int nt = 0; nt < (kPutBy ? NT : 0); ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i % 2 == 0) first_map[h % (kPutBy ? H : 1)][nt][i / 2] = kChains == 2 ? c[h][nt][i] + e[h % kE][nt][i] : c[h][nt][i];
+                    c[h][nt][i] = 0.f;
+                    if (kChains == 2) e[h % kE][nt][i] = 0.f;
+                }
+        };
         // values of tokens that do not count, which TMA brought with the others: zero (int8 codes are finite)
         if (TMA && CODE != kS8 && meta.mask != (kTok == 32 ? 0xffffffffu : 0xffffu)) {
             constexpr int kLine = C::kInner / 16;
@@ -956,6 +970,7 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                         // past an odd nks lies the next row, against queries of zero: int8 codes are finite, but an e4m3
                         // code may be NaN
                         if (E4M3 && ks + u >= nks) break;
+                        put_by(ks + u, h);
                         const uint32_t a0 = E4M3 ? e4m3_pair<false>(r[2 * u]) : s8_pair<F16>(r[2 * u]);
                         const uint32_t a1 = E4M3 ? e4m3_pair<false>(r[2 * u + 1]) : s8_pair<F16>(r[2 * u + 1]);
                         const uint32_t a2 = E4M3 ? e4m3_pair<true>(r[2 * u]) : s8_pair<F16>(r[2 * u] >> 8);
@@ -974,6 +989,7 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                 if (ks >= nks) break;
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
+                    put_by(ks, h);
                     uint32_t a0, a1, a2, a3;
                     ldsm_x4(TMA ? piece(st + h * C::kTile, lane & 15, lane >> 4, 2 * ks) : k_ld + h * 16 * krow + ks * 32, a0, a1, a2, a3);
 #pragma unroll
@@ -1000,7 +1016,9 @@ __global__ void __launch_bounds__(32 * Cfg<CODE, DIFF, DB, NT>::kWarps, 1) decod
                     float by = f[DIFF ? i & 1 : 0][i >> 1];
                     if (E4M3 && !F16) by *= q_scale[nt][i & 1];
                     float z = c[h][nt][i];
-                    if (kChains == 2) z = !DIFF ? z + e[h % kE][nt][i] : i & 1 ? e[h % kE][nt][i] : z;
+                    if (kApart) z = i & 1 ? e[h % kE][nt][i] : z;
+                    else if (kPutBy && i % 2 == 0) z = first_map[h % (kPutBy ? H : 1)][nt % (kPutBy ? NT : 1)][i / 2];
+                    else if (kChains == 2) z += e[h % kE][nt][i];
                     c[h][nt][i] = z * by;
                 }
         }

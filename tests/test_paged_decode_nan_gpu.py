@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import scope_b200
-from test_paged_blocks_gpu import E4, decode, make_decode, raw, widened
+from test_paged_blocks_gpu import E4, I8, decode, make_decode, raw, widened
 from test_paged_diff_gpu import diff, make
 from test_paged_gpu import BF, DEV, HF
 
@@ -81,3 +81,35 @@ def test_a_score_of_minus_infinity_leaves_a_token_out_of_its_map(Dk, dtype, m):
     for out, lse in got:
         assert out.isfinite().all() and lse.isfinite().all()
         assert torch.equal(out, got[0][0]) and torch.equal(lse, got[0][1])
+
+
+@pytest.mark.parametrize("D", [32, 48, 64, 96, 128])
+@pytest.mark.parametrize("dtype,pool,block", [(BF, I8, 1), (HF, I8, 16), (BF, I8, 64), (HF, E4, 1), (BF, E4, 16), (BF, E4, 64)])
+@pytest.mark.parametrize("m", [0, 1])
+def test_a_scale_that_is_not_finite_stays_with_its_head(D, dtype, pool, block, m):
+    """A block (or row) of one head of a pair that reads back as NaN: of a key its map's lse, of a value its half of the dims.
+
+    The other map's scores are the same, but the reference of its softmax moves with the pair's: two sums over n tokens of the
+    same terms, each off by (n + 64) 2^-24 and 2^-22 |lse|."""
+    s = make([70, 333, 200], 4, 2, D, D, 64, dtype, pool, block, seed=D + block)
+    b, t = torch.tensor([0, 1, 2], device=DEV), torch.tensor([5, 200, 199], device=DEV)
+    page, j = s["table"].long()[b, t // 64], t % 64 // block
+    bad = torch.tensor([float("nan"), float("inf"), float("nan")], device=DEV)
+    for form in (lambda z: z, far):
+        want, want_lse = diff(form(s), False)
+        for x in "kv":
+            codes, scales = s[x].clone(), s[x + "s"].clone()
+            for p, i in zip(page.tolist(), j.tolist()):
+                raw(codes)[p, i * block:(i + 1) * block, 2 + m] = 0    # as an append leaves it
+            scales[page, j, 2 + m] = bad
+            out, lse = diff(form(dict(s, **{x: codes, x + "s": scales})), False)
+            assert torch.equal(out[:, :2], want[:, :2]) and torch.equal(lse[:, :4], want_lse[:, :4])   # the other pair
+            if x == "k":
+                other, want_other = lse[:, 5 - m::2], want_lse[:, 5 - m::2]
+                assert lse[:, 4 + m::2].isnan().all() and out[:, 2:].isnan().all()
+                assert ((other - want_other).abs() <= 2 * ((333 + 64) * 2.0 ** -24 + 2.0 ** -22 * want_other.abs()) + 2e-6).all()
+            else:
+                mine, others = (slice(h * D, (h + 1) * D) for h in (m, 1 - m))
+                assert out[:, 2:, mine].isnan().all() and torch.equal(out[:, 2:, others], want[:, 2:, others])
+                assert torch.equal(lse, want_lse)
+    assert scope_b200.status_take() == 0

@@ -540,6 +540,7 @@ size_t ws_paged_decode_workspace_size(int B, int Hkv, int G, int Dv);
  *   q [B, 2*H, Dk], H = Hkv/2 * G: map m of head h at q + b*q_stride_b + (2*h + m)*q_stride_h;
  *   lam fp32, head h's at lam + h*lam_stride (0: one for all); norm_weight fp32 [2*Dv] or NULL;
  *   out [B, H, 2*Dv] contiguous in q_dtype; out_lse [B, 2*H] fp32, of each map (NULL: none).
+ * A key that is not finite reaches its own map's scores alone.
  * Dk, Dv at most 128; everything else, the workspace too, as in ws_paged_decode
  * (whose limits hold with Hkv/2 heads of 2*G queries, 2*Dk and 2*Dv dims).
  */

@@ -371,7 +371,10 @@ int plan(const RopeAppendArgs& q, int block, BlockAppendArgs& a, int& warps, int
     if (q.N > INT32_MAX - 4096) return set_error(WS_ERR_UNSUPPORTED, "rope_append: too many tokens");
     // A job is the block of one token where there are few, else those of up to a block of tokens, as long as every SM has 16
     // warps.  A warp takes it, or a CTA where blocks are large and tokens many (17 thousand tokens of 4 + 4 heads of 128 in
-    // blocks of 64, us by warps and by CTAs: 59 and 29; 4.6 thousand of 5 + 5 heads of 80 in blocks of 8: 13 and 20).
+    // blocks of 64, us by warps and by CTAs: 59 and 29; 4.6 thousand of 5 + 5 heads of 80 in blocks of 8: 13 and 20).  Few
+    // tokens are taken for a decode step's, one a block (8 requests, 2 kv heads of 128, blocks of 64, by warps and by CTAs: 3.4
+    // and 3.6; 64 requests, 8 kv heads, blocks of 32: 4.8 and 6.3).  Where they are one request's instead, which the host cannot
+    // see, large blocks pay for it: 64 tokens in blocks of 64 20.6 and 6.7, 512 of 2 kv heads in blocks of 256 89 and 24.
     const int Hkv = a.Hkv = a.kv[0].n, sms = device_sm_count();
     const int64_t each = q.N * 2 * Hkv, units = (int64_t)block * q.lanes;
     warps = units > kThreads && !block_append_small(q.N, Hkv) ? kWarps : 1;

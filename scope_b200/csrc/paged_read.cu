@@ -6,7 +6,7 @@
 // bytes of codes, 32 of output; 16-bit pools: 8 dims) and walks its CTA's tokens, two or four loads in flight.  The tokens'
 // places are looked up once for a CTA.
 // Measured: 16 requests of up to 32768 tokens from the first sixteenth on, 8 heads of 128 in e4m3, 168 us (1.04 GB, 6.2 TB/s,
-// 0.94 of a copy's rate); 1000 tokens of 4 heads 2.8 us.  Loads in flight: 1 took 182 us, 2 169, 4 178, 8 236 (registers,
+// 0.94 of a copy's rate), from a bf16 pool 217 us (1.38 GB, 6.4 TB/s); 1000 tokens of 4 heads 2.8 us and 2.6.  Loads in flight: 1 took 182 us, 2 169, 4 178, 8 236 (registers,
 // so fewer warps); but where all may lie in L2 (18 thousand tokens of 4 heads just written) 2 took 16.6 us and 4 14.0.  CTAs
 // of 16 tokens took 163 us there, but 6.1 us for 4.1 where heads are few; of 64 tokens 183; of 128 threads 181, 512 194.
 #include <cstdio>

@@ -195,7 +195,8 @@ class PagedKVCache:
     Where ``ShardedKVCache`` reserves max_seq tokens for every row, a request here holds only the pages its tokens
     fill, so ``num_pages * page_size`` bounds the requests' summed length.  ``dtype`` bf16, fp16, int8 or
     float8_e4m3fn (codes with one fp32 scale for each head and ``scale_block`` tokens of a page, which it divides; 1: one
-    per row).  Per step:
+    per row).  In 8 bits decode is fastest over pages and blocks of 32, 64, ... tokens, at head dims of 64, 128, ... (8 requests
+    of 16384 to 65536 tokens, 4 heads of 128, with blocks of 32 and of 16: int8 71 us and 78, e4m3 68 and 72).  Per step:
 
         step = cache.begin_step(new_lens, n_tokens)       # pages, slots, positions; lengths advance
         q = cache.append(li, q, k, v, step, cos_sin)      # each layer: rotate, write keys and values

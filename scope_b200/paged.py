@@ -160,7 +160,8 @@ def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positi
     so an open block's earlier int8 rows move by up to half a step each time it grows; e4m3 rows, by powers of two, only
     where they leave the normal range.  Rows behind the last one written are nobody's.  A NaN or an infinity makes the
     whole block read back as NaN.  A block's tokens follow one another in the call in the order of their slots, as
-    ``paged_slots`` lays them; dropped ones may lie between.
+    ``paged_slots`` lays them; dropped ones may lie between.  Strides from token to token and from block to block are below
+    2^32 elements there.
     """
     axis_map, axes = (None, 1) if cos_sin is None else _axes(cos_sin, sections, cyclic)
     return (_c or _load()).rope_append(q, k, v, positions, cos_sin, slots, k_pages, v_pages, k_scales, v_scales, axis_map,
@@ -198,9 +199,9 @@ def paged_diff_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     one after the other, its 2 * Dv values.  q [B, 2 * H, Dk]: map m of head h is q[:, 2 * h + m]; H is a multiple of the
     pairs, heads of a pair side by side.  lam fp32 [H] or one value: exp(lq1 . lk1) - exp(lq2 . lk2) + lam_init of the
     layer's learned vectors.  norm_weight fp32 [2 * Dv] (a factor 1 - lam_init goes into it).  Returns (out [B, H, 2 * Dv]
-    in q's type, lse fp32 [B, 2 * H] of each map).  Dk, Dv at most 128.  Pools, page_table, seq_lens, window and what is
-    left out as in ``paged_decode``; ``rope_append`` writes such a pool with k [N, 2 * pairs, Dk] and
-    v.view(N, 2 * pairs, Dv).
+    in q's type, lse fp32 [B, 2 * H] of each map).  A key that is not finite reaches its own map's scores alone.  Dk, Dv at most
+    128.  Pools, page_table, seq_lens, window and what is left out as in ``paged_decode``; ``rope_append`` writes such a
+    pool with k [N, 2 * pairs, Dk] and v.view(N, 2 * pairs, Dv).
     """
     return (_c or _load()).paged_diff_decode(q, k_pages, v_pages, page_table, seq_lens, scale, window, k_scales, v_scales, out,
                                              lse, lam, norm_weight, norm_eps)

@@ -301,7 +301,7 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
             out = tensor(what, "out", a[7]);
             want_rows(what, "out", out, x.scalar_type(), N, dev);
             if (out.sizes() != x.sizes()) refuse(what, "out must have x's shape");
-            want_apart(out, x, {});
+            want_apart(out, x, {&THPVariable_Unpack(a[1]), &THPVariable_Unpack(a[2])});
         }
         void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
         check(p_rope_append(&r, x.data_ptr(), x.stride(0), x.stride(1), (int)x.size(1), (int)x.size(2), out.data_ptr(),
@@ -389,7 +389,9 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 out = tensor(what, "q_out", a[13]);
                 want_rows(what, "q_out", out, st, N, dev);
                 if (out.sizes() != q.sizes()) refuse(what, "q_out must have q's shape");
-                want_apart(out, q, {&k, &v});
+                want_apart(out, q, {&k, &v, &slots});
+                for (int i = 3; i < 10; ++i)   // positions, turns, the pool
+                    if (i != 5 && a[i] != Py_None) at::assert_no_overlap(out, THPVariable_Unpack(a[i]));
             }
         } else if (a[13] != Py_None) {
             refuse(what, "q_out without q");
@@ -436,10 +438,13 @@ PyObject* decode(const char* what, PyObject* const* a, int maps, F&& call) {
     const c10::cuda::OptionalCUDAGuard guard(dev);
     const at::Tensor out = output(what, "out", a[9], {B, H / maps, maps * p.Dv}, st, dev);
     const at::Tensor lse = output(what, "lse", a[10], {B, H}, at::kFloat, dev);
-    for (const at::Tensor* t : {&q, &table, &lens}) {
-        if (a[9] != Py_None) at::assert_no_overlap(out, *t);
-        if (a[10] != Py_None) at::assert_no_overlap(lse, *t);
+    for (const int i : {9, 10}) {
+        if (a[i] == Py_None) continue;
+        const at::Tensor& t = i == 9 ? out : lse;
+        for (const int j : {0, 1, 2, 3, 4, 7, 8})
+            if (a[j] != Py_None) at::assert_no_overlap(t, THPVariable_Unpack(a[j]));
     }
+    if (a[9] != Py_None && a[10] != Py_None) at::assert_no_overlap(out, lse);
     void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
     const Workspace ws = workspace(g_decode_ws, dev, stream);
     call(q, type, (int)B, (int)(H / p.Hkv), p, table, lens, (int)std::min<int64_t>(window, INT32_MAX), (float)scale, out, lse, ws,
